@@ -282,6 +282,72 @@ enum { PKV_WTYPE_Q8_0 = 8, PKV_WTYPE_Q4K = 12, PKV_WTYPE_Q5K = 13, PKV_WTYPE_Q6K
 int pkv_gated_oproj(const float *attn, const float *gate, const void *w, int w_type, float *out,
                     int batch, int in_dim, int out_dim, pkv_stream stream);
 
+/* ---- the rest of a Gated-DeltaNet layer, prompts and single tokens ---- */
+/* Short causal convolution (depthwise_conv1d, ops.rs:18-20) with its kept inputs
+ * (conv_state, qn:683-700, 3455-3460) and activation. x: [batch, n, channels] f32, token t
+ * of sequence b at x + b * stride_b + t * stride_t (elements; a slice of a wider
+ * projection is taken as it is). weight: [channels, taps], its last tap weighs the newest
+ * input; bias: [channels] or NULL; state: [batch, channels, taps - 1], oldest input first,
+ * updated in place; out: [batch, n, channels]. out[t] = act(bias + sum_j weight[j] *
+ * input[t - taps + 1 + j]), act = y * sigmoid(y) if silu, else y. lens: device int32
+ * [batch] or NULL: the valid tokens of each sequence of a padded batch (taken into [0, n]):
+ * rows of out behind them are left as they were, and the padding of x is not read. 2, 3 or
+ * 4 taps (else PKV_ERR_UNSUPPORTED). x, out and state must not overlap. */
+int pkv_causal_conv(const float *x, int64_t stride_b, int64_t stride_t, const float *weight,
+                    const float *bias, float *state, const int *lens, float *out, int batch,
+                    int64_t n, int channels, int taps, int silu, pkv_stream stream);
+
+/* The gated delta rule over n tokens (delta_net_chunked, qn:3506-3731): pkv_deltanet_step
+ * token by token. q, k: [batch, n, k_heads, head_dim], v: [batch, n, heads, head_dim] f32,
+ * value head h reading key head h / (heads / k_heads); strides: batch and token stride of
+ * q, of k and of v in elements (slices of the convolution's output are taken as they are;
+ * multiples of 4). gate, beta: [batch, n, heads]; state, gate_offset (NULL or [batch,
+ * heads]): as pkv_deltanet_step, updated in place; lens as pkv_causal_conv: tokens behind a
+ * sequence's end change nothing and their rows of out are left as they were. out: [batch, n,
+ * heads, head_dim]. head_dim 64, 128 or 256 (else PKV_ERR_UNSUPPORTED); q, k, v, state, out
+ * and workspace 16-byte aligned; q, k and v must not overlap out or state. workspace: at
+ * least pkv_deltanet_prompt_workspace() bytes of device memory (may be 0, with NULL), which
+ * the call writes: calls that overlap in time, and graphs that do, need one each. */
+size_t pkv_deltanet_prompt_workspace(int batch, int64_t n, int heads, int head_dim);
+int pkv_deltanet_prompt(const float *q, const float *k, const float *v, const int64_t strides[6],
+                        const float *gate, const float *beta, float *state, float *gate_offset,
+                        const int *lens, float *out, int batch, int64_t n, int k_heads, int heads,
+                        int head_dim, float scale, float eps, void *workspace,
+                        size_t workspace_bytes, pkv_stream stream);
+
+/* Root-mean-square norm of rows, with the residual's addition in front and an output gate
+ * behind (RmsNorm of a layer; the gated norm per head behind the delta rule): h = residual
+ * + x, written back to residual (NULL: h = x), y = h / sqrt(mean(h^2) + eps) * alpha, times
+ * gate * sigmoid(gate) where gate is given. x: [rows, dim] f32, rows `stride` elements
+ * apart; residual, gate, out: [rows, dim] f32; alpha: [dim]. y goes to out, to out_q8_0, or
+ * to both (one may be NULL): out_q8_0 takes pkv_bytes_per_row(PKV_QUANT_Q8_0, dim) bytes a
+ * row, encoded as the cache encodes Q8_0 (a last block is filled up with zeros). dim at most
+ * 32768 (else PKV_ERR_UNSUPPORTED). out or residual may be x itself (of dense rows), out
+ * may be gate; no other buffers may overlap. */
+int pkv_rms_norm(const float *x, int64_t stride, float *residual, const float *alpha,
+                 const float *gate, float eps, float *out, void *out_q8_0, int64_t rows, int dim,
+                 pkv_stream stream);
+
+/* pkv_gated_oproj with a low-rank adapter per row (forward_with_scales_and_lora,
+ * models/with_tracing.rs:253-300, for the rows of many requests at once): out[m] = W x +
+ * lora_scale[a] * B_a (A_a x) with x = attn[m] * sigmoid(gate[m]) and a = adapter_ids[m];
+ * a negative id: no adapter. lora_a: [n_adapters, rank, in_dim], lora_b: [n_adapters,
+ * out_dim, rank], both of lora_type (a lower rank is filled up with zeros); lora_scale: f32
+ * [n_adapters]; adapter_ids: int32 [batch]; all on the device, lora_a and lora_b 16-byte
+ * aligned. An id of n_adapters or more: its row takes no adapter, and pkv_device_status
+ * reports it. rank at most PKV_LORA_MAX_RANK (else PKV_ERR_UNSUPPORTED). workspace: at least
+ * pkv_gated_oproj_lora_workspace() bytes of device memory, 256-byte aligned, which the call
+ * writes (unlike pkv_gated_oproj it allocates nothing): calls that overlap in time, and
+ * graphs that do, need one each. Everything else as pkv_gated_oproj. */
+enum { PKV_LORA_F32 = 0, PKV_LORA_F16 = 1, PKV_LORA_BF16 = 2 };
+#define PKV_LORA_MAX_RANK 128
+size_t pkv_gated_oproj_lora_workspace(int w_type, int batch, int in_dim, int out_dim, int rank);
+int pkv_gated_oproj_lora(const float *attn, const float *gate, const void *w, int w_type,
+                         const void *lora_a, const void *lora_b, int lora_type, int n_adapters,
+                         int rank, const float *lora_scale, const int *adapter_ids, float *out,
+                         int batch, int in_dim, int out_dim, void *workspace,
+                         size_t workspace_bytes, pkv_stream stream);
+
 /* ---- PrefixCache host spill (the survey's next row after the path: the reference keeps
  * prefixes in device memory only, qn:856-864; LocalBackend, paramecia-llm, is the caller
  * that would evict them). A blob is a self-describing host byte image of a prefix:

@@ -9,6 +9,7 @@ from .kv_cache import (  # noqa: F401
     KvCacheQuantization, LayerCheckpoint, LinearAttentionState, ModelKvState, PagedKvPool,
     PagedSequence, PreallocatedQuantizedKvCache,
     PrefixCache, PrefixCacheEntry, PrefixLayerMismatch, QkPrep, RecurrentState, RotaryEmbedding,
-    append_attend_batched, fill_normal, flash_attn, gated_o_proj, scale_channels,
+    append_attend_batched, causal_conv, fill_normal, flash_attn, gated_delta_rule, gated_o_proj,
+    gated_o_proj_lora, rms_norm, scale_channels,
     WTYPE_Q4K, WTYPE_Q5K, WTYPE_Q6K, WTYPE_Q8_0,
 )

@@ -35,7 +35,9 @@ SYMBOLS = (
     "pkv_pool_set_stream", "pkv_seq_create", "pkv_seq_destroy", "pkv_seq_len", "pkv_seq_pages",
     "pkv_seq_fork", "pkv_seq_truncate", "pkv_seq_append", "pkv_seq_attend",
     "pkv_seq_decode_batched", "pkv_seq_get_kv", "pkv_seq_append_batched",
-    "pkv_seq_append_decode_batched",
+    "pkv_seq_append_decode_batched", "pkv_causal_conv", "pkv_deltanet_prompt_workspace",
+    "pkv_deltanet_prompt", "pkv_rms_norm", "pkv_gated_oproj_lora_workspace",
+    "pkv_gated_oproj_lora",
 )
 
 
@@ -138,6 +140,14 @@ def _declare(L: ctypes.CDLL) -> None:
         "pkv_deltanet_step": ([vp] * 8 + [c_int] * 3 + [fl, fl, vp], c_int),
         "pkv_gated_oproj_q4k": ([vp] * 4 + [c_int] * 3 + [vp], c_int),
         "pkv_gated_oproj": ([vp] * 3 + [c_int, vp] + [c_int] * 3 + [vp], c_int),
+        "pkv_causal_conv": ([vp, c_i64, c_i64] + [vp] * 5 + [c_int, c_i64, c_int, c_int, c_int, vp], c_int),
+        "pkv_deltanet_prompt_workspace": ([c_int, c_i64, c_int, c_int], c_sz),
+        "pkv_deltanet_prompt": ([vp] * 3 + [P(c_i64)] + [vp] * 6 +
+                                [c_int, c_i64, c_int, c_int, c_int, fl, fl, vp, c_sz, vp], c_int),
+        "pkv_rms_norm": ([vp, c_i64, vp, vp, vp, fl, vp, vp, c_i64, c_int, vp], c_int),
+        "pkv_gated_oproj_lora_workspace": ([c_int] * 5, c_sz),
+        "pkv_gated_oproj_lora": ([vp] * 3 + [c_int, vp, vp] + [c_int] * 3 + [vp] * 3 + [c_int] * 3 +
+                                 [vp, c_sz, vp], c_int),
         "pkv_prefix_serialized_size": ([vp], c_sz),
         "pkv_prefix_serialize": ([vp, vp, c_sz, vp], c_int),
         "pkv_prefix_deserialize": ([vp, c_sz, P(vp), vp], c_int),

@@ -38,6 +38,10 @@ SOURCES = {
     "pkv_prefill_half.hip": [],
     "pkv_util.hip": [],
     "pkv_deltanet.hip": [],
+    "pkv_deltanet_prompt.hip": [],
+    "pkv_conv.hip": [],
+    "pkv_rmsnorm.hip": ["-ffp-contract=off"],
+    "pkv_lora.hip": [],
     "pkv_oproj.hip": [],
     "pkv_oproj_mfma.hip": [],
     "pkv_prep.hip": ["-ffp-contract=off"],

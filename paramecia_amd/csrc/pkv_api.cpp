@@ -207,6 +207,9 @@ int pkv_device_status(void) {
   if (v == 0) return PKV_OK;
   const unsigned zero = 0;
   PKV_HIP(hipMemcpy(w, &zero, sizeof zero, hipMemcpyHostToDevice));
+  if (v == kStatusAdapterId)
+    return set_error(PKV_ERR_HIP, "a projection was given an adapter id past its adapters: that "
+                                  "row took none");
   return set_error(PKV_ERR_HIP, (v & kStatusBarrierTimeout)
                                     ? "a fused decode step's quantizer barrier timed out: its "
                                       "appended row and attention output are not valid"
@@ -1165,27 +1168,140 @@ int pkv_deltanet_step(const float *q, const float *k, const float *v, const floa
                               head_dim, scale, eps, static_cast<hipStream_t>(stream));
 }
 
-// From this many tokens on, the k-quant projection runs as the batched MFMA form (each
-// decoded weight serves 32 or 64 tokens); below it, per-token GEMV workgroups.
-constexpr int kOprojMfmaMinBatch = 8;
-
 int pkv_gated_oproj(const float *attn, const float *gate, const void *w, int w_type, float *out,
                     int batch, int in_dim, int out_dim, pkv_stream stream) {
   if (!attn || !w || !out) return set_error(PKV_ERR_ARG, "null argument");
   if (batch <= 0 || in_dim <= 0 || out_dim <= 0)
     return set_error(PKV_ERR_ARG, "batch, in_dim and out_dim must be > 0");
-  const auto *wb = static_cast<const uint8_t *>(w);
-  const auto s = static_cast<hipStream_t>(stream);
-  if (batch >= kOprojMfmaMinBatch &&
-      (w_type == PKV_WTYPE_Q4K || w_type == PKV_WTYPE_Q5K || w_type == PKV_WTYPE_Q6K))
-    return launch_oproj_mfma(attn, gate, wb, w_type, out, batch, in_dim, out_dim,
-                             util_workspace(), s);
-  return launch_oproj(attn, gate, wb, w_type, out, batch, in_dim, out_dim, s);
+  return oproj_any(attn, gate, static_cast<const uint8_t *>(w), w_type, out, batch, in_dim, out_dim,
+                   util_workspace(), static_cast<hipStream_t>(stream));
 }
 
 int pkv_gated_oproj_q4k(const float *attn, const float *gate, const void *w_q4k, float *out,
                         int batch, int in_dim, int out_dim, pkv_stream stream) {
   return pkv_gated_oproj(attn, gate, w_q4k, PKV_WTYPE_Q4K, out, batch, in_dim, out_dim, stream);
+}
+
+// Whether [a, a + na) and [b, b + nb) share a byte.
+static bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+  const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + nb && y < x + na;
+}
+
+int pkv_causal_conv(const float *x, int64_t stride_b, int64_t stride_t, const float *weight,
+                    const float *bias, float *state, const int *lens, float *out, int batch,
+                    int64_t n, int channels, int taps, int silu, pkv_stream stream) {
+  if (batch <= 0 || n < 0 || channels <= 0)
+    return set_error(PKV_ERR_ARG, "batch and channels must be > 0, n >= 0");
+  if (n == 0) return PKV_OK;
+  if (!x || !weight || !state || !out) return set_error(PKV_ERR_ARG, "null argument");
+  if (stride_t < channels || stride_b < 0 || (batch > 1 && stride_b < channels))
+    return set_error(PKV_ERR_ARG, "x: a token's row holds `channels` values, and rows do not overlap");
+  const uint64_t span = 4 * ((uint64_t)(batch - 1) * stride_b + (uint64_t)(n - 1) * stride_t + channels);
+  const uint64_t out_bytes = 4 * (uint64_t)batch * n * channels;
+  const uint64_t state_bytes = 4 * (uint64_t)batch * channels * (taps > 0 ? taps - 1 : 0);
+  if (overlap(x, span, out, out_bytes) || overlap(x, span, state, state_bytes) || overlap(out, out_bytes, state, state_bytes))
+    return set_error(PKV_ERR_ARG, "x, out and state must not overlap");
+  return launch_causal_conv(x, stride_b, stride_t, weight, bias, state, lens, out, batch, n,
+                            channels, taps, silu, static_cast<hipStream_t>(stream));
+}
+
+size_t pkv_deltanet_prompt_workspace(int batch, int64_t n, int heads, int head_dim) {
+  if (batch <= 0 || n <= 0 || heads <= 0 || head_dim <= 0) return 0;
+  return deltanet_prompt_workspace(batch, n, heads, head_dim);
+}
+
+int pkv_deltanet_prompt(const float *q, const float *k, const float *v, const int64_t strides[6],
+                        const float *gate, const float *beta, float *state, float *gate_offset,
+                        const int *lens, float *out, int batch, int64_t n, int k_heads, int heads,
+                        int head_dim, float scale, float eps, void *workspace,
+                        size_t workspace_bytes, pkv_stream stream) {
+  if (batch <= 0 || n < 0 || k_heads <= 0 || heads <= 0 || head_dim <= 0 || heads % k_heads != 0)
+    return set_error(PKV_ERR_ARG, "batch, heads and head_dim must be > 0, n >= 0, and heads a "
+                                  "multiple of k_heads");
+  if (n == 0) return PKV_OK;
+  if (!q || !k || !v || !strides || !gate || !beta || !state || !out)
+    return set_error(PKV_ERR_ARG, "null argument");
+  const int width[3] = {k_heads, k_heads, heads};
+  const float *in[3] = {q, k, v};
+  const uint64_t out_bytes = 4 * (uint64_t)batch * n * heads * head_dim;
+  const uint64_t state_bytes = 4 * (uint64_t)batch * heads * head_dim * head_dim;
+  if (overlap(out, out_bytes, state, state_bytes))
+    return set_error(PKV_ERR_ARG, "out and state must not overlap");
+  for (int i = 0; i < 3; ++i) {
+    const int64_t sb = strides[2 * i], st = strides[2 * i + 1], w = (int64_t)width[i] * head_dim;
+    if ((n > 1 && st < w) || (batch > 1 && sb < w) || sb < 0 || st < 0)
+      return set_error(PKV_ERR_ARG, "q, k, v: a token's row holds all its heads, and rows do not overlap");
+    const uint64_t span = 4 * ((uint64_t)(batch - 1) * sb + (uint64_t)(n - 1) * st + w);
+    if (overlap(in[i], span, out, out_bytes) || overlap(in[i], span, state, state_bytes))
+      return set_error(PKV_ERR_ARG, "q, k and v must not overlap out or state");
+  }
+  return launch_deltanet_prompt(q, k, v, strides, gate, beta, state, gate_offset, lens, out, batch,
+                                n, k_heads, heads, head_dim, scale, eps, workspace,
+                                workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+int pkv_rms_norm(const float *x, int64_t stride, float *residual, const float *alpha,
+                 const float *gate, float eps, float *out, void *out_q8_0, int64_t rows, int dim,
+                 pkv_stream stream) {
+  if (rows < 0 || dim <= 0 || (rows > 1 && stride < dim))
+    return set_error(PKV_ERR_ARG, "rows must be >= 0, dim > 0, and x's rows must not overlap");
+  if (rows == 0) return PKV_OK;
+  if (!x || !alpha || (!out && !out_q8_0)) return set_error(PKV_ERR_ARG, "null argument");
+  if (reinterpret_cast<uintptr_t>(out_q8_0) % 2 != 0)
+    return set_error(PKV_ERR_ARG, "the Q8_0 rows must be 2-byte aligned");
+  const uint64_t bytes = 4 * (uint64_t)rows * dim, q8 = out_q8_0 ? (uint64_t)rows * row_bytes(PKV_QUANT_Q8_0, dim) : 0;
+  const uint64_t span = 4 * ((uint64_t)(rows - 1) * stride + dim);
+  // a row is read before it is written, so out or residual may be x itself, and out the gate;
+  // anything else that overlaps would be read half written
+  const bool dense = rows == 1 || stride == dim;
+  const void *reads[3] = {x, residual, gate};
+  const uint64_t read_bytes[3] = {span, residual ? bytes : 0, gate ? bytes : 0};
+  if ((out && residual && overlap(out, bytes, residual, bytes)) ||
+      (out && q8 && overlap(out, bytes, out_q8_0, q8)))
+    return set_error(PKV_ERR_ARG, "out, the Q8_0 rows and residual must not overlap");
+  for (int i = 0; i < 3; ++i) {
+    if (!reads[i] || !read_bytes[i]) continue;
+    if (q8 && overlap(reads[i], read_bytes[i], out_q8_0, q8))
+      return set_error(PKV_ERR_ARG, "the Q8_0 rows must not overlap an input");
+    if (out && overlap(reads[i], read_bytes[i], out, bytes) && !(reads[i] == out && (i == 2 || (i == 0 && dense))))
+      return set_error(PKV_ERR_ARG, "out must not overlap an input, unless it is that input");
+    if (residual && i != 1 && overlap(reads[i], read_bytes[i], residual, bytes) && !(i == 0 && x == residual && dense))
+      return set_error(PKV_ERR_ARG, "residual must not overlap an input, unless it is x");
+  }
+  return launch_rms_norm(x, stride, residual, alpha, gate, eps, out, static_cast<uint8_t *>(out_q8_0),
+                         rows, dim, static_cast<hipStream_t>(stream));
+}
+
+static int check_lora(const void *a, const void *b, int type, int adapters, int rank) {
+  if (!a || !b) return set_error(PKV_ERR_ARG, "null argument");
+  if (type != PKV_LORA_F32 && type != PKV_LORA_F16 && type != PKV_LORA_BF16)
+    return set_error(PKV_ERR_UNSUPPORTED, "adapters are F32, F16 or BF16");
+  if (adapters <= 0 || rank <= 0) return set_error(PKV_ERR_ARG, "n_adapters and rank must be > 0");
+  if (rank > PKV_LORA_MAX_RANK) return set_error(PKV_ERR_UNSUPPORTED, "adapters of rank 128 at most");
+  if (reinterpret_cast<uintptr_t>(a) % 16 != 0 || reinterpret_cast<uintptr_t>(b) % 16 != 0)
+    return set_error(PKV_ERR_ARG, "lora_a and lora_b must be 16-byte aligned");
+  return PKV_OK;
+}
+
+size_t pkv_gated_oproj_lora_workspace(int w_type, int batch, int in_dim, int out_dim, int rank) {
+  if (batch <= 0 || in_dim <= 0 || out_dim <= 0 || rank <= 0) return 0;
+  return oproj_lora_workspace(w_type, batch, in_dim, out_dim, rank);
+}
+
+int pkv_gated_oproj_lora(const float *attn, const float *gate, const void *w, int w_type,
+                         const void *lora_a, const void *lora_b, int lora_type, int n_adapters,
+                         int rank, const float *lora_scale, const int *adapter_ids, float *out,
+                         int batch, int in_dim, int out_dim, void *workspace,
+                         size_t workspace_bytes, pkv_stream stream) {
+  if (!attn || !w || !out || !lora_scale || !adapter_ids || !workspace)
+    return set_error(PKV_ERR_ARG, "null argument");
+  if (batch <= 0 || in_dim <= 0 || out_dim <= 0)
+    return set_error(PKV_ERR_ARG, "batch, in_dim and out_dim must be > 0");
+  if (int rc = check_lora(lora_a, lora_b, lora_type, n_adapters, rank)) return rc;
+  return launch_oproj_lora(attn, gate, static_cast<const uint8_t *>(w), w_type, lora_a, lora_b,
+                           lora_type, n_adapters, rank, lora_scale, adapter_ids, out, batch, in_dim,
+                           out_dim, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 int pkv_fill_normal(float *dst, size_t n, uint64_t seed, uint64_t stream_id, float scale,

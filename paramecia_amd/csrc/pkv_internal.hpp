@@ -43,6 +43,7 @@ inline size_t row_bytes(int quant, int head_dim) {
 // that give up a bounded wait set a bit with an atomic OR; pkv_device_status() reads and
 // clears it.
 constexpr unsigned kStatusBarrierTimeout = 1u;  // the fused quantizer's barrier of waves 0-3
+constexpr unsigned kStatusAdapterId = 2u;       // an adapter id past the call's adapters
 int device_status_word(unsigned **out);
 
 // PKV_ERR_UNSUPPORTED when `s` is capturing a HIP graph: for calls that allocate device
@@ -251,6 +252,31 @@ int launch_oproj(const float *attn, const float *gate, const uint8_t *w, int w_t
 int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, int w_type,
                       float *out, int batch, int in_dim, int out_dim, Workspace &ws,
                       hipStream_t s);
+// The form that a batch takes of the two, and its workspace (0: none).
+int oproj_any(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
+              int batch, int in_dim, int out_dim, Workspace &ws, hipStream_t s);
+size_t oproj_workspace(int w_type, int batch, int in_dim, int out_dim);
+// ---- launchers (pkv_lora.hip): the projection with low-rank adapters, in the caller's workspace
+int launch_oproj_lora(const float *attn, const float *gate, const uint8_t *w, int w_type,
+                      const void *lora_a, const void *lora_b, int lora_type, int adapters,
+                      int rank, const float *scale, const int *ids, float *out, int rows,
+                      int in_dim, int out_dim, void *ws, size_t ws_bytes, hipStream_t s);
+size_t oproj_lora_workspace(int w_type, int rows, int in_dim, int out_dim, int rank);
+// ---- launchers (pkv_conv.hip, pkv_deltanet_prompt.hip, pkv_rmsnorm.hip): the rest of a
+// Gated-DeltaNet layer. lens (device, may be null): the valid tokens of each padded row.
+int launch_causal_conv(const float *x, int64_t stride_b, int64_t stride_t, const float *w,
+                       const float *bias, float *state, const int *lens, float *out, int batch,
+                       int64_t n, int channels, int taps, int silu, hipStream_t s);
+// strides: q batch, q token, k batch, k token, v batch, v token (elements)
+int launch_deltanet_prompt(const float *q, const float *k, const float *v, const int64_t *strides,
+                           const float *gate, const float *beta, float *state, float *gate_offset,
+                           const int *lens, float *out, int batch, int64_t n, int k_heads,
+                           int heads, int head_dim, float scale, float eps, void *ws,
+                           size_t ws_bytes, hipStream_t s);
+size_t deltanet_prompt_workspace(int batch, int64_t n, int heads, int head_dim);
+int launch_rms_norm(const float *x, int64_t x_stride, float *residual, const float *alpha,
+                    const float *gate, float eps, float *out, uint8_t *q8, int64_t rows, int dim,
+                    hipStream_t s);
 int launch_deltanet_step(const float *q, const float *k, const float *v, const float *gate,
                          const float *beta, float *state, float *gate_offset, float *out,
                          int batch, int heads, int head_dim, float scale, float eps,

@@ -508,20 +508,14 @@ __global__ __launch_bounds__(256) void oproj_reduce_kernel(const float *part, co
   }
 }
 
+// How a projection of T tokens is cut: its tiles, its split over K and its workspace.
+struct MxPlan {
+  bool wide;
+  int T_pad, rbs, tbs, per, S;
+  size_t off_xl, off_xs, off_inv, off_part, bytes;
+};
 
-}  // namespace
-
-int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, int w_type,
-                      float *out, int batch, int in_dim, int out_dim, Workspace &ws,
-                      hipStream_t s) {
-  if (w_type != kMQ4K && w_type != kMQ5K && w_type != kMQ6K)
-    return set_error(PKV_ERR_UNSUPPORTED, "batched o_proj: weight type must be Q4K, Q5K or Q6K");
-  if (in_dim % 4096 != 0 || in_dim > 8192)
-    return set_error(PKV_ERR_UNSUPPORTED, "batched o_proj: in_dim must be 4096 or 8192");
-  for (const void *p : {(const void *)attn, (const void *)gate, (const void *)w})
-    if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
-      return set_error(PKV_ERR_ARG, "attn, gate and the weights must be 16-byte aligned");
-  const int T = batch, N = out_dim, K = in_dim;
+MxPlan plan_mx(int w_type, int T, int K, int N) {
   // Tile: 32 tokens x 256 rows per workgroup of 4 waves (32 x 64 per wave), or 64 tokens: Q4K
   // and Q5K with 8 waves (two per SIMD, one's decoding beside the other's MFMAs), Q6K, whose
   // two-plane operands would spill at 256 registers a wave, with 4 waves of 64 x 64. A decoded
@@ -535,27 +529,60 @@ int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, in
   // 227; Q5K 4001 322 / 245; Q6K 512 65.8 / 61.7, 4001 444 / 377; -> 300, Q4K 400 tokens 25.1 /
   // 29.3.
   constexpr int kWideWGs = 40;
-  const int rows = 256, rbs = (N + rows - 1) / rows;
-  const auto wgs = [&](int tokens) { return (int64_t)rbs * ((T + tokens - 1) / tokens); };
-  bool wide = wgs(64) >= kWideWGs;
-  if (w_type == kMQ6K && wgs(64) > 256) wide = 17 * ((wgs(64) + 255) / 256) < 10 * ((wgs(32) + 255) / 256);
-  const int tok = wide ? 64 : 32;
-  const int T_pad = (T + tok - 1) / tok * tok;
-  const int KB = K / 32, SB = K / 256;
+  MxPlan p;
+  const int rows = 256;
+  p.rbs = (N + rows - 1) / rows;
+  const auto wgs = [&](int tokens) { return (int64_t)p.rbs * ((T + tokens - 1) / tokens); };
+  p.wide = wgs(64) >= kWideWGs;
+  if (w_type == kMQ6K && wgs(64) > 256) p.wide = 17 * ((wgs(64) + 255) / 256) < 10 * ((wgs(32) + 255) / 256);
+  const int tok = p.wide ? 64 : 32;
+  p.tbs = (T + tok - 1) / tok;
+  p.T_pad = p.tbs * tok;
+  const int SB = K / 256;
+  const int64_t tiles = (int64_t)p.rbs * p.tbs;
+  p.S = tiles > kMxTargetWGs ? 1 : (int)(kMxTargetWGs / tiles);
+  p.S = p.S > SB ? SB : p.S;
+  p.per = (SB + p.S - 1) / p.S;
+  p.S = (SB + p.per - 1) / p.per;  // no empty split
+  const size_t xhl_bytes = (size_t)p.T_pad * K * 2, xs_bytes = (size_t)p.T_pad * SB * 32;
+  const size_t inv_bytes = (size_t)p.T_pad * 4;
+  const size_t part_bytes = p.S > 1 ? (size_t)p.S * T * N * 4 : 0;
+  p.off_xl = xhl_bytes;
+  p.off_xs = 2 * xhl_bytes;
+  p.off_inv = p.off_xs + xs_bytes;
+  p.off_part = (p.off_inv + inv_bytes + 255) / 256 * 256;
+  p.bytes = p.off_part + part_bytes;
+  return p;
+}
+
+// From this many tokens on, the k-quant projection runs as the batched MFMA form (each
+// decoded weight serves 32 or 64 tokens); below it, per-token GEMV workgroups.
+constexpr int kOprojMfmaMinBatch = 8;
+bool batched_form(int w_type, int batch) {
+  return batch >= kOprojMfmaMinBatch && (w_type == kMQ4K || w_type == kMQ5K || w_type == kMQ6K);
+}
+
+}  // namespace
+
+int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, int w_type,
+                      float *out, int batch, int in_dim, int out_dim, Workspace &ws,
+                      hipStream_t s) {
+  if (w_type != kMQ4K && w_type != kMQ5K && w_type != kMQ6K)
+    return set_error(PKV_ERR_UNSUPPORTED, "batched o_proj: weight type must be Q4K, Q5K or Q6K");
+  if (in_dim % 4096 != 0 || in_dim > 8192)
+    return set_error(PKV_ERR_UNSUPPORTED, "batched o_proj: in_dim must be 4096 or 8192");
+  for (const void *p : {(const void *)attn, (const void *)gate, (const void *)w})
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
+      return set_error(PKV_ERR_ARG, "attn, gate and the weights must be 16-byte aligned");
+  const MxPlan p = plan_mx(w_type, batch, in_dim, out_dim);
+  const bool wide = p.wide;
+  const int T = batch, N = out_dim, K = in_dim, T_pad = p.T_pad, S = p.S, rbs = p.rbs, tbs = p.tbs;
+  const int KB = K / 32, SB = K / 256, per = p.per;
   const int64_t row_bytes = (int64_t)SB * (w_type == kMQ4K ? 144 : w_type == kMQ5K ? 176 : 210);
-  const int tbs = T_pad / tok;
   if ((int64_t)rbs * tbs * SB > (1 << 30))
     return set_error(PKV_ERR_ARG, "batch too large for the batched o_proj");
-  int S = kMxTargetWGs / (rbs * tbs);
-  S = S < 1 ? 1 : (S > SB ? SB : S);
-  const int per = (SB + S - 1) / S;
-  S = (SB + per - 1) / per;  // no empty split
-  const size_t xhl_bytes = (size_t)T_pad * K * 2, xs_bytes = (size_t)T_pad * SB * 32;
-  const size_t inv_bytes = (size_t)T_pad * 4;
-  const size_t part_bytes = S > 1 ? (size_t)S * T * N * 4 : 0;
-  const size_t off_xl = xhl_bytes, off_xs = 2 * xhl_bytes, off_inv = off_xs + xs_bytes;
-  const size_t off_part = (off_inv + inv_bytes + 255) / 256 * 256;
-  if (int rc = ws.reserve(off_part + part_bytes)) return rc;
+  const size_t off_xl = p.off_xl, off_xs = p.off_xs, off_inv = p.off_inv, off_part = p.off_part;
+  if (int rc = ws.reserve(p.bytes)) return rc;
   uint8_t *base = static_cast<uint8_t *>(ws.ptr);
   XprepArgs xa{attn, gate, T, K, reinterpret_cast<u4 *>(base), reinterpret_cast<u4 *>(base + off_xl),
                reinterpret_cast<h4 *>(base + off_xs), reinterpret_cast<float *>(base + off_inv)};
@@ -590,6 +617,17 @@ int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, in
     PKV_HIP(hipGetLastError());
   }
   return PKV_OK;
+}
+
+size_t oproj_workspace(int w_type, int batch, int in_dim, int out_dim) {
+  return batched_form(w_type, batch) ? plan_mx(w_type, batch, in_dim, out_dim).bytes : 0;
+}
+
+int oproj_any(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
+              int batch, int in_dim, int out_dim, Workspace &ws, hipStream_t s) {
+  if (batched_form(w_type, batch))
+    return launch_oproj_mfma(attn, gate, w, w_type, out, batch, in_dim, out_dim, ws, s);
+  return launch_oproj(attn, gate, w, w_type, out, batch, in_dim, out_dim, s);
 }
 
 }  // namespace pkv

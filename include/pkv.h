@@ -335,7 +335,7 @@ int pkv_rms_norm(const float *x, int64_t stride, float *residual, const float *a
  * out_dim, rank], both of lora_type (a lower rank is filled up with zeros); lora_scale: f32
  * [n_adapters]; adapter_ids: int32 [batch]; all on the device, lora_a and lora_b 16-byte
  * aligned. An id of n_adapters or more: its row takes no adapter, and pkv_device_status
- * reports it. rank at most PKV_LORA_MAX_RANK (else PKV_ERR_UNSUPPORTED). workspace: at least
+ * reports it. rank at most PKV_LORA_MAX_RANK (else PKV_ERR_UNSUPPORTED), batch at most 65535. workspace: at least
  * pkv_gated_oproj_lora_workspace() bytes of device memory, 256-byte aligned, which the call
  * writes (unlike pkv_gated_oproj it allocates nothing): calls that overlap in time, and
  * graphs that do, need one each. Everything else as pkv_gated_oproj. */

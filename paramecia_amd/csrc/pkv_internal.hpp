@@ -246,16 +246,30 @@ int launch_copy_segments(void *const *dst, const void *const *src, const size_t 
                          Workspace &ws, hipStream_t s);
 // n words of dst set to zero by a kernel (capturable, unlike hipMemsetAsync).
 int launch_zero_words(uint32_t *dst, size_t n, hipStream_t s);
+// The low-rank term of a projection's rows (pkv_lora.hpp): out[row] += B[ids[row]] t[row],
+// t [S][rows][rank] in parts to be added in order.
+struct LoraTerm {
+  const float *t;
+  const void *b;  // [adapters][out][rank]
+  const int *ids;
+  int type, rank, adapters, S;
+  int64_t plane;  // rows * rank
+};
 int launch_oproj(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
-                 int batch, int in_dim, int out_dim, hipStream_t s);
+                 int batch, int in_dim, int out_dim, hipStream_t s,
+                 const LoraTerm *lora = nullptr);
 // ---- launcher (pkv_oproj_mfma.hip): the batched form, Q4K/Q5K/Q6K ----
 int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, int w_type,
                       float *out, int batch, int in_dim, int out_dim, Workspace &ws,
-                      hipStream_t s);
+                      hipStream_t s, const LoraTerm *lora = nullptr);
 // The form that a batch takes of the two, and its workspace (0: none).
 int oproj_any(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
-              int batch, int in_dim, int out_dim, Workspace &ws, hipStream_t s);
+              int batch, int in_dim, int out_dim, Workspace &ws, hipStream_t s,
+              const LoraTerm *lora = nullptr);
 size_t oproj_workspace(int w_type, int batch, int in_dim, int out_dim);
+// The projection's own checks of its arguments, which both forms make before a launch.
+int check_oproj(const float *attn, const float *gate, const uint8_t *w, int w_type, int batch,
+                int in_dim, int out_dim);
 // ---- launchers (pkv_lora.hip): the projection with low-rank adapters, in the caller's workspace
 int launch_oproj_lora(const float *attn, const float *gate, const uint8_t *w, int w_type,
                       const void *lora_a, const void *lora_b, int lora_type, int adapters,

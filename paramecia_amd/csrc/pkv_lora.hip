@@ -2,124 +2,164 @@
 // (forward_with_scales_and_lora, paramecia-model/src/models/with_tracing.rs:253-300, around
 // pkv_gated_oproj): for row m with adapter a = ids[m],
 //   x = attn * sigmoid(gate), out[m] = W x + scale[a] * B_a (A_a x)
-// and out[m] = W x where the row has none. The small product t = scale A x comes first (t in
-// the workspace), then the projection, then its sum with B t.
-#include "pkv_internal.hpp"
-#include "pkv_scalar.hpp"
+// and out[m] = W x where the row has none.
+//
+// The small product t = scale A x comes first, in a launch of its own (here); the
+// projection's kernels add B t where they have a row's outputs in registers
+// (pkv_lora.hpp): the per-token form in its dot product's sum, the batched form in its
+// reduction over the splits or in its epilogue.
+#include "pkv_lora.hpp"
 
 namespace pkv {
 namespace {
 
-struct LoraArgs {
+struct ShrinkArgs {
   const float *attn, *gate;  // [rows][in]; gate may be null
-  const void *a, *b;         // [adapters][rank][in], [adapters][out][rank]
+  const void *a;             // [adapters][rank][in]
   const float *scale;        // [adapters]
   const int *ids;            // [rows]
-  float *t;                  // [rows][rank]
-  float *out;                // [rows][out]
+  float *t;                  // [S][rows][rank]
   unsigned *status;
-  int rows, in_dim, out_dim, rank, adapters;
+  int rows, in_dim, rank, adapters, slice;  // slice: inputs per workgroup
 };
 
-enum : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
-template <int kType>
-__device__ __forceinline__ float weight(const void *p, int64_t i) {
-  if constexpr (kType == kF32) return reinterpret_cast<const float *>(p)[i];
-  else if constexpr (kType == kF16) return f16_to_f32(reinterpret_cast<const uint16_t *>(p)[i]);
-  else return bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i]);
+__device__ __forceinline__ float fast_sigmoid(float g) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g * 1.4426950408889634f));
 }
 
-// the row's adapter, -1 for none; an id past the adapters flags the device status word
-__device__ __forceinline__ int adapter_of(const LoraArgs &a, int row) {
-  const int id = a.ids[row];
+// A workgroup takes 16 rows and a slice of the inputs, a quarter of it per wave, with
+// v_mfma_f32_16x16x4_f32 (f32 products: 16 rows by 16 ranks, 4 inputs): lane (m, g) holds
+// inputs 8 g .. 8 g + 7 of a 32-input step for row m of x and for rank m of A, and the eight
+// MFMAs of a step take one of each. The rows' adapters are taken one after the other, each
+// for all 16 rows; a row keeps its own one's result. kC tiles of 16 ranks.
+template <int kType, int kC>
+__global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs a) {
+  typedef float v4 __attribute__((ext_vector_type(4)));
+  __shared__ v4 red[4][kC][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int m = lane & 15, g = lane >> 4;
+  const int row0 = blockIdx.x * 16;
+  const int row = row0 + m < a.rows ? row0 + m : a.rows - 1;
+  int id = a.ids[row];
   if (id >= a.adapters) {
-    if (threadIdx.x == 0)
+    if (blockIdx.y == 0 && tid < 16)
       __hip_atomic_fetch_or(a.status, kStatusAdapterId, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return -1;
+    id = -1;
   }
-  return id < 0 ? -1 : id;
-}
-
-// t[row][r]: a wave per rank of a row, lanes along the inputs.
-template <int kType>
-__global__ __launch_bounds__(256) void lora_shrink_kernel(LoraArgs a) {
-  const int row = blockIdx.x, id = adapter_of(a, row);
-  if (id < 0) return;
-  const int lane = threadIdx.x & 63, r = blockIdx.y * 4 + (threadIdx.x >> 6);
-  if (r >= a.rank) return;
-  const int64_t w0 = ((int64_t)id * a.rank + r) * a.in_dim, x0 = (int64_t)row * a.in_dim;
-  float s = 0.0f;
-  for (int i = lane; i < a.in_dim; i += 64) {
-    float x = a.attn[x0 + i];
-    if (a.gate != nullptr) x = x / (1.0f + expf(-a.gate[x0 + i]));
-    s = fmaf(weight<kType>(a.a, w0 + i), x, s);
-  }
+  if (row0 + m >= a.rows) id = -1;
+  unsigned todo = (unsigned)(__ballot(id >= 0) & 0xFFFFu);
+  const int k0 = blockIdx.y * a.slice + wave * (a.slice >> 2) + 8 * g, steps = a.slice >> 7;
+  const float4 *x4 = reinterpret_cast<const float4 *>(a.attn + (int64_t)row * a.in_dim + k0);
+  const float4 *g4 = a.gate == nullptr ? nullptr : reinterpret_cast<const float4 *>(a.gate + (int64_t)row * a.in_dim + k0);
+  while (todo != 0) {
+    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
+    const unsigned mine = (unsigned)(__ballot(id == cur) & 0xFFFFu);
+    todo &= ~mine;
+    v4 acc[kC];
+    int64_t w0[kC];
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-  if (lane == 0) a.t[(int64_t)row * a.rank + r] = s * a.scale[id];
+    for (int c = 0; c < kC; ++c) {
+      acc[c] = v4{0.f, 0.f, 0.f, 0.f};
+      const int r = 16 * c + m < a.rank ? 16 * c + m : a.rank - 1;
+      w0[c] = ((int64_t)cur * a.rank + r) * a.in_dim + k0;
+    }
+    for (int s = 0; s < steps; ++s) {
+      float x[8], w[kC][8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 f = x4[8 * s + h];
+        x[4 * h] = f.x; x[4 * h + 1] = f.y; x[4 * h + 2] = f.z; x[4 * h + 3] = f.w;
+      }
+#pragma unroll
+      for (int c = 0; c < kC; ++c) lora_weights<kType, 8>(a.a, w0[c] + 32 * s, w[c]);
+      if (g4 != nullptr) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 f = g4[8 * s + h];
+          x[4 * h] *= fast_sigmoid(f.x);
+          x[4 * h + 1] *= fast_sigmoid(f.y);
+          x[4 * h + 2] *= fast_sigmoid(f.z);
+          x[4 * h + 3] *= fast_sigmoid(f.w);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+          acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], w[c][i], acc[c], 0, 0, 0);
+    }
+#pragma unroll
+    for (int c = 0; c < kC; ++c) red[wave][c][lane] = acc[c];
+    __syncthreads();
+    const float scale = a.scale[cur];
+    for (int u = tid; u < 64 * kC; u += 256) {
+      const int c = u >> 6, l = u & 63, r = 16 * c + (l & 15);
+      const v4 s = (red[0][c][l] + red[1][c][l]) + (red[2][c][l] + red[3][c][l]);
+      if (r < a.rank) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = 4 * (l >> 4) + i;  // the row within the tile
+          if ((mine >> n) & 1) a.t[((int64_t)blockIdx.y * a.rows + row0 + n) * a.rank + r] = s[i] * scale;
+        }
+      }
+    }
+    __syncthreads();  // the next adapter writes red again
+  }
 }
 
-// out[row][o] += B[o] . t[row]: a lane per output.
 template <int kType>
-__global__ __launch_bounds__(256) void lora_expand_kernel(LoraArgs a) {
-  const int row = blockIdx.x, id = adapter_of(a, row);
-  if (id < 0) return;
-  const int o = blockIdx.y * 256 + threadIdx.x;
-  if (o >= a.out_dim) return;
-  const int64_t w0 = ((int64_t)id * a.out_dim + o) * a.rank;
-  const float *t = a.t + (int64_t)row * a.rank;
-  float s = 0.0f;
-  for (int r = 0; r < a.rank; ++r) s = fmaf(weight<kType>(a.b, w0 + r), t[r], s);
-  a.out[(int64_t)row * a.out_dim + o] += s;
-}
-
-template <int kType>
-int launch_shrink(const LoraArgs &a, hipStream_t s) {
-  const dim3 grid((unsigned)a.rows, (unsigned)((a.rank + 3) / 4));
-  hipLaunchKernelGGL(lora_shrink_kernel<kType>, grid, dim3(256), 0, s, a);
+int launch_shrink(const ShrinkArgs &a, int S, hipStream_t s) {
+  const dim3 grid((unsigned)((a.rows + 15) / 16), (unsigned)S), t(256);
+  if (a.rank <= 16) hipLaunchKernelGGL((lora_shrink_kernel<kType, 1>), grid, t, 0, s, a);
+  else if (a.rank <= 32) hipLaunchKernelGGL((lora_shrink_kernel<kType, 2>), grid, t, 0, s, a);
+  else if (a.rank <= 64) hipLaunchKernelGGL((lora_shrink_kernel<kType, 4>), grid, t, 0, s, a);
+  else hipLaunchKernelGGL((lora_shrink_kernel<kType, 8>), grid, t, 0, s, a);
   PKV_HIP(hipGetLastError());
   return PKV_OK;
 }
-template <int kType>
-int launch_expand(const LoraArgs &a, hipStream_t s) {
-  const dim3 grid((unsigned)a.rows, (unsigned)((a.out_dim + 255) / 256));
-  hipLaunchKernelGGL(lora_expand_kernel<kType>, grid, dim3(256), 0, s, a);
-  PKV_HIP(hipGetLastError());
-  return PKV_OK;
-}
 
-size_t t_bytes(int rows, int rank) { return ((size_t)rows * rank * 4 + 255) / 256 * 256; }
+// The split of the inputs: workgroups for the 256 CUs twice over, at most one per 256 inputs.
+int shrink_splits(int rows, int in_dim) {
+  const int tiles = (rows + 15) / 16;
+  int S = 1;
+  while (S * 2 * tiles <= 512 && in_dim / (S * 2) >= 256) S *= 2;
+  return S;
+}
+size_t t_bytes(int rows, int in_dim, int rank) {
+  return ((size_t)shrink_splits(rows, in_dim) * rows * rank * 4 + 255) / 256 * 256;
+}
 
 }  // namespace
 
 size_t oproj_lora_workspace(int w_type, int rows, int in_dim, int out_dim, int rank) {
-  return t_bytes(rows, rank) + oproj_workspace(w_type, rows, in_dim, out_dim);
+  return t_bytes(rows, in_dim, rank) + oproj_workspace(w_type, rows, in_dim, out_dim);
 }
 
 int launch_oproj_lora(const float *attn, const float *gate, const uint8_t *w, int w_type,
                       const void *lora_a, const void *lora_b, int lora_type, int adapters,
                       int rank, const float *scale, const int *ids, float *out, int rows,
                       int in_dim, int out_dim, void *ws, size_t ws_bytes, hipStream_t s) {
+  if (int rc = check_oproj(attn, gate, w, w_type, rows, in_dim, out_dim)) return rc;
+  if (rows > 65535) return set_error(PKV_ERR_ARG, "batch must be <= 65535");
   if (ws_bytes < oproj_lora_workspace(w_type, rows, in_dim, out_dim, rank))
     return set_error(PKV_ERR_ARG, "the workspace is smaller than pkv_gated_oproj_lora_workspace says");
   if (reinterpret_cast<uintptr_t>(ws) % 256 != 0)
     return set_error(PKV_ERR_ARG, "the workspace must be 256-byte aligned");
-  LoraArgs a{attn, gate, lora_a, lora_b, scale, ids, static_cast<float *>(ws), out, nullptr,
-             rows, in_dim, out_dim, rank, adapters};
+  const int S = shrink_splits(rows, in_dim);
+  const size_t own = t_bytes(rows, in_dim, rank);
+  ShrinkArgs a{attn, gate, lora_a, scale, ids, static_cast<float *>(ws), nullptr,
+               rows, in_dim, rank, adapters, in_dim / S};
   if (int rc = device_status_word(&a.status)) return rc;
-  Workspace base;
-  base.ptr = static_cast<uint8_t *>(ws) + t_bytes(rows, rank);
-  base.bytes = ws_bytes - t_bytes(rows, rank);
-  base.fixed = true;
-  // the projection checks its own shapes and alignment before anything is enqueued
-  if (int rc = oproj_any(attn, gate, w, w_type, out, rows, in_dim, out_dim, base, s)) return rc;
-  int rc = lora_type == PKV_LORA_F32   ? launch_shrink<kF32>(a, s)
-           : lora_type == PKV_LORA_F16 ? launch_shrink<kF16>(a, s)
-                                       : launch_shrink<kBF16>(a, s);
+  const int rc = lora_type == PKV_LORA_F32   ? launch_shrink<PKV_LORA_F32>(a, S, s)
+                 : lora_type == PKV_LORA_F16 ? launch_shrink<PKV_LORA_F16>(a, S, s)
+                                             : launch_shrink<PKV_LORA_BF16>(a, S, s);
   if (rc) return rc;
-  return lora_type == PKV_LORA_F32   ? launch_expand<kF32>(a, s)
-         : lora_type == PKV_LORA_F16 ? launch_expand<kF16>(a, s)
-                                     : launch_expand<kBF16>(a, s);
+  const LoraTerm term{a.t, lora_b, ids, lora_type, rank, adapters, S, (int64_t)rows * rank};
+  Workspace base;
+  base.ptr = static_cast<uint8_t *>(ws) + own;
+  base.bytes = ws_bytes - own;
+  base.fixed = true;
+  return oproj_any(attn, gate, w, w_type, out, rows, in_dim, out_dim, base, s, &term);
 }
 
 }  // namespace pkv

@@ -26,6 +26,7 @@
 #include <type_traits>
 
 #include "pkv_internal.hpp"
+#include "pkv_lora.hpp"
 #include "pkv_scalar.hpp"
 
 namespace pkv {
@@ -45,6 +46,12 @@ struct OprojArgs {
   const uint8_t *w;          // [out_dim][row bytes]
   float *out;                // [batch][out_dim]
   int batch, in_dim, out_dim;
+};
+
+// With the rows' low-rank term: each lane adds its ranks' products to its part of the dot
+// product, which the wave sums anyway. Their loads go out in front of the weight stream.
+struct OprojLoraArgs : OprojArgs {
+  LoraTerm lora;
 };
 
 __host__ __device__ constexpr int block_elems(int fmt) { return fmt == kWQ8_0 ? 32 : 256; }
@@ -106,8 +113,9 @@ __device__ __forceinline__ void bytes_to_f32(uint32_t w, float *f) {
 
 // Q4K / Q5K. kChunks 64-element chunks per lane (in_dim / 4096), kOprojRowsPerWave output
 // rows per wave.
-template <int kFmt, int kChunks, int kOprojRowsPerWave>
-__global__ __launch_bounds__(256) void oproj_k45_kernel(OprojArgs a) {
+template <int kFmt, int kChunks, int kOprojRowsPerWave, typename Args>
+__global__ __launch_bounds__(256) void oproj_k45_kernel(Args a) {
+  constexpr bool kLora = std::is_same<Args, OprojLoraArgs>::value;
   static_assert(kFmt == kWQ4K || kFmt == kWQ5K, "Q4K or Q5K");
   constexpr int kBB = block_bytes(kFmt);
   constexpr int kNibOff = kFmt == kWQ5K ? 48 : 16;  // the nibbles follow the fifth bits
@@ -116,6 +124,12 @@ __global__ __launch_bounds__(256) void oproj_k45_kernel(OprojArgs a) {
   const int nsb = a.in_dim >> 8;
   const int row0 = (blockIdx.x * kOprojWaves + wave) * kOprojRowsPerWave;
   const int b = blockIdx.y;
+  float low[kOprojRowsPerWave];
+#pragma unroll
+  for (int r = 0; r < kOprojRowsPerWave; ++r) {
+    low[r] = 0.0f;
+    if constexpr (kLora) low[r] = lora_lane(a.lora, b, min(row0 + r, a.out_dim - 1), a.out_dim, lane);
+  }
   // the inputs are read before the weights: their loads (L2 hits after the first
   // workgroups) then need not wait behind the weight stream
   constexpr int kIn4 = kChunks * 4;  // float4 of the input row per thread (in_dim / 1024)
@@ -223,7 +237,7 @@ __global__ __launch_bounds__(256) void oproj_k45_kernel(OprojArgs a) {
     }
 #pragma unroll
     for (int r = 0; r < kOprojRowsPerWave; ++r) {
-      const float y = wave64_sum(acc[r]);
+      const float y = wave64_sum(kLora ? acc[r] + low[r] : acc[r]);
       if (lane == 0 && row0 + r < a.out_dim) a.out[(int64_t)b * a.out_dim + row0 + r] = y;
     }
   }
@@ -257,8 +271,9 @@ constexpr int xs_floats(int in) {
   return kFmt == kWQ6K ? in + 4 * (in / 256 + 2 * (in / 128)) : in + 4 * (in / 32);
 }
 
-template <int kFmt, int kChunks, int kOprojRowsPerWave>
-__global__ __launch_bounds__(256) void oproj_staged_kernel(OprojArgs a) {
+template <int kFmt, int kChunks, int kOprojRowsPerWave, typename Args>
+__global__ __launch_bounds__(256) void oproj_staged_kernel(Args a) {
+  constexpr bool kLora = std::is_same<Args, OprojLoraArgs>::value;
   static_assert(kFmt == kWQ6K || kFmt == kWQ8_0, "Q6K or Q8_0");
   constexpr int kIn = 4096 * kChunks;
   constexpr int kRowBytes = kIn / block_elems(kFmt) * block_bytes(kFmt);
@@ -270,6 +285,13 @@ __global__ __launch_bounds__(256) void oproj_staged_kernel(OprojArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int rg0 = blockIdx.x * kRows;  // the workgroup's first row
   const int b = blockIdx.y;
+  float low[kOprojRowsPerWave];
+#pragma unroll
+  for (int r = 0; r < kOprojRowsPerWave; ++r) {
+    low[r] = 0.0f;
+    if constexpr (kLora)
+      low[r] = lora_lane(a.lora, b, min(rg0 + wave * kOprojRowsPerWave + r, a.out_dim - 1), a.out_dim, lane);
+  }
   // the gated input and the rows' bytes: every load goes out before any is used
   constexpr int kIn4 = kIn / 1024;
   float4 x0[kIn4], g0[kIn4];
@@ -415,7 +437,7 @@ __global__ __launch_bounds__(256) void oproj_staged_kernel(OprojArgs a) {
   }
 #pragma unroll
   for (int r = 0; r < kOprojRowsPerWave; ++r) {
-    const float y = wave64_sum(acc[r]);
+    const float y = wave64_sum(kLora ? acc[r] + low[r] : acc[r]);
     const int row = rg0 + wave * kOprojRowsPerWave + r;
     if (lane == 0 && row < a.out_dim) a.out[(int64_t)b * a.out_dim + row] = y;
   }
@@ -423,8 +445,8 @@ __global__ __launch_bounds__(256) void oproj_staged_kernel(OprojArgs a) {
 
 }  // namespace
 
-int launch_oproj(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
-                 int batch, int in_dim, int out_dim, hipStream_t s) {
+int check_oproj(const float *attn, const float *gate, const uint8_t *w, int w_type, int batch,
+                int in_dim, int out_dim) {
   if (w_type != kWQ4K && w_type != kWQ5K && w_type != kWQ6K && w_type != kWQ8_0)
     return set_error(PKV_ERR_UNSUPPORTED, "gated o_proj: weight type must be Q8_0 (8), Q4K (12), "
                                           "Q5K (13) or Q6K (14)");
@@ -433,25 +455,39 @@ int launch_oproj(const float *attn, const float *gate, const uint8_t *w, int w_t
   for (const void *p : {(const void *)attn, (const void *)gate, (const void *)w})
     if (reinterpret_cast<uintptr_t>(p) % 16 != 0)
       return set_error(PKV_ERR_ARG, "attn, gate and the weights must be 16-byte aligned");
+  return PKV_OK;
+}
+
+int launch_oproj(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
+                 int batch, int in_dim, int out_dim, hipStream_t s, const LoraTerm *lora) {
+  if (int rc = check_oproj(attn, gate, w, w_type, batch, in_dim, out_dim)) return rc;
   if (batch > 65535) return set_error(PKV_ERR_ARG, "batch must be <= 65535");
   OprojArgs a{attn, gate, w, out, batch, in_dim, out_dim};
   const int rows_per_wave = batch < 4 ? 1 : 2;
   const int rows_per_wg = kOprojWaves * rows_per_wave;
   const dim3 grid((unsigned)((out_dim + rows_per_wg - 1) / rows_per_wg), (unsigned)batch);
   const int shape = (in_dim / 4096) * 4 + rows_per_wave;  // 5, 6, 9, 10
-#define PKV_OPROJ_CASES(KERNEL, FMT)                                                    \
-  switch (shape) {                                                                    \
-    case 5: hipLaunchKernelGGL((KERNEL<FMT, 1, 1>), grid, dim3(256), 0, s, a); break; \
-    case 6: hipLaunchKernelGGL((KERNEL<FMT, 1, 2>), grid, dim3(256), 0, s, a); break; \
-    case 9: hipLaunchKernelGGL((KERNEL<FMT, 2, 1>), grid, dim3(256), 0, s, a); break; \
-    default: hipLaunchKernelGGL((KERNEL<FMT, 2, 2>), grid, dim3(256), 0, s, a); break; \
+#define PKV_OPROJ_CASES(KERNEL, FMT, ARGS, args)                                          \
+  switch (shape) {                                                                        \
+    case 5: hipLaunchKernelGGL((KERNEL<FMT, 1, 1, ARGS>), grid, dim3(256), 0, s, args); break; \
+    case 6: hipLaunchKernelGGL((KERNEL<FMT, 1, 2, ARGS>), grid, dim3(256), 0, s, args); break; \
+    case 9: hipLaunchKernelGGL((KERNEL<FMT, 2, 1, ARGS>), grid, dim3(256), 0, s, args); break; \
+    default: hipLaunchKernelGGL((KERNEL<FMT, 2, 2, ARGS>), grid, dim3(256), 0, s, args); break; \
   }
-  switch (w_type) {
-    case kWQ4K: PKV_OPROJ_CASES(oproj_k45_kernel, kWQ4K); break;
-    case kWQ5K: PKV_OPROJ_CASES(oproj_k45_kernel, kWQ5K); break;
-    case kWQ6K: PKV_OPROJ_CASES(oproj_staged_kernel, kWQ6K); break;
-    default: PKV_OPROJ_CASES(oproj_staged_kernel, kWQ8_0); break;
+#define PKV_OPROJ_TYPES(ARGS, args)                                                       \
+  switch (w_type) {                                                                       \
+    case kWQ4K: PKV_OPROJ_CASES(oproj_k45_kernel, kWQ4K, ARGS, args); break;              \
+    case kWQ5K: PKV_OPROJ_CASES(oproj_k45_kernel, kWQ5K, ARGS, args); break;              \
+    case kWQ6K: PKV_OPROJ_CASES(oproj_staged_kernel, kWQ6K, ARGS, args); break;           \
+    default: PKV_OPROJ_CASES(oproj_staged_kernel, kWQ8_0, ARGS, args); break;             \
   }
+  if (lora == nullptr) {
+    PKV_OPROJ_TYPES(OprojArgs, a);
+  } else {
+    const OprojLoraArgs la{a, *lora};
+    PKV_OPROJ_TYPES(OprojLoraArgs, la);
+  }
+#undef PKV_OPROJ_TYPES
 #undef PKV_OPROJ_CASES
   PKV_HIP(hipGetLastError());
   return PKV_OK;

@@ -30,6 +30,9 @@
 // LDS between two barriers: the only waits for memory sit right before those stores, and
 // each wave decodes its rows' B fragments from LDS. Tiles are placed on XCDs in compact
 // groups (tile_of) so that an XCD's L2 serves both operands to several workgroups.
+#include <type_traits>
+
+#include "pkv_lora.hpp"
 #include "pkv_mfma_common.hpp"
 
 namespace pkv {
@@ -225,6 +228,10 @@ struct MxArgs {
   int rbs, tbs;  // row blocks, token blocks
 };
 
+struct MxLoraArgs : MxArgs {
+  LoraTerm lora;
+};
+
 // Tile (split, row block, token block) of workgroup `id`. Workgroups are dealt to the 8
 // XCDs in turn (id % 8), and each XCD has its own L2: when the grid divides by 8, XCD x
 // takes tiles x C .. x C + C - 1 (C = grid / 8) of an order in which consecutive tiles
@@ -247,8 +254,9 @@ __device__ __forceinline__ void tile_of(const MxArgs &a, int id, int G, int &spl
 // tiles kTT (w / 4) .. + kTT - 1, so the workgroup (256 kWT threads) owns 64 kRT rows and
 // 16 kTT kWT tokens. With kWT = 2 each SIMD runs two waves, one's VALU work beside the
 // other's MFMAs.
-template <int kFmt, int kWT, int kTT, int kRT>
-__global__ __launch_bounds__(256 * kWT) void oproj_mfma_kernel(MxArgs a) {
+// With MxLoraArgs (only without a split over K) the epilogue adds the tokens' low-rank term.
+template <int kFmt, int kWT, int kTT, int kRT, typename Args>
+__global__ __launch_bounds__(256 * kWT) void oproj_mfma_kernel(Args a) {
   constexpr bool kQ6 = kFmt == kMQ6K;
   using F = WFmt<kFmt>;
   constexpr int kThreads = 256 * kWT;
@@ -464,7 +472,10 @@ __global__ __launch_bounds__(256 * kWT) void oproj_mfma_kernel(MxArgs a) {
   // D layout: lane holds rows (tokens) 4 g + i of the tile, column (weight row) lane & 15
   float *dst = a.S == 1 ? a.out : a.part + (int64_t)split * a.T * a.N;
 #pragma unroll
-  for (int tt = 0; tt < kTT; ++tt)
+  for (int tt = 0; tt < kTT; ++tt) {
+    float low[kRT][4];
+    if constexpr (std::is_same<Args, MxLoraArgs>::value)
+      lora_tile(a.lora, a.T, a.N, tbk * kTok + 16 * (tt0 + tt), row0 + wr * 16 * kRT, lane, low);
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt) {
       const int n = row0 + wr * 16 * kRT + rt * 16 + r16;
@@ -473,9 +484,13 @@ __global__ __launch_bounds__(256 * kWT) void oproj_mfma_kernel(MxArgs a) {
       for (int i = 0; i < 4; ++i) {
         const int t = tbk * kTok + 16 * (tt0 + tt) + 4 * g + i;
         if (t >= a.T) continue;
-        dst[(int64_t)t * a.N + n] = a.S == 1 ? a.inv[t] * fin[tt][rt][i] : fin[tt][rt][i];
+        if constexpr (std::is_same<Args, MxLoraArgs>::value)
+          dst[(int64_t)t * a.N + n] = fmaf(a.inv[t], fin[tt][rt][i], low[rt][i]);
+        else
+          dst[(int64_t)t * a.N + n] = a.S == 1 ? a.inv[t] * fin[tt][rt][i] : fin[tt][rt][i];
       }
     }
+  }
 }
 
 // out[t][n] = 2^-e_t * sum over splits in order: grid y over tokens, x over the row in
@@ -505,6 +520,42 @@ __global__ __launch_bounds__(256) void oproj_reduce_kernel(const float *part, co
         out[r0 + c] = f * s;
       }
     }
+  }
+}
+
+// The same with the rows' low-rank term: a lane per output, t of the row in LDS.
+template <int kType, bool kVec>
+__global__ __launch_bounds__(256) void oproj_reduce_lora_kernel(const float *part, const float *inv,
+                                                                float *out, int T, int N, int S,
+                                                                LoraTerm lora) {
+  __shared__ float ts[PKV_LORA_MAX_RANK];
+  const int64_t plane = (int64_t)T * N;
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  for (int t = blockIdx.y; t < T; t += gridDim.y) {
+    const int id = lora_adapter(lora, t);
+    __syncthreads();
+    if (id >= 0)
+      for (int r = threadIdx.x; r < lora.rank; r += 256) ts[r] = lora_t(lora, t, r);
+    __syncthreads();
+    if (c >= N) continue;
+    const int64_t at = (int64_t)t * N + c;
+    float s = part[at];
+    for (int k = 1; k < S; ++k) s += part[k * plane + at];
+    float low = 0.0f;
+    if (id >= 0) {
+      const int64_t w0 = ((int64_t)id * N + c) * lora.rank;
+      if constexpr (kVec) {
+        for (int r = 0; r < lora.rank; r += 4) {
+          float w[4];
+          lora_weights<kType, 4>(lora.b, w0 + r, w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) low = fmaf(w[i], ts[r + i], low);
+        }
+      } else {
+        for (int r = 0; r < lora.rank; ++r) low = fmaf(lora_weight(lora.b, kType, w0 + r), ts[r], low);
+      }
+    }
+    out[at] = fmaf(inv[t], s, low);
   }
 }
 
@@ -566,7 +617,7 @@ bool batched_form(int w_type, int batch) {
 
 int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, int w_type,
                       float *out, int batch, int in_dim, int out_dim, Workspace &ws,
-                      hipStream_t s) {
+                      hipStream_t s, const LoraTerm *lora) {
   if (w_type != kMQ4K && w_type != kMQ5K && w_type != kMQ6K)
     return set_error(PKV_ERR_UNSUPPORTED, "batched o_proj: weight type must be Q4K, Q5K or Q6K");
   if (in_dim % 4096 != 0 || in_dim > 8192)
@@ -596,19 +647,48 @@ int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, in
             reinterpret_cast<const float *>(base + off_inv), w, row_bytes,
             reinterpret_cast<float *>(base + off_part), out, T, N, KB, SB, per, S, rbs, tbs};
   const dim3 grid((unsigned)(rbs * tbs * S));
-#define PKV_MX(FMT, WT, TT)                                                                  \
-  if (wide)                                                                                  \
-    hipLaunchKernelGGL((oproj_mfma_kernel<FMT, WT, TT, 4>), grid, dim3(256 * WT), 0, s, ma); \
-  else                                                                                       \
-    hipLaunchKernelGGL((oproj_mfma_kernel<FMT, 1, 2, 4>), grid, dim3(256), 0, s, ma)
-  switch (w_type) {
-    case kMQ4K: PKV_MX(kMQ4K, 2, 2); break;
-    case kMQ5K: PKV_MX(kMQ5K, 2, 2); break;
-    default: PKV_MX(kMQ6K, 1, 4); break;
+#define PKV_MX(FMT, WT, TT, ARGS, args)                                                          \
+  if (wide)                                                                                      \
+    hipLaunchKernelGGL((oproj_mfma_kernel<FMT, WT, TT, 4, ARGS>), grid, dim3(256 * WT), 0, s, args); \
+  else                                                                                           \
+    hipLaunchKernelGGL((oproj_mfma_kernel<FMT, 1, 2, 4, ARGS>), grid, dim3(256), 0, s, args)
+#define PKV_MX_TYPES(ARGS, args)                           \
+  switch (w_type) {                                        \
+    case kMQ4K: PKV_MX(kMQ4K, 2, 2, ARGS, args); break;    \
+    case kMQ5K: PKV_MX(kMQ5K, 2, 2, ARGS, args); break;    \
+    default: PKV_MX(kMQ6K, 1, 4, ARGS, args); break;       \
   }
+  if (lora != nullptr && S == 1) {
+    MxLoraArgs la;
+    static_cast<MxArgs &>(la) = ma;
+    la.lora = *lora;
+    PKV_MX_TYPES(MxLoraArgs, la);
+  } else {
+    PKV_MX_TYPES(MxArgs, ma);
+  }
+#undef PKV_MX_TYPES
 #undef PKV_MX
   PKV_HIP(hipGetLastError());
-  if (S > 1) {
+  if (S > 1 && lora != nullptr) {
+    const dim3 rgrid((unsigned)((N + 255) / 256), (unsigned)(T < 65535 ? T : 65535));
+    const float *part = reinterpret_cast<const float *>(base + off_part);
+    const float *inv = reinterpret_cast<const float *>(base + off_inv);
+    const bool vec = lora->rank % 4 == 0;
+#define PKV_REDUCE(TYPE)                                                                          \
+  if (vec)                                                                                        \
+    hipLaunchKernelGGL((oproj_reduce_lora_kernel<TYPE, true>), rgrid, dim3(256), 0, s, part, inv, \
+                       out, T, N, S, *lora);                                                      \
+  else                                                                                            \
+    hipLaunchKernelGGL((oproj_reduce_lora_kernel<TYPE, false>), rgrid, dim3(256), 0, s, part, inv, \
+                       out, T, N, S, *lora)
+    switch (lora->type) {
+      case PKV_LORA_F32: PKV_REDUCE(PKV_LORA_F32); break;
+      case PKV_LORA_F16: PKV_REDUCE(PKV_LORA_F16); break;
+      default: PKV_REDUCE(PKV_LORA_BF16); break;
+    }
+#undef PKV_REDUCE
+    PKV_HIP(hipGetLastError());
+  } else if (S > 1) {
     const int per_row = N % 4 == 0 ? N / 4 : N;
     const dim3 rgrid((unsigned)((per_row + 255) / 256), (unsigned)(T < 65535 ? T : 65535));
     hipLaunchKernelGGL(oproj_reduce_kernel, rgrid, dim3(256), 0, s,
@@ -624,10 +704,11 @@ size_t oproj_workspace(int w_type, int batch, int in_dim, int out_dim) {
 }
 
 int oproj_any(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
-              int batch, int in_dim, int out_dim, Workspace &ws, hipStream_t s) {
+              int batch, int in_dim, int out_dim, Workspace &ws, hipStream_t s,
+              const LoraTerm *lora) {
   if (batched_form(w_type, batch))
-    return launch_oproj_mfma(attn, gate, w, w_type, out, batch, in_dim, out_dim, ws, s);
-  return launch_oproj(attn, gate, w, w_type, out, batch, in_dim, out_dim, s);
+    return launch_oproj_mfma(attn, gate, w, w_type, out, batch, in_dim, out_dim, ws, s, lora);
+  return launch_oproj(attn, gate, w, w_type, out, batch, in_dim, out_dim, s, lora);
 }
 
 }  // namespace pkv

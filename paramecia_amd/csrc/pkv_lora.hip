@@ -8,6 +8,8 @@
 // projection's kernels add B t where they have a row's outputs in registers
 // (pkv_lora.hpp): the per-token form in its dot product's sum, the batched form in its
 // reduction over the splits or in its epilogue.
+#include <algorithm>
+
 #include "pkv_lora.hpp"
 
 namespace pkv {
@@ -30,8 +32,9 @@ __device__ __forceinline__ float fast_sigmoid(float g) {
 // A workgroup takes 16 rows and a slice of the inputs, a quarter of it per wave, with
 // v_mfma_f32_16x16x4_f32 (f32 products: 16 rows by 16 ranks, 4 inputs): lane (m, g) holds
 // inputs 8 g .. 8 g + 7 of a 32-input step for row m of x and for rank m of A, and the eight
-// MFMAs of a step take one of each. The rows' adapters are taken one after the other, each
-// for all 16 rows; a row keeps its own one's result. kC tiles of 16 ranks.
+// MFMAs of a step take one of each. The rows' adapters are taken one after the other (in turn
+// by gridDim.z workgroups), each for all 16 rows; a row keeps its own one's result. kC
+// tiles of 16 ranks.
 template <int kType, int kC>
 __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs a) {
   typedef float v4 __attribute__((ext_vector_type(4)));
@@ -42,7 +45,7 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs a) {
   const int row = row0 + m < a.rows ? row0 + m : a.rows - 1;
   int id = a.ids[row];
   if (id >= a.adapters) {
-    if (blockIdx.y == 0 && tid < 16)
+    if (blockIdx.y == 0 && blockIdx.z == 0 && tid < 16)
       __hip_atomic_fetch_or(a.status, kStatusAdapterId, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     id = -1;
   }
@@ -51,10 +54,11 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs a) {
   const int k0 = blockIdx.y * a.slice + wave * (a.slice >> 2) + 8 * g, steps = a.slice >> 7;
   const float4 *x4 = reinterpret_cast<const float4 *>(a.attn + (int64_t)row * a.in_dim + k0);
   const float4 *g4 = a.gate == nullptr ? nullptr : reinterpret_cast<const float4 *>(a.gate + (int64_t)row * a.in_dim + k0);
-  while (todo != 0) {
+  for (int pass = 0; todo != 0; ++pass) {
     const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
     const unsigned mine = (unsigned)(__ballot(id == cur) & 0xFFFFu);
     todo &= ~mine;
+    if (pass % gridDim.z != blockIdx.z) continue;
     v4 acc[kC];
     int64_t w0[kC];
 #pragma unroll
@@ -63,25 +67,37 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs a) {
       const int r = 16 * c + m < a.rank ? 16 * c + m : a.rank - 1;
       w0[c] = ((int64_t)cur * a.rank + r) * a.in_dim + k0;
     }
+    // the next step's inputs and weights are loaded while this one's products run
+    float4 xn[2], gn[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    float wn[kC][8];
+    auto fetch = [&](int s) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        xn[h] = x4[8 * s + h];
+        if (g4 != nullptr) gn[h] = g4[8 * s + h];
+      }
+#pragma unroll
+      for (int c = 0; c < kC; ++c) lora_weights<kType, 8>(a.a, w0[c] + 32 * s, wn[c]);
+    };
+    fetch(0);
     for (int s = 0; s < steps; ++s) {
       float x[8], w[kC][8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float4 f = x4[8 * s + h];
-        x[4 * h] = f.x; x[4 * h + 1] = f.y; x[4 * h + 2] = f.z; x[4 * h + 3] = f.w;
-      }
-#pragma unroll
-      for (int c = 0; c < kC; ++c) lora_weights<kType, 8>(a.a, w0[c] + 32 * s, w[c]);
-      if (g4 != nullptr) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 f = g4[8 * s + h];
-          x[4 * h] *= fast_sigmoid(f.x);
-          x[4 * h + 1] *= fast_sigmoid(f.y);
-          x[4 * h + 2] *= fast_sigmoid(f.z);
-          x[4 * h + 3] *= fast_sigmoid(f.w);
+        x[4 * h] = xn[h].x; x[4 * h + 1] = xn[h].y; x[4 * h + 2] = xn[h].z; x[4 * h + 3] = xn[h].w;
+        if (g4 != nullptr) {
+          x[4 * h] *= fast_sigmoid(gn[h].x);
+          x[4 * h + 1] *= fast_sigmoid(gn[h].y);
+          x[4 * h + 2] *= fast_sigmoid(gn[h].z);
+          x[4 * h + 3] *= fast_sigmoid(gn[h].w);
         }
       }
+#pragma unroll
+      for (int c = 0; c < kC; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[c][i] = wn[c][i];
+      fetch(s + 1 < steps ? s + 1 : s);
+      __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the products
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -109,7 +125,10 @@ __global__ __launch_bounds__(256) void lora_shrink_kernel(ShrinkArgs a) {
 
 template <int kType>
 int launch_shrink(const ShrinkArgs &a, int S, hipStream_t s) {
-  const dim3 grid((unsigned)((a.rows + 15) / 16), (unsigned)S), t(256);
+  // a tile of 16 rows has as many adapters at most; few tiles take them side by side
+  const int tiles = (a.rows + 15) / 16, most = std::min({a.rows, a.adapters, 16});
+  const int Z = std::clamp(512 / (tiles * S), 1, most);
+  const dim3 grid((unsigned)tiles, (unsigned)S, (unsigned)Z), t(256);
   if (a.rank <= 16) hipLaunchKernelGGL((lora_shrink_kernel<kType, 1>), grid, t, 0, s, a);
   else if (a.rank <= 32) hipLaunchKernelGGL((lora_shrink_kernel<kType, 2>), grid, t, 0, s, a);
   else if (a.rank <= 64) hipLaunchKernelGGL((lora_shrink_kernel<kType, 4>), grid, t, 0, s, a);
@@ -118,11 +137,12 @@ int launch_shrink(const ShrinkArgs &a, int S, hipStream_t s) {
   return PKV_OK;
 }
 
-// The split of the inputs: workgroups for the 256 CUs twice over, at most one per 256 inputs.
+// The split of the inputs: workgroups for the 256 CUs four times over, at most one per 256
+// inputs.
 int shrink_splits(int rows, int in_dim) {
   const int tiles = (rows + 15) / 16;
   int S = 1;
-  while (S * 2 * tiles <= 512 && in_dim / (S * 2) >= 256) S *= 2;
+  while (S * 2 * tiles <= 1024 && in_dim / (S * 2) >= 256) S *= 2;
   return S;
 }
 size_t t_bytes(int rows, int in_dim, int rank) {

@@ -47,81 +47,152 @@ __device__ __forceinline__ void lora_weights(const void *p, int64_t i, float (&w
   }
 }
 
-// t[row][r]: its parts in order
+// t[row][r]: its parts, four loads at a time
 __device__ __forceinline__ float lora_t(const LoraTerm &l, int row, int r) {
   const float *p = l.t + (int64_t)row * l.rank + r;
   float t = p[0];
-  for (int s = 1; s < l.S; ++s) t += p[s * l.plane];
+  int s = 1;
+  for (; s + 4 <= l.S; s += 4) {
+    const float a = p[s * l.plane], b = p[(s + 1) * l.plane];
+    const float c = p[(s + 2) * l.plane], d = p[(s + 3) * l.plane];
+    t += (a + b) + (c + d);
+  }
+  for (; s < l.S; ++s) t += p[s * l.plane];
   return t;
 }
 
-// One lane's share of (B t)[o] of a row, ranks lane, lane + 64: the caller sums over the wave.
+// One lane's share of (B t)[o] of a row: the caller sums over the wave. Up to 64 ranks, the
+// lanes left over take some of the parts of t (with 16 parts of 16 ranks, four each).
 __device__ __forceinline__ float lora_lane(const LoraTerm &l, int row, int o, int out_dim, int lane) {
   const int id = lora_adapter(l, row);
   if (id < 0) return 0.0f;
-  float s = 0.0f;
-  for (int r = lane; r < l.rank; r += 64)
-    s = fmaf(lora_weight(l.b, l.type, ((int64_t)id * out_dim + o) * l.rank + r), lora_t(l, row, r), s);
-  return s;
+  const int64_t w0 = ((int64_t)id * out_dim + o) * l.rank;
+  if (l.rank > 64) {
+    float s = 0.0f;
+    for (int r = lane; r < l.rank; r += 64)
+      s = fmaf(lora_weight(l.b, l.type, w0 + r), lora_t(l, row, r), s);
+    return s;
+  }
+  const int per = 64 / l.rank, s0 = lane / l.rank, r = lane - s0 * l.rank;
+  if (s0 >= per || s0 >= l.S) return 0.0f;
+  const float w = lora_weight(l.b, l.type, w0 + r);
+  const float *p = l.t + (int64_t)row * l.rank + r;
+  float t = 0.0f;
+  int s = s0;
+  for (; s + 3 * per < l.S; s += 4 * per) {
+    const float a = p[s * l.plane], b = p[(s + per) * l.plane];
+    const float c = p[(s + 2 * per) * l.plane], d = p[(s + 3 * per) * l.plane];
+    t += (a + b) + (c + d);
+  }
+  for (; s < l.S; s += per) t += p[s * l.plane];
+  return w * t;
 }
 
-// delta[rt][i] = (B t) of tokens tok0 + 4 g + i and outputs col0 + 16 rt + lane % 16 (g = lane
-// / 16): v_mfma_f32_16x16x4_f32 with t as A and B's rows as B, four ranks a lane at a time.
-// The tokens' adapters are taken one after the other; a token keeps its own one's result by
-// selection, so that nothing of another adapter (a NaN, say) reaches it.
-template <int kType, bool kVec, int kRT>
+// delta[tt][rt][i] = (B t) of tokens tok0 + 16 tt + 4 g + i and outputs col0 + 16 rt + lane % 16
+// (g = lane / 16): v_mfma_f32_16x16x4_f32 with t as A and B's rows as B, four ranks a lane
+// at a time, the loads of 32 ranks in flight together. The tokens' adapters are taken one
+// after the other; a token keeps its own one's result by selection, so that nothing of
+// another adapter (a NaN, say) reaches it.
+template <int kType, bool kVec, int kTT, int kRT>
 __device__ void lora_tile_as(const LoraTerm &l, int tokens, int out_dim, int tok0, int col0,
-                             int lane, float (&delta)[kRT][4]) {
+                             int lane, float (&delta)[kTT][kRT][4]) {
   typedef float v4 __attribute__((ext_vector_type(4)));
   const int m = lane & 15, g = lane >> 4;
-  const int row = tok0 + m < tokens ? tok0 + m : tokens - 1;
-  const int id = tok0 + m < tokens ? lora_adapter(l, row) : -1;
-  unsigned todo = (unsigned)(__ballot(id >= 0) & 0xFFFFu);
+  int row[kTT], id[kTT];
+  unsigned todo[kTT], any = 0;
 #pragma unroll
-  for (int rt = 0; rt < kRT; ++rt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) delta[rt][i] = 0.0f;
-  while (todo != 0) {
-    const int cur = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
-    const unsigned mine = (unsigned)(__ballot(id == cur) & 0xFFFFu);
-    todo &= ~mine;
-    v4 d[kRT];
-#pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) d[rt] = v4{0.f, 0.f, 0.f, 0.f};
-    for (int r0 = 0; r0 < l.rank; r0 += 16) {
-      const int r = r0 + 4 * g;
-      float a[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float t = lora_t(l, row, r + i < l.rank ? r + i : 0);
-        a[i] = id == cur && r + i < l.rank ? t : 0.0f;
-      }
-#pragma unroll
-      for (int rt = 0; rt < kRT; ++rt) {
-        const int col = col0 + 16 * rt + m;
-        const int64_t at = ((int64_t)cur * out_dim + (col < out_dim ? col : out_dim - 1)) * l.rank;
-        float w[4] = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (kVec) {
-          if (r < l.rank) lora_weights<kType, 4>(l.b, at + r, w);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (r + i < l.rank) w[i] = lora_weight(l.b, kType, at + r + i);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], w[i], d[rt], 0, 0, 0);
-      }
-    }
+  for (int tt = 0; tt < kTT; ++tt) {
+    const int t = tok0 + 16 * tt + m;
+    row[tt] = t < tokens ? t : tokens - 1;
+    id[tt] = t < tokens ? lora_adapter(l, row[tt]) : -1;
+    todo[tt] = (unsigned)(__ballot(id[tt] >= 0) & 0xFFFFu);
+    any |= todo[tt];
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        delta[rt][i] = (mine >> (4 * g + i)) & 1 ? d[rt][i] : delta[rt][i];
+      for (int i = 0; i < 4; ++i) delta[tt][rt][i] = 0.0f;
+  }
+  while (any != 0) {
+    // the first adapter that a token still waits for
+    int cur = -1;
+#pragma unroll
+    for (int tt = kTT - 1; tt >= 0; --tt)
+      if (todo[tt] != 0) cur = __builtin_amdgcn_readlane(id[tt], __builtin_ctz(todo[tt]));
+    unsigned mine[kTT];
+    any = 0;
+    v4 d[kTT][kRT];
+#pragma unroll
+    for (int tt = 0; tt < kTT; ++tt) {
+      mine[tt] = (unsigned)(__ballot(id[tt] == cur) & 0xFFFFu);
+      todo[tt] &= ~mine[tt];
+      any |= todo[tt];
+#pragma unroll
+      for (int rt = 0; rt < kRT; ++rt) d[tt][rt] = v4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int r0 = 0; r0 < l.rank; r0 += 32) {
+      float a[2][kTT][4], w[2][kRT][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = r0 + 16 * h + 4 * g;
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt) {
+          const int col = col0 + 16 * rt + m;
+          const int64_t at = ((int64_t)cur * out_dim + (col < out_dim ? col : out_dim - 1)) * l.rank;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[h][rt][i] = 0.0f;
+          if constexpr (kVec) {
+            if (r < l.rank) lora_weights<kType, 4>(l.b, at + r, w[h][rt]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (r + i < l.rank) w[h][rt][i] = lora_weight(l.b, kType, at + r + i);
+          }
+        }
+#pragma unroll
+        for (int tt = 0; tt < kTT; ++tt) {
+          if constexpr (kVec) {
+            const float *p = l.t + (int64_t)row[tt] * l.rank + (r < l.rank ? r : 0);
+            float4 t = *reinterpret_cast<const float4 *>(p);
+            for (int s = 1; s < l.S; ++s) {
+              const float4 f = *reinterpret_cast<const float4 *>(p + s * l.plane);
+              t.x += f.x; t.y += f.y; t.z += f.z; t.w += f.w;
+            }
+            const bool on = id[tt] == cur && r < l.rank;
+            a[h][tt][0] = on ? t.x : 0.0f;
+            a[h][tt][1] = on ? t.y : 0.0f;
+            a[h][tt][2] = on ? t.z : 0.0f;
+            a[h][tt][3] = on ? t.w : 0.0f;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float t = lora_t(l, row[tt], r + i < l.rank ? r + i : 0);
+              a[h][tt][i] = id[tt] == cur && r + i < l.rank ? t : 0.0f;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+            for (int tt = 0; tt < kTT; ++tt)
+              d[tt][rt] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[h][tt][i], w[h][rt][i], d[tt][rt], 0, 0, 0);
+    }
+#pragma unroll
+    for (int tt = 0; tt < kTT; ++tt)
+#pragma unroll
+      for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          delta[tt][rt][i] = (mine[tt] >> (4 * g + i)) & 1 ? d[tt][rt][i] : delta[tt][rt][i];
   }
 }
-template <int kRT>
+template <int kTT, int kRT>
 __device__ __forceinline__ void lora_tile(const LoraTerm &l, int tokens, int out_dim, int tok0,
-                                          int col0, int lane, float (&delta)[kRT][4]) {
+                                          int col0, int lane, float (&delta)[kTT][kRT][4]) {
   const bool vec = (l.rank & 3) == 0;
   if (l.type == PKV_LORA_F32) {
     if (vec) lora_tile_as<PKV_LORA_F32, true>(l, tokens, out_dim, tok0, col0, lane, delta);

@@ -471,11 +471,11 @@ __global__ __launch_bounds__(256 * kWT) void oproj_mfma_kernel(Args a) {
   }
   // D layout: lane holds rows (tokens) 4 g + i of the tile, column (weight row) lane & 15
   float *dst = a.S == 1 ? a.out : a.part + (int64_t)split * a.T * a.N;
+  float low[kTT][kRT][4];
+  if constexpr (std::is_same<Args, MxLoraArgs>::value)
+    lora_tile(a.lora, a.T, a.N, tbk * kTok + 16 * tt0, row0 + wr * 16 * kRT, lane, low);
 #pragma unroll
   for (int tt = 0; tt < kTT; ++tt) {
-    float low[kRT][4];
-    if constexpr (std::is_same<Args, MxLoraArgs>::value)
-      lora_tile(a.lora, a.T, a.N, tbk * kTok + 16 * (tt0 + tt), row0 + wr * 16 * kRT, lane, low);
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt) {
       const int n = row0 + wr * 16 * kRT + rt * 16 + r16;
@@ -485,7 +485,7 @@ __global__ __launch_bounds__(256 * kWT) void oproj_mfma_kernel(Args a) {
         const int t = tbk * kTok + 16 * (tt0 + tt) + 4 * g + i;
         if (t >= a.T) continue;
         if constexpr (std::is_same<Args, MxLoraArgs>::value)
-          dst[(int64_t)t * a.N + n] = fmaf(a.inv[t], fin[tt][rt][i], low[rt][i]);
+          dst[(int64_t)t * a.N + n] = fmaf(a.inv[t], fin[tt][rt][i], low[tt][rt][i]);
         else
           dst[(int64_t)t * a.N + n] = a.S == 1 ? a.inv[t] * fin[tt][rt][i] : fin[tt][rt][i];
       }

@@ -254,7 +254,20 @@ struct LoraTerm {
   const int *ids;
   int type, rank, adapters, S;
   int64_t plane;  // rows * rank
+  // what t is made from (host side only)
+  const float *attn, *gate;
+  const void *a;       // [adapters][rank][in]
+  const float *scale;  // [adapters]
+  int rows, in_dim;
 };
+// Gated inputs of the batched projection: x = (hi + lo) * inv[row], fp16 hi and lo [rows][in].
+struct LoraSplit {
+  const void *hi = nullptr, *lo = nullptr;
+  const float *inv = nullptr;
+};
+// t = scale A x of every row with an adapter, from attn and gate or from their split
+// (pkv_lora.hip).
+int launch_lora_shrink(const LoraTerm &lora, const LoraSplit &split, hipStream_t s);
 int launch_oproj(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
                  int batch, int in_dim, int out_dim, hipStream_t s,
                  const LoraTerm *lora = nullptr);

@@ -462,6 +462,8 @@ int launch_oproj(const float *attn, const float *gate, const uint8_t *w, int w_t
                  int batch, int in_dim, int out_dim, hipStream_t s, const LoraTerm *lora) {
   if (int rc = check_oproj(attn, gate, w, w_type, batch, in_dim, out_dim)) return rc;
   if (batch > 65535) return set_error(PKV_ERR_ARG, "batch must be <= 65535");
+  if (lora != nullptr)
+    if (int rc = launch_lora_shrink(*lora, LoraSplit{}, s)) return rc;
   OprojArgs a{attn, gate, w, out, batch, in_dim, out_dim};
   const int rows_per_wave = batch < 4 ? 1 : 2;
   const int rows_per_wg = kOprojWaves * rows_per_wave;

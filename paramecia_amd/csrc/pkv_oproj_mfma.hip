@@ -642,6 +642,10 @@ int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, in
   else
     hipLaunchKernelGGL(oproj_xprep_kernel<4>, dim3((unsigned)T_pad), dim3(256), 0, s, xa);
   PKV_HIP(hipGetLastError());
+  if (lora != nullptr) {
+    const LoraSplit split{base, base + off_xl, reinterpret_cast<const float *>(base + off_inv)};
+    if (int rc = launch_lora_shrink(*lora, split, s)) return rc;
+  }
   MxArgs ma{reinterpret_cast<const u4 *>(base), reinterpret_cast<const u4 *>(base + off_xl),
             reinterpret_cast<const h4 *>(base + off_xs),
             reinterpret_cast<const float *>(base + off_inv), w, row_bytes,

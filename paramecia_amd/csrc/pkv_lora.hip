@@ -17,6 +17,8 @@ namespace pkv {
 namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 struct ShrinkArgs {
   const float *attn, *gate;  // [rows][in]; gate may be null
@@ -39,7 +41,10 @@ __device__ __forceinline__ float fast_sigmoid(float g) {
 // MFMAs of a step take one of each. The rows' adapters are taken one after the other (in turn
 // by gridDim.z workgroups), each for all 16 rows; a row keeps its own one's result. kC
 // tiles of 16 ranks. kSplit: the inputs come, gated already, as the batched projection's
-// fp16 pairs (hi + lo) 2^-e (half the bytes of x and gate, and written just before).
+// fp16 pairs (hi + lo) 2^-e (half the bytes of x and gate, and written just before), and
+// 16-bit weights take v_mfma_f32_16x16x32 as they are: F16 against hi and lo, BF16 against
+// the three bf16 parts that hi + lo (22 bits) has. 4001 rows, rank 64: 40 us with f32
+// products, of them 10 per 16 ranks.
 constexpr int kShrinkWaves = 8;
 template <int kType, int kC, bool kSplit>
 __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkArgs a) {
@@ -77,52 +82,96 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkAr
       const int r = 16 * c + m < a.rank ? 16 * c + m : a.rank - 1;
       w0[c] = ((int64_t)cur * a.rank + r) * a.in_dim + k0;
     }
-    // the next step's inputs and weights are loaded while this one's products run
-    float4 xn[2], gn[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    float wn[kC][8];
-    h8 hn, ln;
-    auto fetch = [&](int s) {
-      if constexpr (kSplit) {
+    if constexpr (kSplit && kType != PKV_LORA_F32) {
+      u4 wn[kC];
+      h8 hn, ln;
+      auto fetch = [&](int s) {
         hn = h4[4 * s];
         ln = l4[4 * s];
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          xn[h] = x4[8 * s + h];
-          if (g4 != nullptr) gn[h] = g4[8 * s + h];
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < kC; ++c) lora_weights<kType, 8>(a.a, w0[c] + 32 * s, wn[c]);
-    };
-    fetch(0);
-    for (int s = 0; s < steps; ++s) {
-      float x[8], w[kC][8];
-      if constexpr (kSplit) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)hn[i] + (float)ln[i];
-      }
-#pragma unroll
-      for (int h = 0; h < (kSplit ? 0 : 2); ++h) {
-        x[4 * h] = xn[h].x; x[4 * h + 1] = xn[h].y; x[4 * h + 2] = xn[h].z; x[4 * h + 3] = xn[h].w;
-        if (g4 != nullptr) {
-          x[4 * h] *= fast_sigmoid(gn[h].x);
-          x[4 * h + 1] *= fast_sigmoid(gn[h].y);
-          x[4 * h + 2] *= fast_sigmoid(gn[h].z);
-          x[4 * h + 3] *= fast_sigmoid(gn[h].w);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < kC; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[c][i] = wn[c][i];
-      fetch(s + 1 < steps ? s + 1 : s);
-      __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the products
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int c = 0; c < kC; ++c)
-          acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], w[c][i], acc[c], 0, 0, 0);
+          wn[c] = *reinterpret_cast<const u4 *>(reinterpret_cast<const uint16_t *>(a.a) + w0[c] + 32 * s);
+      };
+      fetch(0);
+      for (int s = 0; s < steps; ++s) {
+        const h8 hi = hn, lo = ln;
+        u4 w[kC];
+#pragma unroll
+        for (int c = 0; c < kC; ++c) w[c] = wn[c];
+        fetch(s + 1 < steps ? s + 1 : s);
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the products
+        if constexpr (kType == PKV_LORA_F16) {
+#pragma unroll
+          for (int c = 0; c < kC; ++c)
+            acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, __builtin_bit_cast(h8, w[c]), acc[c], 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < kC; ++c)
+            acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, __builtin_bit_cast(h8, w[c]), acc[c], 0, 0, 0);
+        } else {
+          b8 part[3];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float x = (float)hi[i] + (float)lo[i];
+            part[0][i] = (__bf16)x;
+            const float y = x - (float)part[0][i];
+            part[1][i] = (__bf16)y;
+            part[2][i] = (__bf16)(y - (float)part[1][i]);
+          }
+#pragma unroll
+          for (int p = 0; p < 3; ++p)
+#pragma unroll
+            for (int c = 0; c < kC; ++c)
+              acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(part[p], __builtin_bit_cast(b8, w[c]), acc[c], 0, 0, 0);
+        }
+      }
+    } else {
+      // the next step's inputs and weights are loaded while this one's products run
+      float4 xn[2], gn[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      float wn[kC][8];
+      h8 hn, ln;
+      auto fetch = [&](int s) {
+        if constexpr (kSplit) {
+          hn = h4[4 * s];
+          ln = l4[4 * s];
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            xn[h] = x4[8 * s + h];
+            if (g4 != nullptr) gn[h] = g4[8 * s + h];
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kC; ++c) lora_weights<kType, 8>(a.a, w0[c] + 32 * s, wn[c]);
+      };
+      fetch(0);
+      for (int s = 0; s < steps; ++s) {
+        float x[8], w[kC][8];
+        if constexpr (kSplit) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = (float)hn[i] + (float)ln[i];
+        }
+#pragma unroll
+        for (int h = 0; h < (kSplit ? 0 : 2); ++h) {
+          x[4 * h] = xn[h].x; x[4 * h + 1] = xn[h].y; x[4 * h + 2] = xn[h].z; x[4 * h + 3] = xn[h].w;
+          if (g4 != nullptr) {
+            x[4 * h] *= fast_sigmoid(gn[h].x);
+            x[4 * h + 1] *= fast_sigmoid(gn[h].y);
+            x[4 * h + 2] *= fast_sigmoid(gn[h].z);
+            x[4 * h + 3] *= fast_sigmoid(gn[h].w);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kC; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[c][i] = wn[c][i];
+        fetch(s + 1 < steps ? s + 1 : s);
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the products
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int c = 0; c < kC; ++c)
+            acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], w[c][i], acc[c], 0, 0, 0);
+      }
     }
 #pragma unroll
     for (int c = 0; c < kC; ++c) red[wave][c][lane] = acc[c];
@@ -205,9 +254,10 @@ int launch_lora_shrink(const LoraTerm &l, const LoraSplit &split, hipStream_t s)
   ShrinkArgs a{l.attn, l.gate, split, l.a, l.scale, l.ids, const_cast<float *>(l.t), nullptr,
                l.rows, l.in_dim, l.rank, l.adapters, l.in_dim / l.S};
   if (int rc = device_status_word(&a.status)) return rc;
-  // a tile of 16 rows has as many adapters at most; few tiles take them side by side
+  // a tile of 16 rows has as many adapters at most; few tiles take them side by side (24 rows
+  // of 9 adapters: 5.1 us, one after the other 18.7)
   const int tiles = (a.rows + 15) / 16, most = std::min({a.rows, a.adapters, 16});
-  const int Z = std::clamp(512 / (tiles * l.S), 1, most);
+  const int Z = std::clamp(1024 / (tiles * l.S), 1, most);
   const dim3 grid((unsigned)tiles, (unsigned)l.S, (unsigned)Z);
   switch (l.type) {
     case PKV_LORA_F32: launch_shrink<PKV_LORA_F32>(a, grid, s); break;

@@ -308,7 +308,7 @@ int pkv_causal_conv(const float *x, int64_t stride_b, int64_t stride_t, const fl
  * and workspace 16-byte aligned; q, k and v must not overlap out or state. workspace: at
  * least pkv_deltanet_prompt_workspace() bytes of device memory (may be 0, with NULL), which
  * the call writes: calls that overlap in time, and graphs that do, need one each. */
-size_t pkv_deltanet_prompt_workspace(int batch, int64_t n, int heads, int head_dim);
+size_t pkv_deltanet_prompt_workspace(int batch, int64_t n, int k_heads, int heads, int head_dim);
 int pkv_deltanet_prompt(const float *q, const float *k, const float *v, const int64_t strides[6],
                         const float *gate, const float *beta, float *state, float *gate_offset,
                         const int *lens, float *out, int batch, int64_t n, int k_heads, int heads,

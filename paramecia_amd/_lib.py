@@ -141,7 +141,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "pkv_gated_oproj_q4k": ([vp] * 4 + [c_int] * 3 + [vp], c_int),
         "pkv_gated_oproj": ([vp] * 3 + [c_int, vp] + [c_int] * 3 + [vp], c_int),
         "pkv_causal_conv": ([vp, c_i64, c_i64] + [vp] * 5 + [c_int, c_i64, c_int, c_int, c_int, vp], c_int),
-        "pkv_deltanet_prompt_workspace": ([c_int, c_i64, c_int, c_int], c_sz),
+        "pkv_deltanet_prompt_workspace": ([c_int, c_i64, c_int, c_int, c_int], c_sz),
         "pkv_deltanet_prompt": ([vp] * 3 + [P(c_i64)] + [vp] * 6 +
                                 [c_int, c_i64, c_int, c_int, c_int, fl, fl, vp, c_sz, vp], c_int),
         "pkv_rms_norm": ([vp, c_i64, vp, vp, vp, fl, vp, vp, c_i64, c_int, vp], c_int),

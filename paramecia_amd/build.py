@@ -38,7 +38,7 @@ SOURCES = {
     "pkv_prefill_half.hip": [],
     "pkv_util.hip": [],
     "pkv_deltanet.hip": [],
-    "pkv_deltanet_prompt.hip": [],
+    "pkv_deltanet_prompt.hip": ["-ffp-contract=off"],
     "pkv_conv.hip": [],
     "pkv_rmsnorm.hip": ["-ffp-contract=off"],
     "pkv_lora.hip": [],

@@ -1206,9 +1206,9 @@ int pkv_causal_conv(const float *x, int64_t stride_b, int64_t stride_t, const fl
                             channels, taps, silu, static_cast<hipStream_t>(stream));
 }
 
-size_t pkv_deltanet_prompt_workspace(int batch, int64_t n, int heads, int head_dim) {
-  if (batch <= 0 || n <= 0 || heads <= 0 || head_dim <= 0) return 0;
-  return deltanet_prompt_workspace(batch, n, heads, head_dim);
+size_t pkv_deltanet_prompt_workspace(int batch, int64_t n, int k_heads, int heads, int head_dim) {
+  if (batch <= 0 || n <= 0 || k_heads <= 0 || heads <= 0 || head_dim <= 0) return 0;
+  return deltanet_prompt_workspace(batch, n, k_heads, heads, head_dim);
 }
 
 int pkv_deltanet_prompt(const float *q, const float *k, const float *v, const int64_t strides[6],

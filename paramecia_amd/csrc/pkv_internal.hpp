@@ -300,7 +300,7 @@ int launch_deltanet_prompt(const float *q, const float *k, const float *v, const
                            const int *lens, float *out, int batch, int64_t n, int k_heads,
                            int heads, int head_dim, float scale, float eps, void *ws,
                            size_t ws_bytes, hipStream_t s);
-size_t deltanet_prompt_workspace(int batch, int64_t n, int heads, int head_dim);
+size_t deltanet_prompt_workspace(int batch, int64_t n, int k_heads, int heads, int head_dim);
 int launch_rms_norm(const float *x, int64_t x_stride, float *residual, const float *alpha,
                     const float *gate, float eps, float *out, uint8_t *q8, int64_t rows, int dim,
                     hipStream_t s);

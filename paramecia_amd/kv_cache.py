@@ -586,7 +586,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate: to
         _in_place(out, "out", (b, n, h, d))
     strides = (ctypes.c_int64 * 6)(*(x for t in ins for x in (t.stride(0) if b > 1 else 0,
                                                               t.stride(1) if n > 1 else 0)))
-    need = lib().pkv_deltanet_prompt_workspace(b, n, h, d)
+    need = lib().pkv_deltanet_prompt_workspace(b, n, hk, h, d)
     # torch's allocator orders the workspace with the stream, and gives each graph its own
     ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need else None
     _call(lib().pkv_deltanet_prompt(ins[0].data_ptr(), ins[1].data_ptr(), ins[2].data_ptr(), strides,

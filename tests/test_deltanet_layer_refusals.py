@@ -68,8 +68,8 @@ def test_scan(k, code, word):
 
 
 def test_scan_workspace():
-    need = lib().pkv_deltanet_prompt_workspace(2, 80, 32, 128)
-    assert lib().pkv_deltanet_prompt_workspace(0, 80, 32, 128) == 0
+    need = lib().pkv_deltanet_prompt_workspace(2, 80, 16, 32, 128)
+    assert lib().pkv_deltanet_prompt_workspace(0, 80, 16, 32, 128) == 0
     if need:
         assert scan(wb=need - 1) == ERR_ARG and "workspace" in err()
         assert scan(ws=None) == ERR_ARG and "workspace" in err()

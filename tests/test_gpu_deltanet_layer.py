@@ -193,6 +193,10 @@ def check_scan(pk, ins, scale, lens, out):
     (2, 90, 2, 4, 256, [33, 90]),
     (1, 7, 4, 4, 256, None),
     (1, 1500, 1, 2, 128, None),
+    (16, 200, 16, 32, 128, None),                # more than one segment of chunks
+    (9, 333, 16, 32, 128, [333, 0, 48, 47, 200, 256, 257, 1, 128]),
+    (1, 130, 3, 15, 64, None),                   # an odd number of value heads per key head
+    (2, 70, 8, 8, 256, [70, 65]),
 ])
 def test_scan(pk, b, n, hk, h, d, lens):
     say(f"scan b={b} n={n} hk={hk} h={h} d={d} lens={lens}")
@@ -209,7 +213,7 @@ def test_scan(pk, b, n, hk, h, d, lens):
 
 
 @pytest.mark.parametrize("n", [11, 150])
-@pytest.mark.parametrize("kind", ["slow", "fast", "mixed", "reset", "same_keys", "zero_rows", "large", "small", "closed"])
+@pytest.mark.parametrize("kind", ["slow", "fast", "mixed", "reset", "same_keys", "zero_rows", "large", "small", "closed", "growing", "huge", "far_apart", "late"])
 def test_scan_values(pk, kind, n):
     """Decays from none to whole, keys that all point the same way, zero vectors, magnitudes."""
     say(f"scan values {kind} n={n}")
@@ -237,6 +241,14 @@ def test_scan_values(pk, kind, n):
         v, state = v * 1e15, state * 1e15
     elif kind == "small":
         v, state = v * 1e-15, state * 1e-15
+    elif kind == "growing":  # a positive gate, in one head only
+        gate[:, n // 2, 1] = 0.05
+    elif kind == "huge":  # past what a state in two fp16 parts is scaled for
+        v = v * 1e28
+    elif kind == "far_apart":  # value channels of unlike magnitude share a tile
+        v = v * torch.exp2(torch.arange(d, device="cuda") % 16 - 8.0)
+    elif kind == "late":  # the largest values come last
+        v = v * torch.exp2(torch.linspace(-20, 10, n, device="cuda"))[:, None, None]
     elif kind == "closed":  # sigmoid(beta) = 0: nothing is written
         beta = beta * 0 - 200.0
     out = torch.empty_like(v)
@@ -292,6 +304,31 @@ def test_scan_sequences_do_not_touch(pk):
     for i in (0, 2):
         assert torch.equal(got[i], clean[i]) and torch.equal(s1[i], s0[i])
     assert torch.isnan(got[1]).all()
+
+
+@pytest.mark.parametrize("n,at", [(200, 100), (200, 0), (90, 89), (20, 7)])
+@pytest.mark.parametrize("what", ["q", "k", "v", "gate", "beta"])
+def test_scan_nan_goes_forward_only(pk, n, at, what):
+    """A NaN in one token reaches the tokens behind it, never those in front, and no other
+    key head's value heads."""
+    say(f"scan: NaN in {what} at {at} of {n}")
+    r = gen(9)
+    ins = scan_inputs(r, 1, n, 2, 4, 128)
+    s0, s1 = ins[5].clone(), ins[5].clone()
+    clean = pk.gated_delta_rule(*ins[:5], s0, 0.1, EPS)
+    {"q": ins[0], "k": ins[1], "v": ins[2], "gate": ins[3], "beta": ins[4]}[what][0, at, 1] = float("nan")
+    got = pk.gated_delta_rule(*ins[:5], s1, 0.1, EPS)
+    lim = 2 * scan_limit(n)  # the head with the NaN may go another way
+    hit = slice(2, 4) if what in "qk" else slice(1, 2)
+    other = [h for h in range(4) if h not in range(4)[hit]]
+    assert torch.equal(got[:, :, other], clean[:, :, other]) and torch.equal(s1[:, other], s0[:, other])
+    if at:
+        assert rel(got[:, :at, hit], clean[:, :at, hit]) <= lim
+    assert torch.isnan(got[:, at, hit]).all()
+    if what == "q":
+        assert rel(s1, s0) <= lim
+    elif at + 1 < n:
+        assert torch.isnan(got[:, at + 1:, hit]).any()
 
 
 # ------------------------------------------------------------------ norm

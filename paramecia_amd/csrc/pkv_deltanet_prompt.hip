@@ -228,19 +228,21 @@ struct ChunkArgs {
 __device__ __forceinline__ int tri(int w, int p) { return w < 2 ? w : 2 * w - 2 + p; }
 
 // A chunk of one key head: normalised K and Q as fragments, their products, and for each of
-// its value heads T (by forward substitution in f32: lane c owns column c of T, 64 registers,
-// and reads A's rows as broadcasts) and P. A wave owns 16 tokens, its lanes load q and k in
-// fragment order; the waves take each other's K from LDS.
+// its value heads T and P. A wave owns 16 tokens, its lanes load q and k in fragment order;
+// the waves take each other's K from LDS. T = (I + A)^-1 by blocks of 16, in f32: the
+// diagonal blocks by forward substitution (16 lanes each, a column a lane), then T_ij = -T_ii
+// sum_k A_ik T_kj down the block columns, a wave each, on v_mfma_f32_16x16x4_f32, whose result
+// tiles are the next product's B operand as they are.
 template <int kD>
 __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
   constexpr int kS = kD / 32, kRow = kD + 8, kSq = 68;
-  constexpr int kKB = 2 * kC * kRow * 2, kAB = 3 * kC * kSq * 4;
+  constexpr int kKB = 2 * kC * kRow * 2, kAB = 4 * kC * kSq * 4;
   __shared__ __attribute__((aligned(16))) char lds[kKB > kAB ? kKB : kAB];
   __shared__ double gam[2][kC];
   __shared__ float bet[2][kC];
   __shared__ unsigned bad;
   _Float16(*kh)[kC][kRow] = reinterpret_cast<_Float16(*)[kC][kRow]>(lds);  // [hi, lo][token][k]
-  float(*am)[kC][kSq] = reinterpret_cast<float(*)[kC][kSq]>(lds);           // A or T of two heads, then P
+  float(*am)[kC][kSq] = reinterpret_cast<float(*)[kC][kSq]>(lds);           // A of two heads, then P and T of both
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
   const int64_t chunk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int64_t t0 = a.first + chunk * kC;
@@ -387,62 +389,81 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
           const int t = 16 * w + 4 * g + i, s = 16 * j + m;
           const float dec = s <= t ? expf((float)(gam[e][t] - gam[e][s])) : 0.0f;
           am[e][t][s] = s < t ? bet[e][t] * dec * kk[j][i] : 0.0f;
-          am[2][t][s] = s <= t ? dec * qk[j][i] : 0.0f;
+          am[2 + e][t][s] = s <= t ? dec * qk[j][i] : 0.0f;
         }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        if (p > w >> 1) continue;
-        h8 f[2];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          _Float16 hi, lo;
-          split(am[2][16 * w + m][32 * p + 16 * (i >> 2) + 4 * g + (i & 3)] * kUp, hi, lo);
-          f[0][i] = hi;
-          f[1][i] = lo;
-        }
-        h8 *o = a.w.p + ((out + e) * 6 + tri(w, p)) * kFrag + lane;
-        o[0] = f[0];
-        o[64] = f[1];
-      }
-      __syncthreads();
-    }
-    if (w < heads) {
-      float T[kC];
-#pragma unroll
-      for (int t = 0; t < kC; ++t) {
-        float acc[4] = {t == lane ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int s = 0; s < t; s += 4) {
-          const float4 x = *reinterpret_cast<const float4 *>(&am[w][t][s]);
-          acc[0] = fmaf(-x.x, T[s], acc[0]);
-          if (s + 1 < t) acc[1] = fmaf(-x.y, T[s + 1], acc[1]);
-          if (s + 2 < t) acc[2] = fmaf(-x.z, T[s + 2], acc[2]);
-          if (s + 3 < t) acc[3] = fmaf(-x.w, T[s + 3], acc[3]);
-        }
-        T[t] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-        am[w][t][lane] = T[t];  // row t of A has been read
       }
     }
     __syncthreads();
-    for (int e = 0; e < heads; ++e) {
+    // the fragments of a lower triangular matrix's rows 16 w ..
+    const auto put_rows = [&](const float(*x)[kSq], h8 *o) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         if (p > w >> 1) continue;
         h8 f[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          _Float16 hi, lo;
-          split(am[e][16 * w + m][32 * p + 16 * (i >> 2) + 4 * g + (i & 3)] * kUp, hi, lo);
-          f[0][i] = hi;
-          f[1][i] = lo;
+        for (int c = 0; c < 2; ++c) {
+          const f4 y = *reinterpret_cast<const f4 *>(&x[16 * w + m][32 * p + 16 * c + 4 * g]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            _Float16 hi, lo;
+            split(y[i] * kUp, hi, lo);
+            f[0][4 * c + i] = hi;
+            f[1][4 * c + i] = lo;
+          }
         }
-        h8 *o = a.w.t + ((out + e) * 6 + tri(w, p)) * kFrag + lane;
-        o[0] = f[0];
-        o[64] = f[1];
+        o[tri(w, p) * kFrag + lane] = f[0];
+        o[tri(w, p) * kFrag + 64 + lane] = f[1];
+      }
+    };
+    for (int e = 0; e < heads; ++e) put_rows(am[2 + e], a.w.p + (out + e) * 6 * kFrag);
+    if (w < heads) {  // lane m of block g: column m of its inverse
+      float D[16];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        float acc[4] = {t == m ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < t; s += 4) {
+          const f4 x = *reinterpret_cast<const f4 *>(&am[w][16 * g + t][16 * g + s]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (s + i < t) acc[i] = fmaf(-x[i], D[s + i], acc[i]);
+        }
+        D[t] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+      }
+#pragma unroll
+      for (int t = 0; t < 16; ++t) am[w][16 * g + t][16 * g + m] = D[t];
+    }
+    __syncthreads();
+    for (int e = 0; e < heads; ++e) {
+      const int j = e == 0 ? w : 3 - w;  // long columns beside short ones
+      f4 T[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < j) continue;
+        if (i == j) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) T[i][c] = am[e][16 * j + 4 * g + c][16 * j + m];
+        } else {
+          f4 x = f4{0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll
+          for (int k = 0; k < i; ++k) {
+            if (k < j) continue;
+            const f4 row = *reinterpret_cast<const f4 *>(&am[e][16 * i + m][16 * k + 4 * g]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x = __builtin_amdgcn_mfma_f32_16x16x4f32(row[c], T[k][c], x, 0, 0, 0);
+          }
+          const f4 row = *reinterpret_cast<const f4 *>(&am[e][16 * i + m][16 * i + 4 * g]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) y = __builtin_amdgcn_mfma_f32_16x16x4f32(row[c], x[c], y, 0, 0, 0);
+          T[i] = -y;
+        }
+        // over P, whose zeros above the diagonal are T's too
+#pragma unroll
+        for (int c = 0; c < 4; ++c) am[2 + e][16 * i + 4 * g + c][16 * j + m] = T[i][c];
       }
     }
+    __syncthreads();
+    for (int e = 0; e < heads; ++e) put_rows(am[2 + e], a.w.t + (out + e) * 6 * kFrag);
   }
 }
 
@@ -454,6 +475,19 @@ __device__ __forceinline__ void lds_barrier() {
 }
 __device__ __forceinline__ uint32_t mag(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  const auto dpp = [](uint32_t v, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, decltype(ctrl)::value, 0xF, 0xF, false);
+  };
+  x = umax(x, dpp(x, std::integral_constant<int, 0xB1>{}));
+  x = umax(x, dpp(x, std::integral_constant<int, 0x4E>{}));
+  x = umax(x, dpp(x, std::integral_constant<int, 0x141>{}));
+  x = umax(x, dpp(x, std::integral_constant<int, 0x140>{}));
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = umax(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return umax(b[0], b[1]);
+}
 // The exponent that takes values up to `bound` (finite) below 2^15.
 __device__ __forceinline__ int scale_exp(float bound) {
   const int e = 14 - ((int)(__builtin_bit_cast(uint32_t, bound) >> 23) - 127);
@@ -472,14 +506,17 @@ union StateLds {
   TokenStage<kD> t;
 };
 
-// The chunks of 16 value channels of one head, in order. Wave w owns key channels w d / 4 ..
-// of the state (f32, in an MFMA result's layout) and tokens 16 w .. of each chunk. Its
-// fragments of the next chunk are loaded into the registers that a stage has just used.
+// The chunks of 16 value channels of one head, in order, by eight waves. Waves 0 - 3 carry the
+// state: wave w owns key channels w d / 4 .. of it (f32, in an MFMA result's layout) and
+// tokens 16 w .. of each chunk. Waves 4 - 7 make the outputs of the same tokens beside them, off
+// the path from one chunk to the next. A wave loads its fragments of the next chunk (K and Q:
+// of the one after, where the registers hold both) when a stage has just used them.
 template <int kD>
-__global__ __launch_bounds__(256) void state_kernel(ChunkArgs a) {
+__global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   constexpr int kS = kD / 32, kN = kD / 64;
+  constexpr bool kDeep = kD <= 128;
   __shared__ __attribute__((aligned(16))) StateLds<kD> lds;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, w = wave & 3, m = lane & 15, g = lane >> 4;
   // the workgroups of a key head share an XCD and its L2 (workgroups go to the 8 XCDs in turn)
   const int groups = a.batch * a.k_heads, per = a.s.rep * (kD / 16);
   int grp, in;
@@ -498,97 +535,17 @@ __global__ __launch_bounds__(256) void state_kernel(ChunkArgs a) {
   end = end < stop ? end : stop;
   if (end <= a.first) return;
   const int chunks = (int)((end - a.first + kC - 1) / kC);
-
-  const h8 *kw = a.w.k + ((b * a.chunks * a.k_heads + hk) * 4 + w) * kS * kFrag + lane;
-  const h8 *qw = a.w.q + ((b * a.chunks * a.k_heads + hk) * 4 + w) * kS * kFrag + lane;
-  const h8 *ktw = a.w.kt + ((b * a.chunks * a.k_heads + hk) * (kD / 16) + w * kN) * 2 * kFrag + lane;
-  const h8 *tw = a.w.t + ((b * a.chunks * a.s.heads + h) * 6 + tri(w, 0)) * kFrag + lane;
-  const h8 *pw = a.w.p + ((b * a.chunks * a.s.heads + h) * 6 + tri(w, 0)) * kFrag + lane;
-  const float *meta = a.w.meta + (b * a.chunks * a.s.heads + h) * 3 * kC;
   const int64_t kstep = (int64_t)a.k_heads * 4 * kS * kFrag, tstep = (int64_t)a.s.heads * 6 * kFrag;
-  const float *vp = a.s.v + b * a.s.vb + h * kD + row0 + m;
-  float *op = a.s.out + (b * a.s.n * a.s.heads + h) * kD + row0 + m;
-  float *state = a.s.state + ((b * a.s.heads + h) * kD + row0 + m) * kD + w * (kD / 4) + 4 * g;
+  const int64_t key0 = b * a.chunks * a.k_heads + hk, val0 = b * a.chunks * a.s.heads + h;
+  const float *meta = a.w.meta + val0 * 3 * kC + 16 * w + 4 * g;
+  const int64_t mstep = (int64_t)a.s.heads * 3 * kC;
+  const int64_t tok = a.first + 16 * w + 4 * g;  // the lane's first token of chunk 0
 
   if (tid == 0) lds.c.odd = 0u;
   __syncthreads();
-  for (int c = tid; c < chunks; c += 256)
-    if (a.w.odd[(b * a.chunks + c) * a.s.heads + h] != 0u) lds.c.odd = 1u;
+  for (int c = tid; c < chunks; c += 512)
+    if (a.w.odd[val0 + (int64_t)c * a.s.heads] != 0u) lds.c.odd = 1u;
 
-  h8 kf[kS][2], qf[kS][2], ktf[kN][2][2], tf[2][2], pf[2][2];
-  float v[4];
-  f4 be, eg, ec;
-  float whole;
-  auto load_k = [&](int64_t c) {
-#pragma unroll
-    for (int s = 0; s < kS; ++s)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        kf[s][u] = kw[c * kstep + s * kFrag + 64 * u];
-        qf[s][u] = qw[c * kstep + s * kFrag + 64 * u];
-      }
-  };
-  auto load_t = [&](int64_t c) {
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (p <= w >> 1) tf[p][u] = tw[c * tstep + p * kFrag + 64 * u];
-  };
-  auto load_p = [&](int64_t c) {
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (p <= w >> 1) pf[p][u] = pw[c * tstep + p * kFrag + 64 * u];
-#pragma unroll
-    for (int n = 0; n < kN; ++n)
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) ktf[n][p][u] = ktw[c * kstep + (n * 2 + p) * kFrag + 64 * u];
-  };
-  auto load_v = [&](int64_t c) {
-    const int64_t t = a.first + c * kC + 16 * w + 4 * g;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = t + i < end ? vp[(t + i) * a.s.vt] : 0.0f;
-  };
-  auto load_meta = [&](int64_t c) {
-    const float *p = meta + c * a.s.heads * 3 * kC;
-    be = *reinterpret_cast<const f4 *>(p + 16 * w + 4 * g);
-    eg = *reinterpret_cast<const f4 *>(p + kC + 16 * w + 4 * g);
-    ec = *reinterpret_cast<const f4 *>(p + 2 * kC + 16 * w + 4 * g);
-    whole = p[2 * kC - 1];
-  };
-  load_k(0);
-  load_meta(0);
-  load_v(0);
-  load_t(0);
-  load_p(0);
-  f4 M[kN];
-#pragma unroll
-  for (int n = 0; n < kN; ++n) M[n] = *reinterpret_cast<const f4 *>(state + 16 * n);
-
-  // largest |M| (bits) and |v| of the workgroup; integer order, so that a NaN is larger than
-  // everything
-  auto put_top = [&]() {
-    uint32_t x = 0u, y = 0u;
-#pragma unroll
-    for (int n = 0; n < kN; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x = umax(x, mag(M[n][i]));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y = umax(y, mag(v[i]));
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      x = umax(x, (uint32_t)__shfl_xor((int)x, o));
-      y = umax(y, (uint32_t)__shfl_xor((int)y, o));
-    }
-    if (lane == 0) {
-      lds.c.top[w][0] = x;
-      lds.c.top[w][1] = y;
-    }
-  };
   constexpr float kRoot = kD == 64 ? 8.1f : kD == 128 ? 11.4f : 16.1f;  // above sqrt(d)
   float mtop, vtop;
   bool odd;
@@ -599,141 +556,287 @@ __global__ __launch_bounds__(256) void state_kernel(ChunkArgs a) {
     vtop = __builtin_bit_cast(float, y);
     odd = x > 0x6C800000u || y > 0x6C800000u;  // 2^90
   };
-  auto put_m = [&](float up) {
+  // Scales of a chunk. R and U: the state's rows have norms up to sqrt(d) mtop, to which each
+  // token adds vtop. The next state's, from this chunk's bounds: it is split before its
+  // largest value is known to all waves.
+  const auto exp_u = [&]() { return scale_exp(fmaf(65.0f, vtop, kRoot * mtop)); };
+  const auto exp_m = [&]() { return scale_exp(fmaf(64.0f, vtop, kRoot * mtop)); };
+  // four values' parts as half of a B fragment
+  const auto put4 = [&](h4 (*to)[64][2], const f4 &x) {
+    h4 hi, lo;
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      h4 hi, lo;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        _Float16 x, y;
-        split(M[n][i] * up, x, y);
-        hi[i] = x;
-        lo[i] = y;
-      }
-      const int at = w * kN + n;
-      reinterpret_cast<h4 *>(&lds.c.m[at >> 1][0][lane])[at & 1] = hi;
-      reinterpret_cast<h4 *>(&lds.c.m[at >> 1][1][lane])[at & 1] = lo;
+    for (int i = 0; i < 4; ++i) {
+      _Float16 p, q;
+      split(x[i], p, q);
+      hi[i] = p;
+      lo[i] = q;
     }
+    to[0][lane][w & 1] = hi;
+    to[1][lane][w & 1] = lo;
   };
-  put_top();
-  __syncthreads();
-  get_top();
-  odd = odd || lds.c.odd != 0u;
-  int em = scale_exp(mtop);
-  if (!odd) put_m(pow2(em));
-  lds_barrier();
+  const f4 zero = {0.f, 0.f, 0.f, 0.f};
 
-  for (int c = 0; c < chunks && !odd; ++c) {
-    const int64_t next = c + 1 < chunks ? c + 1 : c;
-    // R and U: the state's rows have norms up to sqrt(d) mtop, to which each token adds vtop
-    const int eu = scale_exp(fmaf(65.0f, vtop, kRoot * mtop));
-    const int em1 = scale_exp(fmaf(64.0f, vtop, kRoot * mtop));  // of the next chunk's state
-    const float up = pow2(eu);
-    // ---- K M and Q M of the wave's tokens
-    f4 km = f4{0.f, 0.f, 0.f, 0.f}, kx = km, qm = km, qx = km;
+  if (wave < 4) {
+    const h8 *kw = a.w.k + (key0 * 4 + w) * kS * kFrag + lane;
+    const h8 *ktw = a.w.kt + (key0 * (kD / 16) + w * kN) * 2 * kFrag + lane;
+    const h8 *tw = a.w.t + (val0 * 6 + tri(w, 0)) * kFrag + lane;
+    const float *vp = a.s.v + b * a.s.vb + tok * a.s.vt + h * kD + row0 + m;
+    float *state = a.s.state + ((b * a.s.heads + h) * kD + row0 + m) * kD + w * (kD / 4) + 4 * g;
+    h8 ka[kS][2], kb[kDeep ? kS : 1][2], ktf[kN][2][2], tf[2][2];
+    f4 v, be, eg, ec;
+    float whole;
+    const auto load_k = [&](int c, h8 (*f)[2]) {
+      const h8 *p = kw + (c < chunks ? c : chunks - 1) * kstep;
 #pragma unroll
-    for (int s = 0; s < kS; ++s) {
-      const h8 hi = lds.c.m[s][0][lane], lo = lds.c.m[s][1][lane];
-      km = mfma(kf[s][0], hi, km);
-      qm = mfma(qf[s][0], hi, qm);
-      kx = mfma(kf[s][0], lo, kx);
-      qx = mfma(qf[s][0], lo, qx);
-      kx = mfma(kf[s][1], hi, kx);
-      qx = mfma(qf[s][1], hi, qx);
-    }
-    load_k(next);
-    const float dm = kDown * pow2(-em);
-    h4 hi4, lo4;
+      for (int s = 0; s < kS; ++s)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float r = be[i] * (v[i] - eg[i] * ((km[i] + kx[i]) * dm));
-      _Float16 x, y;
-      split(r * up, x, y);
-      hi4[i] = x;
-      lo4[i] = y;
-    }
-    lds.c.r[w >> 1][0][lane][w & 1] = hi4;
-    lds.c.r[w >> 1][1][lane][w & 1] = lo4;
-    load_v(next);
-    lds_barrier();
-    // ---- U = T R
-    f4 u = f4{0.f, 0.f, 0.f, 0.f}, ux = u;
+        for (int u = 0; u < 2; ++u) f[s][u] = p[s * kFrag + 64 * u];
+    };
+    const auto load_t = [&](int c) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      if (p > w >> 1) continue;
-      const h8 hi = *reinterpret_cast<const h8 *>(lds.c.r[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.r[p][1][lane]);
-      u = mfma(tf[p][0], hi, u);
-      ux = mfma(tf[p][0], lo, ux);
-      ux = mfma(tf[p][1], hi, ux);
-    }
-    load_t(next);
-    h4 hc, lc;
+      for (int p = 0; p < 2; ++p)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float z = (u[i] + ux[i]) * kDown;  // 2^eu U
-      _Float16 x, y;
-      split(z, x, y);
-      hi4[i] = x;
-      lo4[i] = y;
-      split(z * ec[i], x, y);
-      hc[i] = x;
-      lc[i] = y;
-    }
-    lds.c.u[w >> 1][0][lane][w & 1] = hi4;
-    lds.c.u[w >> 1][1][lane][w & 1] = lo4;
-    lds.c.v[w >> 1][0][lane][w & 1] = hc;
-    lds.c.v[w >> 1][1][lane][w & 1] = lc;
-    lds_barrier();
-    // ---- the next state, then the outputs
-    f4 n0[kN], nx[kN];
+        for (int u = 0; u < 2; ++u)
+          if (p <= w >> 1) tf[p][u] = tw[c * tstep + p * kFrag + 64 * u];
+    };
+    const auto load_kt = [&](int c) {
 #pragma unroll
-    for (int n = 0; n < kN; ++n) n0[n] = nx[n] = f4{0.f, 0.f, 0.f, 0.f};
-    f4 o = f4{0.f, 0.f, 0.f, 0.f}, ox = o;
+      for (int n = 0; n < kN; ++n)
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const h8 hi = *reinterpret_cast<const h8 *>(lds.c.v[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.v[p][1][lane]);
+        for (int p = 0; p < 2; ++p)
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        n0[n] = mfma(ktf[n][p][0], hi, n0[n]);
-        nx[n] = mfma(ktf[n][p][0], lo, nx[n]);
-        nx[n] = mfma(ktf[n][p][1], hi, nx[n]);
-      }
-      if (p > w >> 1) continue;
-      const h8 uh = *reinterpret_cast<const h8 *>(lds.c.u[p][0][lane]), ul = *reinterpret_cast<const h8 *>(lds.c.u[p][1][lane]);
-      o = mfma(pf[p][0], uh, o);
-      ox = mfma(pf[p][0], ul, ox);
-      ox = mfma(pf[p][1], uh, ox);
-    }
-    load_p(next);
-    const float du = kDown * pow2(-eu);
-#pragma unroll
-    for (int n = 0; n < kN; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) M[n][i] = fmaf(M[n][i], whole, (n0[n][i] + nx[n][i]) * du);
-    put_m(pow2(em1));
-    put_top();
-    {
-      const int64_t t = a.first + (int64_t)c * kC + 16 * w + 4 * g;
+          for (int u = 0; u < 2; ++u) ktf[n][p][u] = ktw[c * kstep + (n * 2 + p) * kFrag + 64 * u];
+    };
+    const auto load_v = [&](int c, f4 &x) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (t + i < end)
-          op[(t + i) * a.s.heads * kD] = a.s.scale * fmaf(eg[i], (qm[i] + qx[i]) * dm, (o[i] + ox[i]) * du);
-    }
-    load_meta(next);
-    em = em1;
-    lds_barrier();
+        x[i] = tok + (int64_t)c * kC + i < end ? vp[((int64_t)c * kC + i) * a.s.vt] : 0.0f;
+    };
+    const auto load_meta = [&](int c, f4 &x, f4 &y, f4 &z, float &all) {
+      const float *p = meta + c * mstep;
+      x = *reinterpret_cast<const f4 *>(p);
+      y = *reinterpret_cast<const f4 *>(p + kC);
+      z = *reinterpret_cast<const f4 *>(p + 2 * kC);
+      all = p[2 * kC - 1 - (16 * w + 4 * g)];  // e^(G_63)
+    };
+    load_meta(0, be, eg, ec, whole);
+    load_v(0, v);
+    load_k(0, ka);
+    if constexpr (kDeep) load_k(1, kb);
+    load_t(0);
+    load_kt(0);
+    f4 M[kN];
+#pragma unroll
+    for (int n = 0; n < kN; ++n) M[n] = *reinterpret_cast<const f4 *>(state + 16 * n);
+    // largest |M| and |v| of the wave: as integers, so that a NaN is larger than everything
+    const auto put_top = [&]() {
+      uint32_t x = 0u, y = 0u;
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x = umax(x, mag(M[n][i]));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y = umax(y, mag(v[i]));
+      x = wave_max(x);
+      y = wave_max(y);
+      if (lane == 0) {
+        lds.c.top[w][0] = x;
+        lds.c.top[w][1] = y;
+      }
+    };
+    const auto put_m = [&](float up) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        h4 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          _Float16 x, y;
+          split(M[n][i] * up, x, y);
+          hi[i] = x;
+          lo[i] = y;
+        }
+        const int at = w * kN + n;
+        reinterpret_cast<h4 *>(&lds.c.m[at >> 1][0][lane])[at & 1] = hi;
+        reinterpret_cast<h4 *>(&lds.c.m[at >> 1][1][lane])[at & 1] = lo;
+      }
+    };
+    put_top();
+    __syncthreads();
     get_top();
+    odd = odd || lds.c.odd != 0u;
+    int em = scale_exp(mtop);
+    if (!odd) put_m(pow2(em));
+    lds_barrier();
+
+    const auto step = [&](int c, h8 (*kf)[2]) {
+      const int next = c + 1 < chunks ? c + 1 : c;
+      f4 vn, bn, gn, cn;
+      float wn;
+      load_meta(next, bn, gn, cn, wn);
+      load_v(next, vn);
+      const int eu = exp_u(), em1 = exp_m();
+      // ---- R = be (V - e^G K M)
+      f4 km = zero, kx = zero, ky = zero;
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        const h8 hi = lds.c.m[s][0][lane], lo = lds.c.m[s][1][lane];
+        km = mfma(kf[s][0], hi, km);
+        kx = mfma(kf[s][0], lo, kx);
+        ky = mfma(kf[s][1], hi, ky);
+      }
+      load_k(c + (kDeep ? 2 : 1), kf);
+      const float dm = kDown * pow2(-em), up = pow2(eu);
+      f4 r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = (be[i] * up) * (v[i] - eg[i] * ((km[i] + (kx[i] + ky[i])) * dm));
+      put4(lds.c.r[w >> 1], r);
+      lds_barrier();
+      // ---- U = T R, times 2^eu
+      f4 u = zero, ux = zero, uy = zero;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        if (p > w >> 1) continue;
+        const h8 hi = *reinterpret_cast<const h8 *>(lds.c.r[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.r[p][1][lane]);
+        u = mfma(tf[p][0], hi, u);
+        ux = mfma(tf[p][0], lo, ux);
+        uy = mfma(tf[p][1], hi, uy);
+      }
+      load_t(next);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = (u[i] + (ux[i] + uy[i])) * kDown;
+      put4(lds.c.u[w >> 1], u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] *= ec[i];
+      put4(lds.c.v[w >> 1], u);
+      lds_barrier();
+      // ---- the next state
+      f4 n0[kN], nx[kN], ny[kN];
+#pragma unroll
+      for (int n = 0; n < kN; ++n) n0[n] = nx[n] = ny[n] = zero;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const h8 hi = *reinterpret_cast<const h8 *>(lds.c.v[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.v[p][1][lane]);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          n0[n] = mfma(ktf[n][p][0], hi, n0[n]);
+          nx[n] = mfma(ktf[n][p][0], lo, nx[n]);
+          ny[n] = mfma(ktf[n][p][1], hi, ny[n]);
+        }
+      }
+      load_kt(next);
+      const float du = kDown * pow2(-eu);
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) M[n][i] = fmaf(M[n][i], whole, (n0[n][i] + (nx[n][i] + ny[n][i])) * du);
+      put_m(pow2(em1));
+      v = vn;
+      be = bn;
+      eg = gn;
+      ec = cn;
+      whole = wn;
+      em = em1;
+      put_top();
+      lds_barrier();
+      get_top();
+    };
+    if constexpr (kDeep) {
+      for (int c = 0; c < chunks && !odd; c += 2) {
+        step(c, ka);
+        if (c + 1 < chunks && !odd) step(c + 1, kb);
+      }
+    } else {
+      for (int c = 0; c < chunks && !odd; ++c) step(c, ka);
+    }
+    if (!odd) {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) *reinterpret_cast<f4 *>(state + 16 * n) = M[n];
+    }
+  } else {
+    const h8 *qw = a.w.q + (key0 * 4 + w) * kS * kFrag + lane;
+    const h8 *pw = a.w.p + (val0 * 6 + tri(w, 0)) * kFrag + lane;
+    float *op = a.s.out + ((b * a.s.n + tok) * a.s.heads + h) * kD + row0 + m;
+    h8 qa[kS][2], qb[kDeep ? kS : 1][2], pf[2][2];
+    f4 eg;
+    const auto load_q = [&](int c, h8 (*f)[2]) {
+      const h8 *p = qw + (c < chunks ? c : chunks - 1) * kstep;
+#pragma unroll
+      for (int s = 0; s < kS; ++s)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) f[s][u] = p[s * kFrag + 64 * u];
+    };
+    const auto load_p = [&](int c) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          if (p <= w >> 1) pf[p][u] = pw[c * tstep + p * kFrag + 64 * u];
+    };
+    eg = *reinterpret_cast<const f4 *>(meta + kC);
+    load_q(0, qa);
+    if constexpr (kDeep) load_q(1, qb);
+    load_p(0);
+    __syncthreads();
+    get_top();
+    odd = odd || lds.c.odd != 0u;
+    int em = scale_exp(mtop);
+    lds_barrier();
+
+    const auto step = [&](int c, h8 (*qf)[2]) {
+      const int next = c + 1 < chunks ? c + 1 : c;
+      const f4 gn = *reinterpret_cast<const f4 *>(meta + next * mstep + kC);
+      const int eu = exp_u(), em1 = exp_m();
+      f4 qm = zero, qx = zero, qy = zero;
+#pragma unroll
+      for (int s = 0; s < kS; ++s) {
+        const h8 hi = lds.c.m[s][0][lane], lo = lds.c.m[s][1][lane];
+        qm = mfma(qf[s][0], hi, qm);
+        qx = mfma(qf[s][0], lo, qx);
+        qy = mfma(qf[s][1], hi, qy);
+      }
+      load_q(c + (kDeep ? 2 : 1), qf);
+      const float dm = kDown * pow2(-em) * a.s.scale, du = kDown * pow2(-eu) * a.s.scale;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qm[i] = eg[i] * ((qm[i] + (qx[i] + qy[i])) * dm);
+      lds_barrier();
+      lds_barrier();
+      f4 o = zero, ox = zero, oy = zero;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        if (p > w >> 1) continue;
+        const h8 hi = *reinterpret_cast<const h8 *>(lds.c.u[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.u[p][1][lane]);
+        o = mfma(pf[p][0], hi, o);
+        ox = mfma(pf[p][0], lo, ox);
+        oy = mfma(pf[p][1], hi, oy);
+      }
+      load_p(next);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (tok + (int64_t)c * kC + i < end)
+          op[((int64_t)c * kC + i) * a.s.heads * kD] = fmaf(o[i] + (ox[i] + oy[i]), du, qm[i]);
+      eg = gn;
+      em = em1;
+      lds_barrier();
+      get_top();
+    };
+    if constexpr (kDeep) {
+      for (int c = 0; c < chunks && !odd; c += 2) {
+        step(c, qa);
+        if (c + 1 < chunks && !odd) step(c + 1, qb);
+      }
+    } else {
+      for (int c = 0; c < chunks && !odd; ++c) step(c, qa);
+    }
   }
   if (odd) {
     __syncthreads();
+    if (wave >= 4) return;  // a wave that has ended takes no part in the barriers below
     scan_tokens<kD>(a.s, lds.t, b, h, row0, a.first, end);
     return;
   }
-#pragma unroll
-  for (int n = 0; n < kN; ++n) *reinterpret_cast<f4 *>(state + 16 * n) = M[n];
   if (a.s.gate_offset != nullptr && row0 == 0 && tid == 0) {
     double sum = (double)a.s.gate_offset[b * a.s.heads + h];
-    for (int c = 0; c < chunks; ++c) sum += a.w.gates[(b * a.chunks + c) * a.s.heads + h];
+    for (int c = 0; c < chunks; ++c) sum += a.w.gates[val0 + (int64_t)c * a.s.heads];
     a.s.gate_offset[b * a.s.heads + h] = (float)sum;
   }
 }
@@ -784,7 +887,7 @@ int launch(const ScanArgs &a, const SegmentPlan &plan, int batch, int k_heads, v
     hipLaunchKernelGGL((chunk_kernel<kD>), dim3((unsigned)ca.chunks, (unsigned)k_heads, (unsigned)batch),
                        dim3(256), 0, s, ca);
     PKV_HIP(hipGetLastError());
-    hipLaunchKernelGGL((state_kernel<kD>), dim3((unsigned)(batch * a.heads * (kD / 16))), dim3(256), 0, s, ca);
+    hipLaunchKernelGGL((state_kernel<kD>), dim3((unsigned)(batch * a.heads * (kD / 16))), dim3(512), 0, s, ca);
     PKV_HIP(hipGetLastError());
   }
   return PKV_OK;

@@ -23,7 +23,7 @@
 // NaN then reaches the tokens behind it and no others, as there).
 #include <type_traits>
 
-#include "pkv_internal.hpp"
+#include "pkv_q8_common.hpp"
 
 namespace pkv {
 namespace {
@@ -189,12 +189,6 @@ constexpr int kC = 64;           // tokens per chunk
 constexpr float kUp = 1024.0f;   // scale of the fp16 parts of k, q, T and P (at most 1)
 constexpr float kDown = 1.0f / 1024.0f;
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
 // The empty asm pins x: where x is a product, the compiler otherwise rounds one use of hi from
 // the exact product (v_fma_mixlo_f16) and another from its f32 value; now and then the two
 // differ by a step of hi, which lo then does not make up for (a value off by 2^-12).
@@ -227,6 +221,31 @@ struct ChunkArgs {
 };
 __device__ __forceinline__ int tri(int w, int p) { return w < 2 ? w : 2 * w - 2 + p; }
 
+__device__ __forceinline__ double read_lane(double x, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
+// Sums of x over the lanes up to each one, in 64 bits: DPP shifts within rows of 16 lanes
+// (0 comes in), then the rows in front.
+__device__ __forceinline__ double prefix64(float x) {
+  double G = (double)x;
+  const auto add = [&](auto ctrl) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, G);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, decltype(ctrl)::value, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), decltype(ctrl)::value, 0xF, 0xF, true);
+    G += __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+  };
+  add(std::integral_constant<int, 0x111>{});  // row_shr:1, 2, 4, 8
+  add(std::integral_constant<int, 0x112>{});
+  add(std::integral_constant<int, 0x114>{});
+  add(std::integral_constant<int, 0x118>{});
+  const double a = read_lane(G, 15), b = read_lane(G, 31), c = read_lane(G, 47);
+  const int row = (threadIdx.x >> 4) & 3;
+  return G + (row == 0 ? 0.0 : row == 1 ? a : row == 2 ? a + b : (a + b) + c);
+}
+
 // A chunk of one key head: normalised K and Q as fragments, their products, and for each of
 // its value heads T and P. A wave owns 16 tokens, its lanes load q and k in fragment order;
 // the waves take each other's K from LDS. T = (I + A)^-1 by blocks of 16, in f32: the
@@ -238,8 +257,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
   constexpr int kS = kD / 32, kRow = kD + 8, kSq = 68;
   constexpr int kKB = 2 * kC * kRow * 2, kAB = 4 * kC * kSq * 4;
   __shared__ __attribute__((aligned(16))) char lds[kKB > kAB ? kKB : kAB];
-  __shared__ double gam[2][kC];
-  __shared__ float bet[2][kC];
+  __shared__ float4 gam[2][kC];  // a token's sum of gates (base 2) in two parts, be
   __shared__ unsigned bad;
   _Float16(*kh)[kC][kRow] = reinterpret_cast<_Float16(*)[kC][kRow]>(lds);  // [hi, lo][token][k]
   float(*am)[kC][kSq] = reinterpret_cast<float(*)[kC][kSq]>(lds);           // A of two heads, then P and T of both
@@ -249,6 +267,15 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
   const int64_t left = valid_tokens(a.s.lens, b, a.s.n) - t0;
   if (left <= 0) return;
   if (tid == 0) bad = 0u;
+  // the gates of the first two value heads, a wave each, asked for before everything else
+  float gv = 0.0f, bv = 0.0f;
+  const auto load_gates = [&](int r) {
+    const int64_t at = (b * a.s.n + t0 + lane) * a.s.heads + hk * a.s.rep + r + w;
+    const bool on = w < 2 && r + w < a.s.rep && lane < left;
+    gv = on ? a.s.gate[at] : 0.0f;
+    bv = on ? a.s.beta[at] : 0.0f;
+  };
+  load_gates(0);
   const int64_t slot = (b * a.chunks + chunk) * a.k_heads + hk;
 
   // ---- q and k of token t0 + 16 w + m
@@ -324,10 +351,10 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
         const h4 y = *reinterpret_cast<const h4 *>(&kh[u][16 * j + m][32 * s + 16 + 4 * g]);
         bf[u] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
       }
-      kk[j] = mfma(kf[s][0], bf[0], kk[j]);
-      qk[j] = mfma(qf[s][0], bf[0], qk[j]);
-      kx = mfma(kf[s][1], bf[0], mfma(kf[s][0], bf[1], kx));
-      qx = mfma(qf[s][1], bf[0], mfma(qf[s][0], bf[1], qx));
+      kk[j] = mfma32(kf[s][0], bf[0], kk[j]);
+      qk[j] = mfma32(qf[s][0], bf[0], qk[j]);
+      kx = mfma32(kf[s][1], bf[0], mfma32(kf[s][0], bf[1], kx));
+      qx = mfma32(qf[s][1], bf[0], mfma32(qf[s][0], bf[1], qx));
     }
     kk[j] = (kk[j] + kx) * (kDown * kDown);
     qk[j] = (qk[j] + qx) * (kDown * kDown);
@@ -353,42 +380,39 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
     const int64_t out = (b * a.chunks + chunk) * a.s.heads + h0;
     __syncthreads();  // kh, or the heads before, are done with; bad is set
     if (w < heads) {
-      const bool on = lane < left;
-      const int64_t at = (b * a.s.n + t0 + (on ? lane : 0)) * a.s.heads + h0 + w;
-      const float gv = on ? a.s.gate[at] : 0.0f, bv = on ? a.s.beta[at] : 0.0f;
-      const bool odd = !(gv <= 0.0f) || bv != bv;
-      // e^-10000 is 0: a smaller gate does the same
-      double G = (double)fmaxf(gv, -10000.0f), sum = on && !odd ? (double)gv : 0.0;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(G, o);
-        G += lane >= o ? up : 0.0;
-        sum += __shfl_xor(sum, o);
-      }
-      const double last = __shfl(G, 63);
-      const float be = on ? 1.0f / (1.0f + expf(-bv)) : 0.0f;
-      gam[w][lane] = G;
-      bet[w][lane] = be;
+      // e^-10000 is 0, but its sums would leave no bits for the others: the token path's
+      const bool fit = gv <= 0.0f && gv >= -10000.0f && bv == bv;
+      const double G = prefix64(gv), last = read_lane(G, 63);
+      const float be = lane < left ? 1.0f / (1.0f + expf(-bv)) : 0.0f;
+      const double G2 = G * 1.4426950408889634;
+      const float hi = (float)G2;
+      gam[w][lane] = float4{hi, (float)(G2 - (double)hi), be, 0.0f};
       float *meta = a.w.meta + (out + w) * 3 * kC + lane;
       meta[0] = be;
       meta[kC] = expf((float)G);
       meta[2 * kC] = expf((float)(last - G));
-      const bool any = __ballot(odd) != 0;
+      const bool all = __ballot(!fit) == 0;
       if (lane == 0) {
-        a.w.gates[out + w] = sum;
-        a.w.odd[out + w] = any || bad != 0u ? 1u : 0u;
+        a.w.gates[out + w] = last;
+        a.w.odd[out + w] = all && bad == 0u ? 0u : 1u;
       }
     }
     __syncthreads();
+    load_gates(r0 + 2);
     for (int e = 0; e < heads; ++e) {
+      float4 row[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) row[i] = gam[e][16 * w + 4 * g + i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (j > (w | 1)) continue;  // a fragment covers two tiles
+        const float4 col = gam[e][16 * j + m];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          // 2^(G_t - G_s): the difference of the high parts is rounded once, as it is itself
           const int t = 16 * w + 4 * g + i, s = 16 * j + m;
-          const float dec = s <= t ? expf((float)(gam[e][t] - gam[e][s])) : 0.0f;
-          am[e][t][s] = s < t ? bet[e][t] * dec * kk[j][i] : 0.0f;
+          const float dec = __builtin_amdgcn_exp2f((row[i].x - col.x) + (row[i].y - col.y));
+          am[e][t][s] = s < t ? row[i].z * dec * kk[j][i] : 0.0f;
           am[2 + e][t][s] = s <= t ? dec * qk[j][i] : 0.0f;
         }
       }
@@ -457,7 +481,11 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
           for (int c = 0; c < 4; ++c) y = __builtin_amdgcn_mfma_f32_16x16x4f32(row[c], x[c], y, 0, 0, 0);
           T[i] = -y;
         }
-        // over P, whose zeros above the diagonal are T's too
+      }
+      // over P, whose zeros above the diagonal are T's too
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < j) continue;
 #pragma unroll
         for (int c = 0; c < 4; ++c) am[2 + e][16 * i + 4 * g + c][16 * j + m] = T[i][c];
       }
@@ -467,12 +495,6 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
   }
 }
 
-// Barrier that orders LDS only: loads of the next chunk stay in flight.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
 __device__ __forceinline__ uint32_t mag(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
 __device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
@@ -488,6 +510,13 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
   const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   return umax(b[0], b[1]);
 }
+// the largest magnitude of eight fp16 values, as bits (a NaN is larger than everything)
+__device__ __forceinline__ uint32_t top16(h8 x) {
+  uint32_t t = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t = umax(t, (uint32_t)__builtin_bit_cast(uint16_t, x[i]) & 0x7FFFu);
+  return t;
+}
 // The exponent that takes values up to `bound` (finite) below 2^15.
 __device__ __forceinline__ int scale_exp(float bound) {
   const int e = 14 - ((int)(__builtin_bit_cast(uint32_t, bound) >> 23) - 127);
@@ -499,24 +528,40 @@ template <int kD>
 union StateLds {
   struct {
     h8 m[kD / 32][2][64];   // the state's fragments
-    h4 r[2][2][64][2], u[2][2][64][2], v[2][2][64][2];  // R, U and U e^(G_63 - G): [k step][part][lane][half]
-    uint32_t top[4][2];     // largest |M| and |v| of each wave
+    uint2 r[2][2][64][2], u[2][2][64][2], v[2][2][64][2];  // R, U, U e^(G_63 - G): [k step][part][lane][half]
+    uint32_t top[2][3][4];  // [chunk's parity][maximum][wave], bits of magnitudes
     unsigned odd;
   } c;
   TokenStage<kD> t;
 };
 
+// One load at a wave-uniform address and a lane's byte offset.
+template <typename T>
+__device__ __forceinline__ T at(const void *base, uint32_t off) {
+  return *reinterpret_cast<const T *>(static_cast<const char *>(base) + off);
+}
+// Four values (not MFMA results themselves: lo_pair is inline asm) as fp16 parts.
+__device__ __forceinline__ void split4(const f4 &x, uint2 &hi, uint2 &lo) {
+  float y[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("" : "+v"(y[i]));
+  hi = uint2{as_u(h2{(_Float16)y[0], (_Float16)y[1]}), as_u(h2{(_Float16)y[2], (_Float16)y[3]})};
+  lo = uint2{lo_pair(y[0], y[1], hi.x), lo_pair(y[2], y[3], hi.y)};
+}
+
 // The chunks of 16 value channels of one head, in order, by eight waves. Waves 0 - 3 carry the
 // state: wave w owns key channels w d / 4 .. of it (f32, in an MFMA result's layout) and
 // tokens 16 w .. of each chunk. Waves 4 - 7 make the outputs of the same tokens beside them, off
-// the path from one chunk to the next. A wave loads its fragments of the next chunk (K and Q:
-// of the one after, where the registers hold both) when a stage has just used them.
+// the path from one chunk to the next, and the bounds that the scales come from. A wave
+// loads its fragments of the next chunk (K and Q: of the one after, where the registers hold
+// both) when a stage has just used them.
 template <int kD>
 __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   constexpr int kS = kD / 32, kN = kD / 64;
   constexpr bool kDeep = kD <= 128;
   __shared__ __attribute__((aligned(16))) StateLds<kD> lds;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, w = wave & 3, m = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3;
   // the workgroups of a key head share an XCD and its L2 (workgroups go to the 8 XCDs in turn)
   const int groups = a.batch * a.k_heads, per = a.s.rep * (kD / 16);
   int grp, in;
@@ -534,53 +579,57 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   const int64_t stop = a.first + (int64_t)a.chunks * kC;
   end = end < stop ? end : stop;
   if (end <= a.first) return;
-  const int chunks = (int)((end - a.first + kC - 1) / kC);
+  const int tokens = (int)(end - a.first), chunks = (tokens + kC - 1) / kC;
   const int64_t kstep = (int64_t)a.k_heads * 4 * kS * kFrag, tstep = (int64_t)a.s.heads * 6 * kFrag;
   const int64_t key0 = b * a.chunks * a.k_heads + hk, val0 = b * a.chunks * a.s.heads + h;
-  const float *meta = a.w.meta + val0 * 3 * kC + 16 * w + 4 * g;
   const int64_t mstep = (int64_t)a.s.heads * 3 * kC;
-  const int64_t tok = a.first + 16 * w + 4 * g;  // the lane's first token of chunk 0
+  const float *meta = a.w.meta + val0 * 3 * kC;
+  const float *v0 = a.s.v + b * a.s.vb + a.first * a.s.vt + h * kD + row0;
+  const uint32_t moff = 4u * (uint32_t)(16 * w + 4 * g), foff = 16u * (uint32_t)lane;
+  // v of the lane's four tokens; past the end the last token's, whose weight there is 0
+  const auto load_v = [&](int c) {
+    const float *p = v0 + (int64_t)c * kC * a.s.vt;
+    const int last = (tokens - c * kC < kC ? tokens - c * kC : kC) - 1;
+    f4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 16 * w + 4 * g + i < last ? 16 * w + 4 * g + i : last;
+      x[i] = at<float>(p, 4u * ((uint32_t)t * (uint32_t)a.s.vt + (uint32_t)m));
+    }
+    return x;
+  };
 
   if (tid == 0) lds.c.odd = 0u;
   __syncthreads();
   for (int c = tid; c < chunks; c += 512)
     if (a.w.odd[val0 + (int64_t)c * a.s.heads] != 0u) lds.c.odd = 1u;
 
+  // The scales of a chunk come from bounds: a row of the state has a norm of at most `root`
+  // = sqrt(d) max |M| of the chunk before + 64 max |v| of that chunk, and each token of this
+  // one adds its |v| at most. So R and U stay below root + 65 max |v|, the next state below
+  // root + 64 max |v|. Waves 4 - 7 find the maxima beside the others' work: top[0] of M in
+  // front of the chunk before, top[1] and top[2] of v in that chunk and in this one.
   constexpr float kRoot = kD == 64 ? 8.1f : kD == 128 ? 11.4f : 16.1f;  // above sqrt(d)
-  float mtop, vtop;
   bool odd;
-  auto get_top = [&]() {
-    const uint32_t x = umax(umax(lds.c.top[0][0], lds.c.top[1][0]), umax(lds.c.top[2][0], lds.c.top[3][0]));
-    const uint32_t y = umax(umax(lds.c.top[0][1], lds.c.top[1][1]), umax(lds.c.top[2][1], lds.c.top[3][1]));
-    mtop = __builtin_bit_cast(float, x);
-    vtop = __builtin_bit_cast(float, y);
-    odd = x > 0x6C800000u || y > 0x6C800000u;  // 2^90
-  };
-  // Scales of a chunk. R and U: the state's rows have norms up to sqrt(d) mtop, to which each
-  // token adds vtop. The next state's, from this chunk's bounds: it is split before its
-  // largest value is known to all waves.
-  const auto exp_u = [&]() { return scale_exp(fmaf(65.0f, vtop, kRoot * mtop)); };
-  const auto exp_m = [&]() { return scale_exp(fmaf(64.0f, vtop, kRoot * mtop)); };
-  // four values' parts as half of a B fragment
-  const auto put4 = [&](h4 (*to)[64][2], const f4 &x) {
-    h4 hi, lo;
+  int eu, em1;
+  const auto get_scales = [&](int c) {
+    uint32_t x[3];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      _Float16 p, q;
-      split(x[i], p, q);
-      hi[i] = p;
-      lo[i] = q;
-    }
-    to[0][lane][w & 1] = hi;
-    to[1][lane][w & 1] = lo;
+    for (int k = 0; k < 3; ++k)
+      x[k] = umax(umax(lds.c.top[c & 1][k][0], lds.c.top[c & 1][k][1]), umax(lds.c.top[c & 1][k][2], lds.c.top[c & 1][k][3]));
+    odd = odd || umax(umax(x[0], x[1]), x[2]) > 0x6C800000u;  // 2^90
+    const float root = fmaf(kRoot, __builtin_bit_cast(float, x[0]), 64.0f * __builtin_bit_cast(float, x[1]));
+    const float vtop = __builtin_bit_cast(float, x[2]);
+    eu = __builtin_amdgcn_readfirstlane(scale_exp(fmaf(65.0f, vtop, root)));
+    em1 = __builtin_amdgcn_readfirstlane(scale_exp(fmaf(64.0f, vtop, root)));
   };
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
+  odd = false;
 
   if (wave < 4) {
-    const h8 *kw = a.w.k + (key0 * 4 + w) * kS * kFrag + lane;
-    const h8 *ktw = a.w.kt + (key0 * (kD / 16) + w * kN) * 2 * kFrag + lane;
-    const h8 *tw = a.w.t + (val0 * 6 + tri(w, 0)) * kFrag + lane;
-    const float *vp = a.s.v + b * a.s.vb + tok * a.s.vt + h * kD + row0 + m;
+    const h8 *kw = a.w.k + (key0 * 4 + w) * kS * kFrag;
+    const h8 *ktw = a.w.kt + (key0 * (kD / 16) + w * kN) * 2 * kFrag;
+    const h8 *tw = a.w.t + (val0 * 6 + tri(w, 0)) * kFrag;
     float *state = a.s.state + ((b * a.s.heads + h) * kD + row0 + m) * kD + w * (kD / 4) + 4 * g;
     h8 ka[kS][2], kb[kDeep ? kS : 1][2], ktf[kN][2][2], tf[2][2];
     f4 v, be, eg, ec;
@@ -590,37 +639,34 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 #pragma unroll
       for (int s = 0; s < kS; ++s)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) f[s][u] = p[s * kFrag + 64 * u];
+        for (int u = 0; u < 2; ++u) f[s][u] = at<h8>(p + s * kFrag + 64 * u, foff);
     };
     const auto load_t = [&](int c) {
+      const h8 *q = tw + c * tstep;
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          if (p <= w >> 1) tf[p][u] = tw[c * tstep + p * kFrag + 64 * u];
+          if (p <= w >> 1) tf[p][u] = at<h8>(q + p * kFrag + 64 * u, foff);
     };
     const auto load_kt = [&](int c) {
+      const h8 *q = ktw + c * kstep;
 #pragma unroll
       for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) ktf[n][p][u] = ktw[c * kstep + (n * 2 + p) * kFrag + 64 * u];
-    };
-    const auto load_v = [&](int c, f4 &x) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[i] = tok + (int64_t)c * kC + i < end ? vp[((int64_t)c * kC + i) * a.s.vt] : 0.0f;
+          for (int u = 0; u < 2; ++u) ktf[n][p][u] = at<h8>(q + (n * 2 + p) * kFrag + 64 * u, foff);
     };
     const auto load_meta = [&](int c, f4 &x, f4 &y, f4 &z, float &all) {
       const float *p = meta + c * mstep;
-      x = *reinterpret_cast<const f4 *>(p);
-      y = *reinterpret_cast<const f4 *>(p + kC);
-      z = *reinterpret_cast<const f4 *>(p + 2 * kC);
-      all = p[2 * kC - 1 - (16 * w + 4 * g)];  // e^(G_63)
+      x = at<f4>(p, moff);
+      y = at<f4>(p + kC, moff);
+      z = at<f4>(p + 2 * kC, moff);
+      all = at<float>(p + 2 * kC - 1, 0u);  // e^(G_63)
     };
     load_meta(0, be, eg, ec, whole);
-    load_v(0, v);
+    v = load_v(0);
     load_k(0, ka);
     if constexpr (kDeep) load_k(1, kb);
     load_t(0);
@@ -628,8 +674,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     f4 M[kN];
 #pragma unroll
     for (int n = 0; n < kN; ++n) M[n] = *reinterpret_cast<const f4 *>(state + 16 * n);
-    // largest |M| and |v| of the wave: as integers, so that a NaN is larger than everything
-    const auto put_top = [&]() {
+    {  // the first chunk's maxima: of M in front of it (nothing before adds to it) and of v
       uint32_t x = 0u, y = 0u;
 #pragma unroll
       for (int n = 0; n < kN; ++n)
@@ -640,55 +685,54 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
       x = wave_max(x);
       y = wave_max(y);
       if (lane == 0) {
-        lds.c.top[w][0] = x;
-        lds.c.top[w][1] = y;
+        lds.c.top[0][0][w] = x;
+        lds.c.top[0][1][w] = 0u;
+        lds.c.top[0][2][w] = y;
       }
-    };
+    }
     const auto put_m = [&](float up) {
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        h4 hi, lo;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          _Float16 x, y;
-          split(M[n][i] * up, x, y);
-          hi[i] = x;
-          lo[i] = y;
-        }
-        const int at = w * kN + n;
-        reinterpret_cast<h4 *>(&lds.c.m[at >> 1][0][lane])[at & 1] = hi;
-        reinterpret_cast<h4 *>(&lds.c.m[at >> 1][1][lane])[at & 1] = lo;
+        uint2 hi, lo;
+        split4(M[n] * up, hi, lo);
+        const int k = w * kN + n;
+        reinterpret_cast<uint2 *>(&lds.c.m[k >> 1][0][lane])[k & 1] = hi;
+        reinterpret_cast<uint2 *>(&lds.c.m[k >> 1][1][lane])[k & 1] = lo;
       }
     };
-    put_top();
+    const auto put4 = [&](uint2 (*to)[64][2], const f4 &x) {
+      uint2 hi, lo;
+      split4(x, hi, lo);
+      to[0][lane][w & 1] = hi;
+      to[1][lane][w & 1] = lo;
+    };
     __syncthreads();
-    get_top();
-    odd = odd || lds.c.odd != 0u;
-    int em = scale_exp(mtop);
+    odd = lds.c.odd != 0u;
+    get_scales(0);
+    int em = em1;  // its bound holds for the chunk's own state too
     if (!odd) put_m(pow2(em));
     lds_barrier();
 
     const auto step = [&](int c, h8 (*kf)[2]) {
       const int next = c + 1 < chunks ? c + 1 : c;
-      f4 vn, bn, gn, cn;
+      f4 bn, gn, cn;
       float wn;
       load_meta(next, bn, gn, cn, wn);
-      load_v(next, vn);
-      const int eu = exp_u(), em1 = exp_m();
+      const f4 vn = load_v(next);
       // ---- R = be (V - e^G K M)
       f4 km = zero, kx = zero, ky = zero;
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         const h8 hi = lds.c.m[s][0][lane], lo = lds.c.m[s][1][lane];
-        km = mfma(kf[s][0], hi, km);
-        kx = mfma(kf[s][0], lo, kx);
-        ky = mfma(kf[s][1], hi, ky);
+        km = mfma32(kf[s][0], hi, km);
+        kx = mfma32(kf[s][0], lo, kx);
+        ky = mfma32(kf[s][1], hi, ky);
       }
       load_k(c + (kDeep ? 2 : 1), kf);
       const float dm = kDown * pow2(-em), up = pow2(eu);
       f4 r;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = (be[i] * up) * (v[i] - eg[i] * ((km[i] + (kx[i] + ky[i])) * dm));
+      for (int i = 0; i < 4; ++i) r[i] = (be[i] * up) * fmaf(-(eg[i] * dm), km[i] + (kx[i] + ky[i]), v[i]);
       put4(lds.c.r[w >> 1], r);
       lds_barrier();
       // ---- U = T R, times 2^eu
@@ -697,17 +741,15 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
       for (int p = 0; p < 2; ++p) {
         if (p > w >> 1) continue;
         const h8 hi = *reinterpret_cast<const h8 *>(lds.c.r[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.r[p][1][lane]);
-        u = mfma(tf[p][0], hi, u);
-        ux = mfma(tf[p][0], lo, ux);
-        uy = mfma(tf[p][1], hi, uy);
+        u = mfma32(tf[p][0], hi, u);
+        ux = mfma32(tf[p][0], lo, ux);
+        uy = mfma32(tf[p][1], hi, uy);
       }
       load_t(next);
 #pragma unroll
       for (int i = 0; i < 4; ++i) u[i] = (u[i] + (ux[i] + uy[i])) * kDown;
+      put4(lds.c.v[w >> 1], u * ec);
       put4(lds.c.u[w >> 1], u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] *= ec[i];
-      put4(lds.c.v[w >> 1], u);
       lds_barrier();
       // ---- the next state
       f4 n0[kN], nx[kN], ny[kN];
@@ -718,9 +760,9 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         const h8 hi = *reinterpret_cast<const h8 *>(lds.c.v[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.v[p][1][lane]);
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
-          n0[n] = mfma(ktf[n][p][0], hi, n0[n]);
-          nx[n] = mfma(ktf[n][p][0], lo, nx[n]);
-          ny[n] = mfma(ktf[n][p][1], hi, ny[n]);
+          n0[n] = mfma32(ktf[n][p][0], hi, n0[n]);
+          nx[n] = mfma32(ktf[n][p][0], lo, nx[n]);
+          ny[n] = mfma32(ktf[n][p][1], hi, ny[n]);
         }
       }
       load_kt(next);
@@ -736,9 +778,8 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
       ec = cn;
       whole = wn;
       em = em1;
-      put_top();
       lds_barrier();
-      get_top();
+      get_scales(c + 1);
     };
     if constexpr (kDeep) {
       for (int c = 0; c < chunks && !odd; c += 2) {
@@ -753,9 +794,11 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
       for (int n = 0; n < kN; ++n) *reinterpret_cast<f4 *>(state + 16 * n) = M[n];
     }
   } else {
-    const h8 *qw = a.w.q + (key0 * 4 + w) * kS * kFrag + lane;
-    const h8 *pw = a.w.p + (val0 * 6 + tri(w, 0)) * kFrag + lane;
-    float *op = a.s.out + ((b * a.s.n + tok) * a.s.heads + h) * kD + row0 + m;
+    const h8 *qw = a.w.q + (key0 * 4 + w) * kS * kFrag;
+    const h8 *pw = a.w.p + (val0 * 6 + tri(w, 0)) * kFrag;
+    const uint32_t row = (uint32_t)a.s.heads * kD * 4u;  // bytes between a token's outputs
+    char *o0 = reinterpret_cast<char *>(a.s.out + ((b * a.s.n + a.first) * a.s.heads + h) * kD + row0);
+    const uint32_t ooff = (uint32_t)(16 * w + 4 * g) * row + 4u * (uint32_t)m;
     h8 qa[kS][2], qb[kDeep ? kS : 1][2], pf[2][2];
     f4 eg;
     const auto load_q = [&](int c, h8 (*f)[2]) {
@@ -763,61 +806,78 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 #pragma unroll
       for (int s = 0; s < kS; ++s)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) f[s][u] = p[s * kFrag + 64 * u];
+        for (int u = 0; u < 2; ++u) f[s][u] = at<h8>(p + s * kFrag + 64 * u, foff);
     };
     const auto load_p = [&](int c) {
+      const h8 *q = pw + c * tstep;
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          if (p <= w >> 1) pf[p][u] = pw[c * tstep + p * kFrag + 64 * u];
+          if (p <= w >> 1) pf[p][u] = at<h8>(q + p * kFrag + 64 * u, foff);
     };
-    eg = *reinterpret_cast<const f4 *>(meta + kC);
+    eg = at<f4>(meta + kC, moff);
+    f4 v = load_v(chunks > 1 ? 1 : 0);
     load_q(0, qa);
     if constexpr (kDeep) load_q(1, qb);
     load_p(0);
     __syncthreads();
-    get_top();
-    odd = odd || lds.c.odd != 0u;
-    int em = scale_exp(mtop);
+    odd = lds.c.odd != 0u;
+    get_scales(0);
+    int em = em1;
+    uint32_t vnow = lds.c.top[0][2][w];  // max |v| of the wave's tokens in this chunk
     lds_barrier();
 
     const auto step = [&](int c, h8 (*qf)[2]) {
       const int next = c + 1 < chunks ? c + 1 : c;
-      const f4 gn = *reinterpret_cast<const f4 *>(meta + next * mstep + kC);
-      const int eu = exp_u(), em1 = exp_m();
+      const f4 gn = at<f4>(meta + next * mstep + kC, moff);
       f4 qm = zero, qx = zero, qy = zero;
+      uint32_t top = 0u;  // largest magnitude of the state's high parts, as fp16 bits
 #pragma unroll
       for (int s = 0; s < kS; ++s) {
         const h8 hi = lds.c.m[s][0][lane], lo = lds.c.m[s][1][lane];
-        qm = mfma(qf[s][0], hi, qm);
-        qx = mfma(qf[s][0], lo, qx);
-        qy = mfma(qf[s][1], hi, qy);
+        qm = mfma32(qf[s][0], hi, qm);
+        qx = mfma32(qf[s][0], lo, qx);
+        qy = mfma32(qf[s][1], hi, qy);
+        if ((s & 3) == w || kS == 2) top = umax(top, top16(hi));  // a quarter of the state each
       }
       load_q(c + (kDeep ? 2 : 1), qf);
       const float dm = kDown * pow2(-em) * a.s.scale, du = kDown * pow2(-eu) * a.s.scale;
 #pragma unroll
       for (int i = 0; i < 4; ++i) qm[i] = eg[i] * ((qm[i] + (qx[i] + qy[i])) * dm);
       lds_barrier();
+      // the next chunk's maxima: M in front of this chunk, v of this chunk and of the next
+      const uint32_t vnext = wave_max(umax(umax(mag(v[0]), mag(v[1])), umax(mag(v[2]), mag(v[3]))));
+      top = wave_max(top);
+      if (lane == 0) {
+        const float x = (float)__builtin_bit_cast(_Float16, (uint16_t)top) * pow2(-em) * 1.001f;
+        lds.c.top[(c + 1) & 1][0][w] = mag(x);
+        lds.c.top[(c + 1) & 1][1][w] = vnow;
+        lds.c.top[(c + 1) & 1][2][w] = vnext;
+      }
+      vnow = vnext;
+      v = load_v(c + 2 < chunks ? c + 2 : chunks - 1);
       lds_barrier();
       f4 o = zero, ox = zero, oy = zero;
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         if (p > w >> 1) continue;
         const h8 hi = *reinterpret_cast<const h8 *>(lds.c.u[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.u[p][1][lane]);
-        o = mfma(pf[p][0], hi, o);
-        ox = mfma(pf[p][0], lo, ox);
-        oy = mfma(pf[p][1], hi, oy);
+        o = mfma32(pf[p][0], hi, o);
+        ox = mfma32(pf[p][0], lo, ox);
+        oy = mfma32(pf[p][1], hi, oy);
       }
       load_p(next);
+      char *op = o0 + (int64_t)c * kC * row;
+      const bool full = tokens - c * kC >= kC;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (tok + (int64_t)c * kC + i < end)
-          op[((int64_t)c * kC + i) * a.s.heads * kD] = fmaf(o[i] + (ox[i] + oy[i]), du, qm[i]);
+        if (full || 16 * w + 4 * g + i < tokens - c * kC)
+          *reinterpret_cast<float *>(op + (ooff + (uint32_t)i * row)) = fmaf(o[i] + (ox[i] + oy[i]), du, qm[i]);
       eg = gn;
       em = em1;
       lds_barrier();
-      get_top();
+      get_scales(c + 1);
     };
     if constexpr (kDeep) {
       for (int c = 0; c < chunks && !odd; c += 2) {
@@ -914,11 +974,13 @@ int launch_deltanet_prompt(const float *q, const float *k, const float *v, const
     return set_error(PKV_ERR_UNSUPPORTED, "delta net prompt: head_dim must be 64, 128 or 256");
   if (n > ((int64_t)1 << 30) || (int64_t)batch * heads > (1 << 24))
     return set_error(PKV_ERR_ARG, "n must be <= 2^30 and batch * heads <= 2^24");
-  const SegmentPlan plan = plan_segment(batch, n, k_heads, heads, head_dim);
+  SegmentPlan plan = plan_segment(batch, n, k_heads, heads, head_dim);
   if (ws_bytes < plan.bytes || (plan.bytes != 0 && ws == nullptr))
     return set_error(PKV_ERR_ARG, "the workspace is smaller than pkv_deltanet_prompt_workspace says");
   if (reinterpret_cast<uintptr_t>(ws) % 16 != 0)
     return set_error(PKV_ERR_ARG, "the workspace must be 16-byte aligned");
+  // a chunk's v and out are addressed by 32-bit byte offsets
+  if (strides[5] >= 1 << 24 || (int64_t)heads * head_dim >= 1 << 24) plan.chunks = 0;
   ScanArgs a{q, k, v, gate, beta, strides[0], strides[1], strides[2], strides[3], strides[4], strides[5],
              state, gate_offset, out, lens, n, heads, heads / k_heads, scale, eps};
   switch (head_dim) {

@@ -540,6 +540,26 @@ template <typename T>
 __device__ __forceinline__ T at(const void *base, uint32_t off) {
   return *reinterpret_cast<const T *>(static_cast<const char *>(base) + off);
 }
+// Element i of lane q of each four lanes to element q of lane i.
+__device__ __forceinline__ f4 transpose4(f4 x) {
+  const auto swap = [](float v, auto ctrl) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, 0xF, 0xF, true));
+  };
+  const bool q1 = threadIdx.x & 1, q2 = threadIdx.x & 2;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const float t = swap(q1 ? x[i] : x[i + 1], std::integral_constant<int, 0xB1>{});  // lane ^ 1
+    x[i] = q1 ? t : x[i];
+    x[i + 1] = q1 ? x[i + 1] : t;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float t = swap(q2 ? x[i] : x[i + 2], std::integral_constant<int, 0x4E>{});  // lane ^ 2
+    x[i] = q2 ? t : x[i];
+    x[i + 2] = q2 ? x[i + 2] : t;
+  }
+  return x;
+}
 // Four values (not MFMA results themselves: lo_pair is inline asm) as fp16 parts.
 __device__ __forceinline__ void split4(const f4 &x, uint2 &hi, uint2 &lo) {
   float y[4] = {x[0], x[1], x[2], x[3]};
@@ -554,7 +574,7 @@ __device__ __forceinline__ void split4(const f4 &x, uint2 &hi, uint2 &lo) {
 // tokens 16 w .. of each chunk. Waves 4 - 7 make the outputs of the same tokens beside them, off
 // the path from one chunk to the next, and the bounds that the scales come from. A wave
 // loads its fragments of the next chunk (K and Q: of the one after, where the registers hold
-// both) when a stage has just used them.
+// both) when a stage has used them, the state's waves once what others wait for is in LDS.
 template <int kD>
 __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   constexpr int kS = kD / 32, kN = kD / 64;
@@ -586,17 +606,14 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   const float *meta = a.w.meta + val0 * 3 * kC;
   const float *v0 = a.s.v + b * a.s.vb + a.first * a.s.vt + h * kD + row0;
   const uint32_t moff = 4u * (uint32_t)(16 * w + 4 * g), foff = 16u * (uint32_t)lane;
-  // v of the lane's four tokens; past the end the last token's, whose weight there is 0
+  // v of token 16 w + 4 g + m % 4, channels 4 (m / 4) .. + 3 (one 16-byte load, 64-byte rows):
+  // the transpose within each four lanes of the MFMA result's layout. Past the end the last
+  // token's, whose weight there is 0.
   const auto load_v = [&](int c) {
     const float *p = v0 + (int64_t)c * kC * a.s.vt;
     const int last = (tokens - c * kC < kC ? tokens - c * kC : kC) - 1;
-    f4 x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int t = 16 * w + 4 * g + i < last ? 16 * w + 4 * g + i : last;
-      x[i] = at<float>(p, 4u * ((uint32_t)t * (uint32_t)a.s.vt + (uint32_t)m));
-    }
-    return x;
+    const int t = 16 * w + 4 * g + (m & 3) < last ? 16 * w + 4 * g + (m & 3) : last;
+    return at<f4>(p, 4u * ((uint32_t)t * (uint32_t)a.s.vt + (uint32_t)(m & 12)));
   };
 
   if (tid == 0) lds.c.odd = 0u;
@@ -666,7 +683,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
       all = at<float>(p + 2 * kC - 1, 0u);  // e^(G_63)
     };
     load_meta(0, be, eg, ec, whole);
-    v = load_v(0);
+    v = transpose4(load_v(0));
     load_k(0, ka);
     if constexpr (kDeep) load_k(1, kb);
     load_t(0);
@@ -728,12 +745,12 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         kx = mfma32(kf[s][0], lo, kx);
         ky = mfma32(kf[s][1], hi, ky);
       }
-      load_k(c + (kDeep ? 2 : 1), kf);
       const float dm = kDown * pow2(-em), up = pow2(eu);
       f4 r;
 #pragma unroll
       for (int i = 0; i < 4; ++i) r[i] = (be[i] * up) * fmaf(-(eg[i] * dm), km[i] + (kx[i] + ky[i]), v[i]);
       put4(lds.c.r[w >> 1], r);
+      load_k(c + (kDeep ? 2 : 1), kf);
       lds_barrier();
       // ---- U = T R, times 2^eu
       f4 u = zero, ux = zero, uy = zero;
@@ -745,11 +762,11 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         ux = mfma32(tf[p][0], lo, ux);
         uy = mfma32(tf[p][1], hi, uy);
       }
-      load_t(next);
 #pragma unroll
       for (int i = 0; i < 4; ++i) u[i] = (u[i] + (ux[i] + uy[i])) * kDown;
       put4(lds.c.v[w >> 1], u * ec);
       put4(lds.c.u[w >> 1], u);
+      load_t(next);
       lds_barrier();
       // ---- the next state
       f4 n0[kN], nx[kN], ny[kN];
@@ -765,14 +782,14 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           ny[n] = mfma32(ktf[n][p][1], hi, ny[n]);
         }
       }
-      load_kt(next);
       const float du = kDown * pow2(-eu);
 #pragma unroll
       for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) M[n][i] = fmaf(M[n][i], whole, (n0[n][i] + (nx[n][i] + ny[n][i])) * du);
       put_m(pow2(em1));
-      v = vn;
+      load_kt(next);
+      v = transpose4(vn);
       be = bn;
       eg = gn;
       ec = cn;
@@ -798,7 +815,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     const h8 *pw = a.w.p + (val0 * 6 + tri(w, 0)) * kFrag;
     const uint32_t row = (uint32_t)a.s.heads * kD * 4u;  // bytes between a token's outputs
     char *o0 = reinterpret_cast<char *>(a.s.out + ((b * a.s.n + a.first) * a.s.heads + h) * kD + row0);
-    const uint32_t ooff = (uint32_t)(16 * w + 4 * g) * row + 4u * (uint32_t)m;
+    const uint32_t ooff = (uint32_t)(16 * w + 4 * g + (m & 3)) * row + 4u * (uint32_t)(m & 12);
     h8 qa[kS][2], qb[kDeep ? kS : 1][2], pf[2][2];
     f4 eg;
     const auto load_q = [&](int c, h8 (*f)[2]) {
@@ -868,15 +885,15 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         oy = mfma32(pf[p][1], hi, oy);
       }
       load_p(next);
-      char *op = o0 + (int64_t)c * kC * row;
-      const bool full = tokens - c * kC >= kC;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (full || 16 * w + 4 * g + i < tokens - c * kC)
-          *reinterpret_cast<float *>(op + (ooff + (uint32_t)i * row)) = fmaf(o[i] + (ox[i] + oy[i]), du, qm[i]);
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(o[i] + (ox[i] + oy[i]), du, qm[i]);
       eg = gn;
       em = em1;
       lds_barrier();
+      // 64 bytes of each token's row, as load_v
+      o = transpose4(o);
+      if (16 * w + 4 * g + (m & 3) < tokens - c * kC)
+        *reinterpret_cast<f4 *>(o0 + (int64_t)c * kC * row + ooff) = o;
       get_scales(c + 1);
     };
     if constexpr (kDeep) {

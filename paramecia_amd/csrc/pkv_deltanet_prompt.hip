@@ -524,11 +524,11 @@ __device__ __forceinline__ int scale_exp(float bound) {
 }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 
-template <int kD>
+template <int kD, int kNT>
 union StateLds {
   struct {
-    h8 m[kD / 32][2][64];   // the state's fragments
-    uint2 r[2][2][64][2], u[2][2][64][2], v[2][2][64][2];  // R, U, U e^(G_63 - G): [k step][part][lane][half]
+    h8 m[kNT][kD / 32][2][64];  // the state's fragments
+    uint2 r[kNT][2][2][64][2], u[kNT][2][2][64][2], v[kNT][2][2][64][2];  // R, U, U e^(G_63 - G): [k step][part][lane][half]
     uint32_t top[2][3][4];  // [chunk's parity][maximum][wave], bits of magnitudes
     unsigned odd;
   } c;
@@ -569,21 +569,21 @@ __device__ __forceinline__ void split4(const f4 &x, uint2 &hi, uint2 &lo) {
   lo = uint2{lo_pair(y[0], y[1], hi.x), lo_pair(y[2], y[3], hi.y)};
 }
 
-// The chunks of 16 value channels of one head, in order, by eight waves. Waves 0 - 3 carry the
+// The chunks of 16 kNT value channels of one head, in order, by eight waves. Waves 0 - 3 carry the
 // state: wave w owns key channels w d / 4 .. of it (f32, in an MFMA result's layout) and
 // tokens 16 w .. of each chunk. Waves 4 - 7 make the outputs of the same tokens beside them, off
 // the path from one chunk to the next, and the bounds that the scales come from. A wave
 // loads its fragments of the next chunk (K and Q: of the one after, where the registers hold
 // both) when a stage has used them, the state's waves once what others wait for is in LDS.
-template <int kD>
+template <int kD, int kNT>
 __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   constexpr int kS = kD / 32, kN = kD / 64;
   constexpr bool kDeep = kD <= 128;
-  __shared__ __attribute__((aligned(16))) StateLds<kD> lds;
+  __shared__ __attribute__((aligned(16))) StateLds<kD, kNT> lds;
   const int tid = threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3;
   // the workgroups of a key head share an XCD and its L2 (workgroups go to the 8 XCDs in turn)
-  const int groups = a.batch * a.k_heads, per = a.s.rep * (kD / 16);
+  const int groups = a.batch * a.k_heads, per = a.s.rep * (kD / (16 * kNT));
   int grp, in;
   if (groups % 8 == 0) {
     const int id = blockIdx.x >> 3;
@@ -593,8 +593,8 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     grp = blockIdx.x / per;
     in = blockIdx.x % per;
   }
-  const int64_t b = grp / a.k_heads, hk = grp % a.k_heads, h = hk * a.s.rep + in / (kD / 16);
-  const int row0 = (in % (kD / 16)) * 16;
+  const int64_t b = grp / a.k_heads, hk = grp % a.k_heads, h = hk * a.s.rep + in / (kD / (16 * kNT));
+  const int row0 = (in % (kD / (16 * kNT))) * 16 * kNT;
   int64_t end = valid_tokens(a.s.lens, b, a.s.n);
   const int64_t stop = a.first + (int64_t)a.chunks * kC;
   end = end < stop ? end : stop;
@@ -609,11 +609,12 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   // v of token 16 w + 4 g + m % 4, channels 4 (m / 4) .. + 3 (one 16-byte load, 64-byte rows):
   // the transpose within each four lanes of the MFMA result's layout. Past the end the last
   // token's, whose weight there is 0.
-  const auto load_v = [&](int c) {
+  const auto load_v = [&](int c, f4 (&x)[kNT]) {
     const float *p = v0 + (int64_t)c * kC * a.s.vt;
     const int last = (tokens - c * kC < kC ? tokens - c * kC : kC) - 1;
     const int t = 16 * w + 4 * g + (m & 3) < last ? 16 * w + 4 * g + (m & 3) : last;
-    return at<f4>(p, 4u * ((uint32_t)t * (uint32_t)a.s.vt + (uint32_t)(m & 12)));
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) x[j] = at<f4>(p + 16 * j, 4u * ((uint32_t)t * (uint32_t)a.s.vt + (uint32_t)(m & 12)));
   };
 
   if (tid == 0) lds.c.odd = 0u;
@@ -649,7 +650,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     const h8 *tw = a.w.t + (val0 * 6 + tri(w, 0)) * kFrag;
     float *state = a.s.state + ((b * a.s.heads + h) * kD + row0 + m) * kD + w * (kD / 4) + 4 * g;
     h8 ka[kS][2], kb[kDeep ? kS : 1][2], ktf[kN][2][2], tf[2][2];
-    f4 v, be, eg, ec;
+    f4 v[kNT], be, eg, ec;
     float whole;
     const auto load_k = [&](int c, h8 (*f)[2]) {
       const h8 *p = kw + (c < chunks ? c : chunks - 1) * kstep;
@@ -683,22 +684,28 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
       all = at<float>(p + 2 * kC - 1, 0u);  // e^(G_63)
     };
     load_meta(0, be, eg, ec, whole);
-    v = transpose4(load_v(0));
+    load_v(0, v);
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) v[j] = transpose4(v[j]);
     load_k(0, ka);
     if constexpr (kDeep) load_k(1, kb);
     load_t(0);
     load_kt(0);
-    f4 M[kN];
+    f4 M[kNT][kN];
 #pragma unroll
-    for (int n = 0; n < kN; ++n) M[n] = *reinterpret_cast<const f4 *>(state + 16 * n);
+    for (int j = 0; j < kNT; ++j)
+#pragma unroll
+      for (int n = 0; n < kN; ++n) M[j][n] = *reinterpret_cast<const f4 *>(state + 16 * j * kD + 16 * n);
     {  // the first chunk's maxima: of M in front of it (nothing before adds to it) and of v
       uint32_t x = 0u, y = 0u;
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
+      for (int j = 0; j < kNT; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x = umax(x, mag(M[n][i]));
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) y = umax(y, mag(v[i]));
+          for (int n = 0; n < kN; ++n) x = umax(x, mag(M[j][n][i]));
+          y = umax(y, mag(v[j][i]));
+        }
       x = wave_max(x);
       y = wave_max(y);
       if (lane == 0) {
@@ -709,13 +716,15 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     }
     const auto put_m = [&](float up) {
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        uint2 hi, lo;
-        split4(M[n] * up, hi, lo);
-        const int k = w * kN + n;
-        reinterpret_cast<uint2 *>(&lds.c.m[k >> 1][0][lane])[k & 1] = hi;
-        reinterpret_cast<uint2 *>(&lds.c.m[k >> 1][1][lane])[k & 1] = lo;
-      }
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int n = 0; n < kN; ++n) {
+          uint2 hi, lo;
+          split4(M[j][n] * up, hi, lo);
+          const int k = w * kN + n;
+          reinterpret_cast<uint2 *>(&lds.c.m[j][k >> 1][0][lane])[k & 1] = hi;
+          reinterpret_cast<uint2 *>(&lds.c.m[j][k >> 1][1][lane])[k & 1] = lo;
+        }
     };
     const auto put4 = [&](uint2 (*to)[64][2], const f4 &x) {
       uint2 hi, lo;
@@ -732,64 +741,83 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 
     const auto step = [&](int c, h8 (*kf)[2]) {
       const int next = c + 1 < chunks ? c + 1 : c;
-      f4 bn, gn, cn;
+      f4 bn, gn, cn, vn[kNT];
       float wn;
       load_meta(next, bn, gn, cn, wn);
-      const f4 vn = load_v(next);
+      load_v(next, vn);
       // ---- R = be (V - e^G K M)
-      f4 km = zero, kx = zero, ky = zero;
+      f4 km[kNT], kx[kNT], ky[kNT];
 #pragma unroll
-      for (int s = 0; s < kS; ++s) {
-        const h8 hi = lds.c.m[s][0][lane], lo = lds.c.m[s][1][lane];
-        km = mfma32(kf[s][0], hi, km);
-        kx = mfma32(kf[s][0], lo, kx);
-        ky = mfma32(kf[s][1], hi, ky);
-      }
+      for (int j = 0; j < kNT; ++j) km[j] = kx[j] = ky[j] = zero;
+#pragma unroll
+      for (int s = 0; s < kS; ++s)
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) {
+          const h8 hi = lds.c.m[j][s][0][lane], lo = lds.c.m[j][s][1][lane];
+          km[j] = mfma32(kf[s][0], hi, km[j]);
+          kx[j] = mfma32(kf[s][0], lo, kx[j]);
+          ky[j] = mfma32(kf[s][1], hi, ky[j]);
+        }
       const float dm = kDown * pow2(-em), up = pow2(eu);
-      f4 r;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = (be[i] * up) * fmaf(-(eg[i] * dm), km[i] + (kx[i] + ky[i]), v[i]);
-      put4(lds.c.r[w >> 1], r);
+      for (int j = 0; j < kNT; ++j) {
+        f4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = (be[i] * up) * fmaf(-(eg[i] * dm), km[j][i] + (kx[j][i] + ky[j][i]), v[j][i]);
+        put4(lds.c.r[j][w >> 1], r);
+      }
       load_k(c + (kDeep ? 2 : 1), kf);
       lds_barrier();
       // ---- U = T R, times 2^eu
-      f4 u = zero, ux = zero, uy = zero;
+      f4 u[kNT], ux[kNT], uy[kNT];
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) u[j] = ux[j] = uy[j] = zero;
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         if (p > w >> 1) continue;
-        const h8 hi = *reinterpret_cast<const h8 *>(lds.c.r[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.r[p][1][lane]);
-        u = mfma32(tf[p][0], hi, u);
-        ux = mfma32(tf[p][0], lo, ux);
-        uy = mfma32(tf[p][1], hi, uy);
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) {
+          const h8 hi = *reinterpret_cast<const h8 *>(lds.c.r[j][p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.r[j][p][1][lane]);
+          u[j] = mfma32(tf[p][0], hi, u[j]);
+          ux[j] = mfma32(tf[p][0], lo, ux[j]);
+          uy[j] = mfma32(tf[p][1], hi, uy[j]);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = (u[i] + (ux[i] + uy[i])) * kDown;
-      put4(lds.c.v[w >> 1], u * ec);
-      put4(lds.c.u[w >> 1], u);
+      for (int j = 0; j < kNT; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[j][i] = (u[j][i] + (ux[j][i] + uy[j][i])) * kDown;
+        put4(lds.c.v[j][w >> 1], u[j] * ec);
+        put4(lds.c.u[j][w >> 1], u[j]);
+      }
       load_t(next);
       lds_barrier();
       // ---- the next state
-      f4 n0[kN], nx[kN], ny[kN];
-#pragma unroll
-      for (int n = 0; n < kN; ++n) n0[n] = nx[n] = ny[n] = zero;
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const h8 hi = *reinterpret_cast<const h8 *>(lds.c.v[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.v[p][1][lane]);
-#pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          n0[n] = mfma32(ktf[n][p][0], hi, n0[n]);
-          nx[n] = mfma32(ktf[n][p][0], lo, nx[n]);
-          ny[n] = mfma32(ktf[n][p][1], hi, ny[n]);
-        }
-      }
       const float du = kDown * pow2(-eu);
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
+      for (int j = 0; j < kNT; ++j) {
+        f4 n0[kN], nx[kN], ny[kN];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) M[n][i] = fmaf(M[n][i], whole, (n0[n][i] + (nx[n][i] + ny[n][i])) * du);
+        for (int n = 0; n < kN; ++n) n0[n] = nx[n] = ny[n] = zero;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const h8 hi = *reinterpret_cast<const h8 *>(lds.c.v[j][p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.v[j][p][1][lane]);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) {
+            n0[n] = mfma32(ktf[n][p][0], hi, n0[n]);
+            nx[n] = mfma32(ktf[n][p][0], lo, nx[n]);
+            ny[n] = mfma32(ktf[n][p][1], hi, ny[n]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) M[j][n][i] = fmaf(M[j][n][i], whole, (n0[n][i] + (nx[n][i] + ny[n][i])) * du);
+      }
       put_m(pow2(em1));
       load_kt(next);
-      v = transpose4(vn);
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) v[j] = transpose4(vn[j]);
       be = bn;
       eg = gn;
       ec = cn;
@@ -808,7 +836,9 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     }
     if (!odd) {
 #pragma unroll
-      for (int n = 0; n < kN; ++n) *reinterpret_cast<f4 *>(state + 16 * n) = M[n];
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int n = 0; n < kN; ++n) *reinterpret_cast<f4 *>(state + 16 * j * kD + 16 * n) = M[j][n];
     }
   } else {
     const h8 *qw = a.w.q + (key0 * 4 + w) * kS * kFrag;
@@ -834,7 +864,8 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           if (p <= w >> 1) pf[p][u] = at<h8>(q + p * kFrag + 64 * u, foff);
     };
     eg = at<f4>(meta + kC, moff);
-    f4 v = load_v(chunks > 1 ? 1 : 0);
+    f4 v[kNT];
+    load_v(chunks > 1 ? 1 : 0, v);
     load_q(0, qa);
     if constexpr (kDeep) load_q(1, qb);
     load_p(0);
@@ -848,23 +879,34 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     const auto step = [&](int c, h8 (*qf)[2]) {
       const int next = c + 1 < chunks ? c + 1 : c;
       const f4 gn = at<f4>(meta + next * mstep + kC, moff);
-      f4 qm = zero, qx = zero, qy = zero;
+      f4 qm[kNT], qx[kNT], qy[kNT];
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) qm[j] = qx[j] = qy[j] = zero;
       uint32_t top = 0u;  // largest magnitude of the state's high parts, as fp16 bits
 #pragma unroll
-      for (int s = 0; s < kS; ++s) {
-        const h8 hi = lds.c.m[s][0][lane], lo = lds.c.m[s][1][lane];
-        qm = mfma32(qf[s][0], hi, qm);
-        qx = mfma32(qf[s][0], lo, qx);
-        qy = mfma32(qf[s][1], hi, qy);
-        if ((s & 3) == w || kS == 2) top = umax(top, top16(hi));  // a quarter of the state each
-      }
+      for (int s = 0; s < kS; ++s)
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) {
+          const h8 hi = lds.c.m[j][s][0][lane], lo = lds.c.m[j][s][1][lane];
+          qm[j] = mfma32(qf[s][0], hi, qm[j]);
+          qx[j] = mfma32(qf[s][0], lo, qx[j]);
+          qy[j] = mfma32(qf[s][1], hi, qy[j]);
+          if ((s & 3) == w || kS == 2) top = umax(top, top16(hi));  // a quarter of the state each
+        }
       load_q(c + (kDeep ? 2 : 1), qf);
       const float dm = kDown * pow2(-em) * a.s.scale, du = kDown * pow2(-eu) * a.s.scale;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) qm[i] = eg[i] * ((qm[i] + (qx[i] + qy[i])) * dm);
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qm[j][i] = eg[i] * ((qm[j][i] + (qx[j][i] + qy[j][i])) * dm);
       lds_barrier();
       // the next chunk's maxima: M in front of this chunk, v of this chunk and of the next
-      const uint32_t vnext = wave_max(umax(umax(mag(v[0]), mag(v[1])), umax(mag(v[2]), mag(v[3]))));
+      uint32_t vnext = 0u;
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vnext = umax(vnext, mag(v[j][i]));
+      vnext = wave_max(vnext);
       top = wave_max(top);
       if (lane == 0) {
         const float x = (float)__builtin_bit_cast(_Float16, (uint16_t)top) * pow2(-em) * 1.001f;
@@ -873,27 +915,36 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         lds.c.top[(c + 1) & 1][2][w] = vnext;
       }
       vnow = vnext;
-      v = load_v(c + 2 < chunks ? c + 2 : chunks - 1);
+      load_v(c + 2 < chunks ? c + 2 : chunks - 1, v);
       lds_barrier();
-      f4 o = zero, ox = zero, oy = zero;
+      f4 o[kNT], ox[kNT], oy[kNT];
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) o[j] = ox[j] = oy[j] = zero;
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         if (p > w >> 1) continue;
-        const h8 hi = *reinterpret_cast<const h8 *>(lds.c.u[p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.u[p][1][lane]);
-        o = mfma32(pf[p][0], hi, o);
-        ox = mfma32(pf[p][0], lo, ox);
-        oy = mfma32(pf[p][1], hi, oy);
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) {
+          const h8 hi = *reinterpret_cast<const h8 *>(lds.c.u[j][p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.u[j][p][1][lane]);
+          o[j] = mfma32(pf[p][0], hi, o[j]);
+          ox[j] = mfma32(pf[p][0], lo, ox[j]);
+          oy[j] = mfma32(pf[p][1], hi, oy[j]);
+        }
       }
       load_p(next);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = fmaf(o[i] + (ox[i] + oy[i]), du, qm[i]);
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[j][i] = fmaf(o[j][i] + (ox[j][i] + oy[j][i]), du, qm[j][i]);
       eg = gn;
       em = em1;
       lds_barrier();
       // 64 bytes of each token's row, as load_v
-      o = transpose4(o);
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) o[j] = transpose4(o[j]);
       if (16 * w + 4 * g + (m & 3) < tokens - c * kC)
-        *reinterpret_cast<f4 *>(o0 + (int64_t)c * kC * row + ooff) = o;
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) *reinterpret_cast<f4 *>(o0 + (int64_t)c * kC * row + 64 * j + ooff) = o[j];
       get_scales(c + 1);
     };
     if constexpr (kDeep) {
@@ -908,19 +959,26 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   if (odd) {
     __syncthreads();
     if (wave >= 4) return;  // a wave that has ended takes no part in the barriers below
-    scan_tokens<kD>(a.s, lds.t, b, h, row0, a.first, end);
+#pragma unroll 1
+    for (int j = 0; j < kNT; ++j) {
+      scan_tokens<kD>(a.s, lds.t, b, h, row0 + 16 * j, a.first, end);
+      __syncthreads();
+    }
     return;
   }
-  if (a.s.gate_offset != nullptr && row0 == 0 && tid == 0) {
-    double sum = (double)a.s.gate_offset[b * a.s.heads + h];
-    for (int c = 0; c < chunks; ++c) sum += a.w.gates[val0 + (int64_t)c * a.s.heads];
-    a.s.gate_offset[b * a.s.heads + h] = (float)sum;
+  if (a.s.gate_offset != nullptr && row0 == 0 && wave == 0) {
+    double sum = 0.0;  // the chunks' sums, 64 at a time, then across the lanes
+    for (int c = lane; c < chunks; c += 64) sum += a.w.gates[val0 + (int64_t)c * a.s.heads];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    float *o = a.s.gate_offset + b * a.s.heads + h;
+    if (lane == 0) *o = (float)((double)*o + sum);
   }
 }
 
 // A segment's chunks, and where its workspace's parts lie.
 constexpr int64_t kChunkedTokens = 48;          // prompts from here on go by chunks
-constexpr size_t kSegmentBytes = (size_t)96 << 20;
+constexpr size_t kSegmentBytes = (size_t)192 << 20;
 struct SegmentPlan {
   int chunks = 0;  // 0: token by token
   size_t k = 0, q = 0, kt = 0, t = 0, p = 0, meta = 0, gates = 0, odd = 0, bytes = 0;
@@ -958,13 +1016,19 @@ int launch(const ScanArgs &a, const SegmentPlan &plan, int batch, int k_heads, v
                   reinterpret_cast<h8 *>(base + plan.kt), reinterpret_cast<h8 *>(base + plan.t),
                   reinterpret_cast<h8 *>(base + plan.p), reinterpret_cast<float *>(base + plan.meta),
                   reinterpret_cast<double *>(base + plan.gates), reinterpret_cast<unsigned *>(base + plan.odd)};
+  constexpr int kWide = kD <= 128 ? 2 : 1;
+  const bool wide = kWide > 1 && (int64_t)batch * a.heads * (kD / 16) > 256;
   const int64_t all = (a.n + kC - 1) / kC;
   for (int64_t c = 0; c < all; c += plan.chunks) {
     ChunkArgs ca{a, w, c * kC, (int)(all - c < plan.chunks ? all - c : plan.chunks), k_heads, batch};
     hipLaunchKernelGGL((chunk_kernel<kD>), dim3((unsigned)ca.chunks, (unsigned)k_heads, (unsigned)batch),
                        dim3(256), 0, s, ca);
     PKV_HIP(hipGetLastError());
-    hipLaunchKernelGGL((state_kernel<kD>), dim3((unsigned)(batch * a.heads * (kD / 16))), dim3(512), 0, s, ca);
+    const unsigned walks = (unsigned)(batch * a.heads * (kD / 16));
+    if (wide)
+      hipLaunchKernelGGL((state_kernel<kD, kWide>), dim3(walks / 2), dim3(512), 0, s, ca);
+    else
+      hipLaunchKernelGGL((state_kernel<kD, 1>), dim3(walks), dim3(512), 0, s, ca);
     PKV_HIP(hipGetLastError());
   }
   return PKV_OK;

@@ -248,7 +248,8 @@ __device__ __forceinline__ double prefix64(float x) {
 
 // A chunk of one key head: normalised K and Q as fragments, their products, and for each of
 // its value heads T and P. A wave owns 16 tokens, its lanes load q and k in fragment order;
-// the waves take each other's K from LDS. T = (I + A)^-1 by blocks of 16, in f32: the
+// the waves take each other's K from LDS (barriers order LDS only: the fragments' stores are
+// not waited for). T = (I + A)^-1 by blocks of 16, in f32: the
 // diagonal blocks by forward substitution (16 lanes each, a column a lane), then T_ij = -T_ii
 // sum_k A_ik T_kj down the block columns, a wave each, on v_mfma_f32_16x16x4_f32, whose result
 // tiles are the next product's B operand as they are.
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
         *reinterpret_cast<h4 *>(&kh[u][16 * w + m][32 * s + 16 + 4 * g]) = __builtin_shufflevector(kf[s][u], kf[s][u], 4, 5, 6, 7);
       }
   }
-  __syncthreads();
+  lds_barrier();
   if (!fine) bad = 1u;
   // ---- k_t . k_s and q_t . k_s of the wave's tokens with tiles 0 .. w
   f4 kk[4], qk[4];
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
     const int heads = a.s.rep - r0 < 2 ? a.s.rep - r0 : 2;
     const int64_t h0 = hk * a.s.rep + r0;
     const int64_t out = (b * a.chunks + chunk) * a.s.heads + h0;
-    __syncthreads();  // kh, or the heads before, are done with; bad is set
+    lds_barrier();  // kh, or the heads before, are done with; bad is set
     if (w < heads) {
       // e^-10000 is 0, but its sums would leave no bits for the others: the token path's
       const bool fit = gv <= 0.0f && gv >= -10000.0f && bv == bv;
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
         a.w.odd[out + w] = all && bad == 0u ? 0u : 1u;
       }
     }
-    __syncthreads();
+    lds_barrier();
     load_gates(r0 + 2);
     for (int e = 0; e < heads; ++e) {
       float4 row[4];
@@ -417,7 +418,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
         }
       }
     }
-    __syncthreads();
+    lds_barrier();
     // the fragments of a lower triangular matrix's rows 16 w ..
     const auto put_rows = [&](const float(*x)[kSq], h8 *o) {
 #pragma unroll
@@ -457,7 +458,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
 #pragma unroll
       for (int t = 0; t < 16; ++t) am[w][16 * g + t][16 * g + m] = D[t];
     }
-    __syncthreads();
+    lds_barrier();
     for (int e = 0; e < heads; ++e) {
       const int j = e == 0 ? w : 3 - w;  // long columns beside short ones
       f4 T[4];
@@ -490,7 +491,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
         for (int c = 0; c < 4; ++c) am[2 + e][16 * i + 4 * g + c][16 * j + m] = T[i][c];
       }
     }
-    __syncthreads();
+    lds_barrier();
     for (int e = 0; e < heads; ++e) put_rows(am[2 + e], a.w.t + (out + e) * 6 * kFrag);
   }
 }

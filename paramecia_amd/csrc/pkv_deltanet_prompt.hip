@@ -978,7 +978,17 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 }
 
 // A segment's chunks, and where its workspace's parts lie.
-constexpr int64_t kChunkedTokens = 48;          // prompts from here on go by chunks
+// Prompts go by chunks from 72 tokens on, from 48 where their heads fill the GPU more than
+// twice (token by token a workgroup per 16 rows). us of the call, by tokens / by chunks, 32 heads
+// of 128: one sequence 64 tokens 19.0 / 20.9, 80 22.6 / 22.6, 128 33.8 / 23.2; four 32 tokens
+// 22.2 / 28.5, 48 31.3 / 29.5; twelve 24 tokens 51.2 / 56.2, 48 75.3 / 58.6. 16 heads of 256: 64
+// tokens 29.1 / 26.0; 32 of 64: 96 tokens 19.7 / 20.2.
+bool by_chunks(int batch, int64_t n, int heads, int d) {
+  return n >= 72 || (n >= 48 && (int64_t)batch * heads * d > 8192);
+}
+// Longer segments have fewer launches and fuller last rounds of workgroups, until the
+// workspace leaves the 256 MB of last-level cache: 8001 tokens, 32 heads of 128, 48 MB 413 us,
+// 96 MB 361, 192 MB 360, all in one (290 MB) 425; seven of 1100 349, 255, 224, 212.
 constexpr size_t kSegmentBytes = (size_t)192 << 20;
 struct SegmentPlan {
   int chunks = 0;  // 0: token by token
@@ -986,7 +996,7 @@ struct SegmentPlan {
 };
 SegmentPlan plan_segment(int batch, int64_t n, int k_heads, int heads, int d) {
   SegmentPlan s;
-  if (n < kChunkedTokens) return s;
+  if (!by_chunks(batch, n, heads, d)) return s;
   const size_t key = (size_t)kC * d * 4;  // one operand of a key head's chunk
   const size_t per = (size_t)batch * (k_heads * 3 * key + heads * (2 * 6 * kFrag * 16 + 3 * kC * 4 + 16));
   const int64_t all = (n + kC - 1) / kC, fit = (int64_t)(kSegmentBytes / per);
@@ -1017,6 +1027,9 @@ int launch(const ScanArgs &a, const SegmentPlan &plan, int batch, int k_heads, v
                   reinterpret_cast<h8 *>(base + plan.kt), reinterpret_cast<h8 *>(base + plan.t),
                   reinterpret_cast<h8 *>(base + plan.p), reinterpret_cast<float *>(base + plan.meta),
                   reinterpret_cast<double *>(base + plan.gates), reinterpret_cast<unsigned *>(base + plan.odd)};
+  // 32 value channels a workgroup halve the fragments' loads, 16 give twice the workgroups: one
+  // sequence of 8001 tokens (256 workgroups of 16) 357 us with 16, 404 with 32; seven of
+  // 1100 282 and 226. Heads of 256 have no registers for 32.
   constexpr int kWide = kD <= 128 ? 2 : 1;
   const bool wide = kWide > 1 && (int64_t)batch * a.heads * (kD / 16) > 256;
   const int64_t all = (a.n + kC - 1) / kC;

@@ -493,30 +493,33 @@ def gated_o_proj(attn_output: torch.Tensor, gate: Optional[torch.Tensor], wo: to
 
 
 # ------------------------------------------------------------------ around the state update
-def _on_device(t: torch.Tensor, name: str, dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """t, refused unless it is a tensor of `dtype` on the current device: a launch goes to the
-    current device's stream, whose work another device's memory is not ordered with."""
-    if not t.is_cuda or t.dtype != dtype:
+def _device() -> int:
+    """The current device, whose current stream the calls go to; -2 where there is none."""
+    if _raw_device is not None and torch.cuda.is_initialized():
+        return _raw_device()
+    return torch.cuda.current_device() if torch.cuda.is_available() else -2
+
+
+def _take(t: Optional[torch.Tensor], name: str, shape, dev: int,
+          dtype: torch.dtype = torch.float32, writes: bool = False):
+    """t (None stays None), contiguous, refused unless it is a tensor of this shape and type on
+    the current device: a launch goes to that device's stream, with which another device's
+    memory is not ordered. A tensor that the call writes has to be contiguous itself."""
+    if t is None or (t.get_device() == dev and t.dtype is dtype and t.shape == shape and t.is_contiguous()):
+        return t
+    if not t.is_cuda or t.dtype is not dtype:
         raise KvCacheError(f"{name} must be a {str(dtype).replace('torch.', '')} device tensor")
-    if t.get_device() != torch.cuda.current_device():
+    if t.get_device() != dev:
         raise KvCacheError(f"{name} is on device {t.get_device()}, not on the current one")
-    return t
-
-
-def _shaped(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype = torch.float32):
-    """t (None stays None), contiguous, refused unless it has this shape."""
-    if t is None:
-        return None
     if tuple(t.shape) != tuple(shape):
         raise KvCacheError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    return _on_device(t, name, dtype).contiguous()
-
-
-def _in_place(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype = torch.float32):
-    """_shaped for a tensor that the call writes: it has to be contiguous itself."""
-    if t is not None and not t.is_contiguous():
+    if writes:
         raise KvCacheError(f"{name} is written in place and must be contiguous")
-    return _shaped(t, name, shape, dtype)
+    return t.contiguous()
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def causal_conv(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor,
@@ -527,27 +530,29 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor,
     taps], state [b, channels, taps - 1] (the inputs kept so far, updated in place), bias
     [channels]. lens: int32 [b], the valid tokens of a padded batch; rows of out behind them
     are left as they were (zeros if out is not given). Returns out [b, n, channels]."""
-    _on_device(x, "x")
+    dev = _device()
     if x.dim() != 3 or weight.dim() != 2:
         raise KvCacheError("causal_conv expects x [b, n, channels] and weight [channels, taps]")
     b, n, ch = x.shape
     if b == 0 or ch == 0:
         raise KvCacheError("causal_conv: b and channels must be > 0")
     taps = weight.shape[1]
-    if n and ((x.stride(2) != 1 and ch > 1) or (n > 1 and x.stride(1) < ch) or (b > 1 and x.stride(0) < ch)):
-        x = x.contiguous()
-    weight, bias = _shaped(weight, "weight", (ch, taps)), _shaped(bias, "bias", (ch,))
-    state = _in_place(state, "state", (b, ch, max(taps - 1, 0)))
-    lens = _shaped(lens, "lens", (b,), torch.int32)
+    sb, st, sc = x.stride()
+    if (x.get_device() != dev or x.dtype is not torch.float32 or
+            (n and ((sc != 1 and ch > 1) or (n > 1 and st < ch) or (b > 1 and sb < ch)))):
+        x = _take(x, "x", x.shape, dev)
+        sb, st, sc = x.stride()
+    weight, bias = _take(weight, "weight", (ch, taps), dev), _take(bias, "bias", (ch,), dev)
+    _take(state, "state", (b, ch, max(taps - 1, 0)), dev, writes=True)
+    lens = _take(lens, "lens", (b,), dev, torch.int32)
     if out is None:
         make = torch.empty if lens is None else torch.zeros
         out = make((b, n, ch), dtype=torch.float32, device=x.device)
     else:
-        _in_place(out, "out", (b, n, ch))
-    _call(lib().pkv_causal_conv(x.data_ptr(), x.stride(0) if b > 1 else 0,
-                                x.stride(1) if n > 1 else ch, weight.data_ptr(), _ptr(bias),
-                                state.data_ptr(), _ptr(lens), out.data_ptr(), b, n, ch, taps,
-                                int(silu), _stream()))
+        _take(out, "out", (b, n, ch), dev, writes=True)
+    _call(lib().pkv_causal_conv(x.data_ptr(), sb if b > 1 else 0, st if n > 1 else ch,
+                                weight.data_ptr(), _at(bias), state.data_ptr(), _at(lens),
+                                out.data_ptr(), b, n, ch, taps, silu, _stream()))
     return out
 
 
@@ -561,38 +566,40 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate: to
     taken as they are), gate (log decay) and beta (pre-sigmoid) [b, n, heads]; state [b,
     heads, d, d] and gate_offset [b, heads] are updated in place. Value head h reads key
     head h // (heads // key heads). lens, out as causal_conv. Returns out [b, n, heads, d]."""
+    dev = _device()
     if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2] or v.shape[3] != q.shape[3]:
         raise KvCacheError("gated_delta_rule expects q, k [b, n, key heads, d] and v [b, n, heads, d]")
     b, n, hk, d = q.shape
     h = v.shape[2]
     if b == 0 or hk == 0 or h % hk:
         raise KvCacheError(f"gated_delta_rule: {h} value heads over {hk} key heads of {b} sequences")
-    ins = []
+    ins, strides = [], []
     for t, name, heads in ((q, "q", hk), (k, "k", hk), (v, "v", h)):
-        _on_device(t, name)
         sb, st, sh, sd = t.stride()
+        if t.get_device() != dev or t.dtype is not torch.float32:
+            t = _take(t, name, t.shape, dev)
         if (sd != 1 or (heads > 1 and sh != d) or (n > 1 and (st < heads * d or st % 4)) or
                 (b > 1 and (sb < heads * d or sb % 4)) or t.data_ptr() % 16):
             t = t.clone(memory_format=torch.contiguous_format)
+            sb, st, sh, sd = t.stride()
         ins.append(t)
-    gate, beta = _shaped(gate, "gate", (b, n, h)), _shaped(beta, "beta", (b, n, h))
-    state = _in_place(state, "state", (b, h, d, d))
-    gate_offset = _in_place(gate_offset, "gate_offset", (b, h))
-    lens = _shaped(lens, "lens", (b,), torch.int32)
+        strides += (sb if b > 1 else 0, st if n > 1 else 0)
+    gate, beta = _take(gate, "gate", (b, n, h), dev), _take(beta, "beta", (b, n, h), dev)
+    _take(state, "state", (b, h, d, d), dev, writes=True)
+    _take(gate_offset, "gate_offset", (b, h), dev, writes=True)
+    lens = _take(lens, "lens", (b,), dev, torch.int32)
     if out is None:
         make = torch.empty if lens is None else torch.zeros
         out = make((b, n, h, d), dtype=torch.float32, device=v.device)
     else:
-        _in_place(out, "out", (b, n, h, d))
-    strides = (ctypes.c_int64 * 6)(*(x for t in ins for x in (t.stride(0) if b > 1 else 0,
-                                                              t.stride(1) if n > 1 else 0)))
+        _take(out, "out", (b, n, h, d), dev, writes=True)
     need = lib().pkv_deltanet_prompt_workspace(b, n, hk, h, d)
     # torch's allocator orders the workspace with the stream, and gives each graph its own
     ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need else None
-    _call(lib().pkv_deltanet_prompt(ins[0].data_ptr(), ins[1].data_ptr(), ins[2].data_ptr(), strides,
-                                    gate.data_ptr(), beta.data_ptr(), state.data_ptr(),
-                                    _ptr(gate_offset), _ptr(lens), out.data_ptr(), b, n, hk, h, d,
-                                    scale, eps, _ptr(ws), need, _stream()))
+    _call(lib().pkv_deltanet_prompt(ins[0].data_ptr(), ins[1].data_ptr(), ins[2].data_ptr(),
+                                    (ctypes.c_int64 * 6)(*strides), gate.data_ptr(), beta.data_ptr(),
+                                    state.data_ptr(), _at(gate_offset), _at(lens), out.data_ptr(),
+                                    b, n, hk, h, d, scale, eps, _at(ws), need, _stream()))
     return out
 
 
@@ -603,20 +610,26 @@ def rms_norm(x: torch.Tensor, alpha: torch.Tensor, eps: float,
     updated to h in place), y = h / sqrt(mean(h^2) + eps) * alpha, times silu(gate) if gate is
     given. Returns (y or None, Q8_0 blocks or None): y as x, the blocks uint8 [.., ceil(d / 32),
     34] (an f16 scale and 32 int8 codes each)."""
-    _on_device(x, "x")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    dev = _device()
+    shape = x.shape
+    if not shape or shape[-1] == 0:
         raise KvCacheError("rms_norm expects rows")
-    d = x.shape[-1]
+    if not f32_out and not q8_0_out:
+        raise KvCacheError("rms_norm: no output is asked for")
+    d = stride = shape[-1]
     rows = x.numel() // d
-    if not x.is_contiguous() and not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= d):
-        x = x.contiguous()
-    alpha = _shaped(alpha, "alpha", (d,))
-    residual, gate = _in_place(residual, "residual", x.shape), _shaped(gate, "gate", x.shape)
-    y = torch.empty(x.shape, dtype=torch.float32, device=x.device) if f32_out else None
-    q8 = torch.empty(x.shape[:-1] + ((d + 31) // 32, 34), dtype=torch.uint8, device=x.device) if q8_0_out else None
-    stride = d if x.is_contiguous() else x.stride(0)
-    _call(lib().pkv_rms_norm(x.data_ptr(), stride, _ptr(residual), alpha.data_ptr(), _ptr(gate), eps,
-                             _ptr(y), _ptr(q8), rows, d, _stream()))
+    if x.get_device() != dev or x.dtype is not torch.float32 or not x.is_contiguous():
+        if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= d and x.get_device() == dev and x.dtype is torch.float32:
+            stride = x.stride(0)
+        else:
+            x = _take(x, "x", shape, dev)
+    alpha = _take(alpha, "alpha", (d,), dev)
+    _take(residual, "residual", shape, dev, writes=True)
+    gate = _take(gate, "gate", shape, dev)
+    y = torch.empty(shape, dtype=torch.float32, device=x.device) if f32_out else None
+    q8 = torch.empty(shape[:-1] + ((d + 31) // 32, 34), dtype=torch.uint8, device=x.device) if q8_0_out else None
+    _call(lib().pkv_rms_norm(x.data_ptr(), stride, _at(residual), alpha.data_ptr(), _at(gate), eps,
+                             _at(y), _at(q8), rows, d, _stream()))
     return y, q8
 
 
@@ -632,8 +645,9 @@ def gated_o_proj_lora(attn_output: torch.Tensor, gate: Optional[torch.Tensor], w
     [adapters, out_dim, rank] in float32, float16 or bfloat16, lora_scale f32 [adapters];
     adapter_ids int32, one per row (attn_output's shape without its last dimension), negative
     for none. Everything else as gated_o_proj."""
-    x = _on_device(attn_output, "attn_output").contiguous()
-    g = _shaped(gate, "gate", x.shape)
+    dev = _device()
+    x = _take(attn_output, "attn_output", attn_output.shape, dev)
+    g = _take(gate, "gate", x.shape, dev)
     if w_type not in _W_BLOCK:
         raise KvCacheError(f"unsupported weight type {w_type} (Q8_0 8, Q4K 12, Q5K 13, Q6K 14)")
     in_dim = x.shape[-1]
@@ -641,20 +655,20 @@ def gated_o_proj_lora(attn_output: torch.Tensor, gate: Optional[torch.Tensor], w
     blk, nbytes = _W_BLOCK[w_type]
     if wo.numel() != out_dim * (in_dim // blk) * nbytes:
         raise KvCacheError(f"wo must hold out_dim x in_dim / {blk} blocks of {nbytes} B")
-    w = _on_device(wo, "wo", torch.uint8).contiguous()
+    w = _take(wo, "wo", wo.shape, dev, torch.uint8)
     if lora_a.dim() != 3 or lora_a.dtype not in _LORA_TYPE:
         raise KvCacheError("lora_a must be a float32, float16 or bfloat16 [adapters, rank, in_dim] tensor")
-    n, rank = lora_a.shape[:2]
-    a = _shaped(lora_a, "lora_a", (n, rank, in_dim), lora_a.dtype)
-    b = _shaped(lora_b, "lora_b", (n, out_dim, rank), lora_a.dtype)
-    scale = _shaped(lora_scale, "lora_scale", (n,))
-    ids = _shaped(adapter_ids, "adapter_ids", x.shape[:-1], torch.int32)
+    n, rank, _ = lora_a.shape
+    a = _take(lora_a, "lora_a", (n, rank, in_dim), dev, lora_a.dtype)
+    b = _take(lora_b, "lora_b", (n, out_dim, rank), dev, lora_a.dtype)
+    scale = _take(lora_scale, "lora_scale", (n,), dev)
+    ids = _take(adapter_ids, "adapter_ids", x.shape[:-1], dev, torch.int32)
     out = torch.empty(x.shape[:-1] + (out_dim,), dtype=torch.float32, device=x.device)
     if rows == 0:
         return out
     need = lib().pkv_gated_oproj_lora_workspace(w_type, rows, in_dim, out_dim, rank)
-    ws = torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
-    _call(lib().pkv_gated_oproj_lora(x.data_ptr(), _ptr(g), w.data_ptr(), w_type, a.data_ptr(),
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _call(lib().pkv_gated_oproj_lora(x.data_ptr(), _at(g), w.data_ptr(), w_type, a.data_ptr(),
                                      b.data_ptr(), _LORA_TYPE[a.dtype], n, rank, scale.data_ptr(),
                                      ids.data_ptr(), out.data_ptr(), rows, in_dim, out_dim,
                                      ws.data_ptr(), need, _stream()))

@@ -83,14 +83,15 @@ __global__ __launch_bounds__(256) void conv_kernel(ConvArgs a) {
     for (int j = 0; j < K - 1; ++j) {
       const int64_t at = end + j;  // of kept inputs followed by new ones
       float v[kV];
-      if (at >= K - 1) {
+      if (kTile > 4 && at >= K - 1) {
         load(at - (K - 1), v);
-      } else {  // a prompt shorter than the kept inputs
+      } else {  // a prompt that the tile's registers hold, or one shorter than the kept inputs
+        constexpr int kHeld = kTile > 4 ? K - 1 : K - 1 + kTile;
 #pragma unroll
         for (int i = 0; i < kV; ++i) {
           v[i] = 0.0f;
 #pragma unroll
-          for (int s = 0; s < K - 1; ++s) v[i] = at == s ? xv[s][i] : v[i];
+          for (int s = 0; s < kHeld; ++s) v[i] = at == s ? xv[s][i] : v[i];
         }
       }
 #pragma unroll

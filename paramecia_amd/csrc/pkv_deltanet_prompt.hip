@@ -18,9 +18,11 @@
 // then walks each head's chunks, its state in registers. Products run on
 // v_mfma_f32_16x16x32_f16 with every operand in two fp16 parts (22 bits; hi hi + hi lo + lo hi),
 // which is exact to about f32: k, q, T and P are at most 1 in magnitude, and M, R and U are
-// scaled by powers of two from bounds that hold while no gate is positive. A head with a
-// positive gate, or a value that is not finite or past 2^90, goes token by token instead (a
-// NaN then reaches the tokens behind it and no others, as there).
+// scaled, each value channel by a power of two of its own, from bounds that hold while no gate
+// is positive. (Within a channel the parts keep 22 bits of a value down to some 2^-20 of the
+// chunk's largest.) A head with a positive gate, with a key or query that normalisation leaves
+// below 2^-8, or with a value that is not finite or past 2^90, goes token by token instead (a NaN
+// then reaches the tokens behind it and no others, as there).
 #include <type_traits>
 
 #include "pkv_q8_common.hpp"
@@ -186,6 +188,7 @@ __global__ __launch_bounds__(256) void scan_tokens_kernel(ScanArgs a) {
 
 // ---- by chunks
 constexpr int kC = 64;           // tokens per chunk
+constexpr int kMeta = 3 * kC + 4;
 constexpr float kUp = 1024.0f;   // scale of the fp16 parts of k, q, T and P (at most 1)
 constexpr float kDown = 1.0f / 1024.0f;
 
@@ -207,7 +210,8 @@ struct ChunkWs {
   h8 *k, *q;       // [b][chunk][key head][row tile 4][d / 32][2][64]
   h8 *kt;          // [b][chunk][key head][d / 16][k step 2][2][64]: rows are key channels
   h8 *t, *p;       // [b][chunk][head][6][2][64]
-  float *meta;     // [b][chunk][head][3][64]: be, e^G, e^(G_63 - G)
+  float *meta;     // [b][chunk][head][kMeta]: be, e^G, e^(G_63 - G) of its tokens; then the
+                   // largest be, the largest be e^(G_63 - G), and e^(G_63)
   double *gates;   // [b][chunk][head]: the chunk's sum
   unsigned *odd;   // [b][chunk][head]: this chunk needs the token path
 };
@@ -221,6 +225,26 @@ struct ChunkArgs {
 };
 __device__ __forceinline__ int tri(int w, int p) { return w < 2 ? w : 2 * w - 2 + p; }
 
+__device__ __forceinline__ uint32_t mag(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ float as_f(uint32_t x) { return __builtin_bit_cast(float, x); }
+// over the four lanes l % 16 apart (all of them receive it)
+__device__ __forceinline__ uint32_t groups_max(uint32_t x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = umax(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return umax(b[0], b[1]);
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  const auto dpp = [](uint32_t v, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, decltype(ctrl)::value, 0xF, 0xF, false);
+  };
+  x = umax(x, dpp(x, std::integral_constant<int, 0xB1>{}));
+  x = umax(x, dpp(x, std::integral_constant<int, 0x4E>{}));
+  x = umax(x, dpp(x, std::integral_constant<int, 0x141>{}));
+  x = umax(x, dpp(x, std::integral_constant<int, 0x140>{}));
+  return groups_max(x);
+}
 __device__ __forceinline__ double read_lane(double x, int lane) {
   const uint64_t u = __builtin_bit_cast(uint64_t, x);
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
@@ -300,17 +324,20 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float sq = 0.0f;
+      bool any = false;
 #pragma unroll
       for (int s = 0; s < kS; ++s)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           x[u][s][i] = on ? x[u][s][i] : 0.0f;
+          any = any || x[u][s][i] != 0.0f;
           sq = fmaf(x[u][s][i], x[u][s][i], sq);
         }
       sq += __shfl_xor(sq, 16);
       sq += __shfl_xor(sq, 32);
       const float up = on ? kUp / __builtin_sqrtf(sq + a.s.eps) : 0.0f;
-      fine = fine && sq < 3.0e38f && up < 3.0e38f;  // false for NaN
+      // false for NaN; an all but vanishing vector would leave its fp16 parts without bits
+      fine = fine && sq < 3.0e38f && up < 3.0e38f && (sq > 0x1p-16f * a.s.eps || !any);
 #pragma unroll
       for (int s = 0; s < kS; ++s)
 #pragma unroll
@@ -388,10 +415,13 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
       const double G2 = G * 1.4426950408889634;
       const float hi = (float)G2;
       gam[w][lane] = float4{hi, (float)(G2 - (double)hi), be, 0.0f};
-      float *meta = a.w.meta + (out + w) * 3 * kC + lane;
-      meta[0] = be;
-      meta[kC] = expf((float)G);
-      meta[2 * kC] = expf((float)(last - G));
+      float *meta = a.w.meta + (out + w) * kMeta;
+      const float ec = expf((float)(last - G));
+      meta[lane] = be;
+      meta[kC + lane] = expf((float)G);
+      meta[2 * kC + lane] = ec;
+      const uint32_t mb = wave_max(mag(be)), mc = wave_max(mag(be * ec));
+      if (lane < 4) meta[3 * kC + lane] = lane == 0 ? as_f(mb) : lane == 1 ? as_f(mc) : expf((float)last);
       const bool all = __ballot(!fit) == 0;
       if (lane == 0) {
         a.w.gates[out + w] = last;
@@ -496,21 +526,6 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
   }
 }
 
-__device__ __forceinline__ uint32_t mag(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
-__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-  const auto dpp = [](uint32_t v, auto ctrl) {
-    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, decltype(ctrl)::value, 0xF, 0xF, false);
-  };
-  x = umax(x, dpp(x, std::integral_constant<int, 0xB1>{}));
-  x = umax(x, dpp(x, std::integral_constant<int, 0x4E>{}));
-  x = umax(x, dpp(x, std::integral_constant<int, 0x141>{}));
-  x = umax(x, dpp(x, std::integral_constant<int, 0x140>{}));
-  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  x = umax(a[0], a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  return umax(b[0], b[1]);
-}
 // the largest magnitude of eight fp16 values, as bits (a NaN is larger than everything)
 __device__ __forceinline__ uint32_t top16(h8 x) {
   uint32_t t = 0u;
@@ -523,6 +538,8 @@ __device__ __forceinline__ int scale_exp(float bound) {
   const int e = 14 - ((int)(__builtin_bit_cast(uint32_t, bound) >> 23) - 127);
   return e > 100 ? 100 : e;
 }
+// 1 / x of a power of two
+__device__ __forceinline__ float inverse2(float x) { return as_f(0x7F000000u - __builtin_bit_cast(uint32_t, x)); }
 __device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (uint32_t)(e + 127) << 23); }
 
 template <int kD, int kNT>
@@ -530,7 +547,7 @@ union StateLds {
   struct {
     h8 m[kNT][kD / 32][2][64];  // the state's fragments
     uint2 r[kNT][2][2][64][2], u[kNT][2][2][64][2], v[kNT][2][2][64][2];  // R, U, U e^(G_63 - G): [k step][part][lane][half]
-    uint32_t top[2][3][4];  // [chunk's parity][maximum][wave], bits of magnitudes
+    uint4 top[2][3][kNT][16];  // [chunk's parity][maximum][..][channel], a word of each wave: bits of magnitudes
     unsigned odd;
   } c;
   TokenStage<kD> t;
@@ -603,8 +620,8 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   const int tokens = (int)(end - a.first), chunks = (tokens + kC - 1) / kC;
   const int64_t kstep = (int64_t)a.k_heads * 4 * kS * kFrag, tstep = (int64_t)a.s.heads * 6 * kFrag;
   const int64_t key0 = b * a.chunks * a.k_heads + hk, val0 = b * a.chunks * a.s.heads + h;
-  const int64_t mstep = (int64_t)a.s.heads * 3 * kC;
-  const float *meta = a.w.meta + val0 * 3 * kC;
+  const int64_t mstep = (int64_t)a.s.heads * kMeta;
+  const float *meta = a.w.meta + val0 * kMeta;
   const float *v0 = a.s.v + b * a.s.vb + a.first * a.s.vt + h * kD + row0;
   const uint32_t moff = 4u * (uint32_t)(16 * w + 4 * g), foff = 16u * (uint32_t)lane;
   // v of token 16 w + 4 g + m % 4, channels 4 (m / 4) .. + 3 (one 16-byte load, 64-byte rows):
@@ -623,24 +640,40 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   for (int c = tid; c < chunks; c += 512)
     if (a.w.odd[val0 + (int64_t)c * a.s.heads] != 0u) lds.c.odd = 1u;
 
-  // The scales of a chunk come from bounds: a row of the state has a norm of at most `root`
-  // = sqrt(d) max |M| of the chunk before + 64 max |v| of that chunk, and each token of this
-  // one adds its |v| at most. So R and U stay below root + 65 max |v|, the next state below
-  // root + 64 max |v|. Waves 4 - 7 find the maxima beside the others' work: top[0] of M in
-  // front of the chunk before, top[1] and top[2] of v in that chunk and in this one.
+  // A channel's scales in a chunk come from bounds. With N on the norm of its row of the state
+  // in front of a chunk, V on its |v| there, w = e^(G_63), x the largest be e^(G_63 - G): each
+  // token adds its |v| at most, so the row behind has a norm of at most N + 64 V, and of w N +
+  // 64 x (N + 65 V), as |u| <= be (|v| + norm). N of this chunk comes from the state in front of
+  // the one before: waves 4 - 7 find the maxima beside the others' work (top[0]: |M| in front
+  // of the chunk before, top[1] and top[2]: |v| in that chunk and in this one).
   constexpr float kRoot = kD == 64 ? 8.1f : kD == 128 ? 11.4f : 16.1f;  // above sqrt(d)
   bool odd;
-  int eu, em1;
+  // 2^e: of the state in front of the chunk, of R and U, of U e^(G_63 - G), of the state behind
+  float sm[kNT], su[kNT], sv[kNT], sm1[kNT];
+  f4 ex0, ex1;  // of the chunk before and of this one: the largest be, x, w
+  const auto behind = [](float N, float V, const f4 &ex) {
+    return fminf(fmaf(64.0f, V, N), fmaf(ex[2], N, 64.0f * ex[1] * fmaf(65.0f, V, N)));
+  };
   const auto get_scales = [&](int c) {
-    uint32_t x[3];
+    uint32_t any = 0u;
 #pragma unroll
-    for (int k = 0; k < 3; ++k)
-      x[k] = umax(umax(lds.c.top[c & 1][k][0], lds.c.top[c & 1][k][1]), umax(lds.c.top[c & 1][k][2], lds.c.top[c & 1][k][3]));
-    odd = odd || umax(umax(x[0], x[1]), x[2]) > 0x6C800000u;  // 2^90
-    const float root = fmaf(kRoot, __builtin_bit_cast(float, x[0]), 64.0f * __builtin_bit_cast(float, x[1]));
-    const float vtop = __builtin_bit_cast(float, x[2]);
-    eu = __builtin_amdgcn_readfirstlane(scale_exp(fmaf(65.0f, vtop, root)));
-    em1 = __builtin_amdgcn_readfirstlane(scale_exp(fmaf(64.0f, vtop, root)));
+    for (int j = 0; j < kNT; ++j) {
+      uint32_t x[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const uint4 t = lds.c.top[c & 1][k][j][m];
+        x[k] = umax(umax(t.x, t.y), umax(t.z, t.w));
+        any = umax(any, x[k]);
+      }
+      const float N = c == 0 ? kRoot * as_f(x[0]) : behind(kRoot * as_f(x[0]), as_f(x[1]), ex0), V = as_f(x[2]);
+      const float bound = fmaf(65.0f, V, N);
+      // U's own errors, which do not shrink with be, must stay in range too
+      const int eu = scale_exp(bound * ex1[0]), ev = scale_exp(bound * ex1[1]);
+      su[j] = pow2(eu);
+      sv[j] = pow2(ev < eu + 24 ? ev : eu + 24);
+      sm1[j] = pow2(scale_exp(behind(N, V, ex1)));
+    }
+    odd = odd || __ballot(any > 0x6C800000u) != 0;  // 2^90
   };
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   odd = false;
@@ -652,7 +685,6 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     float *state = a.s.state + ((b * a.s.heads + h) * kD + row0 + m) * kD + w * (kD / 4) + 4 * g;
     h8 ka[kS][2], kb[kDeep ? kS : 1][2], ktf[kN][2][2], tf[2][2];
     f4 v[kNT], be, eg, ec;
-    float whole;
     const auto load_k = [&](int c, h8 (*f)[2]) {
       const h8 *p = kw + (c < chunks ? c : chunks - 1) * kstep;
 #pragma unroll
@@ -677,14 +709,15 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) ktf[n][p][u] = at<h8>(q + (n * 2 + p) * kFrag + 64 * u, foff);
     };
-    const auto load_meta = [&](int c, f4 &x, f4 &y, f4 &z, float &all) {
+    const auto load_meta = [&](int c, f4 &x, f4 &y, f4 &z, f4 &ex) {
       const float *p = meta + c * mstep;
       x = at<f4>(p, moff);
       y = at<f4>(p + kC, moff);
       z = at<f4>(p + 2 * kC, moff);
-      all = at<float>(p + 2 * kC - 1, 0u);  // e^(G_63)
+      ex = at<f4>(p + 3 * kC, 0u);
     };
-    load_meta(0, be, eg, ec, whole);
+    load_meta(0, be, eg, ec, ex1);
+    ex0 = ex1;
     load_v(0, v);
 #pragma unroll
     for (int j = 0; j < kNT; ++j) v[j] = transpose4(v[j]);
@@ -697,31 +730,30 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     for (int j = 0; j < kNT; ++j)
 #pragma unroll
       for (int n = 0; n < kN; ++n) M[j][n] = *reinterpret_cast<const f4 *>(state + 16 * j * kD + 16 * n);
-    {  // the first chunk's maxima: of M in front of it (nothing before adds to it) and of v
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) {  // the first chunk's maxima: of M in front of it and of v
       uint32_t x = 0u, y = 0u;
 #pragma unroll
-      for (int j = 0; j < kNT; ++j)
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-          for (int n = 0; n < kN; ++n) x = umax(x, mag(M[j][n][i]));
-          y = umax(y, mag(v[j][i]));
-        }
-      x = wave_max(x);
-      y = wave_max(y);
-      if (lane == 0) {
-        lds.c.top[0][0][w] = x;
-        lds.c.top[0][1][w] = 0u;
-        lds.c.top[0][2][w] = y;
+        for (int n = 0; n < kN; ++n) x = umax(x, mag(M[j][n][i]));
+        y = umax(y, mag(v[j][i]));
+      }
+      x = groups_max(x);
+      y = groups_max(y);
+      if (g == 0) {
+        reinterpret_cast<uint32_t *>(&lds.c.top[0][0][j][m])[w] = x;
+        reinterpret_cast<uint32_t *>(&lds.c.top[0][1][j][m])[w] = 0u;
+        reinterpret_cast<uint32_t *>(&lds.c.top[0][2][j][m])[w] = y;
       }
     }
-    const auto put_m = [&](float up) {
+    const auto put_m = [&](const float (&up)[kNT]) {
 #pragma unroll
       for (int j = 0; j < kNT; ++j)
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
           uint2 hi, lo;
-          split4(M[j][n] * up, hi, lo);
+          split4(M[j][n] * up[j], hi, lo);
           const int k = w * kN + n;
           reinterpret_cast<uint2 *>(&lds.c.m[j][k >> 1][0][lane])[k & 1] = hi;
           reinterpret_cast<uint2 *>(&lds.c.m[j][k >> 1][1][lane])[k & 1] = lo;
@@ -736,15 +768,19 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     __syncthreads();
     odd = lds.c.odd != 0u;
     get_scales(0);
-    int em = em1;  // its bound holds for the chunk's own state too
-    if (!odd) put_m(pow2(em));
+    const auto first_scale = [&](int j) {  // of the state as it comes: its largest value is known
+      const uint4 t = lds.c.top[0][0][j][m];
+      return pow2(scale_exp(as_f(umax(umax(t.x, t.y), umax(t.z, t.w)))));
+    };
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) sm[j] = first_scale(j);
+    if (!odd) put_m(sm);
     lds_barrier();
 
     const auto step = [&](int c, h8 (*kf)[2]) {
       const int next = c + 1 < chunks ? c + 1 : c;
-      f4 bn, gn, cn, vn[kNT];
-      float wn;
-      load_meta(next, bn, gn, cn, wn);
+      f4 bn, gn, cn, en, vn[kNT];
+      load_meta(next, bn, gn, cn, en);
       load_v(next, vn);
       // ---- R = be (V - e^G K M)
       f4 km[kNT], kx[kNT], ky[kNT];
@@ -759,17 +795,17 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           kx[j] = mfma32(kf[s][0], lo, kx[j]);
           ky[j] = mfma32(kf[s][1], hi, ky[j]);
         }
-      const float dm = kDown * pow2(-em), up = pow2(eu);
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
         f4 r;
+        const float dm = kDown * inverse2(sm[j]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = (be[i] * up) * fmaf(-(eg[i] * dm), km[j][i] + (kx[j][i] + ky[j][i]), v[j][i]);
+        for (int i = 0; i < 4; ++i) r[i] = (be[i] * su[j]) * fmaf(-(eg[i] * dm), km[j][i] + (kx[j][i] + ky[j][i]), v[j][i]);
         put4(lds.c.r[j][w >> 1], r);
       }
       load_k(c + (kDeep ? 2 : 1), kf);
       lds_barrier();
-      // ---- U = T R, times 2^eu
+      // ---- U = T R, times 2^e
       f4 u[kNT], ux[kNT], uy[kNT];
 #pragma unroll
       for (int j = 0; j < kNT; ++j) u[j] = ux[j] = uy[j] = zero;
@@ -788,15 +824,15 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
       for (int j = 0; j < kNT; ++j) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[j][i] = (u[j][i] + (ux[j][i] + uy[j][i])) * kDown;
-        put4(lds.c.v[j][w >> 1], u[j] * ec);
+        put4(lds.c.v[j][w >> 1], u[j] * (ec * (sv[j] * inverse2(su[j]))));
         put4(lds.c.u[j][w >> 1], u[j]);
       }
       load_t(next);
       lds_barrier();
       // ---- the next state
-      const float du = kDown * pow2(-eu);
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
+        const float dv = kDown * inverse2(sv[j]);
         f4 n0[kN], nx[kN], ny[kN];
 #pragma unroll
         for (int n = 0; n < kN; ++n) n0[n] = nx[n] = ny[n] = zero;
@@ -813,17 +849,19 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) M[j][n][i] = fmaf(M[j][n][i], whole, (n0[n][i] + (nx[n][i] + ny[n][i])) * du);
+          for (int i = 0; i < 4; ++i) M[j][n][i] = fmaf(M[j][n][i], ex1[2], (n0[n][i] + (nx[n][i] + ny[n][i])) * dv);
       }
-      put_m(pow2(em1));
+      put_m(sm1);
       load_kt(next);
 #pragma unroll
       for (int j = 0; j < kNT; ++j) v[j] = transpose4(vn[j]);
       be = bn;
       eg = gn;
       ec = cn;
-      whole = wn;
-      em = em1;
+      ex0 = ex1;
+      ex1 = en;
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) sm[j] = sm1[j];
       lds_barrier();
       get_scales(c + 1);
     };
@@ -865,6 +903,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           if (p <= w >> 1) pf[p][u] = at<h8>(q + p * kFrag + 64 * u, foff);
     };
     eg = at<f4>(meta + kC, moff);
+    ex0 = ex1 = at<f4>(meta + 3 * kC, 0u);
     f4 v[kNT];
     load_v(chunks > 1 ? 1 : 0, v);
     load_q(0, qa);
@@ -873,17 +912,22 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     __syncthreads();
     odd = lds.c.odd != 0u;
     get_scales(0);
-    int em = em1;
-    uint32_t vnow = lds.c.top[0][2][w];  // max |v| of the wave's tokens in this chunk
+    uint32_t vnow[kNT];  // largest |v| of the wave's tokens in this chunk
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) {
+      const uint4 t = lds.c.top[0][0][j][m];
+      sm[j] = pow2(scale_exp(as_f(umax(umax(t.x, t.y), umax(t.z, t.w)))));
+      vnow[j] = reinterpret_cast<const uint32_t *>(&lds.c.top[0][2][j][m])[w];
+    }
     lds_barrier();
 
     const auto step = [&](int c, h8 (*qf)[2]) {
       const int next = c + 1 < chunks ? c + 1 : c;
-      const f4 gn = at<f4>(meta + next * mstep + kC, moff);
+      const f4 gn = at<f4>(meta + next * mstep + kC, moff), en = at<f4>(meta + next * mstep + 3 * kC, 0u);
       f4 qm[kNT], qx[kNT], qy[kNT];
 #pragma unroll
       for (int j = 0; j < kNT; ++j) qm[j] = qx[j] = qy[j] = zero;
-      uint32_t top = 0u;  // largest magnitude of the state's high parts, as fp16 bits
+      uint32_t top[kNT] = {};  // largest magnitudes of the state's high parts, as fp16 bits
 #pragma unroll
       for (int s = 0; s < kS; ++s)
 #pragma unroll
@@ -892,30 +936,30 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           qm[j] = mfma32(qf[s][0], hi, qm[j]);
           qx[j] = mfma32(qf[s][0], lo, qx[j]);
           qy[j] = mfma32(qf[s][1], hi, qy[j]);
-          if ((s & 3) == w || kS == 2) top = umax(top, top16(hi));  // a quarter of the state each
+          if ((s & 3) == w || kS == 2) top[j] = umax(top[j], top16(hi));  // a quarter of the state each
         }
       load_q(c + (kDeep ? 2 : 1), qf);
-      const float dm = kDown * pow2(-em) * a.s.scale, du = kDown * pow2(-eu) * a.s.scale;
 #pragma unroll
-      for (int j = 0; j < kNT; ++j)
+      for (int j = 0; j < kNT; ++j) {
+        const float dm = kDown * inverse2(sm[j]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) qm[j][i] = eg[i] * ((qm[j][i] + (qx[j][i] + qy[j][i])) * dm);
+      }
       lds_barrier();
       // the next chunk's maxima: M in front of this chunk, v of this chunk and of the next
-      uint32_t vnext = 0u;
 #pragma unroll
-      for (int j = 0; j < kNT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vnext = umax(vnext, mag(v[j][i]));
-      vnext = wave_max(vnext);
-      top = wave_max(top);
-      if (lane == 0) {
-        const float x = (float)__builtin_bit_cast(_Float16, (uint16_t)top) * pow2(-em) * 1.001f;
-        lds.c.top[(c + 1) & 1][0][w] = mag(x);
-        lds.c.top[(c + 1) & 1][1][w] = vnow;
-        lds.c.top[(c + 1) & 1][2][w] = vnext;
+      for (int j = 0; j < kNT; ++j) {
+        const f4 x = transpose4(v[j]);
+        const uint32_t vnext = groups_max(umax(umax(mag(x[0]), mag(x[1])), umax(mag(x[2]), mag(x[3]))));
+        const uint32_t mtop = groups_max(top[j]);
+        if (g == 0) {
+          const float t = (float)__builtin_bit_cast(_Float16, (uint16_t)mtop) * inverse2(sm[j]) * 1.001f;
+          reinterpret_cast<uint32_t *>(&lds.c.top[(c + 1) & 1][0][j][m])[w] = mag(t);
+          reinterpret_cast<uint32_t *>(&lds.c.top[(c + 1) & 1][1][j][m])[w] = vnow[j];
+          reinterpret_cast<uint32_t *>(&lds.c.top[(c + 1) & 1][2][j][m])[w] = vnext;
+        }
+        vnow[j] = vnext;
       }
-      vnow = vnext;
       load_v(c + 2 < chunks ? c + 2 : chunks - 1, v);
       lds_barrier();
       f4 o[kNT], ox[kNT], oy[kNT];
@@ -934,11 +978,15 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
       }
       load_p(next);
 #pragma unroll
-      for (int j = 0; j < kNT; ++j)
+      for (int j = 0; j < kNT; ++j) {
+        const float du = kDown * inverse2(su[j]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[j][i] = fmaf(o[j][i] + (ox[j][i] + oy[j][i]), du, qm[j][i]);
+        for (int i = 0; i < 4; ++i) o[j][i] = a.s.scale * fmaf(o[j][i] + (ox[j][i] + oy[j][i]), du, qm[j][i]);
+        sm[j] = sm1[j];
+      }
       eg = gn;
-      em = em1;
+      ex0 = ex1;
+      ex1 = en;
       lds_barrier();
       // 64 bytes of each token's row, as load_v
 #pragma unroll
@@ -998,7 +1046,7 @@ SegmentPlan plan_segment(int batch, int64_t n, int k_heads, int heads, int d) {
   SegmentPlan s;
   if (!by_chunks(batch, n, heads, d)) return s;
   const size_t key = (size_t)kC * d * 4;  // one operand of a key head's chunk
-  const size_t per = (size_t)batch * (k_heads * 3 * key + heads * (2 * 6 * kFrag * 16 + 3 * kC * 4 + 16));
+  const size_t per = (size_t)batch * (k_heads * 3 * key + heads * (2 * 6 * kFrag * 16 + kMeta * 4 + 16));
   const int64_t all = (n + kC - 1) / kC, fit = (int64_t)(kSegmentBytes / per);
   const int64_t parts = (all + (fit < 1 ? 1 : fit) - 1) / (fit < 1 ? 1 : fit);
   s.chunks = (int)((all + parts - 1) / parts);  // segments of about one length
@@ -1008,7 +1056,7 @@ SegmentPlan plan_segment(int batch, int64_t n, int k_heads, int heads, int d) {
   s.t = 3 * s.q;
   s.p = s.t + vals * 6 * kFrag * 16;
   s.meta = s.p + vals * 6 * kFrag * 16;
-  s.gates = s.meta + vals * 3 * kC * 4;
+  s.gates = s.meta + vals * kMeta * 4;
   s.odd = s.gates + vals * 8;
   s.bytes = s.odd + (vals * 4 + 15) / 16 * 16;
   return s;

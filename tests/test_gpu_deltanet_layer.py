@@ -168,7 +168,11 @@ def check_scan(pk, ins, scale, lens, out):
     on = (torch.arange(q.shape[1]) < torch.tensor(ends(lens, *q.shape[:2]))[:, None]).cuda()[..., None, None]
     got, ref = torch.where(on, got, 0.0), torch.where(on, ref, 0.0)
     say(f"  out {rel(got, ref):.2e} state {rel(state, ref_state):.2e} limit {lim:.2e}")
-    assert rel(got, ref) <= lim and rel(state, ref_state) <= lim
+    # f32 holds nothing to a relative precision below its smallest normal value
+    small = 2.0 ** -126
+    for x, y in ((got, ref), (state, ref_state)):
+        assert torch.isfinite(x).all()
+        assert float((x.double() - y).norm()) <= lim * float(y.norm()) + small * y.numel() ** 0.5
     # no single value is far off: 40 times the mean error, of the largest values' size
     assert float((got.double() - ref).abs().max() / ref.abs().max()) <= 40 * lim
     # the gates' sum is rounded once after its own 64 bits (and once more as the offset's)
@@ -193,7 +197,8 @@ def check_scan(pk, ins, scale, lens, out):
     (2, 90, 2, 4, 256, [33, 90]),
     (1, 7, 4, 4, 256, None),
     (1, 1500, 1, 2, 128, None),
-    (16, 200, 16, 32, 128, None),                # more than one segment of chunks
+    (16, 200, 16, 32, 128, None),
+    (16, 700, 16, 32, 128, None),                # more than one segment of chunks
     (9, 333, 16, 32, 128, [333, 0, 48, 47, 200, 256, 257, 1, 128]),
     (1, 130, 3, 15, 64, None),                   # an odd number of value heads per key head
     (2, 70, 8, 8, 256, [70, 65]),
@@ -213,7 +218,8 @@ def test_scan(pk, b, n, hk, h, d, lens):
 
 
 @pytest.mark.parametrize("n", [11, 150])
-@pytest.mark.parametrize("kind", ["slow", "fast", "mixed", "reset", "same_keys", "zero_rows", "large", "small", "closed", "growing", "huge", "far_apart", "late"])
+@pytest.mark.parametrize("kind", ["slow", "fast", "mixed", "reset", "same_keys", "zero_rows", "large", "small", "closed", "growing", "huge", "far_apart", "late",
+                                  "one_write", "one_write_mild", "few_writes", "tiny_keys", "tiny_queries"])
 def test_scan_values(pk, kind, n):
     """Decays from none to whole, keys that all point the same way, zero vectors, magnitudes."""
     say(f"scan values {kind} n={n}")
@@ -246,7 +252,19 @@ def test_scan_values(pk, kind, n):
     elif kind == "huge":  # past what a state in two fp16 parts is scaled for
         v = v * 1e28
     elif kind == "far_apart":  # value channels of unlike magnitude share a tile
-        v = v * torch.exp2(torch.arange(d, device="cuda") % 16 - 8.0)
+        far = torch.exp2(4.0 * (torch.arange(d, device="cuda") % 16) - 32.0)
+        v, state = v * far, state * far[:, None]
+    elif kind.startswith("one_write"):  # one token writes, the decay leaves little of it
+        beta = torch.where(torch.arange(n, device="cuda")[:, None] == 3, beta, -200.0)
+        gate = gate * (2 if kind == "one_write" else 0.4)
+    elif kind == "few_writes":  # the first tokens write, the others all but nothing
+        beta = torch.where(torch.arange(n, device="cuda")[:, None] < 8, beta, -25.0)
+        state = state * 0
+    elif kind == "tiny_keys":  # what eps leaves of them is far below one
+        k = k * 1e-9
+        state = state * 0
+    elif kind == "tiny_queries":
+        q = q * 1e-9
     elif kind == "late":  # the largest values come last
         v = v * torch.exp2(torch.linspace(-20, 10, n, device="cuda"))[:, None, None]
     elif kind == "closed":  # sigmoid(beta) = 0: nothing is written
@@ -257,7 +275,15 @@ def test_scan_values(pk, kind, n):
         got = pk.gated_delta_rule(q, k, v, gate, beta, state, 0.1, EPS)
         assert rel(got, ref) <= scan_limit(n) and rel(state, ref_state) <= scan_limit(n)
         return
-    check_scan(pk, (q, k, v, gate.contiguous(), beta, state, offset), 0.1, None, out)
+    ins = (q, k, v, gate.contiguous(), beta, state, offset)
+    ref, ref_state, _ = scan64(*ins[:6], 0.1, None, out, offset)
+    got = check_scan(pk, ins, 0.1, None, out)
+    # each head and value channel by itself, of the output and of the state
+    lim = 4 * scan_limit(n)
+    for x, y, over in ((got, ref, 1), (state, ref_state, 3)):
+        err, mag = (x.double() - y).norm(dim=over), y.norm(dim=over)
+        room = lim * mag + 2.0 ** -126 * x.shape[over] ** 0.5  # f32's smallest normal value
+        assert bool((err <= room).all()), float((err / room).max())
 
 
 def test_scan_pieces_and_tokens(pk):
@@ -289,6 +315,30 @@ def test_scan_is_deterministic(pk):
         state = ins[5].clone()
         got.append((pk.gated_delta_rule(*ins[:5], state, 0.1, EPS), state))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+def test_scan_token_path_of_some_heads(pk):
+    """Heads that cannot go by chunks beside heads that do, 32 value channels a workgroup, over
+    several segments, the odd values in the first, a middle and the last one."""
+    say("scan: some heads token by token")
+    r = gen(14)
+    b, n, hk, h, d = 16, 700, 16, 32, 128
+    q, k, v, gate, beta, state, offset = scan_inputs(r, b, n, hk, h, d)
+    gate[2, 5, 7] = 0.02
+    gate[3, 350, 0] = float("-inf")
+    k[4, 690, 3] *= 1e-30
+    v[5, 300, 9] *= 1e28
+    ref, ref_state, ref_offset = scan64(q, k, v, gate, beta, state, 0.1, None, torch.zeros_like(v), offset)
+    got = pk.gated_delta_rule(q, k, v, gate, beta, state, 0.1, EPS, gate_offset=offset)
+    lim = scan_limit(n)
+    err, mag = (got.double() - ref).norm(dim=(1, 3)), ref.norm(dim=(1, 3))
+    assert bool((err <= lim * mag).all())
+    err, mag = (state.double() - ref_state).norm(dim=(2, 3)), ref_state.norm(dim=(2, 3))
+    assert bool((err <= lim * mag).all())
+    fin = torch.isfinite(ref_offset)
+    assert torch.equal(offset[~fin].double(), ref_offset[~fin])
+    # a rounding per segment
+    assert bool(((offset.double() - ref_offset)[fin].abs() <= 6 * E * (ref_offset[fin].abs() + 1)).all())
 
 
 def test_scan_sequences_do_not_touch(pk):
@@ -467,6 +517,9 @@ W_BYTES = {8: 34 / 32, 12: 144 / 256, 13: 176 / 256, 14: 210 / 256}
     (130, 4096, 300, 64, 3, "bfloat16", 12, True),
     (257, 4096, 513, 20, 4, "float16", 14, True),
     (600, 4096, 64, 8, 2, "float32", 12, True),
+    (2, 4096, 40, 100, 3, "float16", 14, True),
+    (5, 8192, 33, 128, 2, "float32", 8, False),
+    (64, 4096, 257, 16, 50, "float16", 12, True),
 ])
 def test_lora(pk, orc, rows, inner, width, rank, n, dtype, w_type, gated):
     from kquant_blocks import random_weight_bytes

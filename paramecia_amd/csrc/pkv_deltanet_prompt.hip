@@ -767,7 +767,6 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     };
     __syncthreads();
     odd = lds.c.odd != 0u;
-    get_scales(0);
     const auto first_scale = [&](int j) {  // of the state as it comes: its largest value is known
       const uint4 t = lds.c.top[0][0][j][m];
       return pow2(scale_exp(as_f(umax(umax(t.x, t.y), umax(t.z, t.w)))));
@@ -795,6 +794,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           kx[j] = mfma32(kf[s][0], lo, kx[j]);
           ky[j] = mfma32(kf[s][1], hi, ky[j]);
         }
+      get_scales(c);  // what an odd chunk leaves is not used
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
         f4 r;
@@ -863,7 +863,6 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 #pragma unroll
       for (int j = 0; j < kNT; ++j) sm[j] = sm1[j];
       lds_barrier();
-      get_scales(c + 1);
     };
     if constexpr (kDeep) {
       for (int c = 0; c < chunks && !odd; c += 2) {
@@ -911,7 +910,6 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     load_p(0);
     __syncthreads();
     odd = lds.c.odd != 0u;
-    get_scales(0);
     uint32_t vnow[kNT];  // largest |v| of the wave's tokens in this chunk
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
@@ -938,6 +936,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           qy[j] = mfma32(qf[s][1], hi, qy[j]);
           if ((s & 3) == w || kS == 2) top[j] = umax(top[j], top16(hi));  // a quarter of the state each
         }
+      get_scales(c);
       load_q(c + (kDeep ? 2 : 1), qf);
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
@@ -994,7 +993,6 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
       if (16 * w + 4 * g + (m & 3) < tokens - c * kC)
 #pragma unroll
         for (int j = 0; j < kNT; ++j) *reinterpret_cast<f4 *>(o0 + (int64_t)c * kC * row + 64 * j + ooff) = o[j];
-      get_scales(c + 1);
     };
     if constexpr (kDeep) {
       for (int c = 0; c < chunks && !odd; c += 2) {

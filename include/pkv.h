@@ -292,7 +292,7 @@ int pkv_gated_oproj(const float *attn, const float *gate, const void *w, int w_t
  * input[t - taps + 1 + j]), act = y * sigmoid(y) if silu, else y. lens: device int32
  * [batch] or NULL: the valid tokens of each sequence of a padded batch (taken into [0, n]):
  * rows of out behind them are left as they were, and the padding of x is not read. 2, 3 or
- * 4 taps (else PKV_ERR_UNSUPPORTED). x, out and state must not overlap. */
+ * 4 taps (else PKV_ERR_UNSUPPORTED), n at most 1048560, at most 2^24 channels. x, out and state must not overlap. */
 int pkv_causal_conv(const float *x, int64_t stride_b, int64_t stride_t, const float *weight,
                     const float *bias, float *state, const int *lens, float *out, int batch,
                     int64_t n, int channels, int taps, int silu, pkv_stream stream);
@@ -304,10 +304,11 @@ int pkv_causal_conv(const float *x, int64_t stride_b, int64_t stride_t, const fl
  * multiples of 4). gate, beta: [batch, n, heads]; state, gate_offset (NULL or [batch,
  * heads]): as pkv_deltanet_step, updated in place; lens as pkv_causal_conv: tokens behind a
  * sequence's end change nothing and their rows of out are left as they were. out: [batch, n,
- * heads, head_dim]. head_dim 64, 128 or 256 (else PKV_ERR_UNSUPPORTED); q, k, v, state, out
- * and workspace 16-byte aligned; q, k and v must not overlap out or state. workspace: at
- * least pkv_deltanet_prompt_workspace() bytes of device memory (may be 0, with NULL), which
- * the call writes: calls that overlap in time, and graphs that do, need one each. */
+ * heads, head_dim]. head_dim 64, 128 or 256 (else PKV_ERR_UNSUPPORTED), n at most 2^30, batch *
+ * heads * head_dim at most 2^26; q, k, v, state, out and workspace 16-byte aligned; q, k and v,
+ * out, state and workspace must not overlap. workspace: at least
+ * pkv_deltanet_prompt_workspace() bytes of device memory (may be 0, with NULL), which the call
+ * writes: calls that overlap in time, and graphs that do, need one each. */
 size_t pkv_deltanet_prompt_workspace(int batch, int64_t n, int k_heads, int heads, int head_dim);
 int pkv_deltanet_prompt(const float *q, const float *k, const float *v, const int64_t strides[6],
                         const float *gate, const float *beta, float *state, float *gate_offset,
@@ -322,7 +323,8 @@ int pkv_deltanet_prompt(const float *q, const float *k, const float *v, const in
  * apart; residual, gate, out: [rows, dim] f32; alpha: [dim]. y goes to out, to out_q8_0, or
  * to both (one may be NULL): out_q8_0 takes pkv_bytes_per_row(PKV_QUANT_Q8_0, dim) bytes a
  * row, encoded as the cache encodes Q8_0 (a last block is filled up with zeros). dim at most
- * 32768 (else PKV_ERR_UNSUPPORTED). out or residual may be x itself (of dense rows), out
+ * 32768, and rows below 2^31 / 1024 (dim up to 8192: / 256, 512: / 64, 128: / 16; else
+ * PKV_ERR_UNSUPPORTED). out or residual may be x itself (of dense rows), out
  * may be gate; no other buffers may overlap. */
 int pkv_rms_norm(const float *x, int64_t stride, float *residual, const float *alpha,
                  const float *gate, float eps, float *out, void *out_q8_0, int64_t rows, int dim,
@@ -338,7 +340,8 @@ int pkv_rms_norm(const float *x, int64_t stride, float *residual, const float *a
  * reports it. rank at most PKV_LORA_MAX_RANK (else PKV_ERR_UNSUPPORTED), batch at most 65535. workspace: at least
  * pkv_gated_oproj_lora_workspace() bytes of device memory, 256-byte aligned, which the call
  * writes (unlike pkv_gated_oproj it allocates nothing): calls that overlap in time, and
- * graphs that do, need one each. Everything else as pkv_gated_oproj. */
+ * graphs that do, need one each. attn and gate, out, and the workspace must not overlap.
+ * Everything else as pkv_gated_oproj. */
 enum { PKV_LORA_F32 = 0, PKV_LORA_F16 = 1, PKV_LORA_BF16 = 2 };
 #define PKV_LORA_MAX_RANK 128
 size_t pkv_gated_oproj_lora_workspace(int w_type, int batch, int in_dim, int out_dim, int rank);

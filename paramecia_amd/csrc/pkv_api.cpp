@@ -207,13 +207,12 @@ int pkv_device_status(void) {
   if (v == 0) return PKV_OK;
   const unsigned zero = 0;
   PKV_HIP(hipMemcpy(w, &zero, sizeof zero, hipMemcpyHostToDevice));
-  if (v == kStatusAdapterId)
-    return set_error(PKV_ERR_HIP, "a projection was given an adapter id past its adapters: that "
-                                  "row took none");
-  return set_error(PKV_ERR_HIP, (v & kStatusBarrierTimeout)
-                                    ? "a fused decode step's quantizer barrier timed out: its "
-                                      "appended row and attention output are not valid"
-                                    : "device status " + std::to_string(v));
+  std::string what;
+  if (v & kStatusBarrierTimeout)
+    what = "a fused decode step's quantizer barrier timed out: its appended row and attention output are not valid";
+  if (v & kStatusAdapterId)
+    what += std::string(what.empty() ? "" : "; ") + "a projection was given an adapter id past its adapters: that row took none";
+  return set_error(PKV_ERR_HIP, what.empty() ? "device status " + std::to_string(v) : what);
 }
 const char *pkv_version(void) { return "paramecia_amd pkv 0.1 (gfx950)"; }
 
@@ -1228,6 +1227,9 @@ int pkv_deltanet_prompt(const float *q, const float *k, const float *v, const in
   const uint64_t state_bytes = 4 * (uint64_t)batch * heads * head_dim * head_dim;
   if (overlap(out, out_bytes, state, state_bytes))
     return set_error(PKV_ERR_ARG, "out and state must not overlap");
+  const uint64_t used = workspace ? deltanet_prompt_workspace(batch, n, k_heads, heads, head_dim) : 0;
+  if (used && (overlap(workspace, used, out, out_bytes) || overlap(workspace, used, state, state_bytes)))
+    return set_error(PKV_ERR_ARG, "the workspace must not overlap another buffer");
   for (int i = 0; i < 3; ++i) {
     const int64_t sb = strides[2 * i], st = strides[2 * i + 1], w = (int64_t)width[i] * head_dim;
     if ((n > 1 && st < w) || (batch > 1 && sb < w) || sb < 0 || st < 0)
@@ -1235,6 +1237,8 @@ int pkv_deltanet_prompt(const float *q, const float *k, const float *v, const in
     const uint64_t span = 4 * ((uint64_t)(batch - 1) * sb + (uint64_t)(n - 1) * st + w);
     if (overlap(in[i], span, out, out_bytes) || overlap(in[i], span, state, state_bytes))
       return set_error(PKV_ERR_ARG, "q, k and v must not overlap out or state");
+    if (used && overlap(in[i], span, workspace, used))
+      return set_error(PKV_ERR_ARG, "the workspace must not overlap another buffer");
   }
   return launch_deltanet_prompt(q, k, v, strides, gate, beta, state, gate_offset, lens, out, batch,
                                 n, k_heads, heads, head_dim, scale, eps, workspace,
@@ -1285,7 +1289,7 @@ static int check_lora(const void *a, const void *b, int type, int adapters, int 
 }
 
 size_t pkv_gated_oproj_lora_workspace(int w_type, int batch, int in_dim, int out_dim, int rank) {
-  if (batch <= 0 || in_dim <= 0 || out_dim <= 0 || rank <= 0) return 0;
+  if (batch <= 0 || batch > 65535 || in_dim <= 0 || out_dim <= 0 || rank <= 0) return 0;  // refused by the call
   return oproj_lora_workspace(w_type, batch, in_dim, out_dim, rank);
 }
 
@@ -1299,6 +1303,11 @@ int pkv_gated_oproj_lora(const float *attn, const float *gate, const void *w, in
   if (batch <= 0 || in_dim <= 0 || out_dim <= 0)
     return set_error(PKV_ERR_ARG, "batch, in_dim and out_dim must be > 0");
   if (int rc = check_lora(lora_a, lora_b, lora_type, n_adapters, rank)) return rc;
+  const uint64_t in_bytes = 4 * (uint64_t)batch * in_dim, out_bytes = 4 * (uint64_t)batch * out_dim;
+  if (overlap(attn, in_bytes, out, out_bytes) || (gate && overlap(gate, in_bytes, out, out_bytes)) ||
+      overlap(workspace, workspace_bytes, out, out_bytes) || overlap(workspace, workspace_bytes, attn, in_bytes) ||
+      (gate && overlap(workspace, workspace_bytes, gate, in_bytes)))
+    return set_error(PKV_ERR_ARG, "attn and gate, out, and the workspace must not overlap");
   return launch_oproj_lora(attn, gate, static_cast<const uint8_t *>(w), w_type, lora_a, lora_b,
                            lora_type, n_adapters, rank, lora_scale, adapter_ids, out, batch, in_dim,
                            out_dim, workspace, workspace_bytes, static_cast<hipStream_t>(stream));

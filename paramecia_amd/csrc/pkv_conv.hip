@@ -144,6 +144,7 @@ int launch_causal_conv(const float *x, int64_t stride_b, int64_t stride_t, const
                        const float *bias, float *state, const int *lens, float *out, int batch,
                        int64_t n, int channels, int taps, int silu, hipStream_t s) {
   if (batch > 65535) return set_error(PKV_ERR_ARG, "batch must be <= 65535");
+  if (channels > 1 << 24) return set_error(PKV_ERR_ARG, "causal conv: at most 2^24 channels");
   const auto at16 = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
   const bool wide = channels % 4 == 0 && stride_b % 4 == 0 && stride_t % 4 == 0 && at16(x) && at16(out);
   ConvArgs a{x, w, bias, state, lens, out, stride_b, stride_t, n, channels, silu};

@@ -1113,8 +1113,8 @@ int launch_deltanet_prompt(const float *q, const float *k, const float *v, const
   if (heads > 65535 || batch > 65535) return set_error(PKV_ERR_ARG, "heads and batch must be <= 65535");
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return set_error(PKV_ERR_UNSUPPORTED, "delta net prompt: head_dim must be 64, 128 or 256");
-  if (n > ((int64_t)1 << 30) || (int64_t)batch * heads > (1 << 24))
-    return set_error(PKV_ERR_ARG, "n must be <= 2^30 and batch * heads <= 2^24");
+  if (n > ((int64_t)1 << 30) || (int64_t)batch * heads * head_dim > (1 << 26))  // walks of 512 lanes: below 2^32
+    return set_error(PKV_ERR_ARG, "n must be <= 2^30 and batch * heads * head_dim <= 2^26");
   SegmentPlan plan = plan_segment(batch, n, k_heads, heads, head_dim);
   if (ws_bytes < plan.bytes || (plan.bytes != 0 && ws == nullptr))
     return set_error(PKV_ERR_ARG, "the workspace is smaller than pkv_deltanet_prompt_workspace says");

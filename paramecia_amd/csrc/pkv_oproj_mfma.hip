@@ -582,7 +582,7 @@ MxPlan plan_mx(int w_type, int T, int K, int N) {
   constexpr int kWideWGs = 40;
   MxPlan p;
   const int rows = 256;
-  p.rbs = (N + rows - 1) / rows;
+  p.rbs = (int)(((int64_t)N + rows - 1) / rows);
   const auto wgs = [&](int tokens) { return (int64_t)p.rbs * ((T + tokens - 1) / tokens); };
   p.wide = wgs(64) >= kWideWGs;
   if (w_type == kMQ6K && wgs(64) > 256) p.wide = 17 * ((wgs(64) + 255) / 256) < 10 * ((wgs(32) + 255) / 256);

@@ -160,8 +160,10 @@ __global__ __launch_bounds__(kLanes < 256 ? 256 : kLanes) void rms_norm_kernel(N
 }
 
 template <int kLanes, int kQuads>
-void launch(const NormArgs &a, bool wide, hipStream_t s) {
+int launch(const NormArgs &a, bool wide, hipStream_t s) {
   constexpr int kThreads = kLanes < 256 ? 256 : kLanes, kRows = kThreads / kLanes;
+  if (a.rows > INT32_MAX / kLanes)  // a launch holds fewer than 2^32 lanes; half of that is kept to
+    return set_error(PKV_ERR_UNSUPPORTED, "rms norm: too many rows of this length for one call");
   const dim3 grid((unsigned)((a.rows + kRows - 1) / kRows)), t(kThreads);
   if (a.q8 != nullptr) {
     if (wide) hipLaunchKernelGGL((rms_norm_kernel<kLanes, kQuads, true, true>), grid, t, 0, s, a);
@@ -170,6 +172,8 @@ void launch(const NormArgs &a, bool wide, hipStream_t s) {
     if (wide) hipLaunchKernelGGL((rms_norm_kernel<kLanes, kQuads, true, false>), grid, t, 0, s, a);
     else hipLaunchKernelGGL((rms_norm_kernel<kLanes, kQuads, false, false>), grid, t, 0, s, a);
   }
+  PKV_HIP(hipGetLastError());
+  return PKV_OK;
 }
 
 }  // namespace
@@ -181,15 +185,12 @@ int launch_rms_norm(const float *x, int64_t x_stride, float *residual, const flo
   const bool wide = dim % 4 == 0 && x_stride % 4 == 0 && at16(x) && at16(residual) && at16(alpha) &&
                     at16(gate) && at16(out);
   NormArgs a{x, residual, alpha, gate, out, q8, rows, x_stride, dim, (double)eps};
-  if (rows > INT32_MAX) return set_error(PKV_ERR_ARG, "rms norm: at most 2^31 - 1 rows");
-  if (dim <= 128) launch<16, 2>(a, wide, s);
-  else if (dim <= 512) launch<64, 2>(a, wide, s);
-  else if (dim <= 2048) launch<256, 2>(a, wide, s);
-  else if (dim <= 8192) launch<256, 8>(a, wide, s);
-  else if (dim <= 32768) launch<1024, 8>(a, wide, s);
-  else return set_error(PKV_ERR_UNSUPPORTED, "rms norm: rows of at most 32768 values");
-  PKV_HIP(hipGetLastError());
-  return PKV_OK;
+  if (dim <= 128) return launch<16, 2>(a, wide, s);
+  if (dim <= 512) return launch<64, 2>(a, wide, s);
+  if (dim <= 2048) return launch<256, 2>(a, wide, s);
+  if (dim <= 8192) return launch<256, 8>(a, wide, s);
+  if (dim <= 32768) return launch<1024, 8>(a, wide, s);
+  return set_error(PKV_ERR_UNSUPPORTED, "rms norm: rows of at most 32768 values");
 }
 
 }  // namespace pkv

@@ -33,6 +33,7 @@ def conv(**k):
     (dict(state=D + 4), ERR_ARG, "overlap"), (dict(taps=1), ERR_UNSUPPORTED, "taps"),
     (dict(taps=5), ERR_UNSUPPORTED, "taps"), (dict(b=70000, sb=80 * 64), ERR_ARG, "65535"),
     (dict(b=1, n=1 << 24), ERR_ARG, "n must be"),
+    (dict(b=1, ch=(1 << 24) + 4, st=(1 << 24) + 4, x=A, out=G << 4), ERR_ARG, "2^24 channels"),
 ])
 def test_conv(k, code, word):
     assert conv(**k) == code and word in err()
@@ -62,6 +63,8 @@ def scan(**k):
     (dict(st=[80 * 8192, 1024] + [80 * 8192, 8192] * 2), ERR_ARG, "rows do not overlap"),
     (dict(out=A + 4096), ERR_ARG, "overlap"), (dict(state=A + 64), ERR_ARG, "overlap"),
     (dict(out=D), ERR_ARG, "overlap"), (dict(b=70000), ERR_ARG, "65535"),
+    (dict(b=16385, q=A, k=A + (1 << 43), v=A + (1 << 44), gate=1 << 60, beta=1 << 60, state=1 << 61, out=1 << 62), ERR_ARG, "2^26"),
+    (dict(b=1, n=(1 << 30) + 1, out=1 << 62, state=1 << 61, ws=1 << 60), ERR_ARG, "2^30"),
 ])
 def test_scan(k, code, word):
     assert scan(**k) == code and word in err()
@@ -74,6 +77,8 @@ def test_scan_workspace():
         assert scan(wb=need - 1) == ERR_ARG and "workspace" in err()
         assert scan(ws=None) == ERR_ARG and "workspace" in err()
         assert scan(ws=G + 8) == ERR_ARG
+        for at in (A, D, F, A - 16):
+            assert scan(ws=at) == ERR_ARG and "overlap" in err()
 
 
 def norm(**k):
@@ -88,7 +93,9 @@ def norm(**k):
     (dict(d=32769, st=32769), ERR_UNSUPPORTED, "32768"), (dict(q8=D + 1), ERR_ARG, "2-byte"),
     (dict(out=A + 4), ERR_ARG, "overlap"), (dict(res=A + 1024), ERR_ARG, "overlap"),
     (dict(res=C), ERR_ARG, "overlap"), (dict(out=A, st=260), ERR_ARG, "overlap"), (dict(q8=A), ERR_ARG, "overlap"),
-    (dict(gate=F, res=F), ERR_ARG, "overlap"), (dict(rows=1 << 31), ERR_ARG, "rows"), (dict(q8=C), ERR_ARG, "overlap"),
+    (dict(gate=F, res=F), ERR_ARG, "overlap"), (dict(q8=C), ERR_ARG, "overlap"),
+    (dict(rows=1 << 31, out=1 << 61), ERR_UNSUPPORTED, "rows"), (dict(rows=1 << 25, out=1 << 61), ERR_UNSUPPORTED, "rows"),
+    (dict(rows=1 << 21, d=8193, st=8193, out=1 << 61), ERR_UNSUPPORTED, "rows"),
 ])
 def test_norm(k, code, word):
     assert norm(**k) == code and word in err()
@@ -107,6 +114,8 @@ def lora(**k):
     (dict(lb=None), ERR_ARG, "null"), (dict(s=None), ERR_ARG, "null"), (dict(ids=None), ERR_ARG, "null"),
     (dict(ws=None), ERR_ARG, "null"), (dict(b=0), ERR_ARG, "batch"), (dict(n=0), ERR_ARG, "n_adapters"),
     (dict(r=0), ERR_ARG, "rank"), (dict(r=129), ERR_UNSUPPORTED, "rank"), (dict(lt=3), ERR_UNSUPPORTED, "F32, F16"),
+    (dict(out=A), ERR_ARG, "overlap"), (dict(g=F), ERR_ARG, "overlap"), (dict(ws=F), ERR_ARG, "overlap"), (dict(ws=A), ERR_ARG, "overlap"),
+    (dict(b=65536, wb=1 << 32), ERR_ARG, "65535"),
     (dict(la=C + 8), ERR_ARG, "16-byte"), (dict(wb=0), ERR_ARG, "workspace"), (dict(ws=G + 16), ERR_ARG, "256-byte"),
 ])
 def test_lora(k, code, word):
@@ -115,7 +124,7 @@ def test_lora(k, code, word):
 
 def test_lora_workspace():
     f = lib().pkv_gated_oproj_lora_workspace
-    assert f(12, 0, 4096, 64, 16) == 0
+    assert f(12, 0, 4096, 64, 16) == 0 and f(12, 65536, 4096, 64, 16) == 0 and f(12, 2**31 - 1, 4096, 64, 16) == 0
     assert f(12, 20, 4096, 64, 16) > 20 * 4096 * 4  # the batched projection's operands and the small product
     assert f(8, 20, 4096, 64, 16) >= 20 * 16 * 4
 

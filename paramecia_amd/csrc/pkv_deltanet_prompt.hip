@@ -23,6 +23,7 @@
 // chunk's largest.) A head with a positive gate, with a key or query that normalisation leaves
 // below 2^-8, or with a value that is not finite or past 2^90, goes token by token instead (a NaN
 // then reaches the tokens behind it and no others, as there).
+#include <algorithm>
 #include <type_traits>
 
 #include "pkv_q8_common.hpp"
@@ -208,7 +209,6 @@ __device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) {
 // from w = 2 on, six fragments.
 struct ChunkWs {
   h8 *k, *q;       // [b][chunk][key head][row tile 4][d / 32][2][64]
-  h8 *kt;          // [b][chunk][key head][d / 16][k step 2][2][64]: rows are key channels
   h8 *t, *p;       // [b][chunk][head][6][2][64]
   float *meta;     // [b][chunk][head][kMeta]: be, e^G, e^(G_63 - G) of its tokens; then the
                    // largest be, the largest be e^(G_63 - G), and e^(G_63)
@@ -387,20 +387,6 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
     kk[j] = (kk[j] + kx) * (kDown * kDown);
     qk[j] = (qk[j] + qx) * (kDown * kDown);
   }
-  // ---- K^T's fragments: rows are key channels 16 at + m, k the chunk's tokens
-#pragma unroll
-  for (int c = 0; c < kD / 64; ++c) {
-    const int at = w * (kD / 64) + c;
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        h8 f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = kh[u][32 * p + 16 * (i >> 2) + 4 * g + (i & 3)][16 * at + m];
-        a.w.kt[((slot * (kD / 16) + at) * 2 + p) * kFrag + 64 * u + lane] = f;
-      }
-  }
   // ---- two value heads at a time
   for (int r0 = 0; r0 < a.s.rep; r0 += 2) {
     const int heads = a.s.rep - r0 < 2 ? a.s.rep - r0 : 2;
@@ -547,6 +533,7 @@ union StateLds {
   struct {
     h8 m[kNT][kD / 32][2][64];  // the state's fragments
     uint2 r[kNT][2][2][64][2], u[kNT][2][2][64][2], v[kNT][2][2][64][2];  // R, U, U e^(G_63 - G): [k step][part][lane][half]
+    h8 k[2][kC][kD / 8];  // K of the chunk, [part][token][.. in keys_at's order]
     uint4 top[2][3][kNT][16];  // [chunk's parity][maximum][..][channel], a word of each wave: bits of magnitudes
     unsigned odd;
   } c;
@@ -585,6 +572,21 @@ __device__ __forceinline__ void split4(const f4 &x, uint2 &hi, uint2 &lo) {
   for (int i = 0; i < 4; ++i) asm("" : "+v"(y[i]));
   hi = uint2{as_u(h2{(_Float16)y[0], (_Float16)y[1]}), as_u(h2{(_Float16)y[2], (_Float16)y[3]})};
   lo = uint2{lo_pair(y[0], y[1], hi.x), lo_pair(y[2], y[3], hi.y)};
+}
+
+// K in LDS, from which K^T's fragments are read: eight channels (a lane's of a fragment) are 16
+// bytes, whose place in a token's row is turned by the token, so that neither eight tokens'
+// stores nor the four tokens' loads of sixteen lanes meet in a bank.
+template <int kD>
+__device__ __forceinline__ int keys_at(int token, int c) {
+  return c ^ ((((token & 3) << 2) | ((token >> 2) & 3)) & (kD / 8 - 1));
+}
+// Four 16-bit values a lane, transposed within 16 lanes: they load four rows of 16, lane l the
+// values 4 (l % 4) .. of row l / 4, and receive a column each.
+__device__ __forceinline__ h4 load_columns(const _Float16 *p) {
+  typedef __fp16 v4h __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4h lds_v4h;
+  return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h *)(p)));
 }
 
 // The chunks of 16 kNT value channels of one head, in order, by eight waves. Waves 0 - 3 carry the
@@ -680,7 +682,6 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 
   if (wave < 4) {
     const h8 *kw = a.w.k + (key0 * 4 + w) * kS * kFrag;
-    const h8 *ktw = a.w.kt + (key0 * (kD / 16) + w * kN) * 2 * kFrag;
     const h8 *tw = a.w.t + (val0 * 6 + tri(w, 0)) * kFrag;
     float *state = a.s.state + ((b * a.s.heads + h) * kD + row0 + m) * kD + w * (kD / 4) + 4 * g;
     h8 ka[kS][2], kb[kDeep ? kS : 1][2], ktf[kN][2][2], tf[2][2];
@@ -700,14 +701,30 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         for (int u = 0; u < 2; ++u)
           if (p <= w >> 1) tf[p][u] = at<h8>(q + p * kFrag + 64 * u, foff);
     };
-    const auto load_kt = [&](int c) {
-      const h8 *q = ktw + c * kstep;
+    const auto put_k = [&](h8 (*f)[2]) {
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
+      for (int s = 0; s < kS; ++s)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) lds.c.k[u][16 * w + m][keys_at<kD>(16 * w + m, 4 * s + g)] = f[s][u];
+    };
+    // K^T's fragments: rows are key channels w d / 4 + 16 n + m, k the chunk's tokens
+    const auto get_kt = [&]() {
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        const int at = w * kN + n;
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) ktf[n][p][u] = at<h8>(q + (n * 2 + p) * kFrag + 64 * u, foff);
+          for (int u = 0; u < 2; ++u) {
+            h4 x[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int t = 32 * p + 16 * c + 4 * g + (m >> 2);
+              x[c] = load_columns(reinterpret_cast<const _Float16 *>(&lds.c.k[u][t][keys_at<kD>(t, 4 * (at >> 1) + (m & 3))]) + 4 * (at & 1));
+            }
+            ktf[n][p][u] = __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+      }
     };
     const auto load_meta = [&](int c, f4 &x, f4 &y, f4 &z, f4 &ex) {
       const float *p = meta + c * mstep;
@@ -724,7 +741,6 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     load_k(0, ka);
     if constexpr (kDeep) load_k(1, kb);
     load_t(0);
-    load_kt(0);
     f4 M[kNT][kN];
 #pragma unroll
     for (int j = 0; j < kNT; ++j)
@@ -803,6 +819,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         for (int i = 0; i < 4; ++i) r[i] = (be[i] * su[j]) * fmaf(-(eg[i] * dm), km[j][i] + (kx[j][i] + ky[j][i]), v[j][i]);
         put4(lds.c.r[j][w >> 1], r);
       }
+      put_k(kf);
       load_k(c + (kDeep ? 2 : 1), kf);
       lds_barrier();
       // ---- U = T R, times 2^e
@@ -820,6 +837,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           uy[j] = mfma32(tf[p][1], hi, uy[j]);
         }
       }
+      get_kt();
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
 #pragma unroll
@@ -852,7 +870,6 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           for (int i = 0; i < 4; ++i) M[j][n][i] = fmaf(M[j][n][i], ex1[2], (n0[n][i] + (nx[n][i] + ny[n][i])) * dv);
       }
       put_m(sm1);
-      load_kt(next);
 #pragma unroll
       for (int j = 0; j < kNT; ++j) v[j] = transpose4(vn[j]);
       be = bn;
@@ -1026,32 +1043,35 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 // A segment's chunks, and where its workspace's parts lie.
 // Prompts go by chunks from 72 tokens on, from 48 where their heads fill the GPU more than
 // twice (token by token a workgroup per 16 rows). us of the call, by tokens / by chunks, 32 heads
-// of 128: one sequence 64 tokens 19.0 / 20.9, 80 22.6 / 22.6, 128 33.8 / 23.2; four 32 tokens
-// 22.2 / 28.5, 48 31.3 / 29.5; twelve 24 tokens 51.2 / 56.2, 48 75.3 / 58.6. 16 heads of 256: 64
-// tokens 29.1 / 26.0; 32 of 64: 96 tokens 19.7 / 20.2.
+// of 128: one sequence 64 tokens 18.1 / 19.5, 72 21.8 / 21.1, 128 33.7 / 22.1; four 32 tokens
+// 22.7 / 27.9, 48 30.4 / 28.5; twelve 24 tokens 50.6 / 54.8, 48 73.9 / 56.8. 16 heads of 256: 64
+// tokens 28.6 / 26.6; 32 of 64: 96 tokens 19.0 / 17.7.
 bool by_chunks(int batch, int64_t n, int heads, int d) {
   return n >= 72 || (n >= 48 && (int64_t)batch * heads * d > 8192);
 }
-// Longer segments have fewer launches and fuller last rounds of workgroups, until the
-// workspace leaves the 256 MB of last-level cache: 8001 tokens, 32 heads of 128, 48 MB 413 us,
-// 96 MB 361, 192 MB 360, all in one (290 MB) 425; seven of 1100 349, 255, 224, 212.
-constexpr size_t kSegmentBytes = (size_t)192 << 20;
+// A segment's operands should stay in the 256 MB of last-level cache, but what a walk pays for
+// each segment (its state, the last round of workgroups) should not weigh either. us by bytes of a
+// segment 64 / 128 / 192 / 512 MB, 32 heads of 128: one sequence of 8001 tokens 350 / 331 / 332 / 363,
+// of 40000 1666 / 1495 / 1731 / 1667; 14 of 1100 (4, 5, 6, 18 chunks a segment) 883 / 643 /
+// 600 / 519; 28 of 2000 (2, 3, 4, 11 chunks) 4072 / 2966 / 2614 / 1992, 1 GB (16) 1845.
+constexpr size_t kSegmentBytes = (size_t)128 << 20, kSegmentMost = (size_t)1 << 30;
+constexpr int64_t kSegmentChunks = 32;  // up to kSegmentMost
 struct SegmentPlan {
   int chunks = 0;  // 0: token by token
-  size_t k = 0, q = 0, kt = 0, t = 0, p = 0, meta = 0, gates = 0, odd = 0, bytes = 0;
+  size_t q = 0, t = 0, p = 0, meta = 0, gates = 0, odd = 0, bytes = 0;
 };
 SegmentPlan plan_segment(int batch, int64_t n, int k_heads, int heads, int d) {
   SegmentPlan s;
   if (!by_chunks(batch, n, heads, d)) return s;
   const size_t key = (size_t)kC * d * 4;  // one operand of a key head's chunk
-  const size_t per = (size_t)batch * (k_heads * 3 * key + heads * (2 * 6 * kFrag * 16 + kMeta * 4 + 16));
-  const int64_t all = (n + kC - 1) / kC, fit = (int64_t)(kSegmentBytes / per);
+  const size_t per = (size_t)batch * (k_heads * 2 * key + heads * (2 * 6 * kFrag * 16 + kMeta * 4 + 16));
+  const int64_t all = (n + kC - 1) / kC;
+  const int64_t fit = std::max((int64_t)(kSegmentBytes / per), std::min((int64_t)(kSegmentMost / per), kSegmentChunks));
   const int64_t parts = (all + (fit < 1 ? 1 : fit) - 1) / (fit < 1 ? 1 : fit);
   s.chunks = (int)((all + parts - 1) / parts);  // segments of about one length
   const size_t keys = (size_t)batch * s.chunks * k_heads, vals = (size_t)batch * s.chunks * heads;
   s.q = keys * key;
-  s.kt = 2 * s.q;
-  s.t = 3 * s.q;
+  s.t = 2 * s.q;
   s.p = s.t + vals * 6 * kFrag * 16;
   s.meta = s.p + vals * 6 * kFrag * 16;
   s.gates = s.meta + vals * kMeta * 4;
@@ -1070,12 +1090,12 @@ int launch(const ScanArgs &a, const SegmentPlan &plan, int batch, int k_heads, v
   }
   char *base = static_cast<char *>(ws);
   const ChunkWs w{reinterpret_cast<h8 *>(base), reinterpret_cast<h8 *>(base + plan.q),
-                  reinterpret_cast<h8 *>(base + plan.kt), reinterpret_cast<h8 *>(base + plan.t),
-                  reinterpret_cast<h8 *>(base + plan.p), reinterpret_cast<float *>(base + plan.meta),
+                  reinterpret_cast<h8 *>(base + plan.t), reinterpret_cast<h8 *>(base + plan.p),
+                  reinterpret_cast<float *>(base + plan.meta),
                   reinterpret_cast<double *>(base + plan.gates), reinterpret_cast<unsigned *>(base + plan.odd)};
   // 32 value channels a workgroup halve the fragments' loads, 16 give twice the workgroups: one
-  // sequence of 8001 tokens (256 workgroups of 16) 357 us with 16, 404 with 32; seven of
-  // 1100 282 and 226. Heads of 256 have no registers for 32.
+  // sequence of 8001 tokens (256 workgroups of 16) 333 us with 16, 395 with 32; two of 4000
+  // 306 and 251, seven of 1100 360 and 289. Heads of 256 have no registers for 32.
   constexpr int kWide = kD <= 128 ? 2 : 1;
   const bool wide = kWide > 1 && (int64_t)batch * a.heads * (kD / 16) > 256;
   const int64_t all = (a.n + kC - 1) / kC;

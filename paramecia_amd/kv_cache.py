@@ -595,7 +595,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate: to
         _take(out, "out", (b, n, h, d), dev, writes=True)
     need = lib().pkv_deltanet_prompt_workspace(b, n, hk, h, d)
     # torch's allocator orders the workspace with the stream, and gives each graph its own
-    ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need else None
+    ws = state.new_empty(need, dtype=torch.uint8) if need else None
     _call(lib().pkv_deltanet_prompt(ins[0].data_ptr(), ins[1].data_ptr(), ins[2].data_ptr(),
                                     (ctypes.c_int64 * 6)(*strides), gate.data_ptr(), beta.data_ptr(),
                                     state.data_ptr(), _at(gate_offset), _at(lens), out.data_ptr(),
@@ -626,7 +626,8 @@ def rms_norm(x: torch.Tensor, alpha: torch.Tensor, eps: float,
     alpha = _take(alpha, "alpha", (d,), dev)
     _take(residual, "residual", shape, dev, writes=True)
     gate = _take(gate, "gate", shape, dev)
-    y = torch.empty(shape, dtype=torch.float32, device=x.device) if f32_out else None
+    # empty_like costs half of torch.empty; a strided x has no dense like
+    y = (torch.empty_like(x) if stride == d else x.new_empty(shape)) if f32_out else None
     q8 = torch.empty(shape[:-1] + ((d + 31) // 32, 34), dtype=torch.uint8, device=x.device) if q8_0_out else None
     _call(lib().pkv_rms_norm(x.data_ptr(), stride, _at(residual), alpha.data_ptr(), _at(gate), eps,
                              _at(y), _at(q8), rows, d, _stream()))
@@ -663,11 +664,11 @@ def gated_o_proj_lora(attn_output: torch.Tensor, gate: Optional[torch.Tensor], w
     b = _take(lora_b, "lora_b", (n, out_dim, rank), dev, lora_a.dtype)
     scale = _take(lora_scale, "lora_scale", (n,), dev)
     ids = _take(adapter_ids, "adapter_ids", x.shape[:-1], dev, torch.int32)
-    out = torch.empty(x.shape[:-1] + (out_dim,), dtype=torch.float32, device=x.device)
+    out = x.new_empty(x.shape[:-1] + (out_dim,))
     if rows == 0:
         return out
     need = lib().pkv_gated_oproj_lora_workspace(w_type, rows, in_dim, out_dim, rank)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    ws = w.new_empty(need)
     _call(lib().pkv_gated_oproj_lora(x.data_ptr(), _at(g), w.data_ptr(), w_type, a.data_ptr(),
                                      b.data_ptr(), _LORA_TYPE[a.dtype], n, rank, scale.data_ptr(),
                                      ids.data_ptr(), out.data_ptr(), rows, in_dim, out_dim,

@@ -8,7 +8,10 @@
 //
 // HBM-bound: 2 K flops for 8 bytes. A lane owns four neighbouring channels (16-byte
 // accesses, a wave reads 1 KB of a token's row) and kTile tokens of them, whose inputs it
-// holds in registers: K-1 inputs of the tile in front are read again, from L2.
+// holds in registers: K-1 inputs of the tile in front are read again, from L2 (3 of 16).
+// 8001 tokens of 8192 channels, 4 taps: 104 us for 525 MB, 5.0 TB/s, as a large copy. Calls of up
+// to 4 tokens take tiles of 4, whose registers hold whatever the kept inputs become (a tile of
+// 16 reads them once more from memory, behind its weights): 16 sequences of one token 4.3 us.
 #include "pkv_internal.hpp"
 
 namespace pkv {

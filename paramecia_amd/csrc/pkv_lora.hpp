@@ -92,7 +92,9 @@ __device__ __forceinline__ float lora_lane(const LoraTerm &l, int row, int o, in
 // (g = lane / 16): v_mfma_f32_16x16x4_f32 with t as A and B's rows as B, four ranks a lane
 // at a time, the loads of 32 ranks in flight together. The tokens' adapters are taken one
 // after the other; a token keeps its own one's result by selection, so that nothing of
-// another adapter (a NaN, say) reaches it.
+// another adapter (a NaN, say) reaches it. 4001 tokens of 2048 outputs, rank 64 in bf16: the
+// projection's kernel takes 251 us with it and 222 without: f32 products (7 us of matrix time an
+// adapter) behind two latencies that nothing is left to hide.
 template <int kType, bool kVec, int kTT, int kRT>
 __device__ void lora_tile_as(const LoraTerm &l, int tokens, int out_dim, int tok0, int col0,
                              int lane, float (&delta)[kTT][kRT][4]) {

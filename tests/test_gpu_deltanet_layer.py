@@ -198,7 +198,10 @@ def check_scan(pk, ins, scale, lens, out):
     (1, 7, 4, 4, 256, None),
     (1, 1500, 1, 2, 128, None),
     (16, 200, 16, 32, 128, None),
-    (16, 700, 16, 32, 128, None),                # more than one segment of chunks
+    (16, 700, 16, 32, 128, None),
+    (1, 4700, 16, 32, 128, None),                # more than one segment of chunks
+    (2, 2400, 16, 32, 128, [2399, 700]),         # the second sequence ends in the first segment
+    (1, 2000, 3, 9, 64, None),                   # three value heads over two workgroups
     (9, 333, 16, 32, 128, [333, 0, 48, 47, 200, 256, 257, 1, 128]),
     (1, 130, 3, 15, 64, None),                   # an odd number of value heads per key head
     (2, 70, 8, 8, 256, [70, 65]),

@@ -724,3 +724,62 @@ def test_two_streams(pk):
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert torch.equal(g, w)
+
+
+# ------------------------------------------------------------------ offsets past 2^32 bytes
+def test_long_prompt(pk):
+    """131109 tokens of 8192 channels (4.3 GB): the convolution's last tokens are those of its
+    last inputs alone, and the scan over slices of such rows is the scan in two pieces."""
+    say("long prompt")
+    r = gen(51)
+    n, ch, hk, h, d, tail = 131109, 8192, 16, 32, 128, 1000
+    x, w = r(1, n, ch), r(ch, 4)
+    state = torch.zeros(1, ch, 3, device="cuda")
+    y = pk.causal_conv(x, w, state)
+    torch.cuda.synchronize()
+    at = n - tail
+    s = x[:, at - 3:at].transpose(1, 2).contiguous()
+    assert torch.equal(pk.causal_conv(x[:, at:], w, s), y[:, at:]) and torch.equal(s, state)
+    assert torch.equal(state[0], x[0, -3:].T)
+    say("  scan")
+    q, k, v = (t.view(1, n, -1, d) for t in (y[..., :2048], y[..., 2048:4096], y[..., 4096:]))
+    gate, beta = -0.1 * r(1, n, h).abs(), r(1, n, h)
+    s1, s2 = torch.zeros(1, h, d, d, device="cuda"), torch.zeros(1, h, d, d, device="cuda")
+    whole = pk.gated_delta_rule(q, k, v, gate, beta, s1, d ** -0.5, EPS)
+    parts = [pk.gated_delta_rule(*(t[:, a:z].contiguous() for t in (q, k, v, gate, beta)), s2, d ** -0.5, EPS)
+             for a, z in ((0, at), (at, n))]
+    # each is off by the errors that the state has kept: those of some 1 / 0.08 tokens, as its
+    # gates are -0.08 on average; a hundred are allowed for
+    assert rel(whole[:, at:], parts[1]) <= 2 * scan_limit(100) and rel(s1, s2) <= 2 * scan_limit(100)
+    assert rel(whole[:, :at], parts[0]) <= 2 * scan_limit(100)
+
+
+def test_many_rows(pk):
+    """600037 rows of 2048 (4.9 GB): the last ones are the norm of these rows alone."""
+    say("many rows")
+    r = gen(52)
+    rows, d = 600037, 2048
+    x, res, alpha = r(rows, d), r(rows, d), 1 + 0.1 * r(d)
+    xs, rs = x[-50:].clone(), res[-50:].clone()
+    y, q8 = pk.rms_norm(x, alpha, EPS, residual=res, q8_0_out=True)
+    ys, qs = pk.rms_norm(xs, alpha, EPS, residual=rs, q8_0_out=True)
+    assert torch.equal(y[-50:], ys) and torch.equal(q8[-50:], qs) and torch.equal(res[-50:], rs)
+
+
+@pytest.mark.parametrize("rows", [2, 9])
+def test_many_adapters(pk, rows):
+    """2200 adapters of rank 128 over 8192 inputs (4.6 GB), the last one beside itself alone."""
+    from kquant_blocks import random_weight_bytes
+    say(f"many adapters rows={rows}")
+    r = gen(53)
+    n, rank, inner, width = 2200, 128, 8192, 64
+    wb = torch.from_numpy(random_weight_bytes(np.random.default_rng(1), 12, width, inner, d_scale=1e-4)).cuda()
+    a = torch.zeros(n, rank, inner, dtype=torch.bfloat16, device="cuda")
+    b = torch.zeros(n, width, rank, dtype=torch.bfloat16, device="cuda")
+    a[-1], b[-1] = (r(rank, inner) * inner ** -0.5).bfloat16(), (r(width, rank) * rank ** -0.5).bfloat16()
+    x, scale = r(rows, inner), torch.ones(n, device="cuda")
+    ids = torch.full((rows,), n - 1, dtype=torch.int32, device="cuda")
+    many = pk.gated_o_proj_lora(x, None, wb, width, a, b, scale, ids)
+    one = pk.gated_o_proj_lora(x, None, wb, width, a[-1:], b[-1:], scale[-1:], torch.zeros_like(ids))
+    assert torch.equal(many, one)
+    assert float((many - pk.gated_o_proj(x, None, wb, width)).abs().max()) > 0

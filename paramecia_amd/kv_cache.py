@@ -556,6 +556,9 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor,
     return out
 
 
+_Strides = ctypes.c_int64 * 6
+
+
 def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate: torch.Tensor,
                      beta: torch.Tensor, state: torch.Tensor, scale: float, eps: float,
                      gate_offset: Optional[torch.Tensor] = None,
@@ -567,22 +570,26 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate: to
     heads, d, d] and gate_offset [b, heads] are updated in place. Value head h reads key
     head h // (heads // key heads). lens, out as causal_conv. Returns out [b, n, heads, d]."""
     dev = _device()
-    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2] or v.shape[3] != q.shape[3]:
+    qs, vs = q.shape, v.shape
+    if len(qs) != 4 or k.shape != qs or len(vs) != 4 or vs[0] != qs[0] or vs[1] != qs[1] or vs[3] != qs[3]:
         raise KvCacheError("gated_delta_rule expects q, k [b, n, key heads, d] and v [b, n, heads, d]")
-    b, n, hk, d = q.shape
-    h = v.shape[2]
+    b, n, hk, d = qs
+    h = vs[2]
     if b == 0 or hk == 0 or h % hk:
         raise KvCacheError(f"gated_delta_rule: {h} value heads over {hk} key heads of {b} sequences")
-    ins, strides = [], []
+    at, kept, strides = [], [], []
     for t, name, heads in ((q, "q", hk), (k, "k", hk), (v, "v", h)):
         sb, st, sh, sd = t.stride()
         if t.get_device() != dev or t.dtype is not torch.float32:
-            t = _take(t, name, t.shape, dev)
-        if (sd != 1 or (heads > 1 and sh != d) or (n > 1 and (st < heads * d or st % 4)) or
-                (b > 1 and (sb < heads * d or sb % 4)) or t.data_ptr() % 16):
+            _take(t, name, t.shape, dev)
+        p, w = t.data_ptr(), heads * d
+        if (sd != 1 or (sh != d and heads > 1) or ((st < w or st % 4) and n > 1) or
+                ((sb < w or sb % 4) and b > 1) or p % 16):
             t = t.clone(memory_format=torch.contiguous_format)
+            kept.append(t)
+            p = t.data_ptr()
             sb, st, sh, sd = t.stride()
-        ins.append(t)
+        at.append(p)
         strides += (sb if b > 1 else 0, st if n > 1 else 0)
     gate, beta = _take(gate, "gate", (b, n, h), dev), _take(beta, "beta", (b, n, h), dev)
     _take(state, "state", (b, h, d, d), dev, writes=True)
@@ -596,8 +603,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, gate: to
     need = lib().pkv_deltanet_prompt_workspace(b, n, hk, h, d)
     # torch's allocator orders the workspace with the stream, and gives each graph its own
     ws = state.new_empty(need, dtype=torch.uint8) if need else None
-    _call(lib().pkv_deltanet_prompt(ins[0].data_ptr(), ins[1].data_ptr(), ins[2].data_ptr(),
-                                    (ctypes.c_int64 * 6)(*strides), gate.data_ptr(), beta.data_ptr(),
+    _call(lib().pkv_deltanet_prompt(*at, _Strides(*strides), gate.data_ptr(), beta.data_ptr(),
                                     state.data_ptr(), _at(gate_offset), _at(lens), out.data_ptr(),
                                     b, n, hk, h, d, scale, eps, _at(ws), need, _stream()))
     return out
@@ -663,8 +669,9 @@ def gated_o_proj_lora(attn_output: torch.Tensor, gate: Optional[torch.Tensor], w
     a = _take(lora_a, "lora_a", (n, rank, in_dim), dev, lora_a.dtype)
     b = _take(lora_b, "lora_b", (n, out_dim, rank), dev, lora_a.dtype)
     scale = _take(lora_scale, "lora_scale", (n,), dev)
-    ids = _take(adapter_ids, "adapter_ids", x.shape[:-1], dev, torch.int32)
-    out = x.new_empty(x.shape[:-1] + (out_dim,))
+    lead = x.shape[:-1]
+    ids = _take(adapter_ids, "adapter_ids", lead, dev, torch.int32)
+    out = x.new_empty(lead + (out_dim,))
     if rows == 0:
         return out
     need = lib().pkv_gated_oproj_lora_workspace(w_type, rows, in_dim, out_dim, rank)

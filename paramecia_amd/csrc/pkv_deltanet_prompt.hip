@@ -279,7 +279,7 @@ __device__ __forceinline__ double prefix64(float x) {
 // diagonal blocks by forward substitution (16 lanes each, a column a lane), then T_ij = -T_ii
 // sum_k A_ik T_kj down the block columns, a wave each, on v_mfma_f32_16x16x4_f32, whose result
 // tiles are the next product's B operand as they are. 63 chunks of 16 key heads of 128 with 32 value
-// heads: 47 us for 115 MB written, two workgroups a CU (LDS); alone a workgroup takes 12 us, a
+// heads: 46 us for 115 MB written, two workgroups a CU (LDS); alone a workgroup takes 12 us, a
 // quarter of it its first loads.
 template <int kD>
 __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
@@ -354,20 +354,25 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
         }
     }
   }
-  {
+#pragma unroll
+  for (int s = 0; s < kS; ++s)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      *reinterpret_cast<h4 *>(&kh[u][16 * w + m][32 * s + 4 * g]) = __builtin_shufflevector(kf[s][u], kf[s][u], 0, 1, 2, 3);
+      *reinterpret_cast<h4 *>(&kh[u][16 * w + m][32 * s + 16 + 4 * g]) = __builtin_shufflevector(kf[s][u], kf[s][u], 4, 5, 6, 7);
+    }
+  const auto put_kq = [&]() {
+    if (part != 0) return;
     h8 *ko = a.w.k + (slot * 4 + w) * kS * kFrag + lane, *qo = a.w.q + (slot * 4 + w) * kS * kFrag + lane;
 #pragma unroll
     for (int s = 0; s < kS; ++s)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        if (part == 0) {
-          ko[s * kFrag + 64 * u] = kf[s][u];
-          qo[s * kFrag + 64 * u] = qf[s][u];
-        }
-        *reinterpret_cast<h4 *>(&kh[u][16 * w + m][32 * s + 4 * g]) = __builtin_shufflevector(kf[s][u], kf[s][u], 0, 1, 2, 3);
-        *reinterpret_cast<h4 *>(&kh[u][16 * w + m][32 * s + 16 + 4 * g]) = __builtin_shufflevector(kf[s][u], kf[s][u], 4, 5, 6, 7);
+        ko[s * kFrag + 64 * u] = kf[s][u];
+        qo[s * kFrag + 64 * u] = qf[s][u];
       }
-  }
+  };
+  if constexpr (kD > 128) put_kq();  // two workgroups a CU have no registers to keep them
   lds_barrier();
   if (!fine) bad = 1u;
   // ---- k_t . k_s and q_t . k_s of the wave's tokens with tiles 0 .. w
@@ -441,6 +446,8 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
         }
       }
     }
+    if constexpr (kD <= 128)
+      if (r0 == rep0) put_kq();  // 63 chunks 45.5 us, 48.7 with these stores in front of the products
     lds_barrier();
     // the fragments of a lower triangular matrix's rows 16 w ..
     const auto put_rows = [&](const float(*x)[kSq], h8 *o) {

@@ -341,7 +341,8 @@ int pkv_rms_norm(const float *x, int64_t stride, float *residual, const float *a
  * pkv_gated_oproj_lora_workspace() bytes of device memory, 256-byte aligned, which the call
  * writes (unlike pkv_gated_oproj it allocates nothing): calls that overlap in time, and
  * graphs that do, need one each. attn and gate, out, and the workspace must not overlap.
- * Everything else as pkv_gated_oproj. */
+ * Everything else as pkv_gated_oproj, whose bits the rows without an adapter have, but for many
+ * rows of Q8_0 weights, which are batched here. */
 enum { PKV_LORA_F32 = 0, PKV_LORA_F16 = 1, PKV_LORA_BF16 = 2 };
 #define PKV_LORA_MAX_RANK 128
 size_t pkv_gated_oproj_lora_workspace(int w_type, int batch, int in_dim, int out_dim, int rank);

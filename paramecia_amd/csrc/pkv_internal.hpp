@@ -275,7 +275,7 @@ int launch_oproj(const float *attn, const float *gate, const uint8_t *w, int w_t
 int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, int w_type,
                       float *out, int batch, int in_dim, int out_dim, Workspace &ws,
                       hipStream_t s, const LoraTerm *lora = nullptr);
-// The form that a batch takes of the two, and its workspace (0: none).
+// The form that a batch takes, and its workspace with adapters (0: none).
 int oproj_any(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
               int batch, int in_dim, int out_dim, Workspace &ws, hipStream_t s,
               const LoraTerm *lora = nullptr);

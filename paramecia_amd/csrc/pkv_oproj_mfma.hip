@@ -589,6 +589,96 @@ __global__ __launch_bounds__(256) void oproj_reduce_lora_kernel(const float *par
   }
 }
 
+// Q8_0 weights for the rows of many requests (the projection with adapters; the one without
+// them stays token by token): a wave owns 64 weight rows and 64 tokens, a block of 32 weights is
+// one v_mfma_f32_16x16x32_f16 for hi and one for lo (a code is exact in fp16), and its scale
+// multiplies the block's product in f32. Codes and inputs of the next block are loaded while
+// this one's products run. What bounds it is their way through L1 (a row's block is 34 bytes, its
+// inputs half a line): 599 rows of 4096 into 2048, rank 64, with all launches 172 us, with 16 or 32
+// weight rows a wave 251 and 207, with 512 workgroups instead of 1024 197 (token by token 1252).
+struct Q8Args {
+  const u4 *xh, *xl;  // [T_pad][K / 8]
+  const uint8_t *w;   // [N][K / 32] blocks of 34 bytes
+  float *part;        // [S][T][N]
+  int T, N, K, per;   // per: blocks of a split
+};
+constexpr int kQ8Cols = 256;  // weight rows of a workgroup
+__global__ __launch_bounds__(256) void oproj_q8_kernel(Q8Args a) {
+  constexpr int kTT = 4, kRT = kQ8Cols / 64;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * kQ8Cols + (threadIdx.x >> 6) * 16 * kRT + m, t0 = blockIdx.y * 64;
+  const int kb0 = blockIdx.z * a.per;
+  const uint8_t *blk[kRT];
+  f4 acc[kTT][kRT];
+#pragma unroll
+  for (int r = 0; r < kRT; ++r) {
+    const int n = n0 + 16 * r;
+    blk[r] = a.w + ((int64_t)(n < a.N ? n : a.N - 1) * (a.K / 32) + kb0) * 34;
+#pragma unroll
+    for (int tt = 0; tt < kTT; ++tt) acc[tt][r] = f4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int64_t x0 = ((int64_t)(t0 + m) * a.K + 32 * kb0 + 8 * g) / 8;
+  const int64_t tile = (int64_t)2 * a.K;  // units of 16 rows
+  uint32_t cn[kRT][2];
+  uint16_t dn[kRT];
+  u4 hn[kTT], ln[kTT];
+  const auto fetch = [&](int k) {
+#pragma unroll
+    for (int r = 0; r < kRT; ++r) {
+      __builtin_memcpy(&dn[r], blk[r] + 34 * k, 2);
+      __builtin_memcpy(cn[r], blk[r] + 34 * k + 2 + 8 * g, 8);  // 2-byte aligned
+    }
+#pragma unroll
+    for (int tt = 0; tt < kTT; ++tt) {
+      hn[tt] = a.xh[x0 + tt * tile + 4 * k];
+      ln[tt] = a.xl[x0 + tt * tile + 4 * k];
+    }
+  };
+  fetch(0);
+  for (int k = 0; k < a.per; ++k) {
+    h8 hi[kTT], lo[kTT], w[kRT];
+    float d[kRT];
+#pragma unroll
+    for (int tt = 0; tt < kTT; ++tt) {
+      hi[tt] = __builtin_bit_cast(h8, hn[tt]);
+      lo[tt] = __builtin_bit_cast(h8, ln[tt]);
+    }
+#pragma unroll
+    for (int r = 0; r < kRT; ++r) {
+      d[r] = (float)__builtin_bit_cast(_Float16, dn[r]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // 0x6400 | u is 1024 + u; the code is u - 128
+        const uint32_t u = __builtin_amdgcn_perm(0x64646464u, cn[r][i >> 1] ^ 0x80808080u, i & 1 ? 0x07030702u : 0x07010700u);
+        const h2 x = __builtin_bit_cast(h2, u) - h2{(_Float16)1152.0f, (_Float16)1152.0f};
+        w[r][2 * i] = x[0];
+        w[r][2 * i + 1] = x[1];
+      }
+    }
+    fetch(k + 1 < a.per ? k + 1 : k);
+    __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the products
+#pragma unroll
+    for (int tt = 0; tt < kTT; ++tt)
+#pragma unroll
+      for (int r = 0; r < kRT; ++r) {
+        const f4 y = mfma32(lo[tt], w[r], mfma32(hi[tt], w[r], f4{0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[tt][r][i] = fmaf(y[i], d[r], acc[tt][r][i]);
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < kRT; ++r) {
+    const int n = n0 + 16 * r;
+    if (n >= a.N) continue;
+#pragma unroll
+    for (int tt = 0; tt < kTT; ++tt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = t0 + 16 * tt + 4 * g + i;
+        if (t < a.T) a.part[((int64_t)blockIdx.z * a.T + t) * a.N + n] = acc[tt][r][i];
+      }
+  }
+}
+
 // How a projection of T tokens is cut: its tiles, its split over K and its workspace.
 struct MxPlan {
   bool wide;
@@ -636,6 +726,60 @@ MxPlan plan_mx(int w_type, int T, int K, int N) {
   return p;
 }
 
+// The same for Q8_0 weights: tiles of 64 tokens by 256, up to 1024 workgroups from splits of 8 blocks at least.
+MxPlan plan_q8(int T, int K, int N) {
+  MxPlan p;
+  p.wide = true;
+  p.rbs = (int)(((int64_t)N + kQ8Cols - 1) / kQ8Cols);
+  p.tbs = (T + 63) / 64;
+  p.T_pad = 64 * p.tbs;
+  p.S = 1;
+  while ((int64_t)p.rbs * p.tbs * p.S * 2 <= 1024 && K / 32 / (2 * p.S) >= 8) p.S *= 2;
+  p.per = K / 32 / p.S;
+  const size_t x_bytes = (size_t)p.T_pad * K * 2;
+  p.off_xl = x_bytes;
+  p.off_xs = 2 * x_bytes;
+  p.off_inv = p.off_xs + (size_t)p.T_pad * (K / 256) * 32;
+  p.off_part = (p.off_inv + (size_t)p.T_pad * 4 + 255) / 256 * 256;
+  p.bytes = p.off_part + (size_t)p.S * T * N * 4;
+  return p;
+}
+
+// out = sum of the splits' partials, scaled back, + the rows' low-rank term
+int reduce_lora(const float *part, const float *inv, float *out, int T, int N, int S,
+                const LoraTerm &lora, hipStream_t s) {
+  const dim3 rgrid((unsigned)((N + 255) / 256), (unsigned)(T < 65535 ? T : 65535));
+  const bool vec = lora.rank % 4 == 0;
+#define PKV_REDUCE(TYPE)                                                                          \
+  if (vec)                                                                                        \
+    hipLaunchKernelGGL((oproj_reduce_lora_kernel<TYPE, true>), rgrid, dim3(256), 0, s, part, inv, \
+                       out, T, N, S, lora);                                                       \
+  else                                                                                            \
+    hipLaunchKernelGGL((oproj_reduce_lora_kernel<TYPE, false>), rgrid, dim3(256), 0, s, part, inv, \
+                       out, T, N, S, lora)
+  switch (lora.type) {
+    case PKV_LORA_F32: PKV_REDUCE(PKV_LORA_F32); break;
+    case PKV_LORA_F16: PKV_REDUCE(PKV_LORA_F16); break;
+    default: PKV_REDUCE(PKV_LORA_BF16); break;
+  }
+#undef PKV_REDUCE
+  PKV_HIP(hipGetLastError());
+  return PKV_OK;
+}
+
+// The gated inputs of T_pad tokens as fp16 pairs, at the start of a plan's workspace.
+int launch_xprep(const float *attn, const float *gate, int T, int K, const MxPlan &p, uint8_t *base,
+                 hipStream_t s) {
+  XprepArgs xa{attn, gate, T, K, reinterpret_cast<u4 *>(base), reinterpret_cast<u4 *>(base + p.off_xl),
+               reinterpret_cast<h4 *>(base + p.off_xs), reinterpret_cast<float *>(base + p.off_inv)};
+  if (K == 4096)
+    hipLaunchKernelGGL(oproj_xprep_kernel<2>, dim3((unsigned)p.T_pad), dim3(256), 0, s, xa);
+  else
+    hipLaunchKernelGGL(oproj_xprep_kernel<4>, dim3((unsigned)p.T_pad), dim3(256), 0, s, xa);
+  PKV_HIP(hipGetLastError());
+  return PKV_OK;
+}
+
 // From this many tokens on, the k-quant projection runs as the batched MFMA form (each
 // decoded weight serves 32 or 64 tokens); below it, per-token GEMV workgroups.
 constexpr int kOprojMfmaMinBatch = 8;
@@ -657,7 +801,7 @@ int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, in
       return set_error(PKV_ERR_ARG, "attn, gate and the weights must be 16-byte aligned");
   const MxPlan p = plan_mx(w_type, batch, in_dim, out_dim);
   const bool wide = p.wide;
-  const int T = batch, N = out_dim, K = in_dim, T_pad = p.T_pad, S = p.S, rbs = p.rbs, tbs = p.tbs;
+  const int T = batch, N = out_dim, K = in_dim, S = p.S, rbs = p.rbs, tbs = p.tbs;
   const int KB = K / 32, SB = K / 256, per = p.per;
   const int64_t row_bytes = (int64_t)SB * (w_type == kMQ4K ? 144 : w_type == kMQ5K ? 176 : 210);
   if ((int64_t)rbs * tbs * SB > (1 << 30))
@@ -665,13 +809,7 @@ int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, in
   const size_t off_xl = p.off_xl, off_xs = p.off_xs, off_inv = p.off_inv, off_part = p.off_part;
   if (int rc = ws.reserve(p.bytes)) return rc;
   uint8_t *base = static_cast<uint8_t *>(ws.ptr);
-  XprepArgs xa{attn, gate, T, K, reinterpret_cast<u4 *>(base), reinterpret_cast<u4 *>(base + off_xl),
-               reinterpret_cast<h4 *>(base + off_xs), reinterpret_cast<float *>(base + off_inv)};
-  if (K == 4096)
-    hipLaunchKernelGGL(oproj_xprep_kernel<2>, dim3((unsigned)T_pad), dim3(256), 0, s, xa);
-  else
-    hipLaunchKernelGGL(oproj_xprep_kernel<4>, dim3((unsigned)T_pad), dim3(256), 0, s, xa);
-  PKV_HIP(hipGetLastError());
+  if (int rc = launch_xprep(attn, gate, T, K, p, base, s)) return rc;
   if (lora != nullptr) {
     const LoraSplit split{base, base + off_xl, reinterpret_cast<const float *>(base + off_inv)};
     if (int rc = launch_lora_shrink(*lora, split, s)) return rc;
@@ -704,24 +842,9 @@ int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, in
 #undef PKV_MX
   PKV_HIP(hipGetLastError());
   if (S > 1 && lora != nullptr) {
-    const dim3 rgrid((unsigned)((N + 255) / 256), (unsigned)(T < 65535 ? T : 65535));
-    const float *part = reinterpret_cast<const float *>(base + off_part);
-    const float *inv = reinterpret_cast<const float *>(base + off_inv);
-    const bool vec = lora->rank % 4 == 0;
-#define PKV_REDUCE(TYPE)                                                                          \
-  if (vec)                                                                                        \
-    hipLaunchKernelGGL((oproj_reduce_lora_kernel<TYPE, true>), rgrid, dim3(256), 0, s, part, inv, \
-                       out, T, N, S, *lora);                                                      \
-  else                                                                                            \
-    hipLaunchKernelGGL((oproj_reduce_lora_kernel<TYPE, false>), rgrid, dim3(256), 0, s, part, inv, \
-                       out, T, N, S, *lora)
-    switch (lora->type) {
-      case PKV_LORA_F32: PKV_REDUCE(PKV_LORA_F32); break;
-      case PKV_LORA_F16: PKV_REDUCE(PKV_LORA_F16); break;
-      default: PKV_REDUCE(PKV_LORA_BF16); break;
-    }
-#undef PKV_REDUCE
-    PKV_HIP(hipGetLastError());
+    if (int rc = reduce_lora(reinterpret_cast<const float *>(base + off_part),
+                             reinterpret_cast<const float *>(base + off_inv), out, T, N, S, *lora, s))
+      return rc;
   } else if (S > 1) {
     const int per_row = N % 4 == 0 ? N / 4 : N;
     const dim3 rgrid((unsigned)((per_row + 255) / 256), (unsigned)(T < 65535 ? T : 65535));
@@ -733,13 +856,39 @@ int launch_oproj_mfma(const float *attn, const float *gate, const uint8_t *w, in
   return PKV_OK;
 }
 
+// The batched form for Q8_0 weights with adapters, past 3 2^25 products (12 rows of 4096 into
+// 2048): token by token / batched, us: 8 rows 24 / 34, 16 40.7 / 35.7, 64 133 / 38; 8192 into 100, 100
+// rows 54.7 / 42.6; into 70, 17 rows 17.1 / 38.5.
+static bool batched_q8(int w_type, int batch, int in_dim, int out_dim) {
+  return w_type == 8 && batch > 8 && (int64_t)batch * in_dim * out_dim > (int64_t)3 << 25;
+}
+
+static int launch_oproj_q8(const float *attn, const float *gate, const uint8_t *w, float *out, int T,
+                           int K, int N, Workspace &ws, hipStream_t s, const LoraTerm &lora) {
+  const MxPlan p = plan_q8(T, K, N);
+  if (int rc = ws.reserve(p.bytes)) return rc;
+  uint8_t *base = static_cast<uint8_t *>(ws.ptr);
+  if (int rc = launch_xprep(attn, gate, T, K, p, base, s)) return rc;
+  const float *inv = reinterpret_cast<const float *>(base + p.off_inv);
+  if (int rc = launch_lora_shrink(lora, LoraSplit{base, base + p.off_xl, inv}, s)) return rc;
+  float *part = reinterpret_cast<float *>(base + p.off_part);
+  const Q8Args a{reinterpret_cast<const u4 *>(base), reinterpret_cast<const u4 *>(base + p.off_xl), w, part, T, N, K, p.per};
+  hipLaunchKernelGGL(oproj_q8_kernel, dim3((unsigned)p.rbs, (unsigned)p.tbs, (unsigned)p.S), dim3(256), 0, s, a);
+  PKV_HIP(hipGetLastError());
+  return reduce_lora(part, inv, out, T, N, p.S, lora, s);
+}
+
+// of a projection with adapters
 size_t oproj_workspace(int w_type, int batch, int in_dim, int out_dim) {
+  if (batched_q8(w_type, batch, in_dim, out_dim)) return plan_q8(batch, in_dim, out_dim).bytes;
   return batched_form(w_type, batch) ? plan_mx(w_type, batch, in_dim, out_dim).bytes : 0;
 }
 
 int oproj_any(const float *attn, const float *gate, const uint8_t *w, int w_type, float *out,
               int batch, int in_dim, int out_dim, Workspace &ws, hipStream_t s,
               const LoraTerm *lora) {
+  if (lora != nullptr && batched_q8(w_type, batch, in_dim, out_dim))
+    return launch_oproj_q8(attn, gate, w, out, batch, in_dim, out_dim, ws, s, *lora);
   if (batched_form(w_type, batch))
     return launch_oproj_mfma(attn, gate, w, w_type, out, batch, in_dim, out_dim, ws, s, lora);
   return launch_oproj(attn, gate, w, w_type, out, batch, in_dim, out_dim, s, lora);

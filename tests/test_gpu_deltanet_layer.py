@@ -517,6 +517,9 @@ W_BYTES = {8: 34 / 32, 12: 144 / 256, 13: 176 / 256, 14: 210 / 256}
     (16, 4096, 130, 17, 6, "float32", 13, True),
     (33, 8192, 72, 128, 3, "bfloat16", 12, False),
     (40, 4096, 96, 5, 40, "bfloat16", 8, True),
+    (130, 4096, 300, 20, 4, "float16", 8, True),    # Q8_0 weights, batched
+    (70, 8192, 513, 33, 5, "float32", 8, False),
+    (13, 4096, 2048, 16, 13, "bfloat16", 8, True),
     (130, 4096, 300, 64, 3, "bfloat16", 12, True),
     (257, 4096, 513, 20, 4, "float16", 14, True),
     (600, 4096, 64, 8, 2, "float32", 12, True),
@@ -549,7 +552,10 @@ def test_lora(pk, orc, rows, inner, width, rank, n, dtype, w_type, gated):
     if rows > 1 and (ids < 0).any():  # rows without an adapter are the projection's
         plain = pk.gated_o_proj(x, g, torch.from_numpy(wb).cuda(), width, w_type=w_type)
         at = torch.from_numpy(ids < 0).cuda()
-        assert torch.equal(got[at], plain[at])
+        if w_type == 8 and rows * inner * width > 3 << 25:  # the projection alone goes token by token
+            assert rel(got[at], plain[at]) < 2 * 2e-6
+        else:
+            assert torch.equal(got[at], plain[at])
     assert pk.lib().pkv_device_status() == 0
 
 

@@ -127,7 +127,7 @@ __device__ void scan_tokens(const ScanArgs &a, TokenStage<kD> &st, int64_t b, in
     }
     qk = row16_sum(qk);
     st.v[buf][r][lane] = vv;
-    if (lane == 0) st.c[buf][r] = float4{expf(gv), t0 + r < end ? 1.0f / (1.0f + expf(-bv)) : 0.0f, qk, gv};
+    if (lane == 0) st.c[buf][r] = float4{expf(gv), 1.0f / (1.0f + expf(-bv)), qk, gv};
   };
 
   float s[4 * kQ];
@@ -146,8 +146,7 @@ __device__ void scan_tokens(const ScanArgs &a, TokenStage<kD> &st, int64_t b, in
     __syncthreads();
     if (t0 + kT < end) fetch(t0 + kT);
     float kept = 0.0f;
-#pragma unroll 4
-    for (int t = 0; t < kT; ++t) {
+    const auto token = [&](int t) {
       const float4 c4 = st.c[buf][t];
       const float vi = st.v[buf][t][r];
       float kk[4 * kQ], dk[2] = {0.0f, 0.0f}, dq[2] = {0.0f, 0.0f};
@@ -168,7 +167,15 @@ __device__ void scan_tokens(const ScanArgs &a, TokenStage<kD> &st, int64_t b, in
       for (int e = 0; e < 4 * kQ; ++e) s[e] = fmaf(u, kk[e], c4.x * s[e]);
       kept = lane == t ? o : kept;  // lane t keeps token t's output
       gates += (double)c4.w;
-    }
+    };
+    // the slots behind the end are left out: their q and k are of zero vectors (NaN with eps = 0),
+    // and 0 times an infinite state is NaN
+    const int slots = end - t0 < kT ? (int)(end - t0) : kT;
+    int done = 0;
+    for (; done + 4 <= slots; done += 4)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) token(done + i);
+    for (; done < slots; ++done) token(done);
     if (lane < kT && t0 + lane < end) out[(t0 + lane) * a.heads * kD + r] = kept;
     if (t0 + kT < end) stage(t0 + kT, buf ^ 1);
   }

@@ -1,0 +1,156 @@
+"""The gated delta rule over prompts (delta_net_chunked, paramecia-model/src/qwen3_next.rs:
+3506-3731) where magnitudes differ: states that decay away, values that fall, rise or jump
+within a chunk, masked tokens, eps = 0, infinite states; at every head size, over chunks,
+segments and the token-by-token form, each token and value channel held by itself.
+
+A row S_i of the state (value channel i) has a norm of at most
+  N_t = exp(gate_t) N_(t-1) + sigmoid(beta_t) |v_ti|,  N_0 = |S_i|
+while no gate is positive, as I - sigmoid(beta) k k^T lengthens nothing (|k| <= 1). A token's
+step rounds some 16 times, by half a step of f32 (E = 2^-24) of values up to N_t, and what it is
+off decays as N_t does; errors of n tokens that add up as independent ones make
+E (16 + 2 sqrt(n)) N_t of the row, and scale times that of an output, as |q| <= 1."""
+import sys
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+TINY = 2.0 ** -126  # f32's smallest normal value: nothing is held to a relative precision below
+
+
+def say(*a):
+    print(*a, flush=True)
+    sys.stdout.flush()
+
+
+@pytest.fixture(scope="module")
+def pk():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import paramecia_amd
+    paramecia_amd.lib()
+    return paramecia_amd
+
+
+def formula(q, k, v, gate, beta, state, scale, eps, lens=None):
+    """(outputs, state, N of every token, N behind the last) token by token in 64 bits; rows
+    behind a sequence's end are zeros."""
+    b, n, hk, d = q.shape
+    rep = v.shape[2] // hk
+    end = torch.full((b,), n) if lens is None else torch.tensor(lens)
+    end = end.clamp(0, n).to(q.device)
+    q, k, v, gate, beta, s = (t.double() for t in (q, k, v, gate, beta, state))
+    q = (q * scale / (q.square().sum(-1, keepdim=True) + eps).sqrt()).repeat_interleave(rep, 2)
+    k = (k / (k.square().sum(-1, keepdim=True) + eps).sqrt()).repeat_interleave(rep, 2)
+    alpha, be = gate.exp(), torch.sigmoid(beta)
+    out, size, norm = torch.zeros_like(v), torch.zeros_like(v), s.norm(dim=-1)
+    for t in range(n):
+        on = (t < end)[:, None, None]
+        old = s * alpha[:, t, :, None, None]
+        u = be[:, t, :, None] * (v[:, t] - (old * k[:, t, :, None]).sum(-1))
+        new = old + u[..., None] * k[:, t, :, None]
+        grown = norm * alpha[:, t, :, None] + be[:, t, :, None] * v[:, t].abs()
+        out[:, t] = torch.where(on, (new * q[:, t, :, None]).sum(-1), out[:, t])
+        size[:, t] = torch.where(on, grown, size[:, t])
+        s, norm = torch.where(on[..., None], new, s), torch.where(on, grown, norm)
+    return out, s, size, norm
+
+
+def inputs(seed, b, n, hk, h, d):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
+    return (r(b, n, hk, d), r(b, n, hk, d), r(b, n, h, d), -0.5 * torch.nn.functional.softplus(r(b, n, h)),
+            r(b, n, h), 0.3 * r(b, h, d, d))
+
+
+def check(pk, q, k, v, gate, beta, state, eps=1e-6, lens=None, scale=0.1):
+    n = q.shape[1]
+    want, want_state, size, norm = formula(q, k, v, gate, beta, state, scale, eps, lens)
+    out = torch.zeros_like(v)
+    dl = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    pk.gated_delta_rule(q, k, v, gate.contiguous(), beta.contiguous(), state, scale, eps, lens=dl, out=out)
+    lim = E * (16 + 2 * n ** 0.5)
+    assert torch.isfinite(out).all() and torch.isfinite(state).all()
+    off = ((out.double() - want).abs() / (scale * (lim * size + TINY))).max()
+    # what decays by more than e^-87 within a chunk may be taken for nothing
+    off_state = ((state.double() - want_state).norm(dim=-1) / (lim * norm + TINY * state.shape[-1] ** 0.5)).max()
+    say(f"  off by {float(off):.2e} of the limit, the state by {float(off_state):.2e}")
+    assert off <= 1 and off_state <= 1
+    return out
+
+
+KINDS = ["plain", "silent", "whisper", "falling", "falling_chunk", "early", "late", "jump", "masked_jump", "masked_token",
+         "fast", "forgetful", "opened"]
+
+
+def shaped(kind, q, k, v, gate, beta, state):
+    n = q.shape[1]
+    t = torch.arange(n, device="cuda")
+    ramp = torch.linspace(0, 1, n, device="cuda")[:, None, None]
+    if kind in ("silent", "whisper"):  # a decay of e^-31, then values of zero, or next to it
+        gate = torch.where(t[:, None] == 3, -30.0, -1e-3).expand_as(gate)
+        v = v * (0.0 if kind == "silent" else 1e-20)
+    elif kind == "falling":  # values far below the state in front of them, which decays
+        gate, v = gate * 0 - 1.0, v * 1e-8
+    elif kind == "falling_chunk":  # from one chunk to the next
+        gate, v = gate * 0 - 1.0, torch.where((t < 64)[:, None, None], v, v * 1e-6)
+        state = state * 0
+    elif kind == "early":
+        v, state = v * torch.exp2(-60 * ramp), state * 0
+    elif kind == "late":
+        v, state = v * torch.exp2(60 * ramp - 60), state * 0
+    elif kind == "jump":  # one token's values outweigh those in front of it in its chunk
+        v, state = torch.where((t % 64 == 50)[:, None, None], v * 2.0 ** 30, v), state * 0
+    elif kind == "masked_jump":  # sigmoid(beta) = 0: nothing of them is written
+        at = t % 64 == 20
+        v, beta = torch.where(at[:, None, None], v * 2.0 ** 40, v), torch.where(at[:, None], -200.0, beta)
+    elif kind == "masked_token":  # next to nothing of them is written
+        at = t % 64 == 20
+        v, beta = torch.where(at[:, None, None], v * 2.0 ** 20, v), torch.where(at[:, None], -25.0, beta)
+    elif kind == "fast":
+        gate = gate * 0 - 11.0
+    elif kind == "forgetful":  # a large state gone at once, small values behind
+        gate, v, state = torch.where(t[:, None] % 64 == 7, -60.0, gate), v * 1e-10, state * 1e6
+    elif kind == "opened":  # the first tokens write all but nothing
+        beta, state = torch.where((t < 40)[:, None], -30.0, beta), state * 0
+    return q, k, v, gate, beta, state
+
+
+def workspace(pk, q, v):
+    b, n, hk, d = q.shape
+    return pk.lib().pkv_deltanet_prompt_workspace(b, n, hk, v.shape[2], d)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_magnitudes_of_few_tokens(pk, kind):
+    say(f"magnitudes {kind}, token by token")
+    ins = shaped(kind, *inputs(41, 1, 41, 1, 2, 128))
+    assert workspace(pk, ins[0], ins[2]) == 0
+    check(pk, *ins)
+
+
+@pytest.mark.parametrize("b,n,d,lens", [(1, 1, 128, None), (2, 5, 64, None), (1, 17, 128, None), (1, 7, 256, None),
+                                        (3, 40, 128, [40, 3, 0]), (1, 100, 128, None), (2, 90, 256, [90, 70])])
+def test_eps_zero(pk, b, n, d, lens):
+    """Without eps every key and query has a norm to divide by; padding has none."""
+    say(f"eps=0 b={b} n={n} d={d}")
+    check(pk, *inputs(n, b, n, 2, 4, d), eps=0.0, lens=lens)
+
+
+@pytest.mark.parametrize("b,n,d,lens", [(1, 5, 128, None), (1, 3, 256, None), (2, 40, 64, [40, 19]), (1, 100, 128, None)])
+def test_infinite_state_is_kept(pk, b, n, d, lens):
+    """The last token writes an infinity: what the slots behind it hold changes nothing."""
+    say(f"infinite state b={b} n={n} d={d}")
+    ins = inputs(n, b, n, 1, 2, d)
+    for i, e in enumerate([n] * b if lens is None else lens):
+        ins[2][i, e - 1, 1, 3] = float("inf")
+    _, want, _, _ = formula(*ins, 0.1, 1e-6, lens)
+    dl = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    pk.gated_delta_rule(*ins, 0.1, 1e-6, lens=dl)
+    assert torch.isinf(want[:, 1, 3]).all() and torch.equal(ins[5][:, 1, 3].double(), want[:, 1, 3])
+    fine = torch.isfinite(want)
+    lim = E * (16 + 2 * n ** 0.5)
+    assert bool(((ins[5].double() - want)[fine].abs() <= 40 * lim).all())

@@ -995,7 +995,9 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         const uint32_t vnext = groups_max(umax(umax(mag(x[0]), mag(x[1])), umax(mag(x[2]), mag(x[3]))));
         const uint32_t mtop = groups_max(top[j]);
         if (g == 0) {
-          const float t = (float)__builtin_bit_cast(_Float16, (uint16_t)mtop) * inverse2(sm[j]) * 1.001f;
+          // a high part of zero leaves up to half its smallest step, 2^-24, of the state: taken for none,
+          // the next scale would make infinities of it
+          const float t = (float)__builtin_bit_cast(_Float16, (uint16_t)umax(mtop, 1u)) * inverse2(sm[j]) * 1.001f;
           reinterpret_cast<uint32_t *>(&lds.c.top[(c + 1) & 1][0][j][m])[w] = mag(t);
           reinterpret_cast<uint32_t *>(&lds.c.top[(c + 1) & 1][1][j][m])[w] = vnow[j];
           reinterpret_cast<uint32_t *>(&lds.c.top[(c + 1) & 1][2][j][m])[w] = vnext;

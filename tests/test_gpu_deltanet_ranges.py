@@ -154,3 +154,16 @@ def test_infinite_state_is_kept(pk, b, n, d, lens):
     fine = torch.isfinite(want)
     lim = E * (16 + 2 * n ** 0.5)
     assert bool(((ins[5].double() - want)[fine].abs() <= 40 * lim).all())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [193, 200, 256, 320])
+@pytest.mark.parametrize("kind", ["silent", "whisper"])
+def test_vanishing_state_stays_finite(pk, kind, n, d):
+    """What is left of a state far below its scale, with no values to hide it."""
+    say(f"vanishing state {kind} n={n} d={d}")
+    q, k, v, gate, beta, state = shaped(kind, *inputs(n + d, 1, n, 1, 2, d))
+    assert workspace(pk, q, v) > 0
+    out = pk.gated_delta_rule(q, k, v, gate.contiguous(), beta, state, 0.1, 1e-6)
+    assert torch.isfinite(out).all() and torch.isfinite(state).all()
+    assert float(state.abs().max()) < 1e-9 and float(out[:, 64:].abs().max()) < 1e-9

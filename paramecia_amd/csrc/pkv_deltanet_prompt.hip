@@ -15,14 +15,21 @@
 //   R = diag(be) (V - diag(e^G) K M),  U = T R,
 //   O = diag(e^G) Q M + P U,  M' = e^(G_63) M + K^T diag(e^(G_63 - G)) U.
 // chunk_kernel makes T, P and the operands of K and Q for all chunks at once; state_kernel
-// then walks each head's chunks, its state in registers. Products run on
-// v_mfma_f32_16x16x32_f16 with every operand in two fp16 parts (22 bits; hi hi + hi lo + lo hi),
-// which is exact to about f32: k, q, T and P are at most 1 in magnitude, and M, R and U are
-// scaled, each value channel by a power of two of its own, from bounds that hold while no gate
-// is positive. (Within a channel the parts keep 22 bits of a value down to some 2^-20 of the
-// chunk's largest.) A head with a positive gate, with a key or query that normalisation leaves
-// below 2^-8, or with a value that is not finite or past 2^90, goes token by token instead (a NaN
-// then reaches the tokens behind it and no others, as there).
+// then walks each head's chunks, its state in registers. Products run on 16-bit MFMA:
+//   K, Q, M, W = diag(e^(G_63 - G)) U: two fp16 parts (22 bits; hi hi + hi lo + lo hi). K and Q are
+//     at most 1. M and W are scaled, each value channel in each chunk by a power of two of its
+//     own: what they are off by relative to a channel's largest is all that counts of them. With
+//     N = |M_i| in front of the chunk and Y = max be_s e^(G_63 - G_s) |v_si|, both stay below
+//     e^(G_63) N + 65 Y, as a token lengthens M_i by be |v| at most, and |u_s| <= be_s (|v_si| + |M_i|).
+//   T, P, R, U: three bf16 parts (24 bits and f32's exponents; the six products down to 2^-16). A
+//     token's values may be small beside those of tokens behind it, for which a common scale
+//     would leave no bits.
+// What an output or a state is off by is thus some roundings of the largest that the token's state
+// can be, as token by token (a state that later tokens erase is held to that too); what decays
+// by more than e^-87 within a chunk is held to 2^-126 of what it was. The bounds want gates that are
+// not positive: a head with a positive gate, with a gate below -10000, with a key or query that
+// normalisation leaves below 2^-8, or with a value or state that is not finite or past 2^90 goes
+// token by token instead (a NaN then reaches the tokens behind it and no others, as there).
 #include <algorithm>
 #include <type_traits>
 
@@ -68,7 +75,7 @@ __device__ __forceinline__ int64_t valid_tokens(const int *lens, int64_t b, int6
 // every row reads them back. Both products of a token are taken with the state in front of
 // it (S_new . qn = exp(gate) S . qn + u (kn . qn)), so that their reductions run beside each
 // other. 5 tokens of 32 heads of 128: 7.0 us, mostly the 4 MB of state and two memory latencies;
-// each token more 0.25 us, the chain from one state to the next.
+// each token more 0.2 us, the chain from one state to the next.
 template <int kD>
 struct TokenStage {
   static constexpr int kT = kD == 256 ? 8 : 16;
@@ -197,8 +204,8 @@ __global__ __launch_bounds__(256) void scan_tokens_kernel(ScanArgs a) {
 
 // ---- by chunks
 constexpr int kC = 64;           // tokens per chunk
-constexpr int kMeta = 3 * kC + 4;
-constexpr float kUp = 1024.0f;   // scale of the fp16 parts of k, q, T and P (at most 1)
+constexpr int kMeta = 4 * kC + 4;
+constexpr float kUp = 1024.0f;   // scale of the fp16 parts of k and q (at most 1)
 constexpr float kDown = 1.0f / 1024.0f;
 
 // The empty asm pins x: where x is a product, the compiler otherwise rounds one use of hi from
@@ -210,20 +217,44 @@ __device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) {
   lo = (_Float16)(x - (float)hi);
 }
 
-// Workspace of a segment. An operand fragment is 16 rows by 32 k in two parts (hi, lo) of 64
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ f4 mfma32(b8 a, b8 b, f4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// Two values as three bf16 parts each, together exact; a pair of parts a word.
+__device__ __forceinline__ void split3(float x, float y, uint32_t (&o)[3]) {
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    o[p] = __builtin_bit_cast(uint32_t, b2{(__bf16)x, (__bf16)y});
+    x -= __builtin_bit_cast(float, o[p] << 16);
+    y -= __builtin_bit_cast(float, o[p] & 0xFFFF0000u);
+  }
+}
+// a b of three parts each, the sums by size
+__device__ __forceinline__ void mfma3(const b8 (&a)[3], const b8 (&b)[3], f4 (&c)[3]) {
+  c[0] = mfma32(a[0], b[0], c[0]);
+  c[1] = mfma32(a[0], b[1], c[1]);
+  c[2] = mfma32(a[0], b[2], c[2]);
+  c[1] = mfma32(a[1], b[0], c[1]);
+  c[2] = mfma32(a[1], b[1], c[2]);
+  c[2] = mfma32(a[2], b[0], c[2]);
+}
+
+// Workspace of a segment. An operand fragment is 16 rows by 32 k in two or three parts of 64
 // lanes x 16 bytes: lane (m, g) holds row m, k 4 g .. 4 g + 3 and 16 + 4 g .. 16 + 4 g + 3,
 // the order in which an MFMA's result tiles become the next one's B operand without moving
 // between lanes. T and P are lower triangular: row tile w needs k step 1 (tokens 32 .. 63)
 // from w = 2 on, six fragments.
 struct ChunkWs {
   h8 *k, *q;       // [b][chunk][key head][row tile 4][d / 32][2][64]
-  h8 *t, *p;       // [b][chunk][head][6][2][64]
-  float *meta;     // [b][chunk][head][kMeta]: be, e^G, e^(G_63 - G) of its tokens; then the
-                   // largest be, the largest be e^(G_63 - G), and e^(G_63)
+  b8 *t, *p;       // [b][chunk][head][6][3][64]
+  float *meta;     // [b][chunk][head][kMeta]: be, e^G, e^(G_63 - G) and be e^(G_63 - G) (not below
+                   // 2^-126 where be is not) of its tokens; then e^(G_63)
   double *gates;   // [b][chunk][head]: the chunk's sum
   unsigned *odd;   // [b][chunk][head]: this chunk needs the token path
 };
-constexpr size_t kFrag = 2 * 64;  // h8 per fragment
+constexpr size_t kFrag = 2 * 64, kFrag3 = 3 * 64;  // units of 16 bytes per fragment
 struct ChunkArgs {
   ScanArgs s;
   ChunkWs w;
@@ -243,16 +274,6 @@ __device__ __forceinline__ uint32_t groups_max(uint32_t x) {
   x = umax(a[0], a[1]);
   const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   return umax(b[0], b[1]);
-}
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-  const auto dpp = [](uint32_t v, auto ctrl) {
-    return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, decltype(ctrl)::value, 0xF, 0xF, false);
-  };
-  x = umax(x, dpp(x, std::integral_constant<int, 0xB1>{}));
-  x = umax(x, dpp(x, std::integral_constant<int, 0x4E>{}));
-  x = umax(x, dpp(x, std::integral_constant<int, 0x141>{}));
-  x = umax(x, dpp(x, std::integral_constant<int, 0x140>{}));
-  return groups_max(x);
 }
 __device__ __forceinline__ double read_lane(double x, int lane) {
   const uint64_t u = __builtin_bit_cast(uint64_t, x);
@@ -286,8 +307,8 @@ __device__ __forceinline__ double prefix64(float x) {
 // diagonal blocks by forward substitution (16 lanes each, a column a lane), then T_ij = -T_ii
 // sum_k A_ik T_kj down the block columns, a wave each, on v_mfma_f32_16x16x4_f32, whose result
 // tiles are the next product's B operand as they are. 63 chunks of 16 key heads of 128 with 32 value
-// heads: 46 us for 115 MB written, two workgroups a CU (LDS); alone a workgroup takes 12 us, a
-// quarter of it its first loads.
+// heads: 48 us for 142 MB written, two workgroups a CU (LDS). 8 chunks, a round of 256 workgroups with
+// a value head each, 18 us: the chain of loads, norm, products, inverse and stores.
 template <int kD>
 __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
   constexpr int kS = kD / 32, kRow = kD + 8, kSq = 68;
@@ -425,8 +446,8 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
       meta[lane] = be;
       meta[kC + lane] = expf((float)G);
       meta[2 * kC + lane] = ec;
-      const uint32_t mb = wave_max(mag(be)), mc = wave_max(mag(be * ec));
-      if (lane < 4) meta[3 * kC + lane] = lane == 0 ? as_f(mb) : lane == 1 ? as_f(mc) : expf((float)last);
+      meta[3 * kC + lane] = fmaxf(be * ec, fminf(be, 0x1p-126f));
+      if (lane < 4) meta[4 * kC + lane] = expf((float)last);
       const bool all = __ballot(!fit) == 0;
       if (lane == 0) {
         a.w.gates[out + w] = last;
@@ -454,30 +475,30 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
       }
     }
     if constexpr (kD <= 128)
-      if (r0 == rep0) put_kq();  // 63 chunks 45.5 us, 48.7 with these stores in front of the products
+      if (r0 == rep0) put_kq();  // in front of the products these stores cost 3 us of 48
     lds_barrier();
     // the fragments of a lower triangular matrix's rows 16 w ..
-    const auto put_rows = [&](const float(*x)[kSq], h8 *o) {
+    const auto put_rows = [&](const float(*x)[kSq], b8 *o) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         if (p > w >> 1) continue;
-        h8 f[2];
+        u4 f[3];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const f4 y = *reinterpret_cast<const f4 *>(&x[16 * w + m][32 * p + 16 * c + 4 * g]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            _Float16 hi, lo;
-            split(y[i] * kUp, hi, lo);
-            f[0][4 * c + i] = hi;
-            f[1][4 * c + i] = lo;
+          for (int i = 0; i < 2; ++i) {
+            uint32_t o3[3];
+            split3(y[2 * i], y[2 * i + 1], o3);
+#pragma unroll
+            for (int u = 0; u < 3; ++u) f[u][2 * c + i] = o3[u];
           }
         }
-        o[tri(w, p) * kFrag + lane] = f[0];
-        o[tri(w, p) * kFrag + 64 + lane] = f[1];
+#pragma unroll
+        for (int u = 0; u < 3; ++u) o[tri(w, p) * kFrag3 + 64 * u + lane] = __builtin_bit_cast(b8, f[u]);
       }
     };
-    for (int e = 0; e < heads; ++e) put_rows(am[2 + e], a.w.p + (out + e) * 6 * kFrag);
+    for (int e = 0; e < heads; ++e) put_rows(am[2 + e], a.w.p + (out + e) * 6 * kFrag3);
     if (w < heads) {  // lane m of block g: column m of its inverse
       float D[16];
 #pragma unroll
@@ -529,21 +550,14 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
       }
     }
     lds_barrier();
-    for (int e = 0; e < heads; ++e) put_rows(am[2 + e], a.w.t + (out + e) * 6 * kFrag);
+    for (int e = 0; e < heads; ++e) put_rows(am[2 + e], a.w.t + (out + e) * 6 * kFrag3);
   }
 }
 
-// the largest magnitude of eight fp16 values, as bits (a NaN is larger than everything)
-__device__ __forceinline__ uint32_t top16(h8 x) {
-  uint32_t t = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t = umax(t, (uint32_t)__builtin_bit_cast(uint16_t, x[i]) & 0x7FFFu);
-  return t;
-}
 // The exponent that takes values up to `bound` (finite) below 2^15.
 __device__ __forceinline__ int scale_exp(float bound) {
   const int e = 14 - ((int)(__builtin_bit_cast(uint32_t, bound) >> 23) - 127);
-  return e > 100 ? 100 : e;
+  return e > 126 ? 126 : e;
 }
 // 1 / x of a power of two
 __device__ __forceinline__ float inverse2(float x) { return as_f(0x7F000000u - __builtin_bit_cast(uint32_t, x)); }
@@ -553,9 +567,11 @@ template <int kD, int kNT>
 union StateLds {
   struct {
     h8 m[kNT][kD / 32][2][64];  // the state's fragments
-    uint2 r[kNT][2][2][64][2], u[kNT][2][2][64][2], v[kNT][2][2][64][2];  // R, U, U e^(G_63 - G): [k step][part][lane][half]
+    // [k step][part][lane][half]: R and U, and U e^(G_63 - G), scaled
+    uint2 r[kNT][2][3][64][2], u[kNT][2][3][64][2], v[kNT][2][2][64][2];
     h8 k[2][kC][kD / 8];  // K of the chunk, [part][token][.. in keys_at's order]
-    uint4 top[2][3][kNT][16];  // [chunk's parity][maximum][..][channel], a word of each wave: bits of magnitudes
+    uint4 n[kNT][16], y[kNT][16];  // [channel], a word of each wave: bits of its N and Y
+    float scale[kNT][16];          // of U e^(G_63 - G) and of the state behind the chunk
     unsigned odd;
   } c;
   TokenStage<kD> t;
@@ -614,13 +630,16 @@ __device__ __forceinline__ h4 load_columns(const _Float16 *p) {
 // The chunks of 16 kNT value channels of one head, in order, by eight waves. Waves 0 - 3 carry the
 // state: wave w owns key channels w d / 4 .. of it (f32, in an MFMA result's layout) and
 // tokens 16 w .. of each chunk. Waves 4 - 7 make the outputs of the same tokens beside them, off
-// the path from one chunk to the next, and the bounds that the scales come from. A wave
+// the path from one chunk to the next. A wave
 // loads its fragments of the next chunk (K and Q: of the one after, where the registers hold
 // both) when a stage has used them, the state's waves once what others wait for is in LDS. K^T
 // comes from the K that the state's waves hold anyway, through LDS.
-// 63 chunks of 32 heads of 128, 256 workgroups: 123 us, 1.95 a chunk: 1.5 for the three stages one
-// behind the other, the rest for the 92 KB of fragments that a CU takes from L2 (124 KB, with K^T
-// of its own from memory: 145 us). A stage less (the product T R) would save 0.1 us a chunk.
+// The scales are found by the outputs' waves: Y of the next chunk while the others make U, the
+// scale itself beside their product Q M.
+// 63 chunks of 32 heads of 128, 256 workgroups: 130 us, 2.06 a chunk: the three stages one
+// behind the other, and the 104 KB of fragments that a CU takes from L2 beside them.
+// (T, P, R and U in two fp16 parts with a scale per channel: 118 us, and wrong where a channel's tokens
+// differ by more than 2^10. Y and the scale by the state's waves themselves: 140.)
 template <int kD, int kNT>
 __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   constexpr int kS = kD / 32, kN = kD / 64;
@@ -646,7 +665,7 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   end = end < stop ? end : stop;
   if (end <= a.first) return;
   const int tokens = (int)(end - a.first), chunks = (tokens + kC - 1) / kC;
-  const int64_t kstep = (int64_t)a.k_heads * 4 * kS * kFrag, tstep = (int64_t)a.s.heads * 6 * kFrag;
+  const int64_t kstep = (int64_t)a.k_heads * 4 * kS * kFrag, tstep = (int64_t)a.s.heads * 6 * kFrag3;
   const int64_t key0 = b * a.chunks * a.k_heads + hk, val0 = b * a.chunks * a.s.heads + h;
   const int64_t mstep = (int64_t)a.s.heads * kMeta;
   const float *meta = a.w.meta + val0 * kMeta;
@@ -668,50 +687,26 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
   for (int c = tid; c < chunks; c += 512)
     if (a.w.odd[val0 + (int64_t)c * a.s.heads] != 0u) lds.c.odd = 1u;
 
-  // A channel's scales in a chunk come from bounds. With N on the norm of its row of the state
-  // in front of a chunk, V on its |v| there, w = e^(G_63), x the largest be e^(G_63 - G): each
-  // token adds its |v| at most, so the row behind has a norm of at most N + 64 V, and of w N +
-  // 64 x (N + 65 V), as |u| <= be (|v| + norm). N of this chunk comes from the state in front of
-  // the one before: waves 4 - 7 find the maxima beside the others' work (top[0]: |M| in front
-  // of the chunk before, top[1] and top[2]: |v| in that chunk and in this one).
   constexpr float kRoot = kD == 64 ? 8.1f : kD == 128 ? 11.4f : 16.1f;  // above sqrt(d)
-  bool odd;
-  // 2^e: of the state in front of the chunk, of R and U, of U e^(G_63 - G), of the state behind
-  float sm[kNT], su[kNT], sv[kNT], sm1[kNT];
-  f4 ex0, ex1;  // of the chunk before and of this one: the largest be, x, w
-  const auto behind = [](float N, float V, const f4 &ex) {
-    return fminf(fmaf(64.0f, V, N), fmaf(ex[2], N, 64.0f * ex[1] * fmaf(65.0f, V, N)));
+  constexpr uint32_t kLargest = 0x6C800000u;  // 2^90; infinities and NaN are larger
+  bool odd = false;
+  uint32_t largest = 0u;  // magnitude of a value or of a state so far
+  const auto all_done = [&]() {
+    if (largest > kLargest) lds.c.odd = 1u;
+    lds_barrier();
+    odd = lds.c.odd != 0u;
   };
-  const auto get_scales = [&](int c) {
-    uint32_t any = 0u;
-#pragma unroll
-    for (int j = 0; j < kNT; ++j) {
-      uint32_t x[3];
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        const uint4 t = lds.c.top[c & 1][k][j][m];
-        x[k] = umax(umax(t.x, t.y), umax(t.z, t.w));
-        any = umax(any, x[k]);
-      }
-      const float N = c == 0 ? kRoot * as_f(x[0]) : behind(kRoot * as_f(x[0]), as_f(x[1]), ex0), V = as_f(x[2]);
-      const float bound = fmaf(65.0f, V, N);
-      // U's own errors, which do not shrink with be, must stay in range too
-      const int eu = scale_exp(bound * ex1[0]), ev = scale_exp(bound * ex1[1]);
-      su[j] = pow2(eu);
-      sv[j] = pow2(ev < eu + 24 ? ev : eu + 24);
-      sm1[j] = pow2(scale_exp(behind(N, V, ex1)));
-    }
-    odd = odd || __ballot(any > 0x6C800000u) != 0;  // 2^90
-  };
+  const auto whole = [&](const uint4 &t) { return as_f(umax(umax(t.x, t.y), umax(t.z, t.w))); };
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  odd = false;
 
   if (wave < 4) {
     const h8 *kw = a.w.k + (key0 * 4 + w) * kS * kFrag;
-    const h8 *tw = a.w.t + (val0 * 6 + tri(w, 0)) * kFrag;
+    const b8 *tw = a.w.t + (val0 * 6 + tri(w, 0)) * kFrag3;
     float *state = a.s.state + ((b * a.s.heads + h) * kD + row0 + m) * kD + w * (kD / 4) + 4 * g;
-    h8 ka[kS][2], kb[kDeep ? kS : 1][2], ktf[kN][2][2], tf[2][2];
+    h8 ka[kS][2], kb[kDeep ? kS : 1][2], ktf[kN][2][2];
+    b8 tf[2][3];
     f4 v[kNT], be, eg, ec;
+    float decay, sm[kNT];   // e^(G_63); the scale of the state's fragments
     const auto load_k = [&](int c, h8 (*f)[2]) {
       const h8 *p = kw + (c < chunks ? c : chunks - 1) * kstep;
 #pragma unroll
@@ -720,12 +715,12 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         for (int u = 0; u < 2; ++u) f[s][u] = at<h8>(p + s * kFrag + 64 * u, foff);
     };
     const auto load_t = [&](int c) {
-      const h8 *q = tw + c * tstep;
+      const b8 *q = tw + c * tstep;
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (p <= w >> 1) tf[p][u] = at<h8>(q + p * kFrag + 64 * u, foff);
+        for (int u = 0; u < 3; ++u)
+          if (p <= w >> 1) tf[p][u] = at<b8>(q + p * kFrag3 + 64 * u, foff);
     };
     const auto put_k = [&](h8 (*f)[2]) {
 #pragma unroll
@@ -752,15 +747,14 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           }
       }
     };
-    const auto load_meta = [&](int c, f4 &x, f4 &y, f4 &z, f4 &ex) {
+    const auto load_meta = [&](int c, f4 &x, f4 &y, f4 &z, float &e) {
       const float *p = meta + c * mstep;
       x = at<f4>(p, moff);
       y = at<f4>(p + kC, moff);
       z = at<f4>(p + 2 * kC, moff);
-      ex = at<f4>(p + 3 * kC, 0u);
+      e = at<float>(p + 4 * kC, 0u);
     };
-    load_meta(0, be, eg, ec, ex1);
-    ex0 = ex1;
+    load_meta(0, be, eg, ec, decay);
     load_v(0, v);
 #pragma unroll
     for (int j = 0; j < kNT; ++j) v[j] = transpose4(v[j]);
@@ -772,55 +766,51 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     for (int j = 0; j < kNT; ++j)
 #pragma unroll
       for (int n = 0; n < kN; ++n) M[j][n] = *reinterpret_cast<const f4 *>(state + 16 * j * kD + 16 * n);
+    const auto put_n = [&]() {  // the wave's part of max |M_i|
 #pragma unroll
-    for (int j = 0; j < kNT; ++j) {  // the first chunk's maxima: of M in front of it and of v
-      uint32_t x = 0u, y = 0u;
+      for (int j = 0; j < kNT; ++j) {
+        uint32_t x = 0u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+        for (int n = 0; n < kN; ++n)
 #pragma unroll
-        for (int n = 0; n < kN; ++n) x = umax(x, mag(M[j][n][i]));
-        y = umax(y, mag(v[j][i]));
+          for (int i = 0; i < 4; ++i) x = umax(x, mag(M[j][n][i]));
+        largest = umax(largest, x);
+        x = groups_max(x);
+        if (g == 0) reinterpret_cast<uint32_t *>(&lds.c.n[j][m])[w] = x;
       }
-      x = groups_max(x);
-      y = groups_max(y);
-      if (g == 0) {
-        reinterpret_cast<uint32_t *>(&lds.c.top[0][0][j][m])[w] = x;
-        reinterpret_cast<uint32_t *>(&lds.c.top[0][1][j][m])[w] = 0u;
-        reinterpret_cast<uint32_t *>(&lds.c.top[0][2][j][m])[w] = y;
-      }
-    }
-    const auto put_m = [&](const float (&up)[kNT]) {
+    };
+    put_n();
+    const auto put_m = [&]() {
 #pragma unroll
-      for (int j = 0; j < kNT; ++j)
+      for (int j = 0; j < kNT; ++j) {
 #pragma unroll
         for (int n = 0; n < kN; ++n) {
           uint2 hi, lo;
-          split4(M[j][n] * up[j], hi, lo);
+          split4(M[j][n] * sm[j], hi, lo);
           const int k = w * kN + n;
           reinterpret_cast<uint2 *>(&lds.c.m[j][k >> 1][0][lane])[k & 1] = hi;
           reinterpret_cast<uint2 *>(&lds.c.m[j][k >> 1][1][lane])[k & 1] = lo;
         }
+      }
     };
-    const auto put4 = [&](uint2 (*to)[64][2], const f4 &x) {
-      uint2 hi, lo;
-      split4(x, hi, lo);
-      to[0][lane][w & 1] = hi;
-      to[1][lane][w & 1] = lo;
+    const auto put3 = [&](uint2 (*to)[64][2], const f4 &x) {
+      uint32_t a2[3], b2[3];
+      split3(x[0], x[1], a2);
+      split3(x[2], x[3], b2);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) to[p][lane][w & 1] = uint2{a2[p], b2[p]};
     };
     __syncthreads();
     odd = lds.c.odd != 0u;
-    const auto first_scale = [&](int j) {  // of the state as it comes: its largest value is known
-      const uint4 t = lds.c.top[0][0][j][m];
-      return pow2(scale_exp(as_f(umax(umax(t.x, t.y), umax(t.z, t.w)))));
-    };
 #pragma unroll
-    for (int j = 0; j < kNT; ++j) sm[j] = first_scale(j);
-    if (!odd) put_m(sm);
+    for (int j = 0; j < kNT; ++j) sm[j] = pow2(scale_exp(whole(lds.c.n[j][m])));
+    if (!odd) put_m();
     lds_barrier();
 
     const auto step = [&](int c, h8 (*kf)[2]) {
       const int next = c + 1 < chunks ? c + 1 : c;
-      f4 bn, gn, cn, en, vn[kNT];
+      f4 bn, gn, cn, vn[kNT];
+      float en;
       load_meta(next, bn, gn, cn, en);
       load_v(next, vn);
       // ---- R = be (V - e^G K M)
@@ -836,47 +826,49 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           kx[j] = mfma32(kf[s][0], lo, kx[j]);
           ky[j] = mfma32(kf[s][1], hi, ky[j]);
         }
-      get_scales(c);  // what an odd chunk leaves is not used
+      put_k(kf);
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
         f4 r;
         const float dm = kDown * inverse2(sm[j]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = (be[i] * su[j]) * fmaf(-(eg[i] * dm), km[j][i] + (kx[j][i] + ky[j][i]), v[j][i]);
-        put4(lds.c.r[j][w >> 1], r);
+        for (int i = 0; i < 4; ++i) r[i] = be[i] * fmaf(-eg[i], (km[j][i] + (kx[j][i] + ky[j][i])) * dm, v[j][i]);
+        put3(lds.c.r[j][w >> 1], r);
       }
-      put_k(kf);
       load_k(c + (kDeep ? 2 : 1), kf);
       lds_barrier();
-      // ---- U = T R, times 2^e
-      f4 u[kNT], ux[kNT], uy[kNT];
+      // ---- U = T R, and U e^(G_63 - G) at the scale that holds the next state too
+      f4 u[kNT][3];
 #pragma unroll
-      for (int j = 0; j < kNT; ++j) u[j] = ux[j] = uy[j] = zero;
+      for (int j = 0; j < kNT; ++j) u[j][0] = u[j][1] = u[j][2] = zero;
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         if (p > w >> 1) continue;
 #pragma unroll
         for (int j = 0; j < kNT; ++j) {
-          const h8 hi = *reinterpret_cast<const h8 *>(lds.c.r[j][p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.r[j][p][1][lane]);
-          u[j] = mfma32(tf[p][0], hi, u[j]);
-          ux[j] = mfma32(tf[p][0], lo, ux[j]);
-          uy[j] = mfma32(tf[p][1], hi, uy[j]);
+          b8 r[3];
+#pragma unroll
+          for (int i = 0; i < 3; ++i) r[i] = *reinterpret_cast<const b8 *>(lds.c.r[j][p][i][lane]);
+          mfma3(tf[p], r, u[j]);
         }
       }
       get_kt();
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[j][i] = (u[j][i] + (ux[j][i] + uy[j][i])) * kDown;
-        put4(lds.c.v[j][w >> 1], u[j] * (ec * (sv[j] * inverse2(su[j]))));
-        put4(lds.c.u[j][w >> 1], u[j]);
+        sm[j] = lds.c.scale[j][m];
+        const f4 x = u[j][0] + (u[j][1] + u[j][2]);
+        uint2 hi, lo;
+        split4(x * (ec * sm[j]), hi, lo);
+        lds.c.v[j][w >> 1][0][lane][w & 1] = hi;
+        lds.c.v[j][w >> 1][1][lane][w & 1] = lo;
+        put3(lds.c.u[j][w >> 1], x);
       }
-      load_t(next);
+      if constexpr (kDeep) load_t(next);
       lds_barrier();
       // ---- the next state
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
-        const float dv = kDown * inverse2(sv[j]);
+        const float dv = kDown * inverse2(sm[j]);
         f4 n0[kN], nx[kN], ny[kN];
 #pragma unroll
         for (int n = 0; n < kN; ++n) n0[n] = nx[n] = ny[n] = zero;
@@ -893,28 +885,28 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 #pragma unroll
         for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) M[j][n][i] = fmaf(M[j][n][i], ex1[2], (n0[n][i] + (nx[n][i] + ny[n][i])) * dv);
+          for (int i = 0; i < 4; ++i) M[j][n][i] = fmaf(M[j][n][i], decay, (n0[n][i] + (nx[n][i] + ny[n][i])) * dv);
       }
-      put_m(sm1);
+      put_m();
+      put_n();
+      if constexpr (!kDeep) load_t(next);
 #pragma unroll
       for (int j = 0; j < kNT; ++j) v[j] = transpose4(vn[j]);
       be = bn;
       eg = gn;
       ec = cn;
-      ex0 = ex1;
-      ex1 = en;
-#pragma unroll
-      for (int j = 0; j < kNT; ++j) sm[j] = sm1[j];
+      decay = en;
       lds_barrier();
     };
     if constexpr (kDeep) {
       for (int c = 0; c < chunks && !odd; c += 2) {
         step(c, ka);
-        if (c + 1 < chunks && !odd) step(c + 1, kb);
+        if (c + 1 < chunks) step(c + 1, kb);
       }
     } else {
       for (int c = 0; c < chunks && !odd; ++c) step(c, ka);
     }
+    all_done();
     if (!odd) {
 #pragma unroll
       for (int j = 0; j < kNT; ++j)
@@ -923,11 +915,12 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     }
   } else {
     const h8 *qw = a.w.q + (key0 * 4 + w) * kS * kFrag;
-    const h8 *pw = a.w.p + (val0 * 6 + tri(w, 0)) * kFrag;
+    const b8 *pw = a.w.p + (val0 * 6 + tri(w, 0)) * kFrag3;
     const uint32_t row = (uint32_t)a.s.heads * kD * 4u;  // bytes between a token's outputs
     char *o0 = reinterpret_cast<char *>(a.s.out + ((b * a.s.n + a.first) * a.s.heads + h) * kD + row0);
     const uint32_t ooff = (uint32_t)(16 * w + 4 * g + (m & 3)) * row + 4u * (uint32_t)(m & 12);
-    h8 qa[kS][2], qb[kDeep ? kS : 1][2], pf[2][2];
+    h8 qa[kS][2], qb[kDeep ? kS : 1][2];
+    b8 pf[2][3];
     f4 eg;
     const auto load_q = [&](int c, h8 (*f)[2]) {
       const h8 *p = qw + (c < chunks ? c : chunks - 1) * kstep;
@@ -937,38 +930,53 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
         for (int u = 0; u < 2; ++u) f[s][u] = at<h8>(p + s * kFrag + 64 * u, foff);
     };
     const auto load_p = [&](int c) {
-      const h8 *q = pw + c * tstep;
+      const b8 *q = pw + c * tstep;
 #pragma unroll
       for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (p <= w >> 1) pf[p][u] = at<h8>(q + p * kFrag + 64 * u, foff);
+        for (int u = 0; u < 3; ++u)
+          if (p <= w >> 1) pf[p][u] = at<b8>(q + p * kFrag3 + 64 * u, foff);
+    };
+    f4 v[kNT], cy;  // of the chunk whose Y comes next
+    float decay = at<float>(meta + 4 * kC, 0u), sm[kNT];
+    const auto load_y = [&](int c) {
+      load_v(c < chunks ? c : chunks - 1, v);
+      cy = at<f4>(meta + (c < chunks ? c : chunks - 1) * mstep + 3 * kC, moff);
+    };
+    const auto put_y = [&]() {  // the wave's part of Y
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) {
+        const f4 x = transpose4(v[j]);
+        uint32_t y = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          y = umax(y, mag(cy[i] * x[i]));
+          largest = umax(largest, mag(x[i]));
+        }
+        y = groups_max(y);
+        if (g == 0) reinterpret_cast<uint32_t *>(&lds.c.y[j][m])[w] = y;
+      }
     };
     eg = at<f4>(meta + kC, moff);
-    ex0 = ex1 = at<f4>(meta + 3 * kC, 0u);
-    f4 v[kNT];
-    load_v(chunks > 1 ? 1 : 0, v);
+    load_y(0);
     load_q(0, qa);
     if constexpr (kDeep) load_q(1, qb);
     load_p(0);
+    put_y();
+    load_y(1);
     __syncthreads();
     odd = lds.c.odd != 0u;
-    uint32_t vnow[kNT];  // largest |v| of the wave's tokens in this chunk
 #pragma unroll
-    for (int j = 0; j < kNT; ++j) {
-      const uint4 t = lds.c.top[0][0][j][m];
-      sm[j] = pow2(scale_exp(as_f(umax(umax(t.x, t.y), umax(t.z, t.w)))));
-      vnow[j] = reinterpret_cast<const uint32_t *>(&lds.c.top[0][2][j][m])[w];
-    }
+    for (int j = 0; j < kNT; ++j) sm[j] = pow2(scale_exp(whole(lds.c.n[j][m])));
     lds_barrier();
 
     const auto step = [&](int c, h8 (*qf)[2]) {
       const int next = c + 1 < chunks ? c + 1 : c;
-      const f4 gn = at<f4>(meta + next * mstep + kC, moff), en = at<f4>(meta + next * mstep + 3 * kC, 0u);
+      const f4 gn = at<f4>(meta + next * mstep + kC, moff);
+      const float dn = at<float>(meta + next * mstep + 4 * kC, 0u);
       f4 qm[kNT], qx[kNT], qy[kNT];
 #pragma unroll
       for (int j = 0; j < kNT; ++j) qm[j] = qx[j] = qy[j] = zero;
-      uint32_t top[kNT] = {};  // largest magnitudes of the state's high parts, as fp16 bits
 #pragma unroll
       for (int s = 0; s < kS; ++s)
 #pragma unroll
@@ -977,60 +985,41 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
           qm[j] = mfma32(qf[s][0], hi, qm[j]);
           qx[j] = mfma32(qf[s][0], lo, qx[j]);
           qy[j] = mfma32(qf[s][1], hi, qy[j]);
-          if ((s & 3) == w || kS == 2) top[j] = umax(top[j], top16(hi));  // a quarter of the state each
         }
-      get_scales(c);
       load_q(c + (kDeep ? 2 : 1), qf);
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
         const float dm = kDown * inverse2(sm[j]);
+        sm[j] = pow2(scale_exp(fmaf(fmaxf(decay, 0x1p-126f) * kRoot, whole(lds.c.n[j][m]), 65.0f * whole(lds.c.y[j][m]))));
+        if (w == 0 && g == 0) lds.c.scale[j][m] = sm[j];
 #pragma unroll
         for (int i = 0; i < 4; ++i) qm[j][i] = eg[i] * ((qm[j][i] + (qx[j][i] + qy[j][i])) * dm);
       }
+      decay = dn;
       lds_barrier();
-      // the next chunk's maxima: M in front of this chunk, v of this chunk and of the next
-#pragma unroll
-      for (int j = 0; j < kNT; ++j) {
-        const f4 x = transpose4(v[j]);
-        const uint32_t vnext = groups_max(umax(umax(mag(x[0]), mag(x[1])), umax(mag(x[2]), mag(x[3]))));
-        const uint32_t mtop = groups_max(top[j]);
-        if (g == 0) {
-          // a high part of zero leaves up to half its smallest step, 2^-24, of the state: taken for none,
-          // the next scale would make infinities of it
-          const float t = (float)__builtin_bit_cast(_Float16, (uint16_t)umax(mtop, 1u)) * inverse2(sm[j]) * 1.001f;
-          reinterpret_cast<uint32_t *>(&lds.c.top[(c + 1) & 1][0][j][m])[w] = mag(t);
-          reinterpret_cast<uint32_t *>(&lds.c.top[(c + 1) & 1][1][j][m])[w] = vnow[j];
-          reinterpret_cast<uint32_t *>(&lds.c.top[(c + 1) & 1][2][j][m])[w] = vnext;
-        }
-        vnow[j] = vnext;
-      }
-      load_v(c + 2 < chunks ? c + 2 : chunks - 1, v);
+      put_y();
+      load_y(c + 2);
       lds_barrier();
-      f4 o[kNT], ox[kNT], oy[kNT];
+      f4 o[kNT], o3[kNT][3];
 #pragma unroll
-      for (int j = 0; j < kNT; ++j) o[j] = ox[j] = oy[j] = zero;
+      for (int j = 0; j < kNT; ++j) o3[j][0] = o3[j][1] = o3[j][2] = zero;
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         if (p > w >> 1) continue;
 #pragma unroll
         for (int j = 0; j < kNT; ++j) {
-          const h8 hi = *reinterpret_cast<const h8 *>(lds.c.u[j][p][0][lane]), lo = *reinterpret_cast<const h8 *>(lds.c.u[j][p][1][lane]);
-          o[j] = mfma32(pf[p][0], hi, o[j]);
-          ox[j] = mfma32(pf[p][0], lo, ox[j]);
-          oy[j] = mfma32(pf[p][1], hi, oy[j]);
+          b8 u[3];
+#pragma unroll
+          for (int i = 0; i < 3; ++i) u[i] = *reinterpret_cast<const b8 *>(lds.c.u[j][p][i][lane]);
+          mfma3(pf[p], u, o3[j]);
         }
       }
       load_p(next);
 #pragma unroll
-      for (int j = 0; j < kNT; ++j) {
-        const float du = kDown * inverse2(su[j]);
+      for (int j = 0; j < kNT; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[j][i] = a.s.scale * fmaf(o[j][i] + (ox[j][i] + oy[j][i]), du, qm[j][i]);
-        sm[j] = sm1[j];
-      }
+        for (int i = 0; i < 4; ++i) o[j][i] = a.s.scale * (o3[j][0][i] + (o3[j][1][i] + o3[j][2][i]) + qm[j][i]);
       eg = gn;
-      ex0 = ex1;
-      ex1 = en;
       lds_barrier();
       // 64 bytes of each token's row, as load_v
 #pragma unroll
@@ -1042,11 +1031,12 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
     if constexpr (kDeep) {
       for (int c = 0; c < chunks && !odd; c += 2) {
         step(c, qa);
-        if (c + 1 < chunks && !odd) step(c + 1, qb);
+        if (c + 1 < chunks) step(c + 1, qb);
       }
     } else {
       for (int c = 0; c < chunks && !odd; ++c) step(c, qa);
     }
+    all_done();
   }
   if (odd) {
     __syncthreads();
@@ -1071,18 +1061,20 @@ __global__ __launch_bounds__(512) void state_kernel(ChunkArgs a) {
 // A segment's chunks, and where its workspace's parts lie.
 // Prompts go by chunks from 72 tokens on, from 48 where their heads fill the GPU more than
 // twice (token by token a workgroup per 16 rows). us of the call, by tokens / by chunks, 32 heads
-// of 128: one sequence 64 tokens 18.1 / 19.5, 72 21.8 / 21.1, 128 33.7 / 22.1; four 32 tokens
-// 22.7 / 27.9, 48 30.4 / 28.5; twelve 24 tokens 50.6 / 54.8, 48 73.9 / 56.8. 16 heads of 256: 64
-// tokens 28.6 / 26.6; 32 of 64: 96 tokens 19.0 / 17.7.
+// of 128 over 16 key heads: one sequence 64 tokens 19.0 / 19.7, 72 20.8 / 21.4, 96 25.8 / 21.6; four 32 tokens
+// 23.4 / 31.6, 48 33.0 / 31.8; twelve 32 tokens 54.1 / 60.5, 48 74.7 / 62.1. More value heads per key head
+// change little: 20 over 4 key heads 72 tokens 20.5 / 21.8, 32 over 32 20.6 / 22.2. 16 heads of 256: 72 tokens
+// 31.9 / 30.8; 32 of 64: 80 tokens 16.2 / 17.5, 96 18.8 / 17.6.
 bool by_chunks(int batch, int64_t n, int heads, int d) {
   return n >= 72 || (n >= 48 && (int64_t)batch * heads * d > 8192);
 }
 // A segment's operands should stay in the 256 MB of last-level cache, but what a walk pays for
 // each segment (its state, the last round of workgroups) should not weigh either. us by bytes of a
-// segment 64 / 128 / 192 / 512 MB, 32 heads of 128: one sequence of 8001 tokens 350 / 331 / 332 / 363,
-// of 40000 1666 / 1495 / 1731 / 1667; 14 of 1100 (4, 5, 6, 18 chunks a segment) 883 / 643 /
-// 600 / 519; 28 of 2000 (2, 3, 4, 11 chunks) 4072 / 2966 / 2614 / 1992, 1 GB (16) 1845.
-constexpr size_t kSegmentBytes = (size_t)128 << 20, kSegmentMost = (size_t)1 << 30;
+// segment 80 / 160 / 240 / 640 MB, 32 heads of 128: one sequence of 8001 tokens 345 / 334 / 334 / 394,
+// of 40000 1815 / 1717 / 1957 / 1862; 14 of 1100 (2, 5, 6, 18 chunks a segment) 939 / 737 /
+// 694 / 593; 28 of 2000 (1, 2, 3, 10 chunks) 4455 / 3327 / 2993 / 2277, 1 GB (16) 2100. A chunk of all
+// sequences is a segment at least, whatever it takes (2.2 MB a sequence there).
+constexpr size_t kSegmentBytes = (size_t)160 << 20, kSegmentMost = (size_t)1 << 30;
 constexpr int64_t kSegmentChunks = 32;  // up to kSegmentMost
 struct SegmentPlan {
   int chunks = 0;  // 0: token by token
@@ -1092,7 +1084,7 @@ SegmentPlan plan_segment(int batch, int64_t n, int k_heads, int heads, int d) {
   SegmentPlan s;
   if (!by_chunks(batch, n, heads, d)) return s;
   const size_t key = (size_t)kC * d * 4;  // one operand of a key head's chunk
-  const size_t per = (size_t)batch * (k_heads * 2 * key + heads * (2 * 6 * kFrag * 16 + kMeta * 4 + 16));
+  const size_t per = (size_t)batch * (k_heads * 2 * key + heads * (2 * 6 * kFrag3 * 16 + kMeta * 4 + 16));
   const int64_t all = (n + kC - 1) / kC;
   const int64_t fit = std::max((int64_t)(kSegmentBytes / per), std::min((int64_t)(kSegmentMost / per), kSegmentChunks));
   const int64_t parts = (all + (fit < 1 ? 1 : fit) - 1) / (fit < 1 ? 1 : fit);
@@ -1100,8 +1092,8 @@ SegmentPlan plan_segment(int batch, int64_t n, int k_heads, int heads, int d) {
   const size_t keys = (size_t)batch * s.chunks * k_heads, vals = (size_t)batch * s.chunks * heads;
   s.q = keys * key;
   s.t = 2 * s.q;
-  s.p = s.t + vals * 6 * kFrag * 16;
-  s.meta = s.p + vals * 6 * kFrag * 16;
+  s.p = s.t + vals * 6 * kFrag3 * 16;
+  s.meta = s.p + vals * 6 * kFrag3 * 16;
   s.gates = s.meta + vals * kMeta * 4;
   s.odd = s.gates + vals * 8;
   s.bytes = s.odd + (vals * 4 + 15) / 16 * 16;
@@ -1118,18 +1110,18 @@ int launch(const ScanArgs &a, const SegmentPlan &plan, int batch, int k_heads, v
   }
   char *base = static_cast<char *>(ws);
   const ChunkWs w{reinterpret_cast<h8 *>(base), reinterpret_cast<h8 *>(base + plan.q),
-                  reinterpret_cast<h8 *>(base + plan.t), reinterpret_cast<h8 *>(base + plan.p),
+                  reinterpret_cast<b8 *>(base + plan.t), reinterpret_cast<b8 *>(base + plan.p),
                   reinterpret_cast<float *>(base + plan.meta),
                   reinterpret_cast<double *>(base + plan.gates), reinterpret_cast<unsigned *>(base + plan.odd)};
   // 32 value channels a workgroup halve the fragments' loads, 16 give twice the workgroups: one
-  // sequence of 8001 tokens (256 workgroups of 16) 333 us with 16, 395 with 32; two of 4000
-  // 306 and 251, seven of 1100 360 and 289. Heads of 256 have no registers for 32.
+  // sequence of 8001 tokens (256 workgroups of 16) 330 us with 16, 445 with 32; two of 4000
+  // 333 and 293, seven of 1100 403 and 329. Heads of 256 have no registers for 32.
   constexpr int kWide = kD <= 128 ? 2 : 1;
   const bool wide = kWide > 1 && (int64_t)batch * a.heads * (kD / 16) > 256;
   const int64_t all = (a.n + kC - 1) / kC;
   // A key head's value heads are shared out to workgroups while all of them have a CU of their
-  // own: 509 tokens, 16 key and 32 value heads of 128: 36.8 to 35.4 us, 4 and 16 39.2 to 32.5 (past
-  // 256, K and Q are worked out twice for nothing: 1000 tokens 47.2, 48.2 with two each).
+  // own: 509 tokens, 16 key and 32 value heads of 128: 41.2 to 39.7 us, 4 and 16 42.2 to 35.6 (past
+  // 256, K and Q are worked out twice for nothing: 1000 tokens 53.0 either way).
   const int64_t groups = (int64_t)plan.chunks * k_heads * batch;
   const int parts = (int)std::clamp<int64_t>(256 / groups, 1, a.rep);
   for (int64_t c = 0; c < all; c += plan.chunks) {

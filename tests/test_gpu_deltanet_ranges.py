@@ -124,12 +124,84 @@ def workspace(pk, q, v):
     return pk.lib().pkv_deltanet_prompt_workspace(b, n, hk, v.shape[2], d)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("n", [193, 256, 330])
+@pytest.mark.parametrize("kind", KINDS)
+def test_magnitudes(pk, kind, n, d):
+    say(f"magnitudes {kind} n={n} d={d}")
+    ins = shaped(kind, *inputs(n + d, 1, n, 1, 2, d))
+    assert workspace(pk, ins[0], ins[2]) > 0  # by chunks
+    check(pk, *ins)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_magnitudes_of_few_tokens(pk, kind):
     say(f"magnitudes {kind}, token by token")
     ins = shaped(kind, *inputs(41, 1, 41, 1, 2, 128))
     assert workspace(pk, ins[0], ins[2]) == 0
     check(pk, *ins)
+
+
+@pytest.mark.parametrize("b,n,hk,h,d,lens", [
+    (1, 72, 1, 1, 256, None),
+    (2, 130, 2, 4, 256, [130, 65]),
+    (1, 300, 2, 2, 256, None),                   # five chunks, an odd number
+    (1, 257, 1, 3, 64, None),
+    (4, 200, 2, 4, 64, [200, 0, 129, 64]),
+    (2, 3100, 8, 16, 256, [3100, 1000]),         # more than one segment
+    (4, 2200, 16, 32, 64, [2200, 2100, 5, 2048]),
+    (2, 80, 16, 32, 128, [80, 33]),              # a padded batch by chunks
+])
+def test_sizes_by_chunks(pk, b, n, hk, h, d, lens):
+    say(f"sizes b={b} n={n} hk={hk} h={h} d={d} lens={lens}")
+    ins = inputs(n + h, b, n, hk, h, d)
+    assert workspace(pk, ins[0], ins[2]) > 0
+    for i, e in enumerate([n] * b if lens is None else lens):
+        for t in ins[:5]:
+            t[i, e:] = float("nan")  # padding is not read
+    clean = [t.nan_to_num() for t in ins[:5]]
+    want, want_state, size, norm = formula(*clean, ins[5], 0.1, 1e-6, lens)
+    out, state = torch.zeros_like(ins[2]), ins[5].clone()
+    dl = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    pk.gated_delta_rule(*ins[:5], state, 0.1, 1e-6, lens=dl, out=out)
+    lim = E * (16 + 2 * n ** 0.5)
+    assert bool(((out.double() - want).abs() <= 0.1 * lim * size).all())
+    assert bool(((state.double() - want_state).norm(dim=-1) <= lim * norm).all())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("what", ["gate", "closed_gate", "key", "value"])
+def test_heads_token_by_token_beside_chunks(pk, what, d):
+    """A head that cannot go by chunks, from its second chunk on, beside one that does."""
+    say(f"odd head: {what} d={d}")
+    q, k, v, gate, beta, state = inputs(d, 1, 300, 2, 4, d)
+    if what == "gate":
+        gate[0, 100, 1] = 0.05
+    elif what == "closed_gate":
+        gate[0, 100, 1] = -20000.0
+    elif what == "key":
+        k[0, 100, 1] *= 1e-30
+    else:
+        v[0, 100, 1] *= 1e28
+    check(pk, q, k, v, gate, beta, state)
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("at", [0, 130, 299])
+def test_nan_goes_forward_only(pk, d, at):
+    say(f"NaN at {at} d={d}")
+    ins = inputs(d + at, 1, 300, 1, 2, d)
+    s0, s1 = ins[5].clone(), ins[5].clone()
+    want, _, size, _ = formula(*ins[:5], s0, 0.1, 1e-6)
+    clean = pk.gated_delta_rule(*ins[:5], s0, 0.1, 1e-6)
+    ins[2][0, at, 1, 5] = float("nan")
+    got = pk.gated_delta_rule(*ins[:5], s1, 0.1, 1e-6)
+    assert torch.equal(got[:, :, 0], clean[:, :, 0]) and torch.equal(s1[:, 0], s0[:, 0])
+    lim = 0.1 * E * (16 + 2 * 300 ** 0.5)
+    assert bool(((got[:, :at, 1].double() - want[:, :at, 1]).abs() <= lim * size[:, :at, 1]).all())
+    assert torch.isnan(got[0, at:, 1, 5]).all() and torch.isnan(s1[0, 1, 5]).all()
+    others = [i for i in range(d) if i != 5]  # a value channel reaches no other
+    assert torch.isfinite(got[0, :, 1, others]).all() and torch.isfinite(s1[0, 1, others]).all()
 
 
 @pytest.mark.parametrize("b,n,d,lens", [(1, 1, 128, None), (2, 5, 64, None), (1, 17, 128, None), (1, 7, 256, None),

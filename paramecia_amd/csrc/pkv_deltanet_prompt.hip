@@ -314,7 +314,7 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
   constexpr int kS = kD / 32, kRow = kD + 8, kSq = 68;
   constexpr int kKB = 2 * kC * kRow * 2, kAB = 4 * kC * kSq * 4;
   __shared__ __attribute__((aligned(16))) char lds[kKB > kAB ? kKB : kAB];
-  __shared__ float4 gam[2][kC];  // a token's sum of gates (base 2) in two parts, be
+  __shared__ float4 gam[2][kC];  // a token's sum of gates, base 2: whole number and rest; be
   __shared__ unsigned bad;
   _Float16(*kh)[kC][kRow] = reinterpret_cast<_Float16(*)[kC][kRow]>(lds);  // [hi, lo][token][k]
   float(*am)[kC][kSq] = reinterpret_cast<float(*)[kC][kSq]>(lds);           // A of two heads, then P and T of both
@@ -438,16 +438,18 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
       const bool fit = gv <= 0.0f && gv >= -10000.0f && bv == bv;
       const double G = prefix64(gv), last = read_lane(G, 63);
       const float be = lane < left ? 1.0f / (1.0f + expf(-bv)) : 0.0f;
-      const double G2 = G * 1.4426950408889634;
-      const float hi = (float)G2;
-      gam[w][lane] = float4{hi, (float)(G2 - (double)hi), be, 0.0f};
+      // 2^(whole + rest): a sum rounded to f32 would cost its power up to 2^-18
+      const double G2 = G * 1.4426950408889634, whole = __builtin_rint(G2);
+      const int gi = (int)whole, li = __builtin_amdgcn_readlane(gi, 63);
+      const float gf = (float)(G2 - whole), lf = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, gf), 63));
+      gam[w][lane] = float4{__builtin_bit_cast(float, gi), gf, be, 0.0f};
       float *meta = a.w.meta + (out + w) * kMeta;
-      const float ec = expf((float)(last - G));
+      const float ec = __builtin_ldexpf(__builtin_amdgcn_exp2f(lf - gf), li - gi);
       meta[lane] = be;
-      meta[kC + lane] = expf((float)G);
+      meta[kC + lane] = __builtin_ldexpf(__builtin_amdgcn_exp2f(gf), gi);
       meta[2 * kC + lane] = ec;
       meta[3 * kC + lane] = fmaxf(be * ec, fminf(be, 0x1p-126f));
-      if (lane < 4) meta[4 * kC + lane] = expf((float)last);
+      if (lane < 4) meta[4 * kC + lane] = __builtin_ldexpf(__builtin_amdgcn_exp2f(lf), li);
       const bool all = __ballot(!fit) == 0;
       if (lane == 0) {
         a.w.gates[out + w] = last;
@@ -466,9 +468,9 @@ __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {
         const float4 col = gam[e][16 * j + m];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          // 2^(G_t - G_s): the difference of the high parts is rounded once, as it is itself
           const int t = 16 * w + 4 * g + i, s = 16 * j + m;
-          const float dec = __builtin_amdgcn_exp2f((row[i].x - col.x) + (row[i].y - col.y));
+          const float dec = __builtin_ldexpf(__builtin_amdgcn_exp2f(row[i].y - col.y),
+                                             __builtin_bit_cast(int, row[i].x) - __builtin_bit_cast(int, col.x));
           am[e][t][s] = s < t ? row[i].z * dec * kk[j][i] : 0.0f;
           am[2 + e][t][s] = s <= t ? dec * qk[j][i] : 0.0f;
         }

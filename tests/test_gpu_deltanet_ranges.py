@@ -239,3 +239,20 @@ def test_vanishing_state_stays_finite(pk, kind, n, d):
     out = pk.gated_delta_rule(q, k, v, gate.contiguous(), beta, state, 0.1, 1e-6)
     assert torch.isfinite(out).all() and torch.isfinite(state).all()
     assert float(state.abs().max()) < 1e-9 and float(out[:, 64:].abs().max()) < 1e-9
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rate", [0.3, 0.97, 1.21])
+def test_one_write_ages(pk, rate, d):
+    """One token writes, along the only key, and decays by up to e^-77 in its chunk: what is left of it
+    is off by the roundings of its tokens' decays."""
+    say(f"one write ages rate={rate} d={d}")
+    n = 128
+    q, k, v, gate, beta, state = inputs(d, 1, n, 1, 2, d)
+    k = k[:, :1].expand_as(k).contiguous()
+    q, gate, state = k.clone(), gate * 0 - rate, state * 0
+    gate[..., 1] *= 1.01
+    for at in (0, 64):
+        b = torch.where((torch.arange(n, device="cuda") == at)[:, None], 3.0, -200.0).expand_as(beta)
+        check(pk, q, k, v, gate, b, state.clone())
+        check(pk, *(t[:, :at + 72].contiguous() for t in (q, k, v, gate, b)), state.clone())

@@ -1298,10 +1298,12 @@ int pkv_gated_oproj_lora(const float *attn, const float *gate, const void *w, in
                          int rank, const float *lora_scale, const int *adapter_ids, float *out,
                          int batch, int in_dim, int out_dim, void *workspace,
                          size_t workspace_bytes, pkv_stream stream) {
-  if (!attn || !w || !out || !lora_scale || !adapter_ids || !workspace)
-    return set_error(PKV_ERR_ARG, "null argument");
   if (batch <= 0 || in_dim <= 0 || out_dim <= 0)
     return set_error(PKV_ERR_ARG, "batch, in_dim and out_dim must be > 0");
+  // in front of the workspace's check: the size of such a call's is 0
+  if (batch > 65535) return set_error(PKV_ERR_ARG, "batch must be <= 65535 with adapters");
+  if (!attn || !w || !out || !lora_scale || !adapter_ids || !workspace)
+    return set_error(PKV_ERR_ARG, "null argument");
   if (int rc = check_lora(lora_a, lora_b, lora_type, n_adapters, rank)) return rc;
   const uint64_t in_bytes = 4 * (uint64_t)batch * in_dim, out_bytes = 4 * (uint64_t)batch * out_dim;
   if (overlap(attn, in_bytes, out, out_bytes) || (gate && overlap(gate, in_bytes, out, out_bytes)) ||

@@ -236,7 +236,6 @@ int launch_oproj_lora(const float *attn, const float *gate, const uint8_t *w, in
                       int rank, const float *scale, const int *ids, float *out, int rows,
                       int in_dim, int out_dim, void *ws, size_t ws_bytes, hipStream_t s) {
   if (int rc = check_oproj(attn, gate, w, w_type, rows, in_dim, out_dim)) return rc;
-  if (rows > 65535) return set_error(PKV_ERR_ARG, "batch must be <= 65535");
   if (ws_bytes < oproj_lora_workspace(w_type, rows, in_dim, out_dim, rank))
     return set_error(PKV_ERR_ARG, "the workspace is smaller than pkv_gated_oproj_lora_workspace says");
   if (reinterpret_cast<uintptr_t>(ws) % 256 != 0)

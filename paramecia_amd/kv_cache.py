@@ -651,7 +651,7 @@ def gated_o_proj_lora(attn_output: torch.Tensor, gate: Optional[torch.Tensor], w
     B_a (A_a x), x = attn_output * sigmoid(gate). lora_a [adapters, rank, in_dim] and lora_b
     [adapters, out_dim, rank] in float32, float16 or bfloat16, lora_scale f32 [adapters];
     adapter_ids int32, one per row (attn_output's shape without its last dimension), negative
-    for none. Everything else as gated_o_proj."""
+    for none; at most 65535 rows. Everything else as gated_o_proj."""
     dev = _device()
     x = _take(attn_output, "attn_output", attn_output.shape, dev)
     g = _take(gate, "gate", x.shape, dev)

@@ -322,7 +322,9 @@ int pkv_deltanet_prompt(const float *q, const float *k, const float *v, const in
  * gate * sigmoid(gate) where gate is given. x: [rows, dim] f32, rows `stride` elements
  * apart; residual, gate, out: [rows, dim] f32; alpha: [dim]. y goes to out, to out_q8_0, or
  * to both (one may be NULL): out_q8_0 takes pkv_bytes_per_row(PKV_QUANT_Q8_0, dim) bytes a
- * row, encoded as the cache encodes Q8_0 (a last block is filled up with zeros). dim at most
+ * row, encoded as the cache encodes Q8_0 (a last block is filled up with zeros). With out_q8_0 the
+ * gate's activation is taken in 64 bits (y is rounded once), else in 32 (y is off by at most 9 half
+ * steps): out with and without out_q8_0 differs by that. dim at most
  * 32768, and rows below 2^31 / 1024 (dim up to 8192: / 256, 512: / 64, 128: / 16; else
  * PKV_ERR_UNSUPPORTED). out or residual may be x itself (of dense rows), out
  * may be gate; no other buffers may overlap. */

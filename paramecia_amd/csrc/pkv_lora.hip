@@ -178,7 +178,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkAr
 #pragma unroll
     for (int c = 0; c < kC; ++c) red[wave][c][lane] = acc[c];
     __syncthreads();
-    const float scale = a.scale[cur];
+    const float scale = a.scale[cur];  // behind inv: their product may be too small to keep its bits
     for (int u = tid; u < 64 * kC; u += 64 * kShrinkWaves) {
       const int c = u >> 6, l = u & 63, r = 16 * c + (l & 15);
       v4 s = red[0][c][l];
@@ -189,8 +189,8 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void lora_shrink_kernel(ShrinkAr
         for (int i = 0; i < 4; ++i) {
           const int n = 4 * (l >> 4) + i;  // the row within the tile
           if ((mine >> n) & 1) {
-            const float f = kSplit ? scale * a.split.inv[row0 + n] : scale;
-            a.t[((int64_t)blockIdx.y * a.rows + row0 + n) * a.rank + r] = s[i] * f;
+            const float y = kSplit ? s[i] * a.split.inv[row0 + n] : s[i];
+            a.t[((int64_t)blockIdx.y * a.rows + row0 + n) * a.rank + r] = y * scale;
           }
         }
       }

@@ -301,7 +301,7 @@ int pkv_causal_conv(const float *x, int64_t stride_b, int64_t stride_t, const fl
  * token by token. q, k: [batch, n, k_heads, head_dim], v: [batch, n, heads, head_dim] f32,
  * value head h reading key head h / (heads / k_heads); strides: batch and token stride of
  * q, of k and of v in elements (slices of the convolution's output are taken as they are;
- * multiples of 4). gate, beta: [batch, n, heads]; state, gate_offset (NULL or [batch,
+ * multiples of 4). gate, beta: [batch, n, heads]; eps >= 0; state, gate_offset (NULL or [batch,
  * heads]): as pkv_deltanet_step, updated in place; lens as pkv_causal_conv: tokens behind a
  * sequence's end change nothing and their rows of out are left as they were. out: [batch, n,
  * heads, head_dim]. head_dim 64, 128 or 256 (else PKV_ERR_UNSUPPORTED), n at most 2^30, batch *

@@ -74,7 +74,7 @@ __device__ __forceinline__ int64_t valid_tokens(const int *lens, int64_t b, int6
 // normalise the next kT tokens' q and k into LDS while they are 16 lanes per token, then
 // every row reads them back. Both products of a token are taken with the state in front of
 // it (S_new . qn = exp(gate) S . qn + u (kn . qn)), so that their reductions run beside each
-// other. 5 tokens of 32 heads of 128: 7.0 us, mostly the 4 MB of state and two memory latencies;
+// other. 5 tokens of 32 heads of 128: 5.0 us, mostly the 4 MB of state and two memory latencies;
 // each token more 0.2 us, the chain from one state to the next.
 template <int kD>
 struct TokenStage {
@@ -307,7 +307,7 @@ __device__ __forceinline__ double prefix64(float x) {
 // diagonal blocks by forward substitution (16 lanes each, a column a lane), then T_ij = -T_ii
 // sum_k A_ik T_kj down the block columns, a wave each, on v_mfma_f32_16x16x4_f32, whose result
 // tiles are the next product's B operand as they are. 63 chunks of 16 key heads of 128 with 32 value
-// heads: 48 us for 142 MB written, two workgroups a CU (LDS). 8 chunks, a round of 256 workgroups with
+// heads: 48 us for 139 MB written, two workgroups a CU (LDS). 8 chunks, a round of 256 workgroups with
 // a value head each, 18 us: the chain of loads, norm, products, inverse and stores.
 template <int kD>
 __global__ __launch_bounds__(256) void chunk_kernel(ChunkArgs a) {

@@ -9,6 +9,7 @@ while no gate is positive, as I - sigmoid(beta) k k^T lengthens nothing (|k| <= 
 step rounds some 16 times, by half a step of f32 (E = 2^-24) of values up to N_t, and what it is
 off decays as N_t does; errors of n tokens that add up as independent ones make
 E (16 + 2 sqrt(n)) N_t of the row, and scale times that of an output, as |q| <= 1."""
+import random
 import sys
 
 import pytest
@@ -256,3 +257,34 @@ def test_one_write_ages(pk, rate, d):
         b = torch.where((torch.arange(n, device="cuda") == at)[:, None], 3.0, -200.0).expand_as(beta)
         check(pk, q, k, v, gate, b, state.clone())
         check(pk, *(t[:, :at + 72].contiguous() for t in (q, k, v, gate, b)), state.clone())
+
+
+@pytest.mark.parametrize("seed", range(32))
+def test_mixes(pk, seed):
+    """Spans of values over tokens and channels, decays, gates, keys and states, mixed at random."""
+    rng = random.Random(seed)
+    d, n, hk, b = rng.choice([64, 128, 256]), rng.choice([72, 100, 128, 193, 256, 330]), rng.choice([1, 2]), rng.choice([1, 2])
+    h = hk * rng.choice([1, 2, 3])
+    q, k, v, _, beta, state = inputs(seed, b, n, hk, h, d)
+    rand = lambda *s: torch.rand(s, device="cuda", generator=g)  # noqa: E731
+    g = torch.Generator(device="cuda").manual_seed(100 + seed)
+    if rng.random() < 0.4:
+        k = k[:, :1] + rng.choice([0, 0.01, 0.3]) * k
+    v = v * torch.exp2(-rng.choice([0, 5, 20, 40, 60]) * rand(b, n, 1, 1) - rng.choice([0, 10, 40]) * rand(1, 1, h, d))
+    v = v * 2.0 ** rng.choice([0, -40, 40, 60])
+    if rng.random() < 0.3:
+        v = v * (rand(b, n, h, 1) < 0.1)
+    gate = -rng.choice([1e-5, 1e-3, 0.1, 1, 5, 20]) * rand(b, n, h) ** rng.choice([1, 4, 16])
+    if rng.random() < 0.3:
+        gate = torch.where(rand(b, n, h) < 0.03, -rng.choice([20.0, 60.0, 90.0, 300.0, 9000.0]), gate)
+    beta = rng.choice([1, 5, 40]) * beta + rng.choice([-5, 0, 5])
+    state = state * rng.choice([0, 1, 1e-8, 1e6])
+    eps = rng.choice([1e-6, 1e-12, 1.0])
+    say(f"mix {seed}: b={b} n={n} hk={hk} h={h} d={d} eps={eps}")
+    want, want_state, size, norm = formula(q, k, v, gate, beta, state, 0.1, eps)
+    # what decays by more than e^-87 within a chunk is held to 2^-126 of the largest so far
+    least = TINY * (1 + float(size.max()) + float(state.norm(dim=-1).max()))
+    out = pk.gated_delta_rule(q, k, v, gate, beta, state, 0.1, eps)
+    lim = E * (16 + 2 * n ** 0.5)
+    assert bool(((out.double() - want).abs() <= 0.1 * (lim * size + least)).all())
+    assert bool(((state.double() - want_state).norm(dim=-1) <= lim * norm + least * d ** 0.5).all())

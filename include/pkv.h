@@ -430,6 +430,92 @@ int pkv_seq_append_decode_batched(pkv_seq *const *seqs, int n, const float *k, c
 /* get_kv (qn:520-575): dequantized [1, n_kv_heads, len, head_dim] f32. */
 int pkv_seq_get_kv(const pkv_seq *s, float *k_out, float *v_out);
 
+/* ---- Pages named by tables on the device: a serving step without the host ----
+ * The pages of F16 or BF16 caches ([n_pages, page_tokens, n_kv_heads, head_dim] each of K and
+ * V: a pool's planes or the caller's memory) and the tables that name them are device memory,
+ * and so are all lengths, so that the launches of a step do not depend on them and a captured
+ * step serves every later one. int is 32 bits. Every buffer that a call writes must overlap no
+ * other one of the call. */
+/* A pool's planes, and pages that the device may hand out: take moves n of the pool's free
+ * pages (PKV_ERR_OVERFLOW, with none taken, when it lacks them) out of its sequences' reach,
+ * give brings such pages back (PKV_ERR_ARG, with none given, for a page that is not taken). */
+int pkv_pool_storage(const pkv_pool *p, void **k_pages, void **v_pages, size_t *page_bytes,
+                     int *page_tokens, int *n_pages);
+int pkv_pool_take_pages(pkv_pool *p, int n, int *pages_host);
+int pkv_pool_give_pages(pkv_pool *p, int n, const int *pages_host);
+/* The pages of a sequence, in token order, into host memory of `capacity` entries
+ * (PKV_ERR_ARG if they are more). */
+int pkv_seq_page_ids(const pkv_seq *s, int *pages_host, int capacity);
+
+/* Request lengths to pages. Request b keeps lens[b] tokens of its cache and gets add[b] new
+ * ones; with total = lens[b] + add[b] it needs ceil(total / page_tokens) pages and holds
+ * held[b], tables[b][0 .. held[b]). First the pages that requests no longer need go back onto
+ * the free stack (free_pages [capacity], its height in free_count[0]), request by request in
+ * the table's order; then requests that need more take them from the stack's top, request by
+ * request. tables [n, max_pages], held [n], free_pages and free_count are updated (the table's
+ * entries behind held[b] mean nothing). starts [n + 1]: the new tokens' first rows, running
+ * sums of add; totals [n]; and for the step's row t of request b, its i-th new token: positions
+ * [max_tokens] lens[b] + i, slots [max_tokens] (64 bits) the page times page_tokens plus its
+ * place there; behind the last row -1 and position 0. status [1]: PKV_OK, or with nothing
+ * moved, all slots -1, starts 0 and totals = lens, PKV_ERR_OVERFLOW (the stack lacks pages) or
+ * PKV_ERR_ARG (a negative length, a table too short, more than max_tokens new tokens, a stack
+ * that would not fit). page_tokens: a power of two in [32, 2^20]; max_tokens below 2^31. */
+int pkv_pages_map(const int *lens, const int *add, int n, int *tables, int max_pages, int *held,
+                  int *free_pages, int *free_count, int capacity, int page_tokens,
+                  int64_t *slots, int *positions, int64_t max_tokens, int *starts, int *totals,
+                  int *status, pkv_stream stream);
+
+/* append_quantized (qn:431-509) of n tokens into their slots: k, v [n, n_kv_heads, head_dim]
+ * f32, tokens `stride` elements apart (slices of a projection are taken as they are), rounded
+ * to quant (PKV_QUANT_F16 or PKV_QUANT_BF16, else PKV_ERR_UNSUPPORTED) as the cache rounds
+ * them. A negative slot: its token is left out; a slot of n_slots (n_pages * page_tokens) or
+ * more too, and pkv_device_status reports it. Two tokens of one slot leave a row whose parts
+ * may be either's. n * n_kv_heads * head_dim below 2^32 (else PKV_ERR_UNSUPPORTED). */
+int pkv_pages_append(int quant, const float *k, const float *v, int64_t k_stride, int64_t v_stride,
+                     const int64_t *slots, int64_t n, void *k_pages, void *v_pages,
+                     int64_t n_slots, int n_kv_heads, int head_dim, pkv_stream stream);
+
+/* The attention of pkv_attend over pages: request b's queries are the rows [starts[b],
+ * starts[b + 1]) of q (starts NULL: row b alone), the last tokens of its lens[b] keys (new ones
+ * included), the pages of tables[b]. A query at position p sees key j iff j <= p and (window
+ * == 0, j > p - window, or j < sinks); scores are scaled, clamped to [-100, 100] and
+ * soft-maxed; a query that sees no key gives zeros. q: [tokens, num_heads, head_dim] f32, tokens
+ * q_stride_t and heads q_stride_h elements apart; out: [tokens, num_heads, head_dim] f32, whose
+ * rows of no request are left as they were. quant PKV_QUANT_F16 or PKV_QUANT_BF16, head_dim 64,
+ * 128 or 256 (else PKV_ERR_UNSUPPORTED); q and out 16-byte aligned, q's strides multiples of 4.
+ * lens and starts are taken into what tables and tokens hold; pages that no key seen lies in are
+ * not read; a key in a page outside [0, n_pages) is not seen, and pkv_device_status reports it.
+ * workspace: at least pkv_pages_attend_workspace() bytes of device memory, 256-byte aligned,
+ * which the call writes: calls that overlap in time, and graphs that do, need one each. */
+size_t pkv_pages_attend_workspace(int n, int64_t tokens, int num_heads, int num_kv_heads,
+                                  int head_dim);
+int pkv_pages_attend(int quant, const float *q, int64_t q_stride_t, int64_t q_stride_h,
+                     const void *k_pages, const void *v_pages, int n_pages, int page_tokens,
+                     const int *tables, int max_pages, const int *lens, const int *starts, int n,
+                     int64_t tokens, int num_heads, int num_kv_heads, int head_dim, float scale,
+                     int window, int sinks, float *out, void *workspace, size_t workspace_bytes,
+                     pkv_stream stream);
+
+/* Drafted tokens against the target's probabilities (the acceptance in front of a rewind,
+ * qn:2755-2762, with the drafts' probabilities of ops.rs:470-491). target: f32 [n, k + 1, vocab],
+ * row i what the target gives behind i accepted drafts, rows target_stride elements apart;
+ * drafts: [n, k], n_drafts: [n] of them valid (NULL: all; taken into [0, k]); draft: f32 [n, k,
+ * vocab], what they were drawn from, rows draft_stride apart (NULL: they were certain); u: f32
+ * [n, k + 1] in [0, 1). Draft i is accepted iff all before it are and u[i] * draft[i][x] <
+ * target[i][x] (a token outside the vocabulary never). The token behind the accepted ones is
+ * drawn with u[k] from max(target - draft, 0) of the first rejected draft's rows (from target
+ * itself where that leaves nothing), or from the target's row behind the last draft: the lowest
+ * one whose running sum exceeds u[k] times the whole sum, in 64 bits; -1 for a row without
+ * weight. tokens: [n, k + 1], the accepted drafts, that token, then -1; accepted: [n]. k at most
+ * 63, n at most 65535 (else PKV_ERR_UNSUPPORTED). workspace: at least
+ * pkv_verify_drafts_workspace(n) bytes of device memory, 8-byte aligned, which the call writes:
+ * calls that overlap in time, and graphs that do, need one each. */
+size_t pkv_verify_drafts_workspace(int n);
+int pkv_verify_drafts(const float *target, int64_t target_stride, const float *draft,
+                      int64_t draft_stride, const int *drafts, const int *n_drafts, const float *u,
+                      int n, int k, int vocab, int *tokens, int *accepted, void *workspace,
+                      size_t workspace_bytes, pkv_stream stream);
+
 /* ---- utilities ---- */
 /* Seeded synthetic data: dst[i] = normal(seed, stream_id, i) * scale, bit-identical
  * to the CPU oracle's generator (Philox4x32-10, Irwin-Hall of eight 22-bit draws). */

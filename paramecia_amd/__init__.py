@@ -13,3 +13,4 @@ from .kv_cache import (  # noqa: F401
     gated_o_proj_lora, rms_norm, scale_channels,
     WTYPE_Q4K, WTYPE_Q5K, WTYPE_Q6K, WTYPE_Q8_0,
 )
+from .pages import PageMap, append_pages, attend_pages, map_pages, verify_drafts  # noqa: F401

@@ -37,7 +37,9 @@ SYMBOLS = (
     "pkv_seq_decode_batched", "pkv_seq_get_kv", "pkv_seq_append_batched",
     "pkv_seq_append_decode_batched", "pkv_causal_conv", "pkv_deltanet_prompt_workspace",
     "pkv_deltanet_prompt", "pkv_rms_norm", "pkv_gated_oproj_lora_workspace",
-    "pkv_gated_oproj_lora",
+    "pkv_gated_oproj_lora", "pkv_pool_storage", "pkv_pool_take_pages", "pkv_pool_give_pages",
+    "pkv_seq_page_ids", "pkv_pages_map", "pkv_pages_append", "pkv_pages_attend_workspace",
+    "pkv_pages_attend", "pkv_verify_drafts_workspace", "pkv_verify_drafts",
 )
 
 
@@ -167,6 +169,17 @@ def _declare(L: ctypes.CDLL) -> None:
         "pkv_seq_get_kv": ([vp, vp, vp], c_int),
         "pkv_seq_append_batched": ([P(vp), c_int, vp, vp], c_int),
         "pkv_seq_append_decode_batched": ([P(vp), c_int, vp, vp, vp, c_int, fl, vp], c_int),
+        "pkv_pool_storage": ([vp, P(vp), P(vp), P(c_sz), P(c_int), P(c_int)], c_int),
+        "pkv_pool_take_pages": ([vp, c_int, P(c_int)], c_int),
+        "pkv_pool_give_pages": ([vp, c_int, P(c_int)], c_int),
+        "pkv_seq_page_ids": ([vp, P(c_int), c_int], c_int),
+        "pkv_pages_map": ([vp, vp, c_int, vp, c_int] + [vp] * 3 + [c_int, c_int, vp, vp, c_i64] + [vp] * 4, c_int),
+        "pkv_pages_append": ([c_int, vp, vp, c_i64, c_i64, vp, c_i64, vp, vp, c_i64, c_int, c_int, vp], c_int),
+        "pkv_pages_attend_workspace": ([c_int, c_i64] + [c_int] * 3, c_sz),
+        "pkv_pages_attend": ([c_int, vp, c_i64, c_i64, vp, vp, c_int, c_int, vp, c_int, vp, vp, c_int, c_i64] +
+                             [c_int] * 3 + [fl, c_int, c_int, vp, vp, c_sz, vp], c_int),
+        "pkv_verify_drafts_workspace": ([c_int], c_sz),
+        "pkv_verify_drafts": ([vp, c_i64, vp, c_i64] + [vp] * 3 + [c_int] * 3 + [vp] * 3 + [c_sz, vp], c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

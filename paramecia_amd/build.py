@@ -45,8 +45,12 @@ SOURCES = {
     "pkv_oproj.hip": [],
     "pkv_oproj_mfma.hip": [],
     "pkv_prep.hip": ["-ffp-contract=off"],
+    "pkv_pages.hip": [],
+    "pkv_pages_attend.hip": [],
+    "pkv_verify.hip": ["-ffp-contract=off"],
     "pkv_api.cpp": ["-x", "hip"],
     "pkv_paged.cpp": ["-x", "hip"],
+    "pkv_pages_api.cpp": ["-x", "hip"],
 }
 
 

@@ -212,6 +212,10 @@ int pkv_device_status(void) {
     what = "a fused decode step's quantizer barrier timed out: its appended row and attention output are not valid";
   if (v & kStatusAdapterId)
     what += std::string(what.empty() ? "" : "; ") + "a projection was given an adapter id past its adapters: that row took none";
+  if (v & kStatusSlot)
+    what += std::string(what.empty() ? "" : "; ") + "an append was given a slot past its pages: that token was left out";
+  if (v & kStatusPage)
+    what += std::string(what.empty() ? "" : "; ") + "an attention's table named a page that is none: its keys were not seen";
   return set_error(PKV_ERR_HIP, what.empty() ? "device status " + std::to_string(v) : what);
 }
 const char *pkv_version(void) { return "paramecia_amd pkv 0.1 (gfx950)"; }

@@ -44,6 +44,8 @@ inline size_t row_bytes(int quant, int head_dim) {
 // clears it.
 constexpr unsigned kStatusBarrierTimeout = 1u;  // the fused quantizer's barrier of waves 0-3
 constexpr unsigned kStatusAdapterId = 2u;       // an adapter id past the call's adapters
+constexpr unsigned kStatusSlot = 4u;            // a row's slot past the pages
+constexpr unsigned kStatusPage = 8u;            // a block table's page that is none
 int device_status_word(unsigned **out);
 
 // PKV_ERR_UNSUPPORTED when `s` is capturing a HIP graph: for calls that allocate device
@@ -304,6 +306,35 @@ size_t deltanet_prompt_workspace(int batch, int64_t n, int k_heads, int heads, i
 int launch_rms_norm(const float *x, int64_t x_stride, float *residual, const float *alpha,
                     const float *gate, float eps, float *out, uint8_t *q8, int64_t rows, int dim,
                     hipStream_t s);
+// ---- launchers (pkv_pages.hip, pkv_pages_attend.hip, pkv_verify.hip): a step over pages that
+// tables on the device name. All pointers are device memory.
+int launch_pages_map(const int *lens, const int *add, int n, int *tables, int max_pages, int *held,
+                     int *free_pages, int *free_count, int capacity, int page_tokens,
+                     int64_t *slots, int *positions, int64_t max_tokens, int *starts, int *totals,
+                     int *status, hipStream_t s);
+int launch_pages_append(int quant, const float *k, const float *v, int64_t k_stride,
+                        int64_t v_stride, const int64_t *slots, int64_t n, void *k_pages,
+                        void *v_pages, int64_t n_slots, int width, hipStream_t s);
+struct PagesAttend {
+  int quant;
+  const float *q;
+  int64_t q_t, q_h;  // elements between tokens and between heads
+  const void *k_pages, *v_pages;
+  int n_pages, page_tokens, max_pages;
+  const int *tables, *lens, *starts;
+  int n;
+  int64_t tokens;
+  int heads, kv_heads, head_dim, window, sinks;
+  float scale;
+  float *out;
+};
+size_t pages_attend_workspace(int n, int64_t tokens, int heads, int kv_heads, int head_dim);
+int launch_pages_attend(const PagesAttend &p, void *ws, hipStream_t s);
+size_t verify_drafts_workspace(int n);
+int launch_verify_drafts(const float *target, int64_t target_row, const float *draft,
+                         int64_t draft_row, const int *drafts, const int *counts, const float *u,
+                         int n, int k, int vocab, int *tokens, int *accepted, void *ws,
+                         hipStream_t s);
 int launch_deltanet_step(const float *q, const float *k, const float *v, const float *gate,
                          const float *beta, float *state, float *gate_offset, float *out,
                          int batch, int heads, int head_dim, float scale, float eps,

@@ -408,6 +408,55 @@ int pkv_pool_set_stream(pkv_pool *p, pkv_stream stream) {
   return PKV_OK;
 }
 
+int pkv_pool_storage(const pkv_pool *p, void **k_pages, void **v_pages, size_t *page_bytes,
+                     int *page_tokens, int *n_pages) {
+  if (!p) return set_error(PKV_ERR_ARG, "null handle");
+  if (k_pages) *k_pages = p->k;
+  if (v_pages) *v_pages = p->v;
+  if (page_bytes) *page_bytes = p->page_bytes;
+  if (page_tokens) *page_tokens = p->page_tokens;
+  if (n_pages) *n_pages = p->n_pages;
+  return PKV_OK;
+}
+
+// A page that the device hands out: no sequence's, and not free.
+static constexpr int32_t kTaken = -1;
+
+int pkv_pool_take_pages(pkv_pool *p, int n, int *pages) {
+  if (!p || n < 0 || (n && !pages)) return set_error(PKV_ERR_ARG, "null argument or n < 0");
+  if ((size_t)n > p->free_list.size())
+    return set_error(PKV_ERR_OVERFLOW, "Paged KV pool overflow: " + std::to_string(n) +
+                                           " more pages needed, " +
+                                           std::to_string(p->free_list.size()) + " free");
+  for (int i = 0; i < n; ++i) {
+    pages[i] = take_page(p);
+    p->refs[(size_t)pages[i]] = kTaken;
+  }
+  return PKV_OK;
+}
+
+int pkv_pool_give_pages(pkv_pool *p, int n, const int *pages) {
+  if (!p || n < 0 || (n && !pages)) return set_error(PKV_ERR_ARG, "null argument or n < 0");
+  for (int i = 0; i < n; ++i) {
+    // (a page named twice is not taken any more the second time)
+    if (pages[i] < 0 || pages[i] >= p->n_pages || p->refs[(size_t)pages[i]] != kTaken) {
+      for (int j = 0; j < i; ++j) p->refs[(size_t)pages[j]] = kTaken;
+      return set_error(PKV_ERR_ARG, "page " + std::to_string(pages[i]) + " is not taken");
+    }
+    p->refs[(size_t)pages[i]] = 0;
+  }
+  for (int i = 0; i < n; ++i) p->free_list.push_back(pages[i]);
+  return PKV_OK;
+}
+
+int pkv_seq_page_ids(const pkv_seq *s, int *pages, int capacity) {
+  if (!s || capacity < 0 || (!s->pages.empty() && !pages)) return set_error(PKV_ERR_ARG, "null argument");
+  if ((size_t)capacity < s->pages.size())
+    return set_error(PKV_ERR_ARG, "the sequence has " + std::to_string(s->pages.size()) + " pages");
+  for (size_t i = 0; i < s->pages.size(); ++i) pages[i] = s->pages[i];
+  return PKV_OK;
+}
+
 int pkv_seq_create(pkv_pool *p, pkv_seq **out) {
   if (!p || !out) return set_error(PKV_ERR_ARG, "null argument");
   *out = nullptr;

@@ -1,0 +1,937 @@
+// Attention over pages that block tables on the device name: the new tokens of many requests
+// (one each, a few drafted ones, prompts) over their F16 or BF16 rows, with a window and some
+// first tokens that stay visible, gfx950.
+//
+// Role: the SDPA of the reference's float cache (paramecia-model/src/qwen3_next.rs:2492-2605)
+// for requests of any lengths in one step. Query i of a request of `len` keys and `new` queries
+// sits at position p = len - new + i and sees key j iff j <= p and (no window, j > p - window,
+// or j < sinks); scores are scaled, clamped to +-100 and soft-maxed; a query that sees nothing
+// gives zeros. Lengths, tables and row counts are read on the device: the launches of a step do
+// not depend on them, so a captured step serves every later one.
+//
+// Work: a tile is 16 kW rows of one request (row = token x query heads of a KV head); its keys
+// are blocks of 32 (one page each), the sinks' blocks first, then the window's. The blocks of all
+// tiles and KV heads lie in one line, which is cut into equal shares, one a workgroup, whatever
+// the lengths are. A share that holds a whole tile writes its rows of out; the parts of a tile
+// that is cut meet in the join, a launch of their own.
+#include "pkv_half_common.hpp"
+#include "pkv_internal.hpp"
+
+namespace pkv {
+namespace {
+
+struct AttendArgs {
+  const float *q;  // token t, head h at t * q_t + h * q_h
+  int64_t q_t, q_h;
+  const uint8_t *k, *v;  // page p at p * page_bytes
+  int64_t page_bytes;
+  const int *tables, *lens, *starts;
+  float *out;
+  int2 *tiles;      // [tile]: request, tile of it
+  int64_t *before;  // [tile + 1]: blocks of the tiles before it
+  int *count;       // tiles
+  float *part;      // [2 workgroup + (not its first piece)][row][head_dim]
+  float2 *ml;       // [..][row]: running max (log2 units), sum
+  unsigned *status;
+  int n, tokens, heads, kv_heads, group, page_lg, n_pages, max_pages, window, sinks, max_tiles, shares;
+  float sl2;  // scale * log2(e)
+};
+
+struct Tile {
+  int b, row0, rows, tok0;  // request, first row, rows, its first token in the step
+  int p0, p1;               // positions of its first and last row's tokens
+  int first;                // position of row 0's token of the request (may be below 0)
+  int sink_blocks, lo, blocks;
+  __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : i - sink_blocks + lo; }
+};
+
+// Request b's queries [q0, q0 + new) and keys, as far as the step and the tables hold them.
+__device__ __forceinline__ void request_of(const AttendArgs &a, int b, int &q0, int &fresh, int &len) {
+  if (a.starts) {
+    int s0 = a.starts[b], s1 = a.starts[b + 1];
+    s0 = s0 < 0 ? 0 : s0 > a.tokens ? a.tokens : s0;
+    s1 = s1 < s0 ? s0 : s1 > a.tokens ? a.tokens : s1;
+    q0 = s0;
+    fresh = s1 - s0;
+  } else {
+    q0 = b;
+    fresh = 1;
+  }
+  const int64_t most = (int64_t)a.max_pages << a.page_lg;
+  len = a.lens[b];
+  len = len < 0 ? 0 : len > most ? (int)most : len;
+}
+
+__device__ __forceinline__ Tile tile_of(const AttendArgs &a, int b, int i, int rows_per_tile) {
+  Tile t;
+  int fresh, len;
+  request_of(a, b, t.tok0, fresh, len);
+  const int all = fresh * a.group;
+  t.b = b;
+  t.row0 = i * rows_per_tile;
+  t.rows = all - t.row0 < rows_per_tile ? all - t.row0 : rows_per_tile;
+  t.first = len - fresh;
+  t.sink_blocks = t.lo = t.blocks = 0;
+  t.p0 = t.p1 = -1;
+  if (t.rows <= 0) return t;
+  t.p0 = t.first + t.row0 / a.group;
+  t.p1 = t.first + (t.row0 + t.rows - 1) / a.group;
+  if (t.p1 < 0) return t;
+  const int from = t.p0 < 0 ? 0 : t.p0;
+  if (a.window > 0 && from >= a.window) {
+    t.lo = (from - a.window + 1) >> 5;
+    const int s = (int)(((int64_t)a.sinks + 31) >> 5);
+    t.sink_blocks = s < t.lo ? s : t.lo;
+  }
+  t.blocks = t.sink_blocks + (t.p1 >> 5) - t.lo + 1;
+  return t;
+}
+
+// Whether the query at position p sees key j.
+__device__ __forceinline__ bool sees(const AttendArgs &a, int p, int j) {
+  return j <= p && (a.window <= 0 || j > p - a.window || j < a.sinks);
+}
+
+// One workgroup: the tiles of all requests and the running count of their blocks.
+constexpr int kPlanThreads = 1024;
+__device__ __forceinline__ int64_t plan_scan(int64_t x, int64_t *part, int64_t &sum) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t y = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t z = __shfl_up(y, o);
+    if (lane >= o) y += z;
+  }
+  __syncthreads();
+  if (lane == 63) part[wave] = y;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    before += w < wave ? part[w] : 0;
+    all += part[w];
+  }
+  sum = all;
+  return before + y - x;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int rows_per_tile) {
+  __shared__ int64_t part[kPlanThreads / 64];
+  const int tid = threadIdx.x;
+  int64_t tiles = 0;
+  for (int b0 = 0; b0 < a.n; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int q0, fresh = 0, len;
+    if (b < a.n) request_of(a, b, q0, fresh, len);
+    const int mine = (int)(((int64_t)fresh * a.group + rows_per_tile - 1) / rows_per_tile);
+    int64_t sum;
+    const int64_t at = tiles + plan_scan(mine, part, sum);
+    for (int i = 0; i < mine && at + i < a.max_tiles; ++i) a.tiles[at + i] = int2{b, i};
+    tiles += sum;
+  }
+  // (starts that run backwards could name more tiles than the step has rows for)
+  const int count = tiles < a.max_tiles ? (int)tiles : a.max_tiles;
+  __syncthreads();
+  int64_t blocks = 0;
+  for (int t0 = 0; t0 < count; t0 += kPlanThreads) {
+    const int t = t0 + tid;
+    int mine = 0;
+    if (t < count) {
+      const int2 x = a.tiles[t];
+      mine = tile_of(a, x.x, x.y, rows_per_tile).blocks;
+    }
+    int64_t sum;
+    const int64_t at = blocks + plan_scan(mine, part, sum);
+    if (t < count) a.before[t] = at;
+    blocks += sum;
+  }
+  if (tid == 0) {
+    a.before[count] = blocks;
+    *a.count = count;
+  }
+}
+
+// The line of all blocks: KV head after KV head, tile after tile.
+struct Line {
+  int tiles, shares;
+  int64_t per_head, all;
+  __device__ __forceinline__ int64_t start(int w) const { return all * w / shares; }
+};
+__device__ __forceinline__ Line line_of(const AttendArgs &a) {
+  Line l;
+  l.tiles = *a.count;
+  l.per_head = a.before[l.tiles];
+  l.all = l.per_head * a.kv_heads;
+  l.shares = l.all < a.shares ? (int)l.all : a.shares;
+  return l;
+}
+// The tile that holds block u of a head (u below the head's blocks).
+__device__ __forceinline__ int tile_at(const AttendArgs &a, int tiles, int64_t u) {
+  int lo = 0, hi = tiles;  // before[lo] <= u < before[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.before[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// A block's rows of K and V of one KV head as buffers: `valid` rows from the block's first one,
+// none where its page is none of the pool's.
+struct Block {
+  __amdgpu_buffer_rsrc_t k, v;
+  int valid;
+};
+__device__ __forceinline__ Block block_of(const AttendArgs &a, const Tile &t, int h, int jb, int head_bytes) {
+  Block r;
+  const int j0 = jb << 5;
+  const uint32_t row = (uint32_t)a.kv_heads * (uint32_t)head_bytes;
+  const int page = __builtin_amdgcn_readfirstlane(a.tables[(int64_t)t.b * a.max_pages + (j0 >> a.page_lg)]);
+  const bool ok = page >= 0 && page < a.n_pages;
+  const int left = t.p1 + 1 - j0;
+  r.valid = !ok ? 0 : left < kBlk ? left : kBlk;
+  const int64_t at = (ok ? (int64_t)page * a.page_bytes : 0) +
+                     (int64_t)(j0 & ((1 << a.page_lg) - 1)) * row + (int64_t)h * head_bytes;
+  const uint32_t span = r.valid > 0 ? (uint32_t)(r.valid - 1) * row + (uint32_t)head_bytes : 0u;
+  r.k = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.k) + at, 0, span, 0x00020000);
+  r.v = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.v) + at, 0, span, 0x00020000);
+  if (!ok && threadIdx.x == 0) atomicOr(a.status, kStatusPage);
+  return r;
+}
+
+// Row `row` of a tile over its blocks [i0, i1) in plain f32 products of the keys that it sees
+// alone: for pieces that met infinities or NaN, where split operands and masked keys' zero
+// weights would make more NaN than the formula does. The lane owns kE elements; m in log2 units.
+template <bool kBf, int kE>
+__device__ __forceinline__ void plain_row(const AttendArgs &a, const Tile &t, int h, int row, int i0, int i1,
+                                          int lane, float &m, float &l, float (&acc)[kE]) {
+  constexpr int kD = 64 * kE;
+  const int r = t.row0 + row, tok = r / a.group, p = t.first + tok;
+  const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + lane * kE;
+  float x[kE];
+  m = -INFINITY;
+  l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    x[e] = q[e] * a.sl2;
+    acc[e] = 0.0f;
+  }
+  const int64_t stride = (int64_t)a.kv_heads * kD;
+  for (int i = i0; i < i1; ++i) {
+    const int j0 = t.block(i) << 5;
+    const int page = a.tables[(int64_t)t.b * a.max_pages + (j0 >> a.page_lg)];
+    if (page < 0 || page >= a.n_pages) continue;
+    const int64_t at = (int64_t)page * a.page_bytes + 2 * ((int64_t)(j0 & ((1 << a.page_lg) - 1)) * stride + (int64_t)h * kD + lane * kE);
+    const uint16_t *k = reinterpret_cast<const uint16_t *>(a.k + at), *v = reinterpret_cast<const uint16_t *>(a.v + at);
+    for (int j = 0; j < kBlk; ++j) {
+      if (!sees(a, p, j0 + j)) continue;
+      float dot = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) dot += x[e] * half_value(k[j * stride + e], kBf);
+      float s = wave_sum(dot);
+      s = s > kClampL2 ? kClampL2 : s < -kClampL2 ? -kClampL2 : s;  // (NaN stays)
+      const float mn = fmaxf(m, s);
+      const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(s - mn);
+      l = l * c + w;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[e] = acc[e] * c + w * half_value(v[j * stride + e], kBf);
+      m = mn;
+    }
+  }
+}
+
+// Where a piece's rows go: out if it is the whole tile, else the share's slot.
+struct Sink {
+  bool whole;
+  int64_t slot;
+};
+__device__ __forceinline__ float *row_out(const AttendArgs &a, const Tile &t, int h, int row, int kD) {
+  const int r = t.row0 + row;
+  return a.out + ((int64_t)(t.tok0 + r / a.group) * a.heads + h * a.group + r % a.group) * kD;
+}
+template <bool kBf, int kE>
+__device__ __forceinline__ void plain_store(const AttendArgs &a, const Tile &t, int h, int row, int i0, int i1, int lane,
+                                            const Sink &to, int rows_per_tile) {
+  constexpr int kD = 64 * kE;
+  float m, l, acc[kE];
+  plain_row<kBf, kE>(a, t, h, row, i0, i1, lane, m, l, acc);
+  const int64_t at = to.slot * rows_per_tile + row;
+  float *o = to.whole ? row_out(a, t, h, row, kD) : a.part + at * kD;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) o[lane * kE + e] = !to.whole ? acc[e] : m == -INFINITY ? 0.0f : acc[e] / l;
+  if (!to.whole && lane == 0) a.ml[at] = float2{m, l};
+}
+
+// The rows of tiles without a key that they see.
+__device__ __forceinline__ void zero_empty(const AttendArgs &a, const Line &l, int rows_per_tile, int kD, int threads) {
+  for (int x = blockIdx.x; x < l.tiles; x += gridDim.x) {
+    if (a.before[x + 1] != a.before[x]) continue;
+    const int2 at = a.tiles[x];
+    const Tile t = tile_of(a, at.x, at.y, rows_per_tile);
+    for (int h = 0; h < a.kv_heads; ++h)
+      for (int i = threadIdx.x; i < t.rows * kD; i += threads) row_out(a, t, h, i / kD, kD)[i % kD] = 0.0f;
+  }
+}
+
+// Queries as MFMA operands: q times scale and log2(e), as sums of 16-bit parts (F16 two, with
+// a power of two per row that keeps both in fp16's range; BF16 three).
+template <bool kBf>
+constexpr int kParts = kBf ? 3 : 2;
+template <bool kBf>
+__device__ __forceinline__ void parts_of(float x0, float x1, uint32_t (&w)[kParts<kBf>]) {
+  if constexpr (kBf) {
+    w[0] = bf2(x0, x1);
+    const float r0 = x0 - bf_lo(w[0]), r1 = x1 - bf_hi(w[0]);
+    w[1] = bf2(r0, r1);
+    w[2] = bf2(r0 - bf_lo(w[1]), r1 - bf_hi(w[1]));
+  } else {
+    const h2 h = {(_Float16)x0, (_Float16)x1};
+    w[0] = as_u(h);
+    w[1] = fp16_sub2(x0, x1, w[0]);
+  }
+}
+template <int kSteps>
+__device__ __forceinline__ float top_of(const float4 (&x)[kSteps][2]) {
+  float m = 0.0f;
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+      m = fmaxf(m, fmaxf(fmaxf(fabsf(x[s][y].x), fabsf(x[s][y].y)), fmaxf(fabsf(x[s][y].z), fabsf(x[s][y].w))));
+  return xmax32(xmax16(m));
+}
+template <bool kBf, int kSteps>
+__device__ __forceinline__ void split_queries(float4 (&x)[kSteps][2], u4 (&qb)[kSteps][kParts<kBf>], float &back) {
+  float f = 1.0f;
+  back = 1.0f;
+  if constexpr (!kBf) {  // a row's elements to [2^14, 2^15)
+    int e = (int)(f2u(top_of(x)) >> 23) - 127;
+    e = e < -100 ? -100 : e > 100 ? 100 : e;
+    f = __builtin_ldexpf(1.0f, 14 - e);
+    back = __builtin_ldexpf(1.0f, e - 14);
+  }
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    uint32_t w[4][kParts<kBf>];
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      parts_of<kBf>(x[s][y].x * f, x[s][y].y * f, w[2 * y]);
+      parts_of<kBf>(x[s][y].z * f, x[s][y].w * f, w[2 * y + 1]);
+    }
+#pragma unroll
+    for (int p = 0; p < kParts<kBf>; ++p) qb[s][p] = u4{w[0][p], w[1][p], w[2][p], w[3][p]};
+  }
+}
+
+// A row's softmax over a block, the lane's eight keys 8 g .. 8 g + 7 of row n: the weights as
+// MFMA operands (a power of two times them, F16), the running max and sum, and the factor that
+// what was summed before takes (1 if it stays).
+template <bool kBf>
+struct Softmax {
+  static constexpr float kUp = kBf ? 1.0f : kPUp, kLazy = kBf ? kBf16Lazy : kF16Lazy;
+  float m = -INFINITY, l = 0.0f;
+  bool bad = false;
+  // s: scores (log2 units); ok(i): key 8 g + i is seen. True if the sums before take `alpha`.
+  template <typename Ok>
+  __device__ __forceinline__ bool step(float (&s)[8], bool all, Ok ok, u4 (&pb)[kParts<kBf>], float &alpha) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool seen = all || ok(i);
+      bad |= seen && !(fabsf(s[i]) < INFINITY);
+      s[i] = seen ? __builtin_amdgcn_fmed3f(s[i], -kClampL2, kClampL2) : -INFINITY;
+    }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
+    top = xmax32(xmax16(top));
+    const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
+    const bool any = __any(raise);
+    alpha = 1.0f;
+    if (any) {
+      const float mn = raise ? top : m;
+      alpha = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      m = mn;
+      l *= alpha;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(s[i] - base) * kUp;
+      l += p[i];
+    }
+    uint32_t w[4][kParts<kBf>];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) parts_of<kBf>(p[2 * i], p[2 * i + 1], w[i]);
+#pragma unroll
+    for (int x = 0; x < kParts<kBf>; ++x) pb[x] = u4{w[0][x], w[1][x], w[2][x], w[3][x]};
+    return any;
+  }
+  __device__ __forceinline__ float sum() const {  // of the row's four lanes
+    float x = l;
+    x += __shfl_xor(x, 16);
+    x += __shfl_xor(x, 32);
+    return x;
+  }
+};
+
+// ---- up to 16 rows a tile. A workgroup of kD / 64 waves: wave w takes elements 64 w .. of all
+// 32 keys of a block for the scores, and columns 64 w .. of V. Rows go from memory straight into
+// registers as MFMA operands, a block ahead; the waves' partial scores meet in LDS, one barrier a
+// block, and every wave runs the same softmax.
+//   scores (transposed, A = K): lane (r, g) holds 8 elements of key 8 (r / 4) + 4 t + r % 4 for
+//   tile t, so that the result (row n, keys 8 g + 4 t + i) is the weights' operand as it is;
+//   out (transposed, A = V): lane (m, g) holds columns 4 m + j (tile j) of keys 8 g .. + 7, pairs
+//   of keys joined by v_perm; the result is columns 16 g + 4 i + j of row n.
+constexpr int kScoreRow = 36;  // floats, 32 keys and a pad that spreads rows over banks
+
+template <bool kBf, int kD>
+__global__ __launch_bounds__(kD) void few_kernel(AttendArgs a) {
+  constexpr int kW = kD / 64;
+  __shared__ __attribute__((aligned(16))) float sc[2][kW][16][kScoreRow];
+  __shared__ uint32_t s_bad;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Line line = line_of(a);
+  zero_empty(a, line, 16, kD, kD);
+  const int share = blockIdx.x;
+  if (share >= line.shares) return;
+  int64_t u = line.start(share);
+  const int64_t u0 = u, end = line.start(share + 1);
+  if (tid == 0) s_bad = 0u;
+  int turn = 0;
+  const uint32_t stride = (uint32_t)a.kv_heads * 2u * kD;
+  while (u < end) {
+    const int h = (int)(u / line.per_head);
+    const int64_t in = u - h * line.per_head;
+    const int x = tile_at(a, line.tiles, in);
+    const int2 where = a.tiles[x];
+    const Tile t = tile_of(a, where.x, where.y, 16);
+    const int i0 = (int)(in - a.before[x]);
+    const int64_t left = end - u;
+    const int i1 = left < t.blocks - i0 ? i0 + (int)left : t.blocks;
+    const Sink to = {i0 == 0 && i1 == t.blocks, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
+
+    u4 kw[2][2];
+    uint2 vw[8];
+    int valid, next_valid = 0;
+    const auto load_k = [&](const Block &b) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t off = (uint32_t)(8 * (n >> 2) + 4 * y + (n & 3)) * stride + 128u * wave + 16u * g;
+#pragma unroll
+        for (int st = 0; st < 2; ++st) kw[y][st] = row_load<u4>(b.k, off + 64 * st);
+      }
+    };
+    const auto load_v = [&](const Block &b) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) vw[k] = row_load<uint2>(b.v, (uint32_t)(8 * g + k) * stride + 128u * wave + 8u * n);
+    };
+    Block blk = block_of(a, t, h, t.block(i0), 2 * kD);
+    valid = blk.valid;
+    load_k(blk);
+    load_v(blk);
+
+    const bool mine = n < t.rows;
+    const int r = t.row0 + (mine ? n : 0), tok = r / a.group;
+    const int pos = mine ? t.first + tok : -1;
+    float4 qv[2][2];
+    const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 64 * wave + 8 * g;
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const float4 f = *reinterpret_cast<const float4 *>(q + 32 * st + 4 * y);
+        const float sl = mine ? a.sl2 : 0.0f;
+        qv[st][y] = mine ? float4{f.x * sl, f.y * sl, f.z * sl, f.w * sl} : float4{0.f, 0.f, 0.f, 0.f};
+      }
+    u4 qb[2][kParts<kBf>];
+    float back;
+    split_queries<kBf, 2>(qv, qb, back);
+
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    f4 acc[4] = {zero, zero, zero, zero};
+    Softmax<kBf> sm;
+    for (int i = i0; i < i1; ++i, turn ^= 1) {
+      const int j0 = t.block(i) << 5;
+      float s[8];
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        f4 c[kParts<kBf>];
+#pragma unroll
+        for (int p = 0; p < kParts<kBf>; ++p) {
+          c[p] = half_mfma<kBf>(kw[y][0], qb[0][p], zero);
+          c[p] = half_mfma<kBf>(kw[y][1], qb[1][p], c[p]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float z = c[kParts<kBf> - 1][e];
+#pragma unroll
+          for (int p = kParts<kBf> - 2; p >= 0; --p) z += c[p][e];
+          s[4 * y + e] = z * back;
+        }
+      }
+      const bool more = i + 1 < i1;
+      if (more) {
+        blk = block_of(a, t, h, t.block(i + 1), 2 * kD);
+        next_valid = blk.valid;
+        load_k(blk);
+      }
+      if constexpr (kW > 1) {
+        float(*to_sc)[16][kScoreRow] = sc[turn];
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          *reinterpret_cast<float4 *>(&to_sc[wave][n][8 * g + 4 * y]) = float4{s[4 * y], s[4 * y + 1], s[4 * y + 2], s[4 * y + 3]};
+        lds_barrier();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kW; ++w)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float4 f = *reinterpret_cast<const float4 *>(&to_sc[w][n][8 * g + 4 * y]);
+            s[4 * y] += f.x;
+            s[4 * y + 1] += f.y;
+            s[4 * y + 2] += f.z;
+            s[4 * y + 3] += f.w;
+          }
+      }
+      const bool all = valid == kBlk && t.rows == 16 && j0 + 31 <= t.p0 && t.p0 >= 0 &&
+                       (a.window <= 0 || j0 > t.p1 - a.window || j0 + 31 < a.sinks);
+      u4 pb[kParts<kBf>];
+      float alpha;
+      if (sm.step(s, all, [&](int e) { return 8 * g + e < valid && sees(a, pos, j0 + 8 * g + e); }, pb, alpha))
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[j][e] *= alpha;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] = j < 2 ? __builtin_amdgcn_perm(vw[2 * k + 1].x, vw[2 * k].x, sel)
+                       : __builtin_amdgcn_perm(vw[2 * k + 1].y, vw[2 * k].y, sel);
+        const u4 A = {w[0], w[1], w[2], w[3]};
+#pragma unroll
+        for (int p = kParts<kBf> - 1; p >= 0; --p) acc[j] = half_mfma<kBf>(A, pb[p], acc[j]);
+      }
+      if (more) load_v(blk);
+      valid = next_valid;
+    }
+    // ---- the piece's rows
+    const float l = sm.sum() * (1.0f / Softmax<kBf>::kUp);
+    bool bad = sm.bad;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[j][e] *= 1.0f / Softmax<kBf>::kUp;
+        bad |= !(fabsf(acc[j][e]) < INFINITY);
+      }
+    if (bad) s_bad = 1u;
+    __syncthreads();
+    const bool redo = s_bad != 0u;
+    __syncthreads();
+    if (redo) {
+      for (int row = wave; row < t.rows; row += kW) plain_store<kBf, kW>(a, t, h, row, i0, i1, lane, to, 16);
+      if (tid == 0) s_bad = 0u;
+    } else if (mine) {
+      const int64_t at = to.slot * 16 + n;
+      float *o = (to.whole ? row_out(a, t, h, n, kD) : a.part + at * kD) + 64 * wave + 16 * g;
+      const float f = !to.whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        reinterpret_cast<float4 *>(o)[e] = float4{acc[0][e] * f, acc[1][e] * f, acc[2][e] * f, acc[3][e] * f};
+      if (!to.whole && wave == 0 && g == 0) a.ml[at] = float2{sm.m, l};
+    }
+    u += i1 - i0;
+  }
+}
+
+// ---- tiles of 16 kW rows, 16 a wave. The workgroup moves a block's rows of K and V into LDS,
+// through registers and a block ahead; every wave then runs its rows from there:
+//   scores (transposed, A = K) with keys in the order of few_kernel; out (transposed, A = V): V's
+//   columns come by transposing reads; the result is columns 16 c + 4 g + i of row n.
+// Pieces of 16 bytes of a row are turned by the row, so that the 16 rows which a quarter of a wave
+// reads at once lie on different banks; V's by 32 bytes, for the 8 rows of a transposing read.
+template <int kD>
+__device__ __forceinline__ int k_piece(int key, int c) {
+  const int r = ((key >> 3) << 2) | (key & 3);
+  if constexpr (kD == 64) return c ^ ((r >> 1) & 7);
+  else return c ^ r;
+}
+template <int kD>
+__device__ __forceinline__ int v_piece(int key, int c) {
+  if constexpr (kD == 64) return c ^ ((((key >> 1) & 1) | ((key >> 3 & 1) << 1)) << 1);
+  else return c ^ (((key & 3) | ((key >> 3 & 1) << 2)) << 1);
+}
+template <bool kBf>
+__device__ __forceinline__ uint2 load_columns(const uint16_t *p) {
+  typedef __fp16 v4h __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) v4h lds_v4h;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h *)(p)));
+}
+
+template <bool kBf, int kD, int kW>
+__global__ __launch_bounds__(64 * kW) void many_kernel(AttendArgs a) {
+  constexpr int kThreads = 64 * kW, kRows = 16 * kW, kSteps = kD / 32, kCols = kD / 16;
+  constexpr int kMoves = 8 * kD / kThreads;  // 16-byte pieces of K and V a thread moves
+  static_assert(kMoves >= 1, "");
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][2][kBlk * kD];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Line line = line_of(a);
+  zero_empty(a, line, kRows, kD, kThreads);
+  // neighbouring shares read the same keys: they go to the same XCD (workgroups go to the 8 in turn)
+  const int share = a.shares % 8 == 0 ? ((int)blockIdx.x % 8) * (a.shares / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
+  if (share >= line.shares) return;
+  int64_t u = line.start(share);
+  const int64_t u0 = u, end = line.start(share + 1);
+  const uint32_t stride = (uint32_t)a.kv_heads * 2u * kD;
+  while (u < end) {
+    const int h = (int)(u / line.per_head);
+    const int64_t in = u - h * line.per_head;
+    const int x = tile_at(a, line.tiles, in);
+    const int2 where = a.tiles[x];
+    const Tile t = tile_of(a, where.x, where.y, kRows);
+    const int i0 = (int)(in - a.before[x]);
+    const int64_t left = end - u;
+    const int i1 = left < t.blocks - i0 ? i0 + (int)left : t.blocks;
+    const Sink to = {i0 == 0 && i1 == t.blocks, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
+
+    u4 hold[kMoves];
+    const auto load = [&](const Block &b) {
+#pragma unroll
+      for (int j = 0; j < kMoves; ++j) {
+        const int piece = j * kThreads + tid, p = piece & (4 * kD - 1);
+        const uint32_t off = (uint32_t)(p / (kD / 8)) * stride + 16u * (uint32_t)(p % (kD / 8));
+        hold[j] = j * kThreads + 64 * wave < 4 * kD ? row_load<u4>(b.k, off) : row_load<u4>(b.v, off);
+      }
+    };
+    const auto store = [&](int buf) {
+#pragma unroll
+      for (int j = 0; j < kMoves; ++j) {
+        const int piece = j * kThreads + tid, p = piece & (4 * kD - 1), key = p / (kD / 8), c = p % (kD / 8);
+        const bool is_k = j * kThreads + 64 * wave < 4 * kD;
+        uint16_t *to_lds = lds[buf][is_k ? 0 : 1] + key * kD + 8 * (is_k ? k_piece<kD>(key, c) : v_piece<kD>(key, c));
+        *reinterpret_cast<u4 *>(to_lds) = hold[j];
+      }
+    };
+    Block blk = block_of(a, t, h, t.block(i0), 2 * kD);
+    int valid = blk.valid, next_valid = 0;
+    load(blk);
+
+    const int row = 16 * wave + n;
+    const bool mine = row < t.rows;
+    const int r = t.row0 + (mine ? row : 0), tok = r / a.group;
+    const int pos = mine ? t.first + tok : -1;
+    // the wave's rows' positions
+    const int w1 = t.rows < 16 * wave + 16 ? t.rows : 16 * wave + 16;  // behind its last row
+    const bool some = 16 * wave < w1;
+    const int wp0 = some ? t.first + (t.row0 + 16 * wave) / a.group : -1;
+    const int wp1 = some ? t.first + (t.row0 + w1 - 1) / a.group : -1;
+    u4 qb[kSteps][kParts<kBf>];
+    float back;
+    {
+      float4 qv[kSteps][2];
+      const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 8 * g;
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float4 f = *reinterpret_cast<const float4 *>(q + 32 * st + 4 * y);
+          qv[st][y] = mine ? float4{f.x * a.sl2, f.y * a.sl2, f.z * a.sl2, f.w * a.sl2} : float4{0.f, 0.f, 0.f, 0.f};
+        }
+      split_queries<kBf, kSteps>(qv, qb, back);
+    }
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    f4 acc[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) acc[c] = zero;
+    Softmax<kBf> sm;
+
+    __syncthreads();  // the last piece's blocks are read
+    store(0);
+    if (i0 + 1 < i1) {
+      blk = block_of(a, t, h, t.block(i0 + 1), 2 * kD);
+      next_valid = blk.valid;
+      load(blk);
+    }
+    lds_barrier();
+    for (int i = i0; i < i1; ++i) {
+      const int buf = (i - i0) & 1, j0 = t.block(i) << 5;
+      int after_valid = 0;
+      if (i + 1 < i1) {
+        store(buf ^ 1);
+        if (i + 2 < i1) {
+          blk = block_of(a, t, h, t.block(i + 2), 2 * kD);
+          after_valid = blk.valid;
+          load(blk);
+        }
+      }
+      // (a block that none of the wave's rows sees: behind them all, or before all their windows)
+      const bool skip = j0 > wp1 || (a.window > 0 && j0 + 31 <= wp0 - a.window && j0 >= a.sinks);
+      if (!skip) {
+        const uint16_t *kb = lds[buf][0], *vb = lds[buf][1];
+        float s[8];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          f4 c[kParts<kBf>];
+#pragma unroll
+          for (int p = 0; p < kParts<kBf>; ++p) c[p] = zero;
+          const int key = 8 * (n >> 2) + 4 * y + (n & 3);
+#pragma unroll
+          for (int st = 0; st < kSteps; ++st) {
+            const u4 A = *reinterpret_cast<const u4 *>(kb + key * kD + 8 * k_piece<kD>(key, 4 * st + g));
+#pragma unroll
+            for (int p = 0; p < kParts<kBf>; ++p) c[p] = half_mfma<kBf>(A, qb[st][p], c[p]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float z = c[kParts<kBf> - 1][e];
+#pragma unroll
+            for (int p = kParts<kBf> - 2; p >= 0; --p) z += c[p][e];
+            s[4 * y + e] = z * back;
+          }
+        }
+        const bool all = valid == kBlk && w1 == 16 * wave + 16 && j0 + 31 <= wp0 &&
+                         (a.window <= 0 || j0 > wp1 - a.window || j0 + 31 < a.sinks);
+        u4 pb[kParts<kBf>];
+        float alpha;
+        if (sm.step(s, all, [&](int e) { return 8 * g + e < valid && sees(a, pos, j0 + 8 * g + e); }, pb, alpha))
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[c][e] *= alpha;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          // lane n of each 16: four values of row n / 4 of keys 8 g .. + 3, then of + 4 .. + 7
+          const int k0 = 8 * g + (n >> 2), at = 2 * c + ((n & 3) >> 1), off = 4 * (n & 1);
+          const uint2 lo = load_columns<kBf>(vb + k0 * kD + 8 * v_piece<kD>(k0, at) + off);
+          const uint2 hi = load_columns<kBf>(vb + (k0 + 4) * kD + 8 * v_piece<kD>(k0 + 4, at) + off);
+          const u4 A = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+          for (int p = kParts<kBf> - 1; p >= 0; --p) acc[c] = half_mfma<kBf>(A, pb[p], acc[c]);
+        }
+      }
+      lds_barrier();
+      valid = next_valid;
+      next_valid = after_valid;
+    }
+    const float l = sm.sum() * (1.0f / Softmax<kBf>::kUp);
+    bool bad = sm.bad;
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[c][e] *= 1.0f / Softmax<kBf>::kUp;
+        bad |= !(fabsf(acc[c][e]) < INFINITY);
+      }
+    if (__any(bad)) {
+      for (int y = 16 * wave; y < w1; ++y) plain_store<kBf, kD / 64>(a, t, h, y, i0, i1, lane, to, kRows);
+    } else if (mine) {
+      const int64_t at = to.slot * kRows + row;
+      float *o = (to.whole ? row_out(a, t, h, row, kD) : a.part + at * kD) + 4 * g;
+      const float f = !to.whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+        *reinterpret_cast<float4 *>(o + 16 * c) = float4{acc[c][0] * f, acc[c][1] * f, acc[c][2] * f, acc[c][3] * f};
+      if (!to.whole && g == 0) a.ml[at] = float2{sm.m, l};
+    }
+    u += i1 - i0;
+  }
+}
+
+// ---- the parts of a tile that was cut, joined. Workgroup: some rows of the tile; kAcross waves
+// share a row's pieces. By tile where there are fewer tiles than cuts, else by cut: the first
+// cut inside a tile joins it.
+template <int kD, int kAcross, int kRowsOf>
+__global__ __launch_bounds__(64 * (kAcross > 4 ? kAcross : 4)) void join_kernel(AttendArgs a, int rows_per_tile, int by_cut) {
+  constexpr int kE = kD / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Line line = line_of(a);
+  int h, x;
+  int64_t first;  // the tile's first block in the line
+  int w0;         // the share that holds it
+  if (by_cut) {
+    const int cut = blockIdx.x + 1;
+    if (cut >= line.shares) return;
+    const int64_t u = line.start(cut);
+    h = (int)(u / line.per_head);
+    x = tile_at(a, line.tiles, u - h * line.per_head);
+    first = h * line.per_head + a.before[x];
+    if (u == first || (cut > 1 && line.start(cut - 1) > first)) return;
+    w0 = cut - 1;
+  } else {
+    h = (int)blockIdx.x % a.kv_heads;
+    x = (int)blockIdx.x / a.kv_heads;
+    if (x >= line.tiles || a.before[x + 1] == a.before[x]) return;
+    first = h * line.per_head + a.before[x];
+    w0 = (int)(first * line.shares / line.all);  // (start(w0) <= first, maybe not the last such)
+    while (line.start(w0 + 1) <= first) ++w0;
+  }
+  const int64_t last = h * line.per_head + a.before[x + 1];  // behind its blocks
+  if (line.start(w0 + 1) >= last) return;                    // not cut
+  int w1 = (int)((last - 1) * line.shares / line.all);
+  while (line.start(w1 + 1) < last) ++w1;
+  const int pieces = w1 - w0 + 1, odd = line.start(w0) < first ? 1 : 0;
+  const int2 where = a.tiles[x];
+  const Tile t = tile_of(a, where.x, where.y, rows_per_tile);
+  const int row0 = blockIdx.y * kRowsOf;
+  const auto at = [&](int i, int row) { return (2 * (int64_t)(w0 + i) + (i == 0 ? odd : 0)) * rows_per_tile + row; };
+  if constexpr (kAcross > 1) {
+    static_assert(kRowsOf == 1, "");
+    __shared__ float part[kAcross][kD], s_m[kAcross], s_l[kAcross];
+    if (row0 >= t.rows) return;
+    float m = -INFINITY, l = 0.0f, acc[kE];
+#pragma unroll
+    for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
+    for (int i = wave; i < pieces; i += kAcross) {
+      const float2 ml = a.ml[at(i, row0)];
+      const float *p = a.part + at(i, row0) * kD + lane * kE;
+      if (ml.x == -INFINITY) continue;
+      const float mn = fmaxf(m, ml.x), c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(ml.x - mn);
+      l = l * c + ml.y * w;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[e] = acc[e] * c + p[e] * w;
+      m = mn;
+    }
+#pragma unroll
+    for (int e = 0; e < kE; ++e) part[wave][lane * kE + e] = acc[e];
+    if (lane == 0) {
+      s_m[wave] = m;
+      s_l[wave] = l;
+    }
+    __syncthreads();
+    if (threadIdx.x >= kD) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kAcross; ++i) top = fmaxf(top, s_m[i]);
+    float sum = 0.0f, all = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAcross; ++i) {
+      const float w = s_m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[i] - top);
+      all += s_l[i] * w;
+      sum += s_m[i] == -INFINITY ? 0.0f : part[i][threadIdx.x] * w;
+    }
+    row_out(a, t, h, row0, kD)[threadIdx.x] = top == -INFINITY ? 0.0f : sum / all;
+  } else {
+    for (int row = row0 + wave; row < row0 + kRowsOf && row < t.rows; row += 4) {
+      float m = -INFINITY, l = 0.0f, acc[kE];
+#pragma unroll
+      for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
+      for (int i = 0; i < pieces; ++i) {
+        const float2 ml = a.ml[at(i, row)];
+        const float *p = a.part + at(i, row) * kD + lane * kE;
+        if (ml.x == -INFINITY) continue;
+        const float mn = fmaxf(m, ml.x), c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(ml.x - mn);
+        l = l * c + ml.y * w;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) acc[e] = acc[e] * c + p[e] * w;
+        m = mn;
+      }
+      float *o = row_out(a, t, h, row, kD) + lane * kE;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) o[e] = m == -INFINITY ? 0.0f : acc[e] / l;
+    }
+  }
+}
+
+// Rows a tile holds, and the workgroups that share the blocks.
+struct Shape {
+  int rows, shares;
+};
+Shape shape_of(int n, int64_t tokens, int group, int head_dim) {
+  const int64_t rows = tokens * group;
+  if (rows <= 16 * (int64_t)n) return Shape{16, 512 * 256 / head_dim};
+  if (rows <= 96 * (int64_t)n) return Shape{64, 512};
+  return Shape{128, 256};
+}
+struct Layout {
+  size_t tiles, before, count, ml, part, all;
+  int max_tiles;
+};
+Layout layout_of(const Shape &sh, int n, int64_t tokens, int group, int head_dim) {
+  Layout l;
+  const auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  l.max_tiles = (int)(n + tokens * group / sh.rows);
+  l.tiles = 0;
+  l.before = up((size_t)l.max_tiles * sizeof(int2));
+  l.count = l.before + up(((size_t)l.max_tiles + 1) * sizeof(int64_t));
+  l.ml = l.count + 256;
+  l.part = l.ml + up((size_t)2 * sh.shares * sh.rows * sizeof(float2));
+  l.all = l.part + (size_t)2 * sh.shares * sh.rows * head_dim * sizeof(float);
+  return l;
+}
+
+template <bool kBf, int kD>
+int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, sh.rows);
+  if (sh.rows == 16)
+    hipLaunchKernelGGL((few_kernel<kBf, kD>), dim3(sh.shares), dim3(kD), 0, s, a);
+  else if (sh.rows == 64)
+    hipLaunchKernelGGL((many_kernel<kBf, kD, 4>), dim3(sh.shares), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((many_kernel<kBf, kD, 8>), dim3(sh.shares), dim3(512), 0, s, a);
+  const int64_t segments = (int64_t)a.max_tiles * a.kv_heads;
+  const int by_cut = segments > sh.shares;
+  const unsigned x = by_cut ? (unsigned)sh.shares : (unsigned)segments;
+  if (segments * 8 <= sh.shares)  // eight parts a tile and more
+    hipLaunchKernelGGL((join_kernel<kD, 16, 1>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
+  else
+    hipLaunchKernelGGL((join_kernel<kD, 1, 16>), dim3(x, sh.rows / 16), dim3(256), 0, s, a, sh.rows, by_cut);
+  PKV_HIP(hipGetLastError());
+  return PKV_OK;
+}
+
+}  // namespace
+
+size_t pages_attend_workspace(int n, int64_t tokens, int heads, int kv_heads, int head_dim) {
+  const int group = heads / kv_heads;
+  return layout_of(shape_of(n, tokens, group, head_dim), n, tokens, group, head_dim).all;
+}
+
+int launch_pages_attend(const PagesAttend &p, void *ws, hipStream_t s) {
+  const int group = p.heads / p.kv_heads;
+  const Shape sh = shape_of(p.n, p.tokens, group, p.head_dim);
+  const Layout l = layout_of(sh, p.n, p.tokens, group, p.head_dim);
+  uint8_t *w = static_cast<uint8_t *>(ws);
+  AttendArgs a;
+  a.q = p.q;
+  a.q_t = p.q_t;
+  a.q_h = p.q_h;
+  a.k = static_cast<const uint8_t *>(p.k_pages);
+  a.v = static_cast<const uint8_t *>(p.v_pages);
+  a.page_bytes = (int64_t)p.page_tokens * p.kv_heads * p.head_dim * 2;
+  a.tables = p.tables;
+  a.lens = p.lens;
+  a.starts = p.starts;
+  a.out = p.out;
+  a.tiles = reinterpret_cast<int2 *>(w + l.tiles);
+  a.before = reinterpret_cast<int64_t *>(w + l.before);
+  a.count = reinterpret_cast<int *>(w + l.count);
+  a.ml = reinterpret_cast<float2 *>(w + l.ml);
+  a.part = reinterpret_cast<float *>(w + l.part);
+  a.n = p.n;
+  a.tokens = (int)p.tokens;
+  a.heads = p.heads;
+  a.kv_heads = p.kv_heads;
+  a.group = group;
+  a.page_lg = __builtin_ctz((unsigned)p.page_tokens);
+  a.n_pages = p.n_pages;
+  a.max_pages = p.max_pages;
+  a.window = p.window;
+  a.sinks = p.sinks;
+  a.max_tiles = l.max_tiles;
+  a.shares = sh.shares;
+  a.sl2 = p.scale * kLog2e;
+  if (const int rc = device_status_word(&a.status)) return rc;
+  const bool bf = p.quant == PKV_QUANT_BF16;
+  if (p.head_dim == 64) return bf ? go<true, 64>(a, sh, s) : go<false, 64>(a, sh, s);
+  if (p.head_dim == 128) return bf ? go<true, 128>(a, sh, s) : go<false, 128>(a, sh, s);
+  return bf ? go<true, 256>(a, sh, s) : go<false, 256>(a, sh, s);
+}
+
+}  // namespace pkv

@@ -327,6 +327,38 @@ class PagedKvPool:
     def sequence(self) -> "PagedSequence":
         return PagedSequence(self)
 
+    def storage(self):
+        """(k_pages, v_pages): the planes of an F16 or BF16 pool as tensors [n_pages, page_tokens,
+        num_kv_heads, head_dim], for append_pages and attend_pages (pkv_pool_storage). They are
+        the pool's memory: they live as long as the pool does."""
+        dtype = self.quant.cache_dtype()
+        if dtype is None:
+            raise KvCacheError("storage: pages of F16 or BF16 rows")
+        kp, vp, page_bytes = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_size_t()
+        _call(lib().pkv_pool_storage(self._h, ctypes.byref(kp), ctypes.byref(vp),
+                                     ctypes.byref(page_bytes), None, None))
+        shape = (self.n_pages, self.page_tokens, self.num_kv_heads, self.head_dim)
+        planes = []
+        for p in (kp, vp):
+            view = _DeviceBytes(p.value, self.n_pages * page_bytes.value)
+            view.pool = self
+            planes.append(torch.as_tensor(view, device="cuda").view(dtype).view(shape))
+        return tuple(planes)
+
+    def take_pages(self, n: int) -> torch.Tensor:
+        """n free pages out of the reach of the pool's sequences, for tables on the device
+        (pkv_pool_take_pages): their ids, int32 on the host."""
+        ids = torch.empty(max(n, 0), dtype=torch.int32)
+        _call(lib().pkv_pool_take_pages(self._h, n, ctypes.cast(ids.data_ptr(), ctypes.POINTER(ctypes.c_int))))
+        return ids
+
+    def give_pages(self, ids: torch.Tensor) -> None:
+        """Pages of take_pages back to the pool's sequences; ids as take_pages gives them."""
+        if ids.is_cuda or ids.dtype is not torch.int32 or ids.dim() != 1:
+            raise KvCacheError("give_pages takes int32 ids on the host")
+        ids = ids.contiguous()
+        _call(lib().pkv_pool_give_pages(self._h, ids.numel(), ctypes.cast(ids.data_ptr(), ctypes.POINTER(ctypes.c_int))))
+
     def append_batched(self, seqs: Sequence["PagedSequence"], new_k: torch.Tensor,
                        new_v: torch.Tensor) -> None:
         """One token per sequence: new_k, new_v [n, num_kv_heads, 1, head_dim] f32
@@ -399,6 +431,12 @@ class PagedSequence:
     @property
     def pages(self) -> int:
         return lib().pkv_seq_pages(self._h)
+
+    def page_ids(self) -> torch.Tensor:
+        """The sequence's pages in token order, int32 on the host: its row of a block table."""
+        ids = torch.empty(self.pages, dtype=torch.int32)
+        _call(lib().pkv_seq_page_ids(self._h, ctypes.cast(ids.data_ptr(), ctypes.POINTER(ctypes.c_int)), ids.numel()))
+        return ids
 
     def fork(self) -> "PagedSequence":
         h = ctypes.c_void_p()

@@ -20,6 +20,7 @@
 namespace pkv {
 namespace {
 
+struct Tile;
 struct AttendArgs {
   const float *q;  // token t, head h at t * q_t + h * q_h
   int64_t q_t, q_h;
@@ -27,8 +28,9 @@ struct AttendArgs {
   int64_t page_bytes;
   const int *tables, *lens, *starts;
   float *out;
-  int2 *tiles;      // [tile]: request, tile of it
+  Tile *tiles;      // [tile]
   int64_t *before;  // [tile + 1]: blocks of the tiles before it
+  int *firsts;      // [share]: the tile that its first block is of
   int *count;       // tiles
   float *part;      // [2 workgroup + (not its first piece)][row][head_dim]
   float2 *ml;       // [..][row]: running max (log2 units), sum
@@ -92,6 +94,35 @@ __device__ __forceinline__ bool sees(const AttendArgs &a, int p, int j) {
   return j <= p && (a.window <= 0 || j > p - a.window || j < a.sinks);
 }
 
+// The line of all blocks: KV head after KV head, tile after tile.
+struct Line {
+  int tiles, shares;
+  int64_t per_head, all;
+  __device__ __forceinline__ int64_t start(int w) const { return all * w / shares; }
+};
+__device__ __forceinline__ Line line_of(const AttendArgs &a, int tiles, int64_t per_head) {
+  Line l;
+  l.tiles = tiles;
+  l.per_head = per_head;
+  l.all = per_head * a.kv_heads;
+  l.shares = l.all < a.shares ? (int)l.all : a.shares;
+  return l;
+}
+__device__ __forceinline__ Line line_of(const AttendArgs &a) {
+  const int tiles = *a.count;
+  return line_of(a, tiles, a.before[tiles]);
+}
+// The tile that holds block u of a head (u below the head's blocks).
+__device__ __forceinline__ int tile_at(const AttendArgs &a, int tiles, int64_t u) {
+  int lo = 0, hi = tiles;  // before[lo] <= u < before[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.before[mid] <= u) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
 // One workgroup: the tiles of all requests and the running count of their blocks.
 constexpr int kPlanThreads = 1024;
 __device__ __forceinline__ int64_t plan_scan(int64_t x, int64_t *part, int64_t &sum) {
@@ -126,7 +157,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int ro
     const int mine = (int)(((int64_t)fresh * a.group + rows_per_tile - 1) / rows_per_tile);
     int64_t sum;
     const int64_t at = tiles + plan_scan(mine, part, sum);
-    for (int i = 0; i < mine && at + i < a.max_tiles; ++i) a.tiles[at + i] = int2{b, i};
+    for (int i = 0; i < mine && at + i < a.max_tiles; ++i) a.tiles[at + i].b = b, a.tiles[at + i].row0 = i;
     tiles += sum;
   }
   // (starts that run backwards could name more tiles than the step has rows for)
@@ -137,8 +168,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int ro
     const int t = t0 + tid;
     int mine = 0;
     if (t < count) {
-      const int2 x = a.tiles[t];
-      mine = tile_of(a, x.x, x.y, rows_per_tile).blocks;
+      const Tile x = tile_of(a, a.tiles[t].b, a.tiles[t].row0, rows_per_tile);
+      a.tiles[t] = x;
+      mine = x.blocks;
     }
     int64_t sum;
     const int64_t at = blocks + plan_scan(mine, part, sum);
@@ -149,31 +181,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int ro
     a.before[count] = blocks;
     *a.count = count;
   }
-}
-
-// The line of all blocks: KV head after KV head, tile after tile.
-struct Line {
-  int tiles, shares;
-  int64_t per_head, all;
-  __device__ __forceinline__ int64_t start(int w) const { return all * w / shares; }
-};
-__device__ __forceinline__ Line line_of(const AttendArgs &a) {
-  Line l;
-  l.tiles = *a.count;
-  l.per_head = a.before[l.tiles];
-  l.all = l.per_head * a.kv_heads;
-  l.shares = l.all < a.shares ? (int)l.all : a.shares;
-  return l;
-}
-// The tile that holds block u of a head (u below the head's blocks).
-__device__ __forceinline__ int tile_at(const AttendArgs &a, int tiles, int64_t u) {
-  int lo = 0, hi = tiles;  // before[lo] <= u < before[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.before[mid] <= u) lo = mid;
-    else hi = mid;
-  }
-  return lo;
+  __syncthreads();
+  const Line line = line_of(a, count, blocks);
+  for (int w = tid; w < line.shares; w += kPlanThreads) a.firsts[w] = tile_at(a, count, line.start(w) % blocks);
 }
 
 // A block's rows of K and V of one KV head as buffers: `valid` rows from the block's first one,
@@ -230,7 +240,7 @@ __device__ __forceinline__ void plain_row(const AttendArgs &a, const Tile &t, in
       for (int e = 0; e < kE; ++e) dot += x[e] * half_value(k[j * stride + e], kBf);
       float s = wave_sum(dot);
       s = s > kClampL2 ? kClampL2 : s < -kClampL2 ? -kClampL2 : s;  // (NaN stays)
-      const float mn = fmaxf(m, s);
+      const float mn = fmaxf(m, s == s ? s : -kClampL2);             // (a key that was seen)
       const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(s - mn);
       l = l * c + w;
 #pragma unroll
@@ -266,8 +276,7 @@ __device__ __forceinline__ void plain_store(const AttendArgs &a, const Tile &t, 
 __device__ __forceinline__ void zero_empty(const AttendArgs &a, const Line &l, int rows_per_tile, int kD, int threads) {
   for (int x = blockIdx.x; x < l.tiles; x += gridDim.x) {
     if (a.before[x + 1] != a.before[x]) continue;
-    const int2 at = a.tiles[x];
-    const Tile t = tile_of(a, at.x, at.y, rows_per_tile);
+    const Tile t = a.tiles[x];
     for (int h = 0; h < a.kv_heads; ++h)
       for (int i = threadIdx.x; i < t.rows * kD; i += threads) row_out(a, t, h, i / kD, kD)[i % kD] = 0.0f;
   }
@@ -401,13 +410,12 @@ __global__ __launch_bounds__(kD) void few_kernel(AttendArgs a) {
   if (tid == 0) s_bad = 0u;
   int turn = 0;
   const uint32_t stride = (uint32_t)a.kv_heads * 2u * kD;
-  while (u < end) {
-    const int h = (int)(u / line.per_head);
-    const int64_t in = u - h * line.per_head;
-    const int x = tile_at(a, line.tiles, in);
-    const int2 where = a.tiles[x];
-    const Tile t = tile_of(a, where.x, where.y, 16);
-    const int i0 = (int)(in - a.before[x]);
+  int x = a.firsts[share], h = (int)(u / line.per_head);
+  for (; u < end; ++x) {
+    if (x == line.tiles) x = 0, ++h;
+    const Tile t = a.tiles[x];
+    if (t.blocks == 0) continue;
+    const int i0 = (int)(u - h * line.per_head - a.before[x]);
     const int64_t left = end - u;
     const int i1 = left < t.blocks - i0 ? i0 + (int)left : t.blocks;
     const Sink to = {i0 == 0 && i1 == t.blocks, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
@@ -590,13 +598,12 @@ __global__ __launch_bounds__(64 * kW) void many_kernel(AttendArgs a) {
   int64_t u = line.start(share);
   const int64_t u0 = u, end = line.start(share + 1);
   const uint32_t stride = (uint32_t)a.kv_heads * 2u * kD;
-  while (u < end) {
-    const int h = (int)(u / line.per_head);
-    const int64_t in = u - h * line.per_head;
-    const int x = tile_at(a, line.tiles, in);
-    const int2 where = a.tiles[x];
-    const Tile t = tile_of(a, where.x, where.y, kRows);
-    const int i0 = (int)(in - a.before[x]);
+  int x = a.firsts[share], h = (int)(u / line.per_head);
+  for (; u < end; ++x) {
+    if (x == line.tiles) x = 0, ++h;
+    const Tile t = a.tiles[x];
+    if (t.blocks == 0) continue;
+    const int i0 = (int)(u - h * line.per_head - a.before[x]);
     const int64_t left = end - u;
     const int i1 = left < t.blocks - i0 ? i0 + (int)left : t.blocks;
     const Sink to = {i0 == 0 && i1 == t.blocks, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
@@ -744,13 +751,64 @@ __global__ __launch_bounds__(64 * kW) void many_kernel(AttendArgs a) {
   }
 }
 
-// ---- the parts of a tile that was cut, joined. Workgroup: some rows of the tile; kAcross waves
-// share a row's pieces. By tile where there are fewer tiles than cuts, else by cut: the first
-// cut inside a tile joins it.
-template <int kD, int kAcross, int kRowsOf>
-__global__ __launch_bounds__(64 * (kAcross > 4 ? kAcross : 4)) void join_kernel(AttendArgs a, int rows_per_tile, int by_cut) {
+// ---- the parts of a tile that was cut, joined: a wave a row, or kAcross waves a row of a tile
+// of many parts. The parts' maxima and sums come side by side, a lane a part; then their rows, four
+// in flight. By tile where there are fewer tiles than cuts, else by cut: the first cut inside a
+// tile joins it.
+template <int kE>
+__device__ __forceinline__ void load_elems(const float *p, float (&x)[kE]) {
+  if constexpr (kE == 4) {
+    const float4 f = *reinterpret_cast<const float4 *>(p);
+    x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+  } else if constexpr (kE == 2) {
+    const float2 f = *reinterpret_cast<const float2 *>(p);
+    x[0] = f.x, x[1] = f.y;
+  } else {
+    x[0] = *p;
+  }
+}
+// Parts [i0, i1) of a row: slot(i) is where part i's row is.
+template <int kE, typename Slot>
+__device__ __forceinline__ void join_parts(const AttendArgs &a, Slot slot, int i0, int i1, int lane, float &m, float &l,
+                                           float (&acc)[kE]) {
+  m = -INFINITY;
+  l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
+  for (int b = i0; b < i1; b += 64) {
+    const int count = i1 - b < 64 ? i1 - b : 64;
+    const float2 ml = lane < count ? a.ml[slot(b + lane)] : float2{-INFINITY, 0.0f};
+    float top = xmax32(xmax16(ml.x));
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if (top == -INFINITY) continue;
+    const float mn = fmaxf(m, top), c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+    // (a part that saw nothing wrote zeros: a weight of 0 takes it out)
+    l = l * c + wave_sum(w * ml.y);
+#pragma unroll
+    for (int e = 0; e < kE; ++e) acc[e] *= c;
+    m = mn;
+    for (int i = 0; i < count; i += 4) {
+      float x[4][kE];
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        load_elems<kE>(a.part + slot(b + (i + y < count ? i + y : count - 1)) * (64 * kE) + lane * kE, x[y]);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        if (i + y >= count) break;  // (the last part again, which may hold infinities)
+        const float f = __shfl(w, i + y);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) acc[e] += f * x[y][e];
+      }
+    }
+  }
+}
+
+template <int kD, int kAcross>
+__global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(AttendArgs a, int rows_per_tile, int by_cut) {
   constexpr int kE = kD / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Line line = line_of(a);
   int h, x;
   int64_t first;  // the tile's first block in the line
@@ -777,27 +835,21 @@ __global__ __launch_bounds__(64 * (kAcross > 4 ? kAcross : 4)) void join_kernel(
   int w1 = (int)((last - 1) * line.shares / line.all);
   while (line.start(w1 + 1) < last) ++w1;
   const int pieces = w1 - w0 + 1, odd = line.start(w0) < first ? 1 : 0;
-  const int2 where = a.tiles[x];
-  const Tile t = tile_of(a, where.x, where.y, rows_per_tile);
-  const int row0 = blockIdx.y * kRowsOf;
-  const auto at = [&](int i, int row) { return (2 * (int64_t)(w0 + i) + (i == 0 ? odd : 0)) * rows_per_tile + row; };
-  if constexpr (kAcross > 1) {
-    static_assert(kRowsOf == 1, "");
+  const Tile t = a.tiles[x];
+  const int row = kAcross > 1 ? (int)blockIdx.y : (int)blockIdx.y * 4 + wave;
+  if (row >= t.rows) return;
+  const auto slot = [&](int i) { return (2 * (int64_t)(w0 + i) + (i == 0 ? odd : 0)) * rows_per_tile + row; };
+  float m, l, acc[kE];
+  if constexpr (kAcross == 1) {
+    join_parts<kE>(a, slot, 0, pieces, lane, m, l, acc);
+    float *o = row_out(a, t, h, row, kD) + lane * kE;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) o[e] = m == -INFINITY ? 0.0f : acc[e] / l;
+  } else {
     __shared__ float part[kAcross][kD], s_m[kAcross], s_l[kAcross];
-    if (row0 >= t.rows) return;
-    float m = -INFINITY, l = 0.0f, acc[kE];
-#pragma unroll
-    for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
-    for (int i = wave; i < pieces; i += kAcross) {
-      const float2 ml = a.ml[at(i, row0)];
-      const float *p = a.part + at(i, row0) * kD + lane * kE;
-      if (ml.x == -INFINITY) continue;
-      const float mn = fmaxf(m, ml.x), c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(ml.x - mn);
-      l = l * c + ml.y * w;
-#pragma unroll
-      for (int e = 0; e < kE; ++e) acc[e] = acc[e] * c + p[e] * w;
-      m = mn;
-    }
+    const int per = (pieces + kAcross - 1) / kAcross;
+    const int i0 = wave * per < pieces ? wave * per : pieces, i1 = i0 + per < pieces ? i0 + per : pieces;
+    join_parts<kE>(a, slot, i0, i1, lane, m, l, acc);
 #pragma unroll
     for (int e = 0; e < kE; ++e) part[wave][lane * kE + e] = acc[e];
     if (lane == 0) {
@@ -814,28 +866,9 @@ __global__ __launch_bounds__(64 * (kAcross > 4 ? kAcross : 4)) void join_kernel(
     for (int i = 0; i < kAcross; ++i) {
       const float w = s_m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[i] - top);
       all += s_l[i] * w;
-      sum += s_m[i] == -INFINITY ? 0.0f : part[i][threadIdx.x] * w;
+      sum += part[i][threadIdx.x] * w;
     }
-    row_out(a, t, h, row0, kD)[threadIdx.x] = top == -INFINITY ? 0.0f : sum / all;
-  } else {
-    for (int row = row0 + wave; row < row0 + kRowsOf && row < t.rows; row += 4) {
-      float m = -INFINITY, l = 0.0f, acc[kE];
-#pragma unroll
-      for (int e = 0; e < kE; ++e) acc[e] = 0.0f;
-      for (int i = 0; i < pieces; ++i) {
-        const float2 ml = a.ml[at(i, row)];
-        const float *p = a.part + at(i, row) * kD + lane * kE;
-        if (ml.x == -INFINITY) continue;
-        const float mn = fmaxf(m, ml.x), c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(ml.x - mn);
-        l = l * c + ml.y * w;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) acc[e] = acc[e] * c + p[e] * w;
-        m = mn;
-      }
-      float *o = row_out(a, t, h, row, kD) + lane * kE;
-#pragma unroll
-      for (int e = 0; e < kE; ++e) o[e] = m == -INFINITY ? 0.0f : acc[e] / l;
-    }
+    row_out(a, t, h, row, kD)[threadIdx.x] = top == -INFINITY ? 0.0f : sum / all;
   }
 }
 
@@ -850,7 +883,7 @@ Shape shape_of(int n, int64_t tokens, int group, int head_dim) {
   return Shape{128, 256};
 }
 struct Layout {
-  size_t tiles, before, count, ml, part, all;
+  size_t tiles, before, firsts, count, ml, part, all;
   int max_tiles;
 };
 Layout layout_of(const Shape &sh, int n, int64_t tokens, int group, int head_dim) {
@@ -858,8 +891,9 @@ Layout layout_of(const Shape &sh, int n, int64_t tokens, int group, int head_dim
   const auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   l.max_tiles = (int)(n + tokens * group / sh.rows);
   l.tiles = 0;
-  l.before = up((size_t)l.max_tiles * sizeof(int2));
-  l.count = l.before + up(((size_t)l.max_tiles + 1) * sizeof(int64_t));
+  l.before = up((size_t)l.max_tiles * sizeof(Tile));
+  l.firsts = l.before + up(((size_t)l.max_tiles + 1) * sizeof(int64_t));
+  l.count = l.firsts + up((size_t)sh.shares * sizeof(int));
   l.ml = l.count + 256;
   l.part = l.ml + up((size_t)2 * sh.shares * sh.rows * sizeof(float2));
   l.all = l.part + (size_t)2 * sh.shares * sh.rows * head_dim * sizeof(float);
@@ -879,9 +913,9 @@ int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
   const int by_cut = segments > sh.shares;
   const unsigned x = by_cut ? (unsigned)sh.shares : (unsigned)segments;
   if (segments * 8 <= sh.shares)  // eight parts a tile and more
-    hipLaunchKernelGGL((join_kernel<kD, 16, 1>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
+    hipLaunchKernelGGL((join_kernel<kD, 16>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
   else
-    hipLaunchKernelGGL((join_kernel<kD, 1, 16>), dim3(x, sh.rows / 16), dim3(256), 0, s, a, sh.rows, by_cut);
+    hipLaunchKernelGGL((join_kernel<kD, 1>), dim3(x, sh.rows / 4), dim3(256), 0, s, a, sh.rows, by_cut);
   PKV_HIP(hipGetLastError());
   return PKV_OK;
 }
@@ -909,8 +943,9 @@ int launch_pages_attend(const PagesAttend &p, void *ws, hipStream_t s) {
   a.lens = p.lens;
   a.starts = p.starts;
   a.out = p.out;
-  a.tiles = reinterpret_cast<int2 *>(w + l.tiles);
+  a.tiles = reinterpret_cast<Tile *>(w + l.tiles);
   a.before = reinterpret_cast<int64_t *>(w + l.before);
+  a.firsts = reinterpret_cast<int *>(w + l.firsts);
   a.count = reinterpret_cast<int *>(w + l.count);
   a.ml = reinterpret_cast<float2 *>(w + l.ml);
   a.part = reinterpret_cast<float *>(w + l.part);

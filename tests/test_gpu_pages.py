@@ -331,6 +331,15 @@ def test_infinities_and_nan_that_are_seen(pk, kind, new):
     assert torch.isfinite(got[2]).all()
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_the_only_key_is_nan(pk, kind):
+    for lens, new in (([1, 1], [1, 1]), ([20, 20], [20, 20])):
+        c = Case(18, lens, new, 16, 2, 256, kind)
+        c.k[int(c.tables[0, 0]), 0, 1, 3] = math.nan
+        got = c.run(pk).view(2, -1, 16, 256)
+        assert torch.isnan(got[0, :, 8:]).all() and torch.isfinite(got[0, :, :8]).all() and torch.isfinite(got[1]).all()
+
+
 def test_pages_that_are_none_are_reported(pk):
     for new in (1, 30):
         c = Case(11, [200, 100], [new, new], 16, 2, 256, "f16")

@@ -29,13 +29,13 @@ struct AttendArgs {
   const int *tables, *lens, *starts;
   float *out;
   Tile *tiles;      // [tile]
-  int64_t *before;  // [tile + 1]: blocks of the tiles before it
+  int64_t *before;  // [tile + 1]: units of the tiles before it
   int *firsts;      // [share]: the tile that its first block is of
   int *count;       // tiles
   float *part;      // [2 workgroup + (not its first piece)][row][head_dim]
   float2 *ml;       // [..][row]: running max (log2 units), sum
   unsigned *status;
-  int n, tokens, heads, kv_heads, group, page_lg, n_pages, max_pages, window, sinks, max_tiles, shares;
+  int n, tokens, heads, kv_heads, group, page_lg, n_pages, max_pages, window, sinks, max_tiles, shares, start;
   float sl2;  // scale * log2(e)
 };
 
@@ -44,6 +44,8 @@ struct Tile {
   int p0, p1;               // positions of its first and last row's tokens
   int first;                // position of row 0's token of the request (may be below 0)
   int sink_blocks, lo, blocks;
+  // a tile's place in the line: what its start costs, in blocks, and its blocks
+  __device__ __forceinline__ int64_t units(int start) const { return blocks ? blocks + start : 0; }
   __device__ __forceinline__ int block(int i) const { return i < sink_blocks ? i : i - sink_blocks + lo; }
 };
 
@@ -94,7 +96,7 @@ __device__ __forceinline__ bool sees(const AttendArgs &a, int p, int j) {
   return j <= p && (a.window <= 0 || j > p - a.window || j < a.sinks);
 }
 
-// The line of all blocks: KV head after KV head, tile after tile.
+// The line of all units: KV head after KV head, tile after tile, of each its start and its blocks.
 struct Line {
   int tiles, shares;
   int64_t per_head, all;
@@ -112,7 +114,7 @@ __device__ __forceinline__ Line line_of(const AttendArgs &a) {
   const int tiles = *a.count;
   return line_of(a, tiles, a.before[tiles]);
 }
-// The tile that holds block u of a head (u below the head's blocks).
+// The tile that holds unit u of a head (u below the head's units).
 __device__ __forceinline__ int tile_at(const AttendArgs &a, int tiles, int64_t u) {
   int lo = 0, hi = tiles;  // before[lo] <= u < before[hi]
   while (hi - lo > 1) {
@@ -123,7 +125,8 @@ __device__ __forceinline__ int tile_at(const AttendArgs &a, int tiles, int64_t u
   return lo;
 }
 
-// One workgroup: the tiles of all requests and the running count of their blocks.
+// One workgroup: the tiles of all requests, the running count of their units, and the tile that
+// each share begins in.
 constexpr int kPlanThreads = 1024;
 __device__ __forceinline__ int64_t plan_scan(int64_t x, int64_t *part, int64_t &sum) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -166,11 +169,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int ro
   int64_t blocks = 0;
   for (int t0 = 0; t0 < count; t0 += kPlanThreads) {
     const int t = t0 + tid;
-    int mine = 0;
+    int64_t mine = 0;
     if (t < count) {
       const Tile x = tile_of(a, a.tiles[t].b, a.tiles[t].row0, rows_per_tile);
       a.tiles[t] = x;
-      mine = x.blocks;
+      mine = x.units(a.start);
     }
     int64_t sum;
     const int64_t at = blocks + plan_scan(mine, part, sum);
@@ -186,27 +189,40 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int ro
   for (int w = tid; w < line.shares; w += kPlanThreads) a.firsts[w] = tile_at(a, count, line.start(w) % blocks);
 }
 
-// A block's rows of K and V of one KV head as buffers: `valid` rows from the block's first one,
-// none where its page is none of the pool's.
+// A block's rows of one KV head, in the plane of K and of V: `valid` rows from byte `at`, none
+// where its page is none of the pool's.
 struct Block {
-  __amdgpu_buffer_rsrc_t k, v;
+  int64_t at;
+  uint32_t span;  // bytes that may be read: loads behind them give zeros
   int valid;
 };
-__device__ __forceinline__ Block block_of(const AttendArgs &a, const Tile &t, int h, int jb, int head_bytes) {
+// 64 entries of a request's table, a lane each: a scalar load a block would be waited for there and
+// then, before the reads of LDS that share its counter.
+struct Table {
+  int first, held;
+  __device__ __forceinline__ void look_at(const AttendArgs &a, int b, int page) {
+    first = page;
+    const int at = page + (int)(threadIdx.x & 63);
+    held = at < a.max_pages ? a.tables[(int64_t)b * a.max_pages + at] : -1;
+  }
+};
+__device__ __forceinline__ Block block_of(const AttendArgs &a, const Tile &t, Table &table, int h, int jb, int head_bytes) {
   Block r;
   const int j0 = jb << 5;
   const uint32_t row = (uint32_t)a.kv_heads * (uint32_t)head_bytes;
-  const int page = __builtin_amdgcn_readfirstlane(a.tables[(int64_t)t.b * a.max_pages + (j0 >> a.page_lg)]);
+  const int nth = j0 >> a.page_lg;
+  if ((uint32_t)(nth - table.first) >= 64u) table.look_at(a, t.b, nth);
+  const int page = __builtin_amdgcn_readlane(table.held, nth - table.first);
   const bool ok = page >= 0 && page < a.n_pages;
   const int left = t.p1 + 1 - j0;
   r.valid = !ok ? 0 : left < kBlk ? left : kBlk;
-  const int64_t at = (ok ? (int64_t)page * a.page_bytes : 0) +
-                     (int64_t)(j0 & ((1 << a.page_lg) - 1)) * row + (int64_t)h * head_bytes;
-  const uint32_t span = r.valid > 0 ? (uint32_t)(r.valid - 1) * row + (uint32_t)head_bytes : 0u;
-  r.k = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.k) + at, 0, span, 0x00020000);
-  r.v = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(a.v) + at, 0, span, 0x00020000);
+  r.at = (ok ? (int64_t)page * a.page_bytes : 0) + (int64_t)(j0 & ((1 << a.page_lg) - 1)) * row + (int64_t)h * head_bytes;
+  r.span = r.valid > 0 ? (uint32_t)(r.valid - 1) * row + (uint32_t)head_bytes : 0u;
   if (!ok && threadIdx.x == 0) atomicOr(a.status, kStatusPage);
   return r;
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const uint8_t *plane, const Block &b) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(plane) + b.at, 0, b.span, 0x00020000);
 }
 
 // Row `row` of a tile over its blocks [i0, i1) in plain f32 products of the keys that it sees
@@ -273,7 +289,7 @@ __device__ __forceinline__ void plain_store(const AttendArgs &a, const Tile &t, 
 }
 
 // The rows of tiles without a key that they see.
-__device__ __forceinline__ void zero_empty(const AttendArgs &a, const Line &l, int rows_per_tile, int kD, int threads) {
+__device__ __forceinline__ void zero_empty(const AttendArgs &a, const Line &l, int kD, int threads) {
   for (int x = blockIdx.x; x < l.tiles; x += gridDim.x) {
     if (a.before[x + 1] != a.before[x]) continue;
     const Tile t = a.tiles[x];
@@ -299,74 +315,100 @@ __device__ __forceinline__ void parts_of(float x0, float x1, uint32_t (&w)[kPart
     w[1] = fp16_sub2(x0, x1, w[0]);
   }
 }
-template <int kSteps>
-__device__ __forceinline__ float top_of(const float4 (&x)[kSteps][2]) {
-  float m = 0.0f;
-#pragma unroll
-  for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-    for (int y = 0; y < 2; ++y)
-      m = fmaxf(m, fmaxf(fmaxf(fabsf(x[s][y].x), fabsf(x[s][y].y)), fmaxf(fabsf(x[s][y].z), fabsf(x[s][y].w))));
-  return xmax32(xmax16(m));
-}
+// A row's elements 32 st + 8 g .. + 7 at q + 32 st, times `by` (zeros unless `mine`). BF16 goes by
+// four steps at a time, F16 needs the row's largest magnitude first.
 template <bool kBf, int kSteps>
-__device__ __forceinline__ void split_queries(float4 (&x)[kSteps][2], u4 (&qb)[kSteps][kParts<kBf>], float &back) {
+__device__ __forceinline__ void split_queries(const float *q, bool mine, float by, u4 (&qb)[kSteps][kParts<kBf>], float &back) {
+  constexpr int kHold = kBf && kSteps > 4 ? 4 : kSteps;
   float f = 1.0f;
   back = 1.0f;
-  if constexpr (!kBf) {  // a row's elements to [2^14, 2^15)
-    int e = (int)(f2u(top_of(x)) >> 23) - 127;
-    e = e < -100 ? -100 : e > 100 ? 100 : e;
-    f = __builtin_ldexpf(1.0f, 14 - e);
-    back = __builtin_ldexpf(1.0f, e - 14);
-  }
 #pragma unroll
-  for (int s = 0; s < kSteps; ++s) {
-    uint32_t w[4][kParts<kBf>];
+  for (int s0 = 0; s0 < kSteps; s0 += kHold) {
+    float x[kHold][8];
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      parts_of<kBf>(x[s][y].x * f, x[s][y].y * f, w[2 * y]);
-      parts_of<kBf>(x[s][y].z * f, x[s][y].w * f, w[2 * y + 1]);
+    for (int st = 0; st < kHold; ++st)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const float4 z = *reinterpret_cast<const float4 *>(q + 32 * (s0 + st) + 4 * y);
+        x[st][4 * y] = z.x, x[st][4 * y + 1] = z.y, x[st][4 * y + 2] = z.z, x[st][4 * y + 3] = z.w;
+      }
+#pragma unroll
+    for (int st = 0; st < kHold; ++st)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[st][i] = mine ? x[st][i] * by : 0.0f;
+    if constexpr (!kBf) {  // a row's elements to [2^14, 2^15)
+      float m = 0.0f;
+#pragma unroll
+      for (int st = 0; st < kHold; ++st)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[st][i]));
+      int e = (int)(f2u(xmax32(xmax16(m))) >> 23) - 127;
+      e = e < -100 ? -100 : e > 100 ? 100 : e;
+      f = __builtin_ldexpf(1.0f, 14 - e);
+      back = __builtin_ldexpf(1.0f, e - 14);
     }
 #pragma unroll
-    for (int p = 0; p < kParts<kBf>; ++p) qb[s][p] = u4{w[0][p], w[1][p], w[2][p], w[3][p]};
+    for (int st = 0; st < kHold; ++st) {
+      uint32_t w[4][kParts<kBf>];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) parts_of<kBf>(x[st][2 * i] * f, x[st][2 * i + 1] * f, w[i]);
+#pragma unroll
+      for (int p = 0; p < kParts<kBf>; ++p) qb[s0 + st][p] = u4{w[0][p], w[1][p], w[2][p], w[3][p]};
+    }
+    if (kHold < kSteps) __builtin_amdgcn_sched_barrier(0);
   }
 }
 
-// A row's softmax over a block, the lane's eight keys 8 g .. 8 g + 7 of row n: the weights as
-// MFMA operands (a power of two times them, F16), the running max and sum, and the factor that
-// what was summed before takes (1 if it stays).
+// Of eight keys from j on, `valid` of them there, the i that the query at position p sees: i <= last,
+// and i > above or i < below.
+struct Seen {
+  int last, above, below;
+};
+__device__ __forceinline__ Seen seen_of(const AttendArgs &a, int p, int j, int valid) {
+  const int x = p - j, y = valid - 1;
+  return Seen{x < y ? x : y, a.window > 0 ? x - a.window : -1, a.sinks - j};
+}
+
+// A row's softmax, the lane's eight keys 8 g .. 8 g + 7 of a block of row n. Scores come in
+// raw, as the MFMA gives them: a score in log2 units is one times `back`, a power of two.
 template <bool kBf>
-struct Softmax {
+struct Row {
   static constexpr float kUp = kBf ? 1.0f : kPUp, kLazy = kBf ? kBf16Lazy : kF16Lazy;
-  float m = -INFINITY, l = 0.0f;
-  bool bad = false;
-  // s: scores (log2 units); ok(i): key 8 g + i is seen. True if the sums before take `alpha`.
-  template <typename Ok>
-  __device__ __forceinline__ bool step(float (&s)[8], bool all, Ok ok, u4 (&pb)[kParts<kBf>], float &alpha) {
+  float m = -INFINITY, l = 0.0f;  // the running max, raised once a score passes it by kLazy; the sum
+  // Masks and clamps c and raises the max: true if any row's was, and what was summed before
+  // takes `alpha`. all: every key is seen, else those of `seen`. (NaN stays: it reaches the sum.)
+  template <typename Which>
+  __device__ __forceinline__ bool raise(float (&c)[8], float back, bool all, Which which, float &alpha) {
+    float top = fmaxf(fmaxf(fmaxf(c[0], c[1]), fmaxf(c[2], c[3])), fmaxf(fmaxf(c[4], c[5]), fmaxf(c[6], c[7])));
+    const float low = fminf(fminf(fminf(c[0], c[1]), fminf(c[2], c[3])), fminf(fminf(c[4], c[5]), fminf(c[6], c[7])));
+    if (!all || __any(top * back > kClampL2 || low * back < -kClampL2)) {
+      const float most = kClampL2 / back;
+      const Seen s = which();
+      top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool seen = all || ok(i);
-      bad |= seen && !(fabsf(s[i]) < INFINITY);
-      s[i] = seen ? __builtin_amdgcn_fmed3f(s[i], -kClampL2, kClampL2) : -INFINITY;
+      for (int i = 0; i < 8; ++i) {
+        const bool seen = (i <= s.last) & ((i > s.above) | (i < s.below));
+        const float x = c[i] > most ? most : c[i] < -most ? -most : c[i];
+        c[i] = seen ? x : -INFINITY;
+        top = fmaxf(top, c[i]);
+      }
     }
-    float top = s[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
-    top = xmax32(xmax16(top));
-    const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
-    const bool any = __any(raise);
-    alpha = 1.0f;
-    if (any) {
-      const float mn = raise ? top : m;
-      alpha = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= alpha;
-    }
+    top = xmax32(xmax16(top)) * back;
+    const bool up = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
+    if (!__any(up)) return false;
+    const float mn = up ? top : m;
+    alpha = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= alpha;
+    return true;
+  }
+  // The weights (times kUp) as MFMA operands.
+  __device__ __forceinline__ void weights(const float (&c)[8], float back, u4 (&pb)[kParts<kBf>]) {
     const float base = m == -INFINITY ? 0.0f : m;
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(s[i] - base) * kUp;
+      p[i] = __builtin_amdgcn_exp2f(fmaf(c[i], back, -base)) * kUp;
       l += p[i];
     }
     uint32_t w[4][kParts<kBf>];
@@ -374,35 +416,38 @@ struct Softmax {
     for (int i = 0; i < 4; ++i) parts_of<kBf>(p[2 * i], p[2 * i + 1], w[i]);
 #pragma unroll
     for (int x = 0; x < kParts<kBf>; ++x) pb[x] = u4{w[0][x], w[1][x], w[2][x], w[3][x]};
-    return any;
   }
   __device__ __forceinline__ float sum() const {  // of the row's four lanes
     float x = l;
     x += __shfl_xor(x, 16);
     x += __shfl_xor(x, 32);
-    return x;
+    return x * (1.0f / kUp);
   }
 };
+// Every query of positions p0 .. p1 (p0 below 0: some see nothing) sees all keys j0 .. j0 + 31.
+__device__ __forceinline__ bool all_seen(const AttendArgs &a, int p0, int p1, int j0) {
+  return (j0 + 31 <= p0) & ((a.window <= 0) | (j0 > p1 - a.window) | (j0 + 31 < a.sinks));
+}
 
-// ---- up to 16 rows a tile. A workgroup of kD / 64 waves: wave w takes elements 64 w .. of all
-// 32 keys of a block for the scores, and columns 64 w .. of V. Rows go from memory straight into
-// registers as MFMA operands, a block ahead; the waves' partial scores meet in LDS, one barrier a
-// block, and every wave runs the same softmax.
+// ---- up to 16 kRT rows a tile, for one token and a few. A workgroup of kD / 64 waves: wave w takes
+// elements 64 w .. of all 32 keys of a block for the scores, and columns 64 w .. of V. Rows go from
+// memory straight into registers as MFMA operands, a block ahead; the waves' partial scores meet
+// in LDS, one barrier a block, and every wave runs the same softmax.
 //   scores (transposed, A = K): lane (r, g) holds 8 elements of key 8 (r / 4) + 4 t + r % 4 for
 //   tile t, so that the result (row n, keys 8 g + 4 t + i) is the weights' operand as it is;
 //   out (transposed, A = V): lane (m, g) holds columns 4 m + j (tile j) of keys 8 g .. + 7, pairs
 //   of keys joined by v_perm; the result is columns 16 g + 4 i + j of row n.
 constexpr int kScoreRow = 36;  // floats, 32 keys and a pad that spreads rows over banks
 
-template <bool kBf, int kD>
-__global__ __launch_bounds__(kD) void few_kernel(AttendArgs a) {
-  constexpr int kW = kD / 64;
-  __shared__ __attribute__((aligned(16))) float sc[2][kW][16][kScoreRow];
+template <bool kBf, int kD, int kRT>
+__global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
+  constexpr int kW = kD / 64, kRows = 16 * kRT, kP = kParts<kBf>;
+  __shared__ __attribute__((aligned(16))) float sc[2][kW][kRows][kScoreRow];
   __shared__ uint32_t s_bad;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Line line = line_of(a);
-  zero_empty(a, line, 16, kD, kD);
+  zero_empty(a, line, kD, kD);
   const int share = blockIdx.x;
   if (share >= line.shares) return;
   int64_t u = line.start(share);
@@ -415,10 +460,12 @@ __global__ __launch_bounds__(kD) void few_kernel(AttendArgs a) {
     if (x == line.tiles) x = 0, ++h;
     const Tile t = a.tiles[x];
     if (t.blocks == 0) continue;
-    const int i0 = (int)(u - h * line.per_head - a.before[x]);
-    const int64_t left = end - u;
-    const int i1 = left < t.blocks - i0 ? i0 + (int)left : t.blocks;
-    const Sink to = {i0 == 0 && i1 == t.blocks, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
+    const int64_t tile0 = h * line.per_head + a.before[x], behind = tile0 + t.units(a.start);
+    const Sink to = {u <= tile0 + a.start && end >= behind, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
+    const int i0 = u <= tile0 + a.start ? 0 : (int)(u - tile0) - a.start;
+    const int i1 = end >= behind ? t.blocks : (int)(end - tile0) - a.start;
+    u = behind;
+    if (i1 <= i0) continue;  // the share ends within the tile's start
 
     u4 kw[2][2];
     uint2 vw[8];
@@ -428,91 +475,96 @@ __global__ __launch_bounds__(kD) void few_kernel(AttendArgs a) {
       for (int y = 0; y < 2; ++y) {
         const uint32_t off = (uint32_t)(8 * (n >> 2) + 4 * y + (n & 3)) * stride + 128u * wave + 16u * g;
 #pragma unroll
-        for (int st = 0; st < 2; ++st) kw[y][st] = row_load<u4>(b.k, off + 64 * st);
+        for (int st = 0; st < 2; ++st) kw[y][st] = row_load<u4>(rsrc_of(a.k, b), off + 64 * st);
       }
     };
     const auto load_v = [&](const Block &b) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) vw[k] = row_load<uint2>(b.v, (uint32_t)(8 * g + k) * stride + 128u * wave + 8u * n);
+      for (int k = 0; k < 8; ++k) vw[k] = row_load<uint2>(rsrc_of(a.v, b), (uint32_t)(8 * g + k) * stride + 128u * wave + 8u * n);
     };
-    Block blk = block_of(a, t, h, t.block(i0), 2 * kD);
+    Table table;
+    table.look_at(a, t.b, (t.block(i0) << 5) >> a.page_lg);
+    Block blk = block_of(a, t, table, h, t.block(i0), 2 * kD);
     valid = blk.valid;
     load_k(blk);
     load_v(blk);
 
-    const bool mine = n < t.rows;
-    const int r = t.row0 + (mine ? n : 0), tok = r / a.group;
-    const int pos = mine ? t.first + tok : -1;
-    float4 qv[2][2];
-    const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 64 * wave + 8 * g;
+    u4 qb[kRT][2][kP];
+    float back[kRT];
+    int pos[kRT];
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const float4 f = *reinterpret_cast<const float4 *>(q + 32 * st + 4 * y);
-        const float sl = mine ? a.sl2 : 0.0f;
-        qv[st][y] = mine ? float4{f.x * sl, f.y * sl, f.z * sl, f.w * sl} : float4{0.f, 0.f, 0.f, 0.f};
-      }
-    u4 qb[2][kParts<kBf>];
-    float back;
-    split_queries<kBf, 2>(qv, qb, back);
-
+    for (int rt = 0; rt < kRT; ++rt) {
+      const bool mine = 16 * rt + n < t.rows;
+      const int r = t.row0 + (mine ? 16 * rt + n : 0), tok = r / a.group;
+      pos[rt] = mine ? t.first + tok : -1;
+      const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 64 * wave + 8 * g;
+      split_queries<kBf, 2>(q, mine, a.sl2, qb[rt], back[rt]);
+    }
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    f4 acc[4] = {zero, zero, zero, zero};
-    Softmax<kBf> sm;
+    f4 acc[kRT][4];
+    Row<kBf> row[kRT];
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[rt][j] = zero;
     for (int i = i0; i < i1; ++i, turn ^= 1) {
       const int j0 = t.block(i) << 5;
-      float s[8];
+      float c[kRT][8];
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        f4 c[kParts<kBf>];
+      for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
-        for (int p = 0; p < kParts<kBf>; ++p) {
-          c[p] = half_mfma<kBf>(kw[y][0], qb[0][p], zero);
-          c[p] = half_mfma<kBf>(kw[y][1], qb[1][p], c[p]);
+        for (int y = 0; y < 2; ++y) {
+          f4 z = zero;
+#pragma unroll
+          for (int p = kP - 1; p >= 0; --p)
+#pragma unroll
+            for (int st = 0; st < 2; ++st) z = half_mfma<kBf>(kw[y][st], qb[rt][st][p], z);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[rt][4 * y + e] = z[e] * back[rt];
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float z = c[kParts<kBf> - 1][e];
-#pragma unroll
-          for (int p = kParts<kBf> - 2; p >= 0; --p) z += c[p][e];
-          s[4 * y + e] = z * back;
-        }
-      }
       const bool more = i + 1 < i1;
       if (more) {
-        blk = block_of(a, t, h, t.block(i + 1), 2 * kD);
+        blk = block_of(a, t, table, h, t.block(i + 1), 2 * kD);
         next_valid = blk.valid;
         load_k(blk);
       }
       if constexpr (kW > 1) {
-        float(*to_sc)[16][kScoreRow] = sc[turn];
+        float(*to_sc)[kRows][kScoreRow] = sc[turn];
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-          *reinterpret_cast<float4 *>(&to_sc[wave][n][8 * g + 4 * y]) = float4{s[4 * y], s[4 * y + 1], s[4 * y + 2], s[4 * y + 3]};
+        for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            *reinterpret_cast<float4 *>(&to_sc[wave][16 * rt + n][8 * g + 4 * y]) =
+                float4{c[rt][4 * y], c[rt][4 * y + 1], c[rt][4 * y + 2], c[rt][4 * y + 3]};
         lds_barrier();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = 0.0f;
+        for (int rt = 0; rt < kRT; ++rt) {
 #pragma unroll
-        for (int w = 0; w < kW; ++w)
+          for (int e = 0; e < 8; ++e) c[rt][e] = 0.0f;
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const float4 f = *reinterpret_cast<const float4 *>(&to_sc[w][n][8 * g + 4 * y]);
-            s[4 * y] += f.x;
-            s[4 * y + 1] += f.y;
-            s[4 * y + 2] += f.z;
-            s[4 * y + 3] += f.w;
-          }
+          for (int w = 0; w < kW; ++w)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float4 f = *reinterpret_cast<const float4 *>(&to_sc[w][16 * rt + n][8 * g + 4 * y]);
+              c[rt][4 * y] += f.x;
+              c[rt][4 * y + 1] += f.y;
+              c[rt][4 * y + 2] += f.z;
+              c[rt][4 * y + 3] += f.w;
+            }
+        }
       }
-      const bool all = valid == kBlk && t.rows == 16 && j0 + 31 <= t.p0 && t.p0 >= 0 &&
-                       (a.window <= 0 || j0 > t.p1 - a.window || j0 + 31 < a.sinks);
-      u4 pb[kParts<kBf>];
-      float alpha;
-      if (sm.step(s, all, [&](int e) { return 8 * g + e < valid && sees(a, pos, j0 + 8 * g + e); }, pb, alpha))
+      const bool all = (valid == kBlk) & (t.rows == kRows) & all_seen(a, t.p0, t.p1, j0);
+      u4 pb[kRT][kP];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+      for (int rt = 0; rt < kRT; ++rt) {
+        float alpha = 1.0f;
+        if (row[rt].raise(c[rt], 1.0f, all, [&] { return seen_of(a, pos[rt], j0 + 8 * g, valid - 8 * g); }, alpha))
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[j][e] *= alpha;
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[rt][j][e] *= alpha;
+        row[rt].weights(c[rt], 1.0f, pb[rt]);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
@@ -523,43 +575,55 @@ __global__ __launch_bounds__(kD) void few_kernel(AttendArgs a) {
                        : __builtin_amdgcn_perm(vw[2 * k + 1].y, vw[2 * k].y, sel);
         const u4 A = {w[0], w[1], w[2], w[3]};
 #pragma unroll
-        for (int p = kParts<kBf> - 1; p >= 0; --p) acc[j] = half_mfma<kBf>(A, pb[p], acc[j]);
+        for (int p = kP - 1; p >= 0; --p)
+#pragma unroll
+          for (int rt = 0; rt < kRT; ++rt) acc[rt][j] = half_mfma<kBf>(A, pb[rt][p], acc[rt][j]);
       }
       if (more) load_v(blk);
       valid = next_valid;
     }
     // ---- the piece's rows
-    const float l = sm.sum() * (1.0f / Softmax<kBf>::kUp);
-    bool bad = sm.bad;
+    float l[kRT];
+    bool bad = false;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int rt = 0; rt < kRT; ++rt) {
+      l[rt] = row[rt].sum();
+      bad |= !(l[rt] < INFINITY);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[j][e] *= 1.0f / Softmax<kBf>::kUp;
-        bad |= !(fabsf(acc[j][e]) < INFINITY);
-      }
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[rt][j][e] *= 1.0f / Row<kBf>::kUp;
+          bad |= !(fabsf(acc[rt][j][e]) < INFINITY);
+        }
+    }
     if (bad) s_bad = 1u;
     __syncthreads();
     const bool redo = s_bad != 0u;
     __syncthreads();
     if (redo) {
-      for (int row = wave; row < t.rows; row += kW) plain_store<kBf, kW>(a, t, h, row, i0, i1, lane, to, 16);
+      for (int y = wave; y < t.rows; y += kW) plain_store<kBf, kW>(a, t, h, y, i0, i1, lane, to, kRows);
       if (tid == 0) s_bad = 0u;
-    } else if (mine) {
-      const int64_t at = to.slot * 16 + n;
-      float *o = (to.whole ? row_out(a, t, h, n, kD) : a.part + at * kD) + 64 * wave + 16 * g;
-      const float f = !to.whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        reinterpret_cast<float4 *>(o)[e] = float4{acc[0][e] * f, acc[1][e] * f, acc[2][e] * f, acc[3][e] * f};
-      if (!to.whole && wave == 0 && g == 0) a.ml[at] = float2{sm.m, l};
+      for (int rt = 0; rt < kRT; ++rt) {
+        const int y = 16 * rt + n;
+        if (y >= t.rows) continue;
+        const int64_t at = to.slot * kRows + y;
+        float *o = (to.whole ? row_out(a, t, h, y, kD) : a.part + at * kD) + 64 * wave + 16 * g;
+        const float f = !to.whole ? 1.0f : l[rt] > 0.0f ? 1.0f / l[rt] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          reinterpret_cast<float4 *>(o)[e] = float4{acc[rt][0][e] * f, acc[rt][1][e] * f, acc[rt][2][e] * f, acc[rt][3][e] * f};
+        if (!to.whole && wave == 0 && g == 0) a.ml[at] = float2{row[rt].m, l[rt]};
+      }
     }
-    u += i1 - i0;
   }
 }
 
-// ---- tiles of 16 kW rows, 16 a wave. The workgroup moves a block's rows of K and V into LDS,
-// through registers and a block ahead; every wave then runs its rows from there:
+// ---- tiles of 16 kW kRT rows, 16 kRT a wave, for prompts. Blocks' rows of K and V go from memory
+// into LDS, three blocks of each, one in use and one or two on their way; every wave runs its rows
+// from there:
 //   scores (transposed, A = K) with keys in the order of few_kernel; out (transposed, A = V): V's
 //   columns come by transposing reads; the result is columns 16 c + 4 g + i of row n.
 // Pieces of 16 bytes of a row are turned by the row, so that the 16 rows which a quarter of a wave
@@ -575,179 +639,271 @@ __device__ __forceinline__ int v_piece(int key, int c) {
   if constexpr (kD == 64) return c ^ ((((key >> 1) & 1) | ((key >> 3 & 1) << 1)) << 1);
   else return c ^ (((key & 3) | ((key >> 3 & 1) << 2)) << 1);
 }
-template <bool kBf>
 __device__ __forceinline__ uint2 load_columns(const uint16_t *p) {
   typedef __fp16 v4h __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) v4h lds_v4h;
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h *)(p)));
 }
 
-template <bool kBf, int kD, int kW>
+// One load of 16 bytes a lane from r + off into LDS from byte `at` (wave-uniform) on, in the lanes'
+// order. In asm, since the compiler would wait for it in front of every later read of LDS: the
+// kernel waits itself (fetched) before the barrier behind which the data is read.
+__device__ __forceinline__ void fetch_rows(uint32_t at, uint32_t off, u4s r) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(at);
+  uint32_t saved;
+  asm volatile(
+      "s_nop 4\n\t"  // SGPRs written by vector instructions: 5 wait states before the load reads them
+      "s_mov_b32 %[sv], m0\n\t"
+      "s_mov_b32 m0, %[m]\n\ts_nop 0\n\t"
+      "buffer_load_dwordx4 %[o], %[r], 0 offen lds\n\t"
+      "s_mov_b32 m0, %[sv]"
+      : [sv] "=&s"(saved)
+      : [m] "s"(m), [o] "v"(off), [r] "s"(r)
+      : "memory");
+}
+// All but the newest `kLeft` loads of this wave have landed.
+template <int kLeft>
+__device__ __forceinline__ void fetched() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(kLeft) : "memory");
+}
+// The lane, from the hardware again rather than from a register.
+__device__ __forceinline__ int this_lane() {
+  int ones = -1;
+  asm volatile("" : "+v"(ones));
+  return __builtin_amdgcn_mbcnt_hi(ones, __builtin_amdgcn_mbcnt_lo(ones, 0));
+}
+// Vector and scalar arithmetic may move across, reads of LDS and matrix products may not.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x406); }
+
+template <bool kBf, int kD, int kW, int kRT>
 __global__ __launch_bounds__(64 * kW) void many_kernel(AttendArgs a) {
-  constexpr int kThreads = 64 * kW, kRows = 16 * kW, kSteps = kD / 32, kCols = kD / 16;
-  constexpr int kMoves = 8 * kD / kThreads;  // 16-byte pieces of K and V a thread moves
+  constexpr int kThreads = 64 * kW, kRows = 16 * kW * kRT, kSteps = kD / 32, kCols = kD / 16, kP = kParts<kBf>;
+  constexpr int kMoves = 4 * kD / kThreads;  // 16-byte pieces of K, and of V, that a thread moves
   static_assert(kMoves >= 1, "");
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2][2][kBlk * kD];
+  __shared__ __attribute__((aligned(1024))) uint16_t lk[3][kBlk * kD], lv[3][kBlk * kD];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Line line = line_of(a);
-  zero_empty(a, line, kRows, kD, kThreads);
+  zero_empty(a, line, kD, kThreads);
   // neighbouring shares read the same keys: they go to the same XCD (workgroups go to the 8 in turn)
   const int share = a.shares % 8 == 0 ? ((int)blockIdx.x % 8) * (a.shares / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
   if (share >= line.shares) return;
   int64_t u = line.start(share);
   const int64_t u0 = u, end = line.start(share + 1);
   const uint32_t stride = (uint32_t)a.kv_heads * 2u * kD;
+  const int row0 = 16 * kRT * wave;  // the wave's first row of a tile
+  // where the pieces that the thread moves come from: of a key's row the one that belongs where it lands
+  uint32_t koff[kMoves], voff[kMoves];
+#pragma unroll
+  for (int j = 0; j < kMoves; ++j) {
+    const int p = j * kThreads + tid, key = p / (kD / 8), c = p % (kD / 8);
+    koff[j] = (uint32_t)key * stride + 16u * (uint32_t)k_piece<kD>(key, c);
+    voff[j] = (uint32_t)key * stride + 16u * (uint32_t)v_piece<kD>(key, c);
+  }
+  // Where the lane reads: K's piece g of key 8 (n / 4) + n % 4, V's row n / 4 of keys 8 g .. + 3 in the
+  // first 16 columns. Later steps and columns turn the place as they turn the piece, by an
+  // exclusive or; the next keys are four rows on. Worked out again in each block: held for all of
+  // them they take registers that the sums need, and what the compiler then puts into scratch
+  // memory comes back behind the loads of LDS.
+  const auto k_place = [] {
+    const int ln = this_lane(), m = ln & 15, key = 8 * (m >> 2) + (m & 3);
+    return key * kD + 8 * k_piece<kD>(key, ln >> 4);
+  };
+  const auto v_place = [] {
+    const int ln = this_lane(), m = ln & 15, key = 8 * (ln >> 4) + (m >> 2);
+    return key * kD + 8 * v_piece<kD>(key, (m & 3) >> 1) + 4 * (m & 1);
+  };
   int x = a.firsts[share], h = (int)(u / line.per_head);
   for (; u < end; ++x) {
     if (x == line.tiles) x = 0, ++h;
     const Tile t = a.tiles[x];
     if (t.blocks == 0) continue;
-    const int i0 = (int)(u - h * line.per_head - a.before[x]);
-    const int64_t left = end - u;
-    const int i1 = left < t.blocks - i0 ? i0 + (int)left : t.blocks;
-    const Sink to = {i0 == 0 && i1 == t.blocks, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
+    const int64_t tile0 = h * line.per_head + a.before[x], behind = tile0 + t.units(a.start);
+    const Sink to = {u <= tile0 + a.start && end >= behind, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
+    const int i0 = u <= tile0 + a.start ? 0 : (int)(u - tile0) - a.start;
+    const int i1 = end >= behind ? t.blocks : (int)(end - tile0) - a.start;
+    u = behind;
+    if (i1 <= i0) continue;  // the share ends within the tile's start
 
-    u4 hold[kMoves];
-    const auto load = [&](const Block &b) {
+    // a block's rows into LDS; rows behind its valid ones are the last one again (never seen)
+    const auto fetch = [&](const uint8_t *plane, const Block &b, const uint32_t (&off)[kMoves], uint16_t *to_lds) {
+      const u4s r = make_rsrc(plane + b.at, b.span);
+      const uint32_t base = (uint32_t)(size_t)((PKV_LDS void *)to_lds) + 1024u * (uint32_t)wave;
+      uint32_t o[kMoves];
 #pragma unroll
-      for (int j = 0; j < kMoves; ++j) {
-        const int piece = j * kThreads + tid, p = piece & (4 * kD - 1);
-        const uint32_t off = (uint32_t)(p / (kD / 8)) * stride + 16u * (uint32_t)(p % (kD / 8));
-        hold[j] = j * kThreads + 64 * wave < 4 * kD ? row_load<u4>(b.k, off) : row_load<u4>(b.v, off);
-      }
-    };
-    const auto store = [&](int buf) {
+      for (int j = 0; j < kMoves; ++j) o[j] = off[j];
+      if (b.valid < kBlk) {
 #pragma unroll
-      for (int j = 0; j < kMoves; ++j) {
-        const int piece = j * kThreads + tid, p = piece & (4 * kD - 1), key = p / (kD / 8), c = p % (kD / 8);
-        const bool is_k = j * kThreads + 64 * wave < 4 * kD;
-        uint16_t *to_lds = lds[buf][is_k ? 0 : 1] + key * kD + 8 * (is_k ? k_piece<kD>(key, c) : v_piece<kD>(key, c));
-        *reinterpret_cast<u4 *>(to_lds) = hold[j];
-      }
-    };
-    Block blk = block_of(a, t, h, t.block(i0), 2 * kD);
-    int valid = blk.valid, next_valid = 0;
-    load(blk);
-
-    const int row = 16 * wave + n;
-    const bool mine = row < t.rows;
-    const int r = t.row0 + (mine ? row : 0), tok = r / a.group;
-    const int pos = mine ? t.first + tok : -1;
-    // the wave's rows' positions
-    const int w1 = t.rows < 16 * wave + 16 ? t.rows : 16 * wave + 16;  // behind its last row
-    const bool some = 16 * wave < w1;
-    const int wp0 = some ? t.first + (t.row0 + 16 * wave) / a.group : -1;
-    const int wp1 = some ? t.first + (t.row0 + w1 - 1) / a.group : -1;
-    u4 qb[kSteps][kParts<kBf>];
-    float back;
-    {
-      float4 qv[kSteps][2];
-      const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 8 * g;
-#pragma unroll
-      for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const float4 f = *reinterpret_cast<const float4 *>(q + 32 * st + 4 * y);
-          qv[st][y] = mine ? float4{f.x * a.sl2, f.y * a.sl2, f.z * a.sl2, f.w * a.sl2} : float4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < kMoves; ++j) {
+          const int over = (j * kThreads + tid) / (kD / 8) - (b.valid - 1);
+          o[j] -= over > 0 ? (uint32_t)over * stride : 0u;
         }
-      split_queries<kBf, kSteps>(qv, qb, back);
-    }
-    const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    f4 acc[kCols];
+      }
 #pragma unroll
-    for (int c = 0; c < kCols; ++c) acc[c] = zero;
-    Softmax<kBf> sm;
-
+      for (int j = 0; j < kMoves; ++j) fetch_rows(base + 1024u * kW * (uint32_t)j, o[j], r);
+    };
+    // (behind the piece's end: the last block again, which nobody looks at)
+    Table table;
+    table.look_at(a, t.b, (t.block(i0) << 5) >> a.page_lg);
+    const auto block = [&](int i) { return block_of(a, t, table, h, t.block(i < i1 ? i : i1 - 1), 2 * kD); };
     __syncthreads();  // the last piece's blocks are read
-    store(0);
-    if (i0 + 1 < i1) {
-      blk = block_of(a, t, h, t.block(i0 + 1), 2 * kD);
-      next_valid = blk.valid;
-      load(blk);
+    Block b0 = block(i0), b1 = block(i0 + 1);
+    fetch(a.k, b0, koff, lk[0]);
+    fetch(a.v, b0, voff, lv[0]);
+    fetch(a.k, b1, koff, lk[1]);
+    fetch(a.v, b1, voff, lv[1]);
+
+    u4 qb[kRT][kSteps][kP];
+    float back[kRT];
+    int pos[kRT];
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+      const int y = row0 + 16 * rt + n;
+      const bool mine = y < t.rows;
+      const int r = t.row0 + (mine ? y : 0), tok = r / a.group;
+      pos[rt] = mine ? t.first + tok : -1;
+      const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 8 * g;
+      split_queries<kBf, kSteps>(q, mine, a.sl2, qb[rt], back[rt]);
     }
+    // the wave's rows' positions
+    const int w1 = t.rows < row0 + 16 * kRT ? t.rows : row0 + 16 * kRT;  // behind its last row
+    const bool some = row0 < w1, full = w1 == row0 + 16 * kRT;
+    const int wp0 = some ? t.first + (t.row0 + row0) / a.group : -1;
+    const int wp1 = some ? t.first + (t.row0 + w1 - 1) / a.group : -1;
+    __builtin_amdgcn_sched_barrier(0);  // (the sums take the registers that the queries came through)
+    const f4 zero = {0.f, 0.f, 0.f, 0.f};
+    f4 acc[kRT][kCols];
+    Row<kBf> row[kRT];
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) acc[rt][c] = zero;
+    f4 sc[kRT][2];
+    // (operands come from LDS kAhead reads ahead of the products that take them)
+    constexpr int kAhead = kBf ? 2 : 4;
+    const auto scores = [&](const uint16_t *kb) {
+      constexpr int kReads = 2 * kSteps;
+      const int kat = k_place();
+      const auto read = [&](int i) {
+        return *reinterpret_cast<const u4 *>(kb + (kat ^ (32 * (i >> 1))) + (i & 1) * 4 * kD);
+      };
+      u4 A[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) A[i] = read(i);
+      keep_order();
+#pragma unroll
+      for (int rt = 0; rt < kRT; ++rt) sc[rt][0] = sc[rt][1] = zero;
+#pragma unroll
+      for (int i = 0; i < kReads; i += 2) {  // (both key tiles in turn: a sum waits for its last product)
+#pragma unroll
+        for (int p = kP - 1; p >= 0; --p)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int rt = 0; rt < kRT; ++rt) sc[rt][y] = half_mfma<kBf>(A[(i + y) % kAhead], qb[rt][i >> 1][p], sc[rt][y]);
+        keep_order();
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          if (i + y + kAhead < kReads) A[(i + y) % kAhead] = read(i + y + kAhead);
+        keep_order();
+      }
+    };
+
+    fetched<2 * kMoves>();  // the first block
     lds_barrier();
-    for (int i = i0; i < i1; ++i) {
-      const int buf = (i - i0) & 1, j0 = t.block(i) << 5;
-      int after_valid = 0;
-      if (i + 1 < i1) {
-        store(buf ^ 1);
-        if (i + 2 < i1) {
-          blk = block_of(a, t, h, t.block(i + 2), 2 * kD);
-          after_valid = blk.valid;
-          load(blk);
-        }
+    // here: block i in LDS, the next one on its way
+    const auto step = [&](int i, auto third) {
+      constexpr int at = decltype(third)::value;  // (i - i0) % 3
+      const int j0 = t.block(i) << 5;
+      const Block b2 = block(i + 2);
+      fetch(a.k, b2, koff, lk[(at + 2) % 3]);
+      fetch(a.v, b2, voff, lv[(at + 2) % 3]);
+      scores(lk[at]);
+      float c[kRT][8];
+#pragma unroll
+      for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[rt][e] = sc[rt][e >> 2][e & 3];
+      const bool all = (b0.valid == kBlk) & full & all_seen(a, wp0, wp1, j0);
+#pragma unroll
+      for (int rt = 0; rt < kRT; ++rt) {
+        float alpha = 1.0f;
+        if (row[rt].raise(c[rt], back[rt], all, [&] { return seen_of(a, pos[rt], j0 + 8 * g, b0.valid - 8 * g); }, alpha))
+#pragma unroll
+          for (int cc = 0; cc < kCols; ++cc)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[rt][cc][e] *= alpha;
       }
-      // (a block that none of the wave's rows sees: behind them all, or before all their windows)
-      const bool skip = j0 > wp1 || (a.window > 0 && j0 + 31 <= wp0 - a.window && j0 >= a.sinks);
-      if (!skip) {
-        const uint16_t *kb = lds[buf][0], *vb = lds[buf][1];
-        float s[8];
+      u4 pb[kRT][kP];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          f4 c[kParts<kBf>];
+      for (int rt = 0; rt < kRT; ++rt) row[rt].weights(c[rt], back[rt], pb[rt]);
+      // lane n of each 16: four values of row n / 4 of keys 8 g .. + 3, then of + 4 .. + 7
+      const int vat = v_place();
+      const auto read = [&](int cc) {
+        const uint16_t *vp = lv[at] + (vat ^ (16 * cc));
+        const uint2 lo = load_columns(vp), hi = load_columns(vp + 4 * kD);
+        return u4{lo.x, lo.y, hi.x, hi.y};
+      };
+      u4 A[kAhead];
 #pragma unroll
-          for (int p = 0; p < kParts<kBf>; ++p) c[p] = zero;
-          const int key = 8 * (n >> 2) + 4 * y + (n & 3);
+      for (int cc = 0; cc < kAhead; ++cc) A[cc] = read(cc);
+      keep_order();
 #pragma unroll
-          for (int st = 0; st < kSteps; ++st) {
-            const u4 A = *reinterpret_cast<const u4 *>(kb + key * kD + 8 * k_piece<kD>(key, 4 * st + g));
+      for (int cc = 0; cc < kCols; cc += 2) {
 #pragma unroll
-            for (int p = 0; p < kParts<kBf>; ++p) c[p] = half_mfma<kBf>(A, qb[st][p], c[p]);
-          }
+        for (int p = kP - 1; p >= 0; --p)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float z = c[kParts<kBf> - 1][e];
+          for (int y = 0; y < 2; ++y)
 #pragma unroll
-            for (int p = kParts<kBf> - 2; p >= 0; --p) z += c[p][e];
-            s[4 * y + e] = z * back;
-          }
-        }
-        const bool all = valid == kBlk && w1 == 16 * wave + 16 && j0 + 31 <= wp0 &&
-                         (a.window <= 0 || j0 > wp1 - a.window || j0 + 31 < a.sinks);
-        u4 pb[kParts<kBf>];
-        float alpha;
-        if (sm.step(s, all, [&](int e) { return 8 * g + e < valid && sees(a, pos, j0 + 8 * g + e); }, pb, alpha))
+            for (int rt = 0; rt < kRT; ++rt)
+              acc[rt][cc + y] = half_mfma<kBf>(A[(cc + y) % kAhead], pb[rt][p], acc[rt][cc + y]);
+        keep_order();
 #pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[c][e] *= alpha;
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          // lane n of each 16: four values of row n / 4 of keys 8 g .. + 3, then of + 4 .. + 7
-          const int k0 = 8 * g + (n >> 2), at = 2 * c + ((n & 3) >> 1), off = 4 * (n & 1);
-          const uint2 lo = load_columns<kBf>(vb + k0 * kD + 8 * v_piece<kD>(k0, at) + off);
-          const uint2 hi = load_columns<kBf>(vb + (k0 + 4) * kD + 8 * v_piece<kD>(k0 + 4, at) + off);
-          const u4 A = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-          for (int p = kParts<kBf> - 1; p >= 0; --p) acc[c] = half_mfma<kBf>(A, pb[p], acc[c]);
-        }
+        for (int y = 0; y < 2; ++y)
+          if (cc + y + kAhead < kCols) A[(cc + y) % kAhead] = read(cc + y + kAhead);
+        keep_order();
       }
+      fetched<2 * kMoves>();  // all but what this step sent for
       lds_barrier();
-      valid = next_valid;
-      next_valid = after_valid;
+      b0 = b1;
+      b1 = b2;
+    };
+    for (int i = i0; i < i1; i += 3) {
+      step(i, std::integral_constant<int, 0>{});
+      if (i + 1 < i1) step(i + 1, std::integral_constant<int, 1>{});
+      if (i + 2 < i1) step(i + 2, std::integral_constant<int, 2>{});
     }
-    const float l = sm.sum() * (1.0f / Softmax<kBf>::kUp);
-    bool bad = sm.bad;
+    fetched<0>();  // (what was sent for behind the end lands before LDS is used again)
+    float l[kRT];
+    bool bad = false;
 #pragma unroll
-    for (int c = 0; c < kCols; ++c)
+    for (int rt = 0; rt < kRT; ++rt) {
+      l[rt] = row[rt].sum();
+      bad |= !(l[rt] < INFINITY);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[c][e] *= 1.0f / Softmax<kBf>::kUp;
-        bad |= !(fabsf(acc[c][e]) < INFINITY);
-      }
+      for (int cc = 0; cc < kCols; ++cc)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[rt][cc][e] *= 1.0f / Row<kBf>::kUp;
+          bad |= !(fabsf(acc[rt][cc][e]) < INFINITY);
+        }
+    }
     if (__any(bad)) {
-      for (int y = 16 * wave; y < w1; ++y) plain_store<kBf, kD / 64>(a, t, h, y, i0, i1, lane, to, kRows);
-    } else if (mine) {
-      const int64_t at = to.slot * kRows + row;
-      float *o = (to.whole ? row_out(a, t, h, row, kD) : a.part + at * kD) + 4 * g;
-      const float f = !to.whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+      for (int y = row0; y < w1; ++y) plain_store<kBf, kD / 64>(a, t, h, y, i0, i1, lane, to, kRows);
+    } else {
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
-        *reinterpret_cast<float4 *>(o + 16 * c) = float4{acc[c][0] * f, acc[c][1] * f, acc[c][2] * f, acc[c][3] * f};
-      if (!to.whole && g == 0) a.ml[at] = float2{sm.m, l};
+      for (int rt = 0; rt < kRT; ++rt) {
+        const int y = row0 + 16 * rt + n;
+        if (y >= t.rows) continue;
+        const int64_t at = to.slot * kRows + y;
+        float *o = (to.whole ? row_out(a, t, h, y, kD) : a.part + at * kD) + 4 * g;
+        const float f = !to.whole ? 1.0f : l[rt] > 0.0f ? 1.0f / l[rt] : 0.0f;
+#pragma unroll
+        for (int cc = 0; cc < kCols; ++cc)
+          *reinterpret_cast<float4 *>(o + 16 * cc) = float4{acc[rt][cc][0] * f, acc[rt][cc][1] * f, acc[rt][cc][2] * f, acc[rt][cc][3] * f};
+        if (!to.whole && g == 0) a.ml[at] = float2{row[rt].m, l[rt]};
+      }
     }
-    u += i1 - i0;
   }
 }
 
@@ -810,31 +966,29 @@ __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(
   constexpr int kE = kD / 64;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Line line = line_of(a);
-  int h, x;
-  int64_t first;  // the tile's first block in the line
-  int w0;         // the share that holds it
+  int h, x, w0;  // w0: the share that holds the tile's first block
   if (by_cut) {
     const int cut = blockIdx.x + 1;
     if (cut >= line.shares) return;
     const int64_t u = line.start(cut);
     h = (int)(u / line.per_head);
     x = tile_at(a, line.tiles, u - h * line.per_head);
-    first = h * line.per_head + a.before[x];
-    if (u == first || (cut > 1 && line.start(cut - 1) > first)) return;
+    const int64_t first = h * line.per_head + a.before[x] + a.start;
+    if (u <= first || (cut > 1 && line.start(cut - 1) > first)) return;
     w0 = cut - 1;
   } else {
     h = (int)blockIdx.x % a.kv_heads;
     x = (int)blockIdx.x / a.kv_heads;
     if (x >= line.tiles || a.before[x + 1] == a.before[x]) return;
-    first = h * line.per_head + a.before[x];
+    const int64_t first = h * line.per_head + a.before[x] + a.start;
     w0 = (int)(first * line.shares / line.all);  // (start(w0) <= first, maybe not the last such)
     while (line.start(w0 + 1) <= first) ++w0;
   }
-  const int64_t last = h * line.per_head + a.before[x + 1];  // behind its blocks
-  if (line.start(w0 + 1) >= last) return;                    // not cut
+  const int64_t tile0 = h * line.per_head + a.before[x], last = h * line.per_head + a.before[x + 1];
+  if (line.start(w0 + 1) >= last) return;  // not cut
   int w1 = (int)((last - 1) * line.shares / line.all);
   while (line.start(w1 + 1) < last) ++w1;
-  const int pieces = w1 - w0 + 1, odd = line.start(w0) < first ? 1 : 0;
+  const int pieces = w1 - w0 + 1, odd = line.start(w0) < tile0 ? 1 : 0;
   const Tile t = a.tiles[x];
   const int row = kAcross > 1 ? (int)blockIdx.y : (int)blockIdx.y * 4 + wave;
   if (row >= t.rows) return;
@@ -872,15 +1026,15 @@ __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(
   }
 }
 
-// Rows a tile holds, and the workgroups that share the blocks.
+// Rows a tile holds, the workgroups that share the blocks, and how many blocks a tile's start costs.
 struct Shape {
-  int rows, shares;
+  int rows, shares, start;
 };
 Shape shape_of(int n, int64_t tokens, int group, int head_dim) {
   const int64_t rows = tokens * group;
-  if (rows <= 16 * (int64_t)n) return Shape{16, 512 * 256 / head_dim};
-  if (rows <= 96 * (int64_t)n) return Shape{64, 512};
-  return Shape{128, 256};
+  for (const int r : {16, 32, 64})
+    if (rows <= r * (int64_t)n) return Shape{r, 512 * 256 / head_dim, 2};
+  return Shape{128, head_dim > 128 ? 256 : 512, 6};
 }
 struct Layout {
   size_t tiles, before, firsts, count, ml, part, all;
@@ -904,16 +1058,21 @@ template <bool kBf, int kD>
 int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, sh.rows);
   if (sh.rows == 16)
-    hipLaunchKernelGGL((few_kernel<kBf, kD>), dim3(sh.shares), dim3(kD), 0, s, a);
+    hipLaunchKernelGGL((few_kernel<kBf, kD, 1>), dim3(sh.shares), dim3(kD), 0, s, a);
+  else if (sh.rows == 32)
+    hipLaunchKernelGGL((few_kernel<kBf, kD, 2>), dim3(sh.shares), dim3(kD), 0, s, a);
   else if (sh.rows == 64)
-    hipLaunchKernelGGL((many_kernel<kBf, kD, 4>), dim3(sh.shares), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((few_kernel<kBf, kD, 4>), dim3(sh.shares), dim3(kD), 0, s, a);
   else
-    hipLaunchKernelGGL((many_kernel<kBf, kD, 8>), dim3(sh.shares), dim3(512), 0, s, a);
-  const int64_t segments = (int64_t)a.max_tiles * a.kv_heads;
-  const int by_cut = segments > sh.shares;
-  const unsigned x = by_cut ? (unsigned)sh.shares : (unsigned)segments;
-  if (segments * 8 <= sh.shares)  // eight parts a tile and more
+    hipLaunchKernelGGL((many_kernel<kBf, kD, (kD == 256 ? 8 : 4), (kD == 256 ? 1 : 2)>), dim3(sh.shares),
+                       dim3(kD == 256 ? 512 : 256), 0, s, a);
+  const int64_t tiles = (int64_t)a.max_tiles * a.kv_heads;
+  const int by_cut = tiles > sh.shares;
+  const unsigned x = by_cut ? (unsigned)sh.shares : (unsigned)tiles;
+  if (tiles * 64 <= sh.shares)  // the parts a tile has on average
     hipLaunchKernelGGL((join_kernel<kD, 16>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
+  else if (tiles * 4 <= sh.shares)
+    hipLaunchKernelGGL((join_kernel<kD, 4>), dim3(x, sh.rows), dim3(256), 0, s, a, sh.rows, by_cut);
   else
     hipLaunchKernelGGL((join_kernel<kD, 1>), dim3(x, sh.rows / 4), dim3(256), 0, s, a, sh.rows, by_cut);
   PKV_HIP(hipGetLastError());
@@ -961,6 +1120,7 @@ int launch_pages_attend(const PagesAttend &p, void *ws, hipStream_t s) {
   a.sinks = p.sinks;
   a.max_tiles = l.max_tiles;
   a.shares = sh.shares;
+  a.start = sh.start;
   a.sl2 = p.scale * kLog2e;
   if (const int rc = device_status_word(&a.status)) return rc;
   const bool bf = p.quant == PKV_QUANT_BF16;

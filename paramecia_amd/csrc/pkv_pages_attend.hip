@@ -315,49 +315,59 @@ __device__ __forceinline__ void parts_of(float x0, float x1, uint32_t (&w)[kPart
     w[1] = fp16_sub2(x0, x1, w[0]);
   }
 }
-// A row's elements 32 st + 8 g .. + 7 at q + 32 st, times `by` (zeros unless `mine`). BF16 goes by
-// four steps at a time, F16 needs the row's largest magnitude first.
+// A row's elements 32 st + 8 g .. + 7 at q + 32 st: sent for, then taken times `by` (zeros unless
+// `mine`). Of a long BF16 row the second half is sent for when the first is taken; F16 needs
+// the row's largest magnitude first.
 template <bool kBf, int kSteps>
-__device__ __forceinline__ void split_queries(const float *q, bool mine, float by, u4 (&qb)[kSteps][kParts<kBf>], float &back) {
-  constexpr int kHold = kBf && kSteps > 4 ? 4 : kSteps;
-  float f = 1.0f;
-  back = 1.0f;
-#pragma unroll
-  for (int s0 = 0; s0 < kSteps; s0 += kHold) {
-    float x[kHold][8];
+struct Queries {
+  static constexpr int kHold = kBf && kSteps > 4 ? 4 : kSteps;
+  float4 x[kHold][2];
+  __device__ __forceinline__ void load(const float *q) {
 #pragma unroll
     for (int st = 0; st < kHold; ++st)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const float4 z = *reinterpret_cast<const float4 *>(q + 32 * (s0 + st) + 4 * y);
-        x[st][4 * y] = z.x, x[st][4 * y + 1] = z.y, x[st][4 * y + 2] = z.z, x[st][4 * y + 3] = z.w;
-      }
+      for (int y = 0; y < 2; ++y) x[st][y] = *reinterpret_cast<const float4 *>(q + 32 * st + 4 * y);
+  }
+  __device__ __forceinline__ void split(const float *q, bool mine, float by, u4 (&qb)[kSteps][kParts<kBf>], float &back) {
+    float f = 1.0f;
+    back = 1.0f;
 #pragma unroll
-    for (int st = 0; st < kHold; ++st)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[st][i] = mine ? x[st][i] * by : 0.0f;
-    if constexpr (!kBf) {  // a row's elements to [2^14, 2^15)
-      float m = 0.0f;
+    for (int s0 = 0; s0 < kSteps; s0 += kHold) {
+      if (s0 > 0) load(q + 32 * s0);
 #pragma unroll
       for (int st = 0; st < kHold; ++st)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[st][i]));
-      int e = (int)(f2u(xmax32(xmax16(m))) >> 23) - 127;
-      e = e < -100 ? -100 : e > 100 ? 100 : e;
-      f = __builtin_ldexpf(1.0f, 14 - e);
-      back = __builtin_ldexpf(1.0f, e - 14);
+        for (int y = 0; y < 2; ++y) {
+          float4 &z = x[st][y];
+          z.x = mine ? z.x * by : 0.0f, z.y = mine ? z.y * by : 0.0f, z.z = mine ? z.z * by : 0.0f, z.w = mine ? z.w * by : 0.0f;
+        }
+      if constexpr (!kBf) {  // a row's elements to [2^14, 2^15)
+        float m = 0.0f;
+#pragma unroll
+        for (int st = 0; st < kHold; ++st)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            m = fmaxf(m, fmaxf(fmaxf(fabsf(x[st][y].x), fabsf(x[st][y].y)), fmaxf(fabsf(x[st][y].z), fabsf(x[st][y].w))));
+        int e = (int)(f2u(xmax32(xmax16(m))) >> 23) - 127;
+        e = e < -100 ? -100 : e > 100 ? 100 : e;
+        f = __builtin_ldexpf(1.0f, 14 - e);
+        back = __builtin_ldexpf(1.0f, e - 14);
+      }
+#pragma unroll
+      for (int st = 0; st < kHold; ++st) {
+        uint32_t w[4][kParts<kBf>];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          parts_of<kBf>(x[st][y].x * f, x[st][y].y * f, w[2 * y]);
+          parts_of<kBf>(x[st][y].z * f, x[st][y].w * f, w[2 * y + 1]);
+        }
+#pragma unroll
+        for (int p = 0; p < kParts<kBf>; ++p) qb[s0 + st][p] = u4{w[0][p], w[1][p], w[2][p], w[3][p]};
+      }
+      if (kHold < kSteps) __builtin_amdgcn_sched_barrier(0);
     }
-#pragma unroll
-    for (int st = 0; st < kHold; ++st) {
-      uint32_t w[4][kParts<kBf>];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) parts_of<kBf>(x[st][2 * i] * f, x[st][2 * i + 1] * f, w[i]);
-#pragma unroll
-      for (int p = 0; p < kParts<kBf>; ++p) qb[s0 + st][p] = u4{w[0][p], w[1][p], w[2][p], w[3][p]};
-    }
-    if (kHold < kSteps) __builtin_amdgcn_sched_barrier(0);
   }
-}
+};
 
 // Of eight keys from j on, `valid` of them there, the i that the query at position p sees: i <= last,
 // and i > above or i < below.
@@ -469,7 +479,7 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
 
     u4 kw[2][2];
     uint2 vw[8];
-    int valid, next_valid = 0;
+    int valid;
     const auto load_k = [&](const Block &b) {
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
@@ -484,6 +494,18 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
     };
     Table table;
     table.look_at(a, t.b, (t.block(i0) << 5) >> a.page_lg);
+    Queries<kBf, 2> qs[kRT];
+    const float *qp[kRT];
+    bool mine[kRT];
+    int pos[kRT];
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+      mine[rt] = 16 * rt + n < t.rows;
+      const int r = t.row0 + (mine[rt] ? 16 * rt + n : 0), tok = r / a.group;
+      pos[rt] = mine[rt] ? t.first + tok : -1;
+      qp[rt] = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 64 * wave + 8 * g;
+      qs[rt].load(qp[rt]);
+    }
     Block blk = block_of(a, t, table, h, t.block(i0), 2 * kD);
     valid = blk.valid;
     load_k(blk);
@@ -491,15 +513,8 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
 
     u4 qb[kRT][2][kP];
     float back[kRT];
-    int pos[kRT];
 #pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      const bool mine = 16 * rt + n < t.rows;
-      const int r = t.row0 + (mine ? 16 * rt + n : 0), tok = r / a.group;
-      pos[rt] = mine ? t.first + tok : -1;
-      const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 64 * wave + 8 * g;
-      split_queries<kBf, 2>(q, mine, a.sl2, qb[rt], back[rt]);
-    }
+    for (int rt = 0; rt < kRT; ++rt) qs[rt].split(qp[rt], mine[rt], a.sl2, qb[rt], back[rt]);
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
     f4 acc[kRT][4];
     Row<kBf> row[kRT];
@@ -509,7 +524,8 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
       for (int j = 0; j < 4; ++j) acc[rt][j] = zero;
     for (int i = i0; i < i1; ++i, turn ^= 1) {
       const int j0 = t.block(i) << 5;
-      float c[kRT][8];
+      const bool more = i + 1 < i1;
+      float(*all_sc)[kRows][kScoreRow] = sc[turn];
 #pragma unroll
       for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
@@ -519,52 +535,11 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
           for (int p = kP - 1; p >= 0; --p)
 #pragma unroll
             for (int st = 0; st < 2; ++st) z = half_mfma<kBf>(kw[y][st], qb[rt][st][p], z);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) c[rt][4 * y + e] = z[e] * back[rt];
+          *reinterpret_cast<float4 *>(&all_sc[wave][16 * rt + n][8 * g + 4 * y]) =
+              float4{z[0] * back[rt], z[1] * back[rt], z[2] * back[rt], z[3] * back[rt]};
         }
-      const bool more = i + 1 < i1;
-      if (more) {
-        blk = block_of(a, t, table, h, t.block(i + 1), 2 * kD);
-        next_valid = blk.valid;
-        load_k(blk);
-      }
-      if constexpr (kW > 1) {
-        float(*to_sc)[kRows][kScoreRow] = sc[turn];
-#pragma unroll
-        for (int rt = 0; rt < kRT; ++rt)
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-            *reinterpret_cast<float4 *>(&to_sc[wave][16 * rt + n][8 * g + 4 * y]) =
-                float4{c[rt][4 * y], c[rt][4 * y + 1], c[rt][4 * y + 2], c[rt][4 * y + 3]};
-        lds_barrier();
-#pragma unroll
-        for (int rt = 0; rt < kRT; ++rt) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) c[rt][e] = 0.0f;
-#pragma unroll
-          for (int w = 0; w < kW; ++w)
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const float4 f = *reinterpret_cast<const float4 *>(&to_sc[w][16 * rt + n][8 * g + 4 * y]);
-              c[rt][4 * y] += f.x;
-              c[rt][4 * y + 1] += f.y;
-              c[rt][4 * y + 2] += f.z;
-              c[rt][4 * y + 3] += f.w;
-            }
-        }
-      }
-      const bool all = (valid == kBlk) & (t.rows == kRows) & all_seen(a, t.p0, t.p1, j0);
-      u4 pb[kRT][kP];
-#pragma unroll
-      for (int rt = 0; rt < kRT; ++rt) {
-        float alpha = 1.0f;
-        if (row[rt].raise(c[rt], 1.0f, all, [&] { return seen_of(a, pos[rt], j0 + 8 * g, valid - 8 * g); }, alpha))
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[rt][j][e] *= alpha;
-        row[rt].weights(c[rt], 1.0f, pb[rt]);
-      }
+      // V's columns as operands; the next block's rows are sent for
+      u4 A[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
@@ -573,14 +548,43 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
         for (int k = 0; k < 4; ++k)
           w[k] = j < 2 ? __builtin_amdgcn_perm(vw[2 * k + 1].x, vw[2 * k].x, sel)
                        : __builtin_amdgcn_perm(vw[2 * k + 1].y, vw[2 * k].y, sel);
-        const u4 A = {w[0], w[1], w[2], w[3]};
+        A[j] = u4{w[0], w[1], w[2], w[3]};
+      }
+      const int now_valid = valid;
+      if (more) {
+        blk = block_of(a, t, table, h, t.block(i + 1), 2 * kD);
+        valid = blk.valid;
+        load_k(blk);
+        load_v(blk);
+      }
+      lds_barrier();
+      const bool all = (now_valid == kBlk) & (t.rows == kRows) & all_seen(a, t.p0, t.p1, j0);
+#pragma unroll
+      for (int rt = 0; rt < kRT; ++rt) {
+        float c[8];
+#pragma unroll
+        for (int w = 0; w < kW; ++w)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float4 f = *reinterpret_cast<const float4 *>(&all_sc[w][16 * rt + n][8 * g + 4 * y]);
+            c[4 * y] = w ? c[4 * y] + f.x : f.x;
+            c[4 * y + 1] = w ? c[4 * y + 1] + f.y : f.y;
+            c[4 * y + 2] = w ? c[4 * y + 2] + f.z : f.z;
+            c[4 * y + 3] = w ? c[4 * y + 3] + f.w : f.w;
+          }
+        float alpha = 1.0f;
+        if (row[rt].raise(c, 1.0f, all, [&] { return seen_of(a, pos[rt], j0 + 8 * g, now_valid - 8 * g); }, alpha))
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[rt][j][e] *= alpha;
+        u4 pb[kP];
+        row[rt].weights(c, 1.0f, pb);
 #pragma unroll
         for (int p = kP - 1; p >= 0; --p)
 #pragma unroll
-          for (int rt = 0; rt < kRT; ++rt) acc[rt][j] = half_mfma<kBf>(A, pb[rt][p], acc[rt][j]);
+          for (int j = 0; j < 4; ++j) acc[rt][j] = half_mfma<kBf>(A[j], pb[p], acc[rt][j]);
       }
-      if (more) load_v(blk);
-      valid = next_valid;
     }
     // ---- the piece's rows
     float l[kRT];
@@ -742,11 +746,24 @@ __global__ __launch_bounds__(64 * kW) void many_kernel(AttendArgs a) {
 #pragma unroll
       for (int j = 0; j < kMoves; ++j) fetch_rows(base + 1024u * kW * (uint32_t)j, o[j], r);
     };
-    // (behind the piece's end: the last block again, which nobody looks at)
     Table table;
     table.look_at(a, t.b, (t.block(i0) << 5) >> a.page_lg);
+    Queries<kBf, kSteps> qs[kRT];
+    const float *qp[kRT];
+    bool mine[kRT];
+    int pos[kRT];
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+      const int y = row0 + 16 * rt + n;
+      mine[rt] = y < t.rows;
+      const int r = t.row0 + (mine[rt] ? y : 0), tok = r / a.group;
+      pos[rt] = mine[rt] ? t.first + tok : -1;
+      qp[rt] = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 8 * g;
+      qs[rt].load(qp[rt]);
+    }
+    // (behind the piece's end: the last block again, which nobody looks at)
     const auto block = [&](int i) { return block_of(a, t, table, h, t.block(i < i1 ? i : i1 - 1), 2 * kD); };
-    __syncthreads();  // the last piece's blocks are read
+    lds_barrier();  // what was sent for behind the last piece's end has landed
     Block b0 = block(i0), b1 = block(i0 + 1);
     fetch(a.k, b0, koff, lk[0]);
     fetch(a.v, b0, voff, lv[0]);
@@ -755,16 +772,8 @@ __global__ __launch_bounds__(64 * kW) void many_kernel(AttendArgs a) {
 
     u4 qb[kRT][kSteps][kP];
     float back[kRT];
-    int pos[kRT];
 #pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      const int y = row0 + 16 * rt + n;
-      const bool mine = y < t.rows;
-      const int r = t.row0 + (mine ? y : 0), tok = r / a.group;
-      pos[rt] = mine ? t.first + tok : -1;
-      const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 8 * g;
-      split_queries<kBf, kSteps>(q, mine, a.sl2, qb[rt], back[rt]);
-    }
+    for (int rt = 0; rt < kRT; ++rt) qs[rt].split(qp[rt], mine[rt], a.sl2, qb[rt], back[rt]);
     // the wave's rows' positions
     const int w1 = t.rows < row0 + 16 * kRT ? t.rows : row0 + 16 * kRT;  // behind its last row
     const bool some = row0 < w1, full = w1 == row0 + 16 * kRT;
@@ -1032,7 +1041,7 @@ struct Shape {
 };
 Shape shape_of(int n, int64_t tokens, int group, int head_dim) {
   const int64_t rows = tokens * group;
-  for (const int r : {16, 32, 64})
+  for (const int r : {16, 32, 48})
     if (rows <= r * (int64_t)n) return Shape{r, 512 * 256 / head_dim, 2};
   return Shape{128, head_dim > 128 ? 256 : 512, 6};
 }
@@ -1061,8 +1070,8 @@ int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
     hipLaunchKernelGGL((few_kernel<kBf, kD, 1>), dim3(sh.shares), dim3(kD), 0, s, a);
   else if (sh.rows == 32)
     hipLaunchKernelGGL((few_kernel<kBf, kD, 2>), dim3(sh.shares), dim3(kD), 0, s, a);
-  else if (sh.rows == 64)
-    hipLaunchKernelGGL((few_kernel<kBf, kD, 4>), dim3(sh.shares), dim3(kD), 0, s, a);
+  else if (sh.rows == 48)
+    hipLaunchKernelGGL((few_kernel<kBf, kD, 3>), dim3(sh.shares), dim3(kD), 0, s, a);
   else
     hipLaunchKernelGGL((many_kernel<kBf, kD, (kD == 256 ? 8 : 4), (kD == 256 ? 1 : 2)>), dim3(sh.shares),
                        dim3(kD == 256 ? 512 : 256), 0, s, a);

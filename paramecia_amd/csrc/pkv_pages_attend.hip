@@ -189,6 +189,93 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int ro
   for (int w = tid; w < line.shares; w += kPlanThreads) a.firsts[w] = tile_at(a, count, line.start(w) % blocks);
 }
 
+// What the plan says, from memory, or worked out by the workgroup itself: a launch less where the
+// requests are a wave's lanes.
+constexpr int kHereTiles = 128;
+struct HerePlan {
+  int before[kHereTiles + 1], count;
+  Tile tiles[kHereTiles];
+};
+// A value that is the same in all lanes, as a scalar.
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ Tile uniform(const Tile &t) {
+  return Tile{uniform(t.b), uniform(t.row0), uniform(t.rows), uniform(t.tok0), uniform(t.p0), uniform(t.p1),
+              uniform(t.first), uniform(t.sink_blocks), uniform(t.lo), uniform(t.blocks)};
+}
+template <bool kHere>
+struct Plan;
+template <>
+struct Plan<false> {
+  Line line;
+  struct Lds {};
+  __device__ __forceinline__ void make(const AttendArgs &a, Lds &, int, int) { line = line_of(a); }
+  __device__ __forceinline__ int64_t before(const AttendArgs &a, int x) const { return a.before[x]; }
+  __device__ __forceinline__ Tile tile(const AttendArgs &a, int x) const { return a.tiles[x]; }
+  __device__ __forceinline__ int first(const AttendArgs &a, int share) const { return a.firsts[share]; }
+  __device__ __forceinline__ int at(const AttendArgs &a, int64_t u) const { return tile_at(a, line.tiles, u); }
+};
+template <>
+struct Plan<true> {
+  Line line;
+  using Lds = HerePlan;
+  const HerePlan *lds;
+  // n at most 64, max_tiles at most kHereTiles, a head's units below 2^31
+  __device__ __forceinline__ void make(const AttendArgs &a, Lds &p, int rows_per_tile, int threads) {
+    const int tid = threadIdx.x;
+    if (tid < 64) {
+      int q0, fresh = 0, len;
+      if (tid < a.n) request_of(a, tid, q0, fresh, len);
+      const int mine = (fresh * a.group + rows_per_tile - 1) / rows_per_tile;
+      int y = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int z = __shfl_up(y, o);
+        if (tid >= o) y += z;
+      }
+      for (int i = 0; i < mine && y - mine + i < a.max_tiles; ++i)
+        p.tiles[y - mine + i].b = tid, p.tiles[y - mine + i].row0 = i;
+      if (tid == 63) p.count = y < a.max_tiles ? y : a.max_tiles;
+    }
+    __syncthreads();
+    const int count = uniform(p.count);
+    for (int t = tid; t < count; t += threads) {
+      const Tile x = tile_of(a, p.tiles[t].b, p.tiles[t].row0, rows_per_tile);
+      p.tiles[t] = x;
+      p.before[t + 1] = (int)x.units(a.start);
+    }
+    __syncthreads();
+    if (tid < 64) {
+      int sum = 0;
+      for (int t0 = 0; t0 < count; t0 += 64) {
+        const int t = t0 + tid;
+        int y = t < count ? p.before[t + 1] : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int z = __shfl_up(y, o);
+          if (tid >= o) y += z;
+        }
+        if (t < count) p.before[t + 1] = sum + y;
+        sum += __shfl(y, 63);
+      }
+      if (tid == 0) p.before[0] = 0;
+    }
+    __syncthreads();
+    lds = &p;
+    line = line_of(a, count, uniform(p.before[count]));
+  }
+  __device__ __forceinline__ int64_t before(const AttendArgs &, int x) const { return uniform(lds->before[x]); }
+  __device__ __forceinline__ Tile tile(const AttendArgs &, int x) const { return uniform(lds->tiles[x]); }
+  __device__ __forceinline__ int first(const AttendArgs &a, int share) const { return at(a, line.start(share) % line.per_head); }
+  __device__ __forceinline__ int at(const AttendArgs &, int64_t u) const {
+    int x = -1;  // tiles that begin at u or before it
+    for (int t0 = 0; t0 < line.tiles; t0 += 64) {
+      const int t = t0 + (int)(threadIdx.x & 63);
+      x += __builtin_popcountll(__ballot(t < line.tiles && lds->before[t < line.tiles ? t : 0] <= u));
+    }
+    return x;
+  }
+};
+
 // A block's rows of one KV head, in the plane of K and of V: `valid` rows from byte `at`, none
 // where its page is none of the pool's.
 struct Block {
@@ -289,10 +376,11 @@ __device__ __forceinline__ void plain_store(const AttendArgs &a, const Tile &t, 
 }
 
 // The rows of tiles without a key that they see.
-__device__ __forceinline__ void zero_empty(const AttendArgs &a, const Line &l, int kD, int threads) {
-  for (int x = blockIdx.x; x < l.tiles; x += gridDim.x) {
-    if (a.before[x + 1] != a.before[x]) continue;
-    const Tile t = a.tiles[x];
+template <typename P>
+__device__ __forceinline__ void zero_empty(const AttendArgs &a, const P &plan, int kD, int threads) {
+  for (int x = blockIdx.x; x < plan.line.tiles; x += gridDim.x) {
+    if (plan.before(a, x + 1) != plan.before(a, x)) continue;
+    const Tile t = plan.tile(a, x);
     for (int h = 0; h < a.kv_heads; ++h)
       for (int i = threadIdx.x; i < t.rows * kD; i += threads) row_out(a, t, h, i / kD, kD)[i % kD] = 0.0f;
   }
@@ -449,15 +537,18 @@ __device__ __forceinline__ bool all_seen(const AttendArgs &a, int p0, int p1, in
 //   of keys joined by v_perm; the result is columns 16 g + 4 i + j of row n.
 constexpr int kScoreRow = 36;  // floats, 32 keys and a pad that spreads rows over banks
 
-template <bool kBf, int kD, int kRT>
+template <bool kBf, int kD, int kRT, bool kHere>
 __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
   constexpr int kW = kD / 64, kRows = 16 * kRT, kP = kParts<kBf>;
   __shared__ __attribute__((aligned(16))) float sc[2][kW][kRows][kScoreRow];
   __shared__ uint32_t s_bad;
+  __shared__ typename Plan<kHere>::Lds s_plan;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Line line = line_of(a);
-  zero_empty(a, line, kD, kD);
+  Plan<kHere> plan;
+  plan.make(a, s_plan, kRows, kD);
+  const Line line = plan.line;
+  zero_empty(a, plan, kD, kD);
   const int share = blockIdx.x;
   if (share >= line.shares) return;
   int64_t u = line.start(share);
@@ -465,12 +556,12 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
   if (tid == 0) s_bad = 0u;
   int turn = 0;
   const uint32_t stride = (uint32_t)a.kv_heads * 2u * kD;
-  int x = a.firsts[share], h = (int)(u / line.per_head);
+  int x = plan.first(a, share), h = (int)(u / line.per_head);
   for (; u < end; ++x) {
     if (x == line.tiles) x = 0, ++h;
-    const Tile t = a.tiles[x];
+    const Tile t = plan.tile(a, x);
     if (t.blocks == 0) continue;
-    const int64_t tile0 = h * line.per_head + a.before[x], behind = tile0 + t.units(a.start);
+    const int64_t tile0 = h * line.per_head + plan.before(a, x), behind = tile0 + t.units(a.start);
     const Sink to = {u <= tile0 + a.start && end >= behind, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
     const int i0 = u <= tile0 + a.start ? 0 : (int)(u - tile0) - a.start;
     const int i1 = end >= behind ? t.blocks : (int)(end - tile0) - a.start;
@@ -687,8 +778,11 @@ __global__ __launch_bounds__(64 * kW) void many_kernel(AttendArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lk[3][kBlk * kD], lv[3][kBlk * kD];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const Line line = line_of(a);
-  zero_empty(a, line, kD, kThreads);
+  Plan<false> plan;
+  Plan<false>::Lds none;
+  plan.make(a, none, kRows, kThreads);
+  const Line line = plan.line;
+  zero_empty(a, plan, kD, kThreads);
   // neighbouring shares read the same keys: they go to the same XCD (workgroups go to the 8 in turn)
   const int share = a.shares % 8 == 0 ? ((int)blockIdx.x % 8) * (a.shares / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
   if (share >= line.shares) return;
@@ -717,12 +811,12 @@ __global__ __launch_bounds__(64 * kW) void many_kernel(AttendArgs a) {
     const int ln = this_lane(), m = ln & 15, key = 8 * (ln >> 4) + (m >> 2);
     return key * kD + 8 * v_piece<kD>(key, (m & 3) >> 1) + 4 * (m & 1);
   };
-  int x = a.firsts[share], h = (int)(u / line.per_head);
+  int x = plan.first(a, share), h = (int)(u / line.per_head);
   for (; u < end; ++x) {
     if (x == line.tiles) x = 0, ++h;
-    const Tile t = a.tiles[x];
+    const Tile t = plan.tile(a, x);
     if (t.blocks == 0) continue;
-    const int64_t tile0 = h * line.per_head + a.before[x], behind = tile0 + t.units(a.start);
+    const int64_t tile0 = h * line.per_head + plan.before(a, x), behind = tile0 + t.units(a.start);
     const Sink to = {u <= tile0 + a.start && end >= behind, 2 * (int64_t)share + (u > u0 ? 1 : 0)};
     const int i0 = u <= tile0 + a.start ? 0 : (int)(u - tile0) - a.start;
     const int i1 = end >= behind ? t.blocks : (int)(end - tile0) - a.start;
@@ -970,35 +1064,38 @@ __device__ __forceinline__ void join_parts(const AttendArgs &a, Slot slot, int i
   }
 }
 
-template <int kD, int kAcross>
+template <int kD, int kAcross, bool kHere>
 __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(AttendArgs a, int rows_per_tile, int by_cut) {
   constexpr int kE = kD / 64;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Line line = line_of(a);
+  __shared__ typename Plan<kHere>::Lds s_plan;
+  Plan<kHere> plan;
+  plan.make(a, s_plan, rows_per_tile, (int)blockDim.x);
+  const Line line = plan.line;
   int h, x, w0;  // w0: the share that holds the tile's first block
   if (by_cut) {
     const int cut = blockIdx.x + 1;
     if (cut >= line.shares) return;
     const int64_t u = line.start(cut);
     h = (int)(u / line.per_head);
-    x = tile_at(a, line.tiles, u - h * line.per_head);
-    const int64_t first = h * line.per_head + a.before[x] + a.start;
+    x = plan.at(a, u - h * line.per_head);
+    const int64_t first = h * line.per_head + plan.before(a, x) + a.start;
     if (u <= first || (cut > 1 && line.start(cut - 1) > first)) return;
     w0 = cut - 1;
   } else {
     h = (int)blockIdx.x % a.kv_heads;
     x = (int)blockIdx.x / a.kv_heads;
-    if (x >= line.tiles || a.before[x + 1] == a.before[x]) return;
-    const int64_t first = h * line.per_head + a.before[x] + a.start;
+    if (x >= line.tiles || plan.before(a, x + 1) == plan.before(a, x)) return;
+    const int64_t first = h * line.per_head + plan.before(a, x) + a.start;
     w0 = (int)(first * line.shares / line.all);  // (start(w0) <= first, maybe not the last such)
     while (line.start(w0 + 1) <= first) ++w0;
   }
-  const int64_t tile0 = h * line.per_head + a.before[x], last = h * line.per_head + a.before[x + 1];
+  const int64_t tile0 = h * line.per_head + plan.before(a, x), last = h * line.per_head + plan.before(a, x + 1);
   if (line.start(w0 + 1) >= last) return;  // not cut
   int w1 = (int)((last - 1) * line.shares / line.all);
   while (line.start(w1 + 1) < last) ++w1;
   const int pieces = w1 - w0 + 1, odd = line.start(w0) < tile0 ? 1 : 0;
-  const Tile t = a.tiles[x];
+  const Tile t = plan.tile(a, x);
   const int row = kAcross > 1 ? (int)blockIdx.y : (int)blockIdx.y * 4 + wave;
   if (row >= t.rows) return;
   const auto slot = [&](int i) { return (2 * (int64_t)(w0 + i) + (i == 0 ? odd : 0)) * rows_per_tile + row; };
@@ -1063,27 +1160,42 @@ Layout layout_of(const Shape &sh, int n, int64_t tokens, int group, int head_dim
   return l;
 }
 
-template <bool kBf, int kD>
-int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, sh.rows);
-  if (sh.rows == 16)
-    hipLaunchKernelGGL((few_kernel<kBf, kD, 1>), dim3(sh.shares), dim3(kD), 0, s, a);
-  else if (sh.rows == 32)
-    hipLaunchKernelGGL((few_kernel<kBf, kD, 2>), dim3(sh.shares), dim3(kD), 0, s, a);
-  else if (sh.rows == 48)
-    hipLaunchKernelGGL((few_kernel<kBf, kD, 3>), dim3(sh.shares), dim3(kD), 0, s, a);
-  else
-    hipLaunchKernelGGL((many_kernel<kBf, kD, (kD == 256 ? 8 : 4), (kD == 256 ? 1 : 2)>), dim3(sh.shares),
-                       dim3(kD == 256 ? 512 : 256), 0, s, a);
+template <int kD, bool kHere>
+void join(AttendArgs &a, const Shape &sh, hipStream_t s) {
   const int64_t tiles = (int64_t)a.max_tiles * a.kv_heads;
   const int by_cut = tiles > sh.shares;
   const unsigned x = by_cut ? (unsigned)sh.shares : (unsigned)tiles;
   if (tiles * 64 <= sh.shares)  // the parts a tile has on average
-    hipLaunchKernelGGL((join_kernel<kD, 16>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
+    hipLaunchKernelGGL((join_kernel<kD, 16, kHere>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
   else if (tiles * 4 <= sh.shares)
-    hipLaunchKernelGGL((join_kernel<kD, 4>), dim3(x, sh.rows), dim3(256), 0, s, a, sh.rows, by_cut);
+    hipLaunchKernelGGL((join_kernel<kD, 4, kHere>), dim3(x, sh.rows), dim3(256), 0, s, a, sh.rows, by_cut);
   else
-    hipLaunchKernelGGL((join_kernel<kD, 1>), dim3(x, sh.rows / 4), dim3(256), 0, s, a, sh.rows, by_cut);
+    hipLaunchKernelGGL((join_kernel<kD, 1, kHere>), dim3(x, sh.rows / 4), dim3(256), 0, s, a, sh.rows, by_cut);
+}
+template <bool kBf, int kD, bool kHere>
+void few(AttendArgs &a, const Shape &sh, hipStream_t s) {
+  const dim3 grid(sh.shares), block(kD);
+  if (sh.rows == 16) hipLaunchKernelGGL((few_kernel<kBf, kD, 1, kHere>), grid, block, 0, s, a);
+  else if (sh.rows == 32) hipLaunchKernelGGL((few_kernel<kBf, kD, 2, kHere>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((few_kernel<kBf, kD, 3, kHere>), grid, block, 0, s, a);
+  join<kD, kHere>(a, sh, s);
+}
+template <bool kBf, int kD>
+int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
+  // a head's units at most, as 32-bit sums of the workgroup's own plan
+  const int64_t most = (int64_t)a.max_tiles * ((((int64_t)a.max_pages << a.page_lg) >> 5) + sh.start + 1);
+  if (sh.rows < 128 && a.n <= 64 && a.max_tiles <= kHereTiles && most < ((int64_t)1 << 31)) {
+    few<kBf, kD, true>(a, sh, s);
+  } else {
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, sh.rows);
+    if (sh.rows < 128) {
+      few<kBf, kD, false>(a, sh, s);
+    } else {
+      hipLaunchKernelGGL((many_kernel<kBf, kD, (kD == 256 ? 8 : 4), (kD == 256 ? 1 : 2)>), dim3(sh.shares),
+                         dim3(kD == 256 ? 512 : 256), 0, s, a);
+      join<kD, false>(a, sh, s);
+    }
+  }
   PKV_HIP(hipGetLastError());
   return PKV_OK;
 }

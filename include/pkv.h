@@ -459,7 +459,8 @@ int pkv_seq_page_ids(const pkv_seq *s, int *pages_host, int capacity);
  * place there; behind the last row -1 and position 0. status [1]: PKV_OK, or with nothing
  * moved, all slots -1, starts 0 and totals = lens, PKV_ERR_OVERFLOW (the stack lacks pages) or
  * PKV_ERR_ARG (a negative length, a table too short, more than max_tokens new tokens, a stack
- * that would not fit). page_tokens: a power of two in [32, 2^20]; max_tokens below 2^31. */
+ * that would not fit). page_tokens: a power of two in [32, 2^20]; max_tokens below 2^31, n * max_pages too (else
+ * PKV_ERR_UNSUPPORTED). */
 int pkv_pages_map(const int *lens, const int *add, int n, int *tables, int max_pages, int *held,
                   int *free_pages, int *free_count, int capacity, int page_tokens,
                   int64_t *slots, int *positions, int64_t max_tokens, int *starts, int *totals,
@@ -508,9 +509,9 @@ int pkv_pages_attend(int quant, const float *q, int64_t q_stride_t, int64_t q_st
  * one whose running sum exceeds u[k] times the whole sum, in 64 bits; -1 for a row without
  * weight. tokens: [n, k + 1], the accepted drafts, that token, then -1; accepted: [n]. k at most
  * 63, n at most 65535 (else PKV_ERR_UNSUPPORTED). workspace: at least
- * pkv_verify_drafts_workspace(n) bytes of device memory, 8-byte aligned, which the call writes:
+ * pkv_verify_drafts_workspace(n, vocab) bytes of device memory, 8-byte aligned, which the call writes:
  * calls that overlap in time, and graphs that do, need one each. */
-size_t pkv_verify_drafts_workspace(int n);
+size_t pkv_verify_drafts_workspace(int n, int vocab);
 int pkv_verify_drafts(const float *target, int64_t target_stride, const float *draft,
                       int64_t draft_stride, const int *drafts, const int *n_drafts, const float *u,
                       int n, int k, int vocab, int *tokens, int *accepted, void *workspace,

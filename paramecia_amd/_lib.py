@@ -178,7 +178,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "pkv_pages_attend_workspace": ([c_int, c_i64] + [c_int] * 3, c_sz),
         "pkv_pages_attend": ([c_int, vp, c_i64, c_i64, vp, vp, c_int, c_int, vp, c_int, vp, vp, c_int, c_i64] +
                              [c_int] * 3 + [fl, c_int, c_int, vp, vp, c_sz, vp], c_int),
-        "pkv_verify_drafts_workspace": ([c_int], c_sz),
+        "pkv_verify_drafts_workspace": ([c_int, c_int], c_sz),
         "pkv_verify_drafts": ([vp, c_i64, vp, c_i64] + [vp] * 3 + [c_int] * 3 + [vp] * 3 + [c_sz, vp], c_int),
     }
     for name, (args, res) in sig.items():

@@ -330,7 +330,7 @@ struct PagesAttend {
 };
 size_t pages_attend_workspace(int n, int64_t tokens, int heads, int kv_heads, int head_dim);
 int launch_pages_attend(const PagesAttend &p, void *ws, hipStream_t s);
-size_t verify_drafts_workspace(int n);
+size_t verify_drafts_workspace(int n, int vocab);
 int launch_verify_drafts(const float *target, int64_t target_row, const float *draft,
                          int64_t draft_row, const int *drafts, const int *counts, const float *u,
                          int n, int k, int vocab, int *tokens, int *accepted, void *ws,

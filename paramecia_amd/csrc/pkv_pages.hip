@@ -11,7 +11,6 @@
 namespace pkv {
 namespace {
 
-constexpr int kMapThreads = 1024, kMapWaves = kMapThreads / 64;
 // Tokens up to which the mapping workgroup writes the slots itself; more are left to a launch
 // of their own.
 constexpr int64_t kMapTokensInline = 4096;
@@ -48,26 +47,34 @@ __device__ __forceinline__ Request request(const MapArgs &a, int b) {
   return r;
 }
 
-// Exclusive sum of x over the workgroup's threads, and the sum. part: one word per wave.
-__device__ __forceinline__ int64_t scan_exclusive(int64_t x, int64_t *part, int64_t &sum) {
+// Pages given, pages taken and tokens added, summed together. (A table holds fewer than 2^31 pages
+// in all; the tokens of a step that is refused may pass 32 bits.)
+struct Sums {
+  int give, take;
+  int64_t add;
+  __device__ __forceinline__ Sums operator+(const Sums &o) const { return {give + o.give, take + o.take, add + o.add}; }
+  __device__ __forceinline__ Sums operator-(const Sums &o) const { return {give - o.give, take - o.take, add - o.add}; }
+};
+// Exclusive sums over the workgroup's threads, and the sums. part: an entry per wave.
+template <int kThreads>
+__device__ __forceinline__ Sums scan_exclusive(const Sums &x, Sums *part, Sums &sum) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t y = x;
+  Sums y = x;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t z = __shfl_up(y, o);
-    if (lane >= o) y += z;
+    const Sums z = {__shfl_up(y.give, o), __shfl_up(y.take, o), __shfl_up(y.add, o)};
+    if (lane >= o) y = y + z;
   }
-  __syncthreads();  // the words' previous readers are done
+  __syncthreads();  // the entries' previous readers are done
   if (lane == 63) part[wave] = y;
   __syncthreads();
-  int64_t before = 0, all = 0;
+  Sums before = {0, 0, 0};
+  sum = {0, 0, 0};
 #pragma unroll
-  for (int w = 0; w < kMapWaves; ++w) {
-    const int64_t p = part[w];
-    before += w < wave ? p : 0;
-    all += p;
+  for (int w = 0; w < kThreads / 64; ++w) {
+    if (w < wave) before = before + part[w];
+    sum = sum + part[w];
   }
-  sum = all;
   return before + y - x;
 }
 
@@ -93,102 +100,104 @@ __device__ __forceinline__ void write_slot(const MapArgs &a, const Starts &start
 }
 
 // One workgroup: the requests' needs and their sums, then (if the step fits) the pages that
-// come back onto the free stack, request by request, then the pages taken from its top. A wave
-// moves the pages of its requests one request at a time, a lane a page.
-__global__ __launch_bounds__(kMapThreads) void pages_map_kernel(MapArgs a) {
-  __shared__ int64_t part[kMapWaves];
+// come back onto the free stack, request by request, then the pages taken from its top. A lane
+// moves the few pages of its request; those of a request that moves more its whole wave, a lane a
+// page. Bound: the chain of its loads and barriers.
+constexpr int kLanePages = 4;
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void pages_map_kernel(MapArgs a) {
+  __shared__ Sums part[kThreads / 64];
   __shared__ int s_starts[kStartsInLds + 1];
-  __shared__ int s_bad;
   const int tid = threadIdx.x, lane = tid & 63;
   const bool staged = a.n <= kStartsInLds;
-  if (tid == 0) s_bad = 0;
   const int count = *a.free_count;
-  const bool one = a.n <= kMapThreads;  // each thread keeps its request
-  int64_t give = 0, take = 0, add = 0;
-  Request mine = request(a, tid);
-  bool bad = mine.bad;
-  for (int b = tid; b < a.n; b += kMapThreads) {
+  const bool one = a.n <= kThreads;  // each thread keeps its request
+  const Request mine = request(a, tid);
+  Sums own = {0, 0, 0};
+  bool bad = false;
+  for (int b = tid; b < a.n; b += kThreads) {
     const Request r = b == tid ? mine : request(a, b);
     bad |= r.bad;
-    give += r.give;
-    take += r.take;
-    add += r.add;
+    own = own + Sums{r.give, r.take, r.bad ? 0 : r.add};
   }
-  int64_t gives, takes, adds;
-  const int64_t give0 = scan_exclusive(give, part, gives);
-  if (bad) s_bad = 1;
-  const int64_t take0 = scan_exclusive(take, part, takes);
-  const int64_t add0 = scan_exclusive(add, part, adds);
-  const int64_t height = (int64_t)count + gives;
-  const bool valid = s_bad == 0 && adds <= a.max_tokens && count >= 0 && count <= a.capacity;
+  // a request that does not fit counts as more tokens than a step holds
+  if (bad) own.add = a.max_tokens + 1;
+  Sums all;
+  const Sums first = scan_exclusive<kThreads>(own, part, all);
+  const int64_t height = (int64_t)count + all.give;
+  const bool valid = all.add <= a.max_tokens && count >= 0 && count <= a.capacity;
   // (pages that come back make the stack higher than its memory only if they were never its own)
-  const bool fits = takes <= height && height <= a.capacity;
-  const bool ok = valid && fits;
+  const bool ok = valid && all.take <= height && height <= a.capacity;
   if (tid == 0) {
-    *a.status = ok ? PKV_OK : valid && takes > height ? PKV_ERR_OVERFLOW : PKV_ERR_ARG;
-    a.starts[a.n] = ok ? (int)adds : 0;
-    if (staged) s_starts[a.n] = ok ? (int)adds : 0;
-    if (ok) *a.free_count = (int)(height - takes);
+    *a.status = ok ? PKV_OK : valid && all.take > height ? PKV_ERR_OVERFLOW : PKV_ERR_ARG;
+    a.starts[a.n] = ok ? (int)all.add : 0;
+    if (staged) s_starts[a.n] = ok ? (int)all.add : 0;
   }
-  // what a wave's lanes' requests move, one after the other
+  // the pages of the wave's requests: back onto the stack from `at` on, or off it down from `at`
   const auto move = [&](const Request &r, int b, int64_t at, bool back) {
-    uint64_t todo = __ballot(back ? r.give > 0 : r.take > 0);
+    const int m = back ? r.give : r.take;
+    int *row = a.tables + (int64_t)b * a.max_pages + (back ? r.need : r.held);
+    if (m <= kLanePages) {
+#pragma unroll
+      for (int j = 0; j < kLanePages; ++j) {
+        if (j >= m) continue;
+        if (back) a.free_pages[at + j] = row[j];
+        else row[j] = a.free_pages[at - j];
+      }
+    }
+    uint64_t todo = __ballot(m > kLanePages);
     while (todo) {
       const int from = __builtin_ctzll(todo);
       todo &= todo - 1;
-      const int m = __shfl(back ? r.give : r.take, from);
-      const int first = __shfl(back ? r.need : r.held, from);
+      const int many = __shfl(m, from), head = __shfl(back ? r.need : r.held, from);
       const int64_t base = __shfl(at, from);
-      int *row = a.tables + (int64_t)__shfl(b, from) * a.max_pages + first;
-      for (int j = lane; j < m; j += 64) {
-        if (back) a.free_pages[base + j] = row[j];
-        else row[j] = a.free_pages[base - j];
+      int *of = a.tables + (int64_t)__shfl(b, from) * a.max_pages + head;
+      for (int j = lane; j < many; j += 64) {
+        if (back) a.free_pages[base + j] = of[j];
+        else of[j] = a.free_pages[base - j];
       }
     }
   };
   if (!ok) {
-    for (int b = tid; b < a.n; b += kMapThreads) {
+    for (int b = tid; b < a.n; b += kThreads) {
       a.totals[b] = a.lens[b];
       a.starts[b] = 0;
       if (staged) s_starts[b] = 0;
     }
   } else {
-    int64_t g = 0, s = 0;
-    for (int b0 = 0; b0 < a.n; b0 += kMapThreads) {
+    Sums run = {0, 0, 0};
+    for (int b0 = 0; b0 < a.n; b0 += kThreads) {
       const int b = b0 + tid;
       const Request r = one ? mine : request(a, b);
-      int64_t gat = give0, sat = add0, gs = 0, ss = 0;
-      if (!one) {
-        gat = g + scan_exclusive(r.give, part, gs);
-        sat = s + scan_exclusive(r.add, part, ss);
-      }
+      Sums at = first, sum = {0, 0, 0};
+      if (!one) at = run + scan_exclusive<kThreads>({r.give, r.take, r.add}, part, sum);
       if (b < a.n) {
         a.totals[b] = (int)r.total;
-        a.starts[b] = (int)sat;
-        if (staged) s_starts[b] = (int)sat;
+        a.starts[b] = (int)at.add;
+        if (staged) s_starts[b] = (int)at.add;
       }
-      if (gives) move(r, b, count + gat, true);
-      g += gs;
-      s += ss;
+      if (all.give) move(r, b, count + (int64_t)at.give, true);
+      run = run + sum;
     }
-    __syncthreads();  // what came back lies on the stack
-    int64_t t = 0;
-    for (int b0 = 0; b0 < a.n; b0 += kMapThreads) {
+    __syncthreads();  // what came back lies on the stack, and its height was read by all
+    run = {0, 0, 0};
+    for (int b0 = 0; b0 < a.n; b0 += kThreads) {
       const int b = b0 + tid;
       const Request r = one ? mine : request(a, b);
-      int64_t tat = take0, ts = 0;
-      if (!one) tat = t + scan_exclusive(r.take, part, ts);
-      if (takes) move(r, b, height - 1 - tat, false);
+      Sums at = first, sum = {0, 0, 0};
+      if (!one) at = run + scan_exclusive<kThreads>({r.give, r.take, r.add}, part, sum);
+      if (all.take) move(r, b, height - 1 - at.take, false);
       if (b < a.n) a.held[b] = r.need;  // its only reader from here on is this thread
-      t += ts;
+      run = run + sum;
     }
+    if (tid == 0) *a.free_count = (int)(height - all.take);
   }
   if (!a.fill) return;
   __syncthreads();
   if (staged) {
-    for (int64_t i = tid; i < a.max_tokens; i += kMapThreads) write_slot(a, s_starts, i);
+    for (int64_t i = tid; i < a.max_tokens; i += kThreads) write_slot(a, s_starts, i);
   } else {
-    for (int64_t i = tid; i < a.max_tokens; i += kMapThreads) write_slot(a, a.starts, i);
+    for (int64_t i = tid; i < a.max_tokens; i += kThreads) write_slot(a, a.starts, i);
   }
 }
 
@@ -275,7 +284,11 @@ int launch_pages_map(const int *lens, const int *add, int n, int *tables, int ma
   a.capacity = capacity;
   a.page_lg = __builtin_ctz((unsigned)page_tokens);
   a.fill = max_tokens <= kMapTokensInline;
-  hipLaunchKernelGGL(pages_map_kernel, dim3(1), dim3(kMapThreads), 0, s, a);
+  // few requests and rows: fewer waves, whose barriers are shorter
+  if (n <= 256 && max_tokens <= 1024)
+    hipLaunchKernelGGL(pages_map_kernel<256>, dim3(1), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(pages_map_kernel<1024>, dim3(1), dim3(1024), 0, s, a);
   if (!a.fill)
     hipLaunchKernelGGL(pages_slots_kernel, dim3((unsigned)((max_tokens + 255) / 256)), dim3(256), 0, s, a);
   PKV_HIP(hipGetLastError());

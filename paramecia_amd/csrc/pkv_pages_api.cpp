@@ -47,6 +47,8 @@ int pkv_pages_map(const int *lens, const int *add, int n, int *tables, int max_p
   if (!page_size(page_tokens)) return refuse_page_size();
   if (max_tokens < 0 || max_tokens >= kMost32)
     return set_error(PKV_ERR_ARG, "max_tokens must be in [0, 2^31)");
+  if ((int64_t)n * max_pages >= kMost32)
+    return set_error(PKV_ERR_UNSUPPORTED, "the tables must hold fewer than 2^31 pages");
   if (!lens || !add || !tables || !held || !free_pages || !free_count || !starts || !totals ||
       !status || (max_tokens && (!slots || !positions)))
     return set_error(PKV_ERR_ARG, "null argument");
@@ -165,7 +167,9 @@ int pkv_pages_attend(int quant, const float *q, int64_t q_stride_t, int64_t q_st
   return launch_pages_attend(p, workspace, static_cast<hipStream_t>(stream));
 }
 
-size_t pkv_verify_drafts_workspace(int n) { return n > 0 ? verify_drafts_workspace(n) : 0; }
+size_t pkv_verify_drafts_workspace(int n, int vocab) {
+  return n > 0 && vocab > 0 ? verify_drafts_workspace(n, vocab) : 0;
+}
 
 int pkv_verify_drafts(const float *target, int64_t target_stride, const float *draft,
                       int64_t draft_stride, const int *drafts, const int *n_drafts, const float *u,
@@ -178,14 +182,14 @@ int pkv_verify_drafts(const float *target, int64_t target_stride, const float *d
     return set_error(PKV_ERR_ARG, "null argument");
   if (target_stride < vocab || (k && draft && draft_stride < vocab))
     return set_error(PKV_ERR_ARG, "rows of probabilities do not overlap");
-  if (workspace_bytes < verify_drafts_workspace(n) || (reinterpret_cast<uintptr_t>(workspace) & 7) != 0)
+  if (workspace_bytes < verify_drafts_workspace(n, vocab) || (reinterpret_cast<uintptr_t>(workspace) & 7) != 0)
     return set_error(PKV_ERR_ARG, "the workspace must hold pkv_verify_drafts_workspace() bytes, 8-byte aligned");
   const uint64_t rows = (uint64_t)n * (k + 1);
   if (clash({{target, 4 * ((rows - 1) * (uint64_t)target_stride + vocab), false},
              {draft, k && draft ? 4 * (((uint64_t)n * k - 1) * (uint64_t)draft_stride + vocab) : 0, false},
              {drafts, 4 * (uint64_t)n * k, false}, {n_drafts, 4 * (uint64_t)n, false}, {u, 4 * rows, false},
              {tokens, 4 * rows, true}, {accepted, 4 * (uint64_t)n, true},
-             {workspace, verify_drafts_workspace(n), true}}))
+             {workspace, verify_drafts_workspace(n, vocab), true}}))
     return set_error(PKV_ERR_ARG, "tokens, accepted and the workspace must not overlap another buffer");
   return launch_verify_drafts(target, target_stride, draft, draft_stride, drafts, n_drafts, u, n, k,
                               vocab, tokens, accepted, workspace, static_cast<hipStream_t>(stream));

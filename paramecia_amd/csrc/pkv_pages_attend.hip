@@ -160,7 +160,20 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int ro
     const int mine = (int)(((int64_t)fresh * a.group + rows_per_tile - 1) / rows_per_tile);
     int64_t sum;
     const int64_t at = tiles + plan_scan(mine, part, sum);
-    for (int i = 0; i < mine && at + i < a.max_tiles; ++i) a.tiles[at + i].b = b, a.tiles[at + i].row0 = i;
+    // a lane names the few tiles of its request; those of a longer one its whole wave
+    const auto name = [&](int64_t t, int of, int i) {
+      if (t < a.max_tiles) a.tiles[t].b = of, a.tiles[t].row0 = i;
+    };
+    if (mine <= 4)
+      for (int i = 0; i < mine; ++i) name(at + i, b, i);
+    uint64_t todo = __ballot(mine > 4);
+    while (todo) {
+      const int from = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      const int many = __shfl(mine, from), of = __shfl(b, from);
+      const int64_t base = __shfl(at, from);
+      for (int i = tid & 63; i < many; i += 64) name(base + i, of, i);
+    }
     tiles += sum;
   }
   // (starts that run backwards could name more tiles than the step has rows for)
@@ -771,10 +784,9 @@ __device__ __forceinline__ int this_lane() {
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x406); }
 
 template <bool kBf, int kD, int kW, int kRT>
-__global__ __launch_bounds__(64 * kW) void many_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2) void many_kernel(AttendArgs a) {
   constexpr int kThreads = 64 * kW, kRows = 16 * kW * kRT, kSteps = kD / 32, kCols = kD / 16, kP = kParts<kBf>;
   constexpr int kMoves = 4 * kD / kThreads;  // 16-byte pieces of K, and of V, that a thread moves
-  static_assert(kMoves >= 1, "");
   __shared__ __attribute__((aligned(1024))) uint16_t lk[3][kBlk * kD], lv[3][kBlk * kD];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1191,8 +1203,7 @@ int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
     if (sh.rows < 128) {
       few<kBf, kD, false>(a, sh, s);
     } else {
-      hipLaunchKernelGGL((many_kernel<kBf, kD, (kD == 256 ? 8 : 4), (kD == 256 ? 1 : 2)>), dim3(sh.shares),
-                         dim3(kD == 256 ? 512 : 256), 0, s, a);
+      hipLaunchKernelGGL((many_kernel<kBf, kD, (kD > 64 ? 8 : 4), (kD > 64 ? 1 : 2)>), dim3(sh.shares), dim3(kD > 64 ? 512 : 256), 0, s, a);
       join<kD, false>(a, sh, s);
     }
   }

@@ -10,23 +10,26 @@
 // (f32); products, differences and sums are taken in 64 bits, since a sum's border decides on a
 // token and a vocabulary's f32 sum is off by more than a token's probability.
 //
-// Bound: one or two rows of the vocabulary a sequence (0.6 MB each), so a row is summed by
-// kParts workgroups (the first launch); the second finds the part, then the token.
+// Bound: one or two rows of the vocabulary a sequence (0.6 MB each), and two dependent loads (the
+// drafts, then their probabilities) in front of them. The first launch sums every 256 elements of the
+// rows, a wave four such chunks at once; the second, a workgroup a sequence, finds the chunk among
+// their sums and the token among its elements.
 #include "pkv_internal.hpp"
 
 namespace pkv {
 namespace {
 
 constexpr int kVThreads = 256, kVWaves = kVThreads / 64;
-constexpr int kParts = 32;
+constexpr int kChunk = 256;  // elements: four a lane
+constexpr int kWaveChunks = 4, kPart = kChunk * kWaveChunks * kVWaves;  // of a workgroup of the first launch
 
 struct VerifyArgs {
   const float *target, *draft, *u;
   const int *drafts, *counts;
   int *tokens, *accepted;
-  double *sums;  // [n][kParts][2]: of the rest, of the row itself
+  double *sums;  // [n][chunks]: of the rest
   int64_t target_row, draft_row;  // elements between rows
-  int n, k, vocab, run;  // run: elements that one thread of a part sums
+  int n, k, vocab, chunks;
 };
 
 // The first rejected draft of sequence b (its count if none is), the same in every lane.
@@ -51,16 +54,10 @@ __device__ __forceinline__ int first_rejected(const VerifyArgs &a, int b, int &c
   return __builtin_amdgcn_readfirstlane(first < count ? first : count);
 }
 
-// What is left of the row behind the accepted drafts: p, and q where a draft was rejected.
+// What is left of the row behind the accepted drafts: p, less q where a draft was rejected.
 struct Rest {
   const float *p, *q;
   int gone;  // the rejected token where the draft was sure of it, else -1
-  // (NaN is no probability: it weighs nothing)
-  __device__ __forceinline__ double raw(float x) const { return x > 0.0f ? (double)x : 0.0; }
-  __device__ __forceinline__ double at(int i, float x, float y) const {
-    const double d = (double)x - (q ? (double)y : i == gone ? 1.0 : 0.0);
-    return d > 0.0 ? d : 0.0;
-  }
 };
 __device__ __forceinline__ Rest rest_of(const VerifyArgs &a, int b, int row, int count) {
   Rest r;
@@ -70,129 +67,151 @@ __device__ __forceinline__ Rest rest_of(const VerifyArgs &a, int b, int row, int
   r.gone = rejected && !a.draft ? a.drafts[(int64_t)b * a.k + row] : -1;
   return r;
 }
-
-// f(i, p_i, q_i) for i in [first, end), in order, with kMost loads in flight.
-template <typename F>
-__device__ __forceinline__ void walk(const Rest &r, int first, int end, F f) {
-  constexpr int kMost = 8;
-  for (int i = first; i < end; i += kMost) {
-    float x[kMost], y[kMost];
+// The lane's four elements of a chunk (zeros behind the row's end); rows begin at any multiple of 4 bytes.
+struct Four {
+  float x[4];
+} __attribute__((packed, aligned(4)));
+__device__ __forceinline__ Four four(const float *row, int64_t first, int vocab) {
+  Four f = {{0.0f, 0.0f, 0.0f, 0.0f}};
+  if (first + 4 <= vocab) {
+    f = *reinterpret_cast<const Four *>(row + first);
+  } else {
 #pragma unroll
-    for (int j = 0; j < kMost; ++j) x[j] = r.p[i + j < end ? i + j : end - 1];
+    for (int i = 0; i < 4; ++i)
+      if (first + i < vocab) f.x[i] = row[first + i];
+  }
+  return f;
+}
+// Their weights: max(p - q, 0), or p alone. (NaN is no probability: it weighs nothing.)
+__device__ __forceinline__ void weigh(const Rest &r, int64_t first, const Four &p, const Four &q, double (&w)[4]) {
 #pragma unroll
-    for (int j = 0; j < kMost; ++j) y[j] = r.q ? r.q[i + j < end ? i + j : end - 1] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < kMost; ++j)
-      if (i + j < end) f(i + j, x[j], y[j]);
+  for (int i = 0; i < 4; ++i) {
+    const double d = (double)p.x[i] - (r.q ? (double)q.x[i] : first + i == r.gone ? 1.0 : 0.0);
+    w[i] = d > 0.0 ? d : 0.0;
   }
 }
-
-// Exclusive sum over the workgroup, and the sum.
-__device__ __forceinline__ double scan_exclusive(double x, double *part, double &sum) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double y = x;
+__device__ __forceinline__ double wave_total(double x) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ __forceinline__ double wave_running(double x) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const double z = __shfl_up(y, o);
-    if (lane >= o) y += z;
+    const double z = __shfl_up(x, o);
+    if (lane >= o) x += z;
   }
-  __syncthreads();
-  if (lane == 63) part[wave] = y;
-  __syncthreads();
-  double before = 0.0, all = 0.0;
-#pragma unroll
-  for (int w = 0; w < kVWaves; ++w) {
-    before += w < wave ? part[w] : 0.0;
-    all += part[w];
-  }
-  const double up = __shfl_up(y, 1);
-  sum = all;
-  return before + (lane ? up : 0.0);
+  return x;
 }
 
 __global__ __launch_bounds__(kVThreads) void verify_sums_kernel(VerifyArgs a) {
-  __shared__ double part[kVWaves];
-  const int b = blockIdx.y;
+  const int b = blockIdx.y, lane = threadIdx.x & 63;
   int count;
   const int row = first_rejected(a, b, count);
   const Rest r = rest_of(a, b, row, count);
-  const int64_t at = ((int64_t)blockIdx.x * kVThreads + threadIdx.x) * a.run;
-  const int first = at < a.vocab ? (int)at : a.vocab;
-  const int end = at + a.run < a.vocab ? (int)(at + a.run) : a.vocab;
-  double rest = 0.0, raw = 0.0;
-  walk(r, first, end, [&](int i, float x, float y) {
-    rest += r.at(i, x, y);
-    raw += r.raw(x);
-  });
-  double rests, raws;
-  scan_exclusive(rest, part, rests);
-  scan_exclusive(raw, part, raws);
-  if (threadIdx.x == 0) {
-    double *o = a.sums + ((int64_t)b * kParts + blockIdx.x) * 2;
-    o[0] = rests;
-    o[1] = raws;
+  const int chunk = ((int)blockIdx.x * kVWaves + (int)(threadIdx.x >> 6)) * kWaveChunks;
+  Four p[kWaveChunks], q[kWaveChunks];
+#pragma unroll
+  for (int c = 0; c < kWaveChunks; ++c) p[c] = four(r.p, (int64_t)(chunk + c) * kChunk + 4 * lane, a.vocab);
+  if (r.q) {
+#pragma unroll
+    for (int c = 0; c < kWaveChunks; ++c) q[c] = four(r.q, (int64_t)(chunk + c) * kChunk + 4 * lane, a.vocab);
+  }
+#pragma unroll
+  for (int c = 0; c < kWaveChunks; ++c) {
+    double w[4];
+    weigh(r, (int64_t)(chunk + c) * kChunk + 4 * lane, p[c], q[c], w);
+    const double sum = wave_total((w[0] + w[1]) + (w[2] + w[3]));
+    if (lane == 0 && chunk + c < a.chunks) a.sums[(int64_t)b * a.chunks + chunk + c] = sum;
   }
 }
 
+// A row's running sums over a workgroup's threads, each with elements [first, end) of `count`,
+// whose values value(i) gives: where the sum first passes u times the whole, or, where rounding or a u
+// of one leaves none, the last with weight; -1 without any. `before`: the sum in front of it.
+template <typename Value>
+__device__ __forceinline__ int pick(int count, float u, Value value, double &bar, double &before) {
+  __shared__ double s_sum[kVWaves], s_before[kVWaves + 1];
+  __shared__ int s_first[kVWaves], s_last[kVWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (count + kVThreads - 1) / kVThreads;
+  const int64_t at = (int64_t)tid * per;
+  const int first = at < count ? (int)at : count, end = at + per < count ? (int)at + per : count;
+  double sum = 0.0;
+  for (int i = first; i < end; ++i) sum += value(i);
+  const double run = wave_running(sum);
+  if (lane == 63) s_sum[wave] = run;
+  __syncthreads();
+  double start = 0.0, all = 0.0;
+#pragma unroll
+  for (int w = 0; w < kVWaves; ++w) {
+    start += w < wave ? s_sum[w] : 0.0;
+    all += s_sum[w];
+  }
+  bar = (double)u * all;
+  double s = start + (run - sum), held = s;
+  int hit = -1, last = -1;
+  for (int i = first; i < end; ++i) {
+    const double w = value(i);
+    if (hit < 0 && w > 0.0) {
+      if (s + w > bar) hit = i;
+      last = i;
+      held = s;
+    }
+    s += w;
+  }
+  const uint64_t hits = __ballot(hit >= 0), some = __ballot(last >= 0);
+  const int from = hits ? __builtin_ctzll(hits) : some ? 63 - __builtin_clzll(some) : 0;
+  const int mine = __shfl(hit >= 0 ? hit : last, from);
+  const double mine_before = __shfl(held, from);
+  if (lane == 0) {
+    s_first[wave] = hits ? mine : -1;
+    s_last[wave] = mine;
+    s_before[wave] = mine_before;
+  }
+  __syncthreads();
+  int got = -1;
+  before = 0.0;
+  for (int w = kVWaves - 1; w >= 0; --w)
+    if (got < 0 && s_last[w] >= 0) got = s_last[w], before = s_before[w];
+  for (int w = kVWaves - 1; w >= 0; --w)
+    if (s_first[w] >= 0) got = s_first[w], before = s_before[w];
+  return got;
+}
+
 __global__ __launch_bounds__(kVThreads) void verify_pick_kernel(VerifyArgs a) {
-  __shared__ double part[kVWaves];
-  __shared__ int s_token;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   int count;
   const int row = first_rejected(a, b, count);
   const Rest r = rest_of(a, b, row, count);
-  // the part whose running sum first exceeds u times the whole: every lane of a wave holds one
-  double rest = lane < kParts ? a.sums[((int64_t)b * kParts + lane) * 2] : 0.0;
-  const double raw = lane < kParts ? a.sums[((int64_t)b * kParts + lane) * 2 + 1] : 0.0;
-  const bool left = __any(rest > 0.0);
-  if (!left) rest = raw;  // nothing is left where p and q are the same: p itself
-  double run = rest;
+  const float u = a.u[(int64_t)b * (a.k + 1) + a.k];
+  const double *sums = a.sums + (int64_t)b * a.chunks;
+  double bar, before;
+  const int chunk = pick(a.chunks, u, [&](int i) { return sums[i]; }, bar, before);
+  int token = -1;
+  if (chunk >= 0) {
+    const int64_t first = (int64_t)chunk * kChunk + 4 * lane;
+    Four q = {{0.0f, 0.0f, 0.0f, 0.0f}};
+    if (r.q) q = four(r.q, first, a.vocab);
+    double w[4];
+    weigh(r, first, four(r.p, first, a.vocab), q, w);
+    const double own = (w[0] + w[1]) + (w[2] + w[3]);
+    double s = before + (wave_running(own) - own);
+    int hit = -1, last = -1;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double z = __shfl_up(run, o);
-    if (lane >= o) run += z;
-  }
-  const double bar = (double)a.u[(int64_t)b * (a.k + 1) + a.k] * __shfl(run, 63);
-  // rounding, or a u of one, may leave no running sum above the bar: the last part with weight
-  const uint64_t over = __ballot(lane < kParts && run > bar && rest > 0.0), some = __ballot(rest > 0.0);
-  const int mine = over ? __builtin_ctzll(over) : some ? 63 - __builtin_clzll(some) : -1;
-  const double before = __shfl(run - rest, mine < 0 ? 0 : mine);
-  if (tid == 0) s_token = -1;
-  if (mine >= 0) {
-    const int64_t at = ((int64_t)mine * kVThreads + tid) * a.run;
-    const int first = at < a.vocab ? (int)at : a.vocab;
-    const int end = at + a.run < a.vocab ? (int)(at + a.run) : a.vocab;
-    double sum = 0.0, all;
-    walk(r, first, end, [&](int i, float x, float y) { sum += left ? r.at(i, x, y) : r.raw(x); });
-    const double s0 = before + scan_exclusive(sum, part, all);
-    // the first thread whose own sums pass the bar; without one the last that has weight
-    double s = s0;
-    int token = -1, last = -1;
-    walk(r, first, end, [&](int i, float x, float y) {
-      const double w = left ? r.at(i, x, y) : r.raw(x);
-      s += w;
-      if (w > 0.0) last = i;
-      if (token < 0 && w > 0.0 && s > bar) token = i;
-    });
-    __shared__ int s_first[kVWaves], s_last[kVWaves];
-    const uint64_t hit = __ballot(token >= 0), any = __ballot(last >= 0);
-    const int f = __shfl(token, hit ? __builtin_ctzll(hit) : 0), l = __shfl(last, any ? 63 - __builtin_clzll(any) : 0);
-    if (lane == 0) {
-      s_first[tid >> 6] = hit ? f : -1;
-      s_last[tid >> 6] = any ? l : -1;
+    for (int i = 0; i < 4; ++i) {
+      s += w[i];
+      if (w[i] > 0.0) last = (int)first + i;
+      if (hit < 0 && w[i] > 0.0 && s > bar) hit = (int)first + i;
     }
+    const uint64_t hits = __ballot(hit >= 0), some = __ballot(last >= 0);
+    token = hits ? __shfl(hit, __builtin_ctzll(hits)) : some ? __shfl(last, 63 - __builtin_clzll(some)) : -1;
+  } else if (row < count) {
+    // nothing is left where q is nowhere below p: p itself, element by element
     __syncthreads();
-    if (tid == 0) {
-      int t = -1;
-      for (int w = 0; w < kVWaves; ++w)
-        if (t < 0) t = s_first[w];
-      for (int w = kVWaves - 1; w >= 0; --w)
-        if (t < 0) t = s_last[w];
-      s_token = t;
-    }
+    token = pick(a.vocab, u, [&](int i) { return r.p[i] > 0.0f ? (double)r.p[i] : 0.0; }, bar, before);
   }
-  __syncthreads();
-  const int token = s_token;
   if (tid <= a.k) {
     const int64_t o = (int64_t)b * (a.k + 1) + tid;
     a.tokens[o] = tid < row ? a.drafts[(int64_t)b * a.k + tid] : tid == row ? token : -1;
@@ -202,7 +221,7 @@ __global__ __launch_bounds__(kVThreads) void verify_pick_kernel(VerifyArgs a) {
 
 }  // namespace
 
-size_t verify_drafts_workspace(int n) { return (size_t)n * kParts * 2 * sizeof(double); }
+size_t verify_drafts_workspace(int n, int vocab) { return (size_t)n * (((size_t)vocab + kChunk - 1) / kChunk) * sizeof(double); }
 
 int launch_verify_drafts(const float *target, int64_t target_row, const float *draft,
                          int64_t draft_row, const int *drafts, const int *counts, const float *u,
@@ -222,8 +241,8 @@ int launch_verify_drafts(const float *target, int64_t target_row, const float *d
   a.n = n;
   a.k = k;
   a.vocab = vocab;
-  a.run = (vocab + kParts * kVThreads - 1) / (kParts * kVThreads);
-  hipLaunchKernelGGL(verify_sums_kernel, dim3(kParts, n), dim3(kVThreads), 0, s, a);
+  a.chunks = (int)(((int64_t)vocab + kChunk - 1) / kChunk);
+  hipLaunchKernelGGL(verify_sums_kernel, dim3((unsigned)(((int64_t)vocab + kPart - 1) / kPart), n), dim3(kVThreads), 0, s, a);
   hipLaunchKernelGGL(verify_pick_kernel, dim3(n), dim3(kVThreads), 0, s, a);
   PKV_HIP(hipGetLastError());
   return PKV_OK;

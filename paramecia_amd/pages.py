@@ -8,6 +8,7 @@ qwen3_next.rs: append_quantized :431-509, the SDPA :2492-2605, truncate and chec
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -17,6 +18,16 @@ from ._lib import lib
 from .kv_cache import KvCacheError, _at, _call, _device, _stream, _take
 
 _PAGES = {torch.float16: _lib.QUANT_F16, torch.bfloat16: _lib.QUANT_BF16}
+
+
+@functools.lru_cache(maxsize=256)
+def _attend_bytes(n: int, tokens: int, heads: int, kv_heads: int, dim: int) -> int:
+    return lib().pkv_pages_attend_workspace(n, tokens, heads, kv_heads, dim)
+
+
+@functools.lru_cache(maxsize=256)
+def _verify_bytes(n: int, vocab: int) -> int:
+    return lib().pkv_verify_drafts_workspace(n, vocab)
 
 
 class PageMap(NamedTuple):
@@ -51,8 +62,9 @@ def map_pages(lens: torch.Tensor, add: torch.Tensor, tables: torch.Tensor, held:
     if out is None:
         if max_tokens < 0:
             raise KvCacheError("map_pages: max_tokens must be >= 0")
-        new = lens.new_empty
-        out = PageMap(new(max_tokens, dtype=torch.int64), new(max_tokens), new(n + 1), new(n), new(1))
+        slots, positions, starts, totals, status = lens.new_empty(3 * max_tokens + 2 * n + 2).split_with_sizes(
+            (2 * max_tokens, max_tokens, n + 1, n, 1))
+        out = PageMap(slots.view(torch.int64), positions, starts, totals, status)
     else:
         for t, name, size, dtype in zip(out, PageMap._fields, (max_tokens, max_tokens, n + 1, n, 1),
                                         (torch.int64, i32, i32, i32, i32)):
@@ -126,7 +138,7 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         out = (torch.empty if starts is None else torch.zeros)((tokens, heads, dim), dtype=torch.float32, device=q.device)
     else:
         _take(out, "out", (tokens, heads, dim), dev, writes=True)
-    need = lib().pkv_pages_attend_workspace(n, tokens, heads, kv_heads, dim)
+    need = _attend_bytes(n, tokens, heads, kv_heads, dim)
     # torch's allocator orders the workspace with the stream, and gives each graph its own
     ws = out.new_empty(need, dtype=torch.uint8) if need else None
     _call(lib().pkv_pages_attend(quant, q.data_ptr(), st, sh, k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
@@ -154,7 +166,7 @@ def verify_drafts(target_probs: torch.Tensor, drafts: torch.Tensor, uniforms: to
     uniforms = _take(uniforms, "uniforms", (n, rows), dev)
     n_drafts = _take(n_drafts, "n_drafts", (n,), dev, torch.int32)
     tokens, accepted = drafts.new_empty((n, rows)), drafts.new_empty(n)
-    need = lib().pkv_verify_drafts_workspace(n)
+    need = _verify_bytes(n, vocab)
     ws = drafts.new_empty(need, dtype=torch.uint8) if need else None
     _call(lib().pkv_verify_drafts(target_probs.data_ptr(), vocab, _at(draft_probs), vocab, drafts.data_ptr(),
                                   _at(n_drafts), uniforms.data_ptr(), n, k, vocab, tokens.data_ptr(),

@@ -32,6 +32,7 @@ def pages_map(**k):
     (dict(n=0), ERR_ARG, "n, max_pages"), (dict(mp=0), ERR_ARG, "max_pages"), (dict(cap=0), ERR_ARG, "capacity"),
     (dict(page=16), ERR_ARG, "power of two"), (dict(page=96), ERR_ARG, "power of two"), (dict(page=1 << 21), ERR_ARG, "power of two"),
     (dict(mt=-1), ERR_ARG, "max_tokens"), (dict(mt=1 << 31), ERR_ARG, "max_tokens"),
+    (dict(mp=1 << 29), ERR_UNSUPPORTED, "2^31 pages"),
     (dict(totals=A), ERR_ARG, "overlap"), (dict(held=C + 4 * 31), ERR_ARG, "overlap"), (dict(pos=H + 120), ERR_ARG, "overlap"),
     (dict(starts=L - 16), ERR_ARG, "overlap"), (dict(count=F + 396), ERR_ARG, "overlap"),
 ])
@@ -96,7 +97,7 @@ def test_attend_workspace():
 def verify(**k):
     a = dict(p=A, ps=1000, q=B, qs=1000, x=C, c=D, u=F, n=3, k=4, v=1000, t=G, acc=H, ws=I, wb=None)
     a.update(k)
-    wb = a["wb"] if a["wb"] is not None else lib().pkv_verify_drafts_workspace(a["n"])
+    wb = a["wb"] if a["wb"] is not None else lib().pkv_verify_drafts_workspace(a["n"], a["v"])
     return lib().pkv_verify_drafts(a["p"], a["ps"], a["q"], a["qs"], a["x"], a["c"], a["u"], a["n"], a["k"], a["v"],
                                    a["t"], a["acc"], a["ws"], wb, None)
 

@@ -729,7 +729,7 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
   }
 }
 
-// ---- tiles of 16 kW kRT rows, 16 kRT a wave, for prompts. Blocks' rows of K and V go from memory
+// ---- tiles of 16 kW rows, 16 a wave, for prompts. Blocks' rows of K and V go from memory
 // into LDS, three blocks of each, one in use and one or two on their way; every wave runs its rows
 // from there:
 //   scores (transposed, A = K) with keys in the order of few_kernel; out (transposed, A = V): V's
@@ -783,9 +783,9 @@ __device__ __forceinline__ int this_lane() {
 // Vector and scalar arithmetic may move across, reads of LDS and matrix products may not.
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x406); }
 
-template <bool kBf, int kD, int kW, int kRT>
-__global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2) void many_kernel(AttendArgs a) {
-  constexpr int kThreads = 64 * kW, kRows = 16 * kW * kRT, kSteps = kD / 32, kCols = kD / 16, kP = kParts<kBf>;
+template <bool kBf, int kD, int kW>
+__global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void many_kernel(AttendArgs a) {
+  constexpr int kThreads = 64 * kW, kRows = 16 * kW, kSteps = kD / 32, kCols = kD / 16, kP = kParts<kBf>;
   constexpr int kMoves = 4 * kD / kThreads;  // 16-byte pieces of K, and of V, that a thread moves
   __shared__ __attribute__((aligned(1024))) uint16_t lk[3][kBlk * kD], lv[3][kBlk * kD];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
@@ -796,12 +796,12 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2)
   const Line line = plan.line;
   zero_empty(a, plan, kD, kThreads);
   // neighbouring shares read the same keys: they go to the same XCD (workgroups go to the 8 in turn)
-  const int share = a.shares % 8 == 0 ? ((int)blockIdx.x % 8) * (a.shares / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
-  if (share >= line.shares) return;
+  const int per_xcd = (line.shares + 7) / 8, share = ((int)blockIdx.x % 8) * per_xcd + (int)blockIdx.x / 8;
+  if ((int)blockIdx.x / 8 >= per_xcd || share >= line.shares) return;
   int64_t u = line.start(share);
   const int64_t u0 = u, end = line.start(share + 1);
   const uint32_t stride = (uint32_t)a.kv_heads * 2u * kD;
-  const int row0 = 16 * kRT * wave;  // the wave's first row of a tile
+  const int row0 = 16 * wave;  // the wave's first row of a tile
   // where the pieces that the thread moves come from: of a key's row the one that belongs where it lands
   uint32_t koff[kMoves], voff[kMoves];
 #pragma unroll
@@ -845,7 +845,7 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2)
       if (b.valid < kBlk) {
 #pragma unroll
         for (int j = 0; j < kMoves; ++j) {
-          const int over = (j * kThreads + tid) / (kD / 8) - (b.valid - 1);
+          const int over = (j * kThreads + tid) / (kD / 8) - (b.valid > 0 ? b.valid - 1 : 0);
           o[j] -= over > 0 ? (uint32_t)over * stride : 0u;
         }
       }
@@ -854,19 +854,12 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2)
     };
     Table table;
     table.look_at(a, t.b, (t.block(i0) << 5) >> a.page_lg);
-    Queries<kBf, kSteps> qs[kRT];
-    const float *qp[kRT];
-    bool mine[kRT];
-    int pos[kRT];
-#pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      const int y = row0 + 16 * rt + n;
-      mine[rt] = y < t.rows;
-      const int r = t.row0 + (mine[rt] ? y : 0), tok = r / a.group;
-      pos[rt] = mine[rt] ? t.first + tok : -1;
-      qp[rt] = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 8 * g;
-      qs[rt].load(qp[rt]);
-    }
+    const int y = row0 + n;
+    const bool mine = y < t.rows;
+    const int r = t.row0 + (mine ? y : 0), tok = r / a.group, pos = mine ? t.first + tok : -1;
+    const float *q = a.q + (int64_t)(t.tok0 + tok) * a.q_t + (int64_t)(h * a.group + r % a.group) * a.q_h + 8 * g;
+    Queries<kBf, kSteps> qs;
+    qs.load(q);
     // (behind the piece's end: the last block again, which nobody looks at)
     const auto block = [&](int i) { return block_of(a, t, table, h, t.block(i < i1 ? i : i1 - 1), 2 * kD); };
     lds_barrier();  // what was sent for behind the last piece's end has landed
@@ -876,24 +869,21 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2)
     fetch(a.k, b1, koff, lk[1]);
     fetch(a.v, b1, voff, lv[1]);
 
-    u4 qb[kRT][kSteps][kP];
-    float back[kRT];
-#pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) qs[rt].split(qp[rt], mine[rt], a.sl2, qb[rt], back[rt]);
+    u4 qb[kSteps][kP];
+    float back;
+    qs.split(q, mine, a.sl2, qb, back);
     // the wave's rows' positions
-    const int w1 = t.rows < row0 + 16 * kRT ? t.rows : row0 + 16 * kRT;  // behind its last row
-    const bool some = row0 < w1, full = w1 == row0 + 16 * kRT;
+    const int w1 = t.rows < row0 + 16 ? t.rows : row0 + 16;  // behind its last row
+    const bool some = row0 < w1, full = w1 == row0 + 16;
     const int wp0 = some ? t.first + (t.row0 + row0) / a.group : -1;
     const int wp1 = some ? t.first + (t.row0 + w1 - 1) / a.group : -1;
     __builtin_amdgcn_sched_barrier(0);  // (the sums take the registers that the queries came through)
     const f4 zero = {0.f, 0.f, 0.f, 0.f};
-    f4 acc[kRT][kCols];
-    Row<kBf> row[kRT];
+    f4 acc[kCols];
+    Row<kBf> row;
 #pragma unroll
-    for (int rt = 0; rt < kRT; ++rt)
-#pragma unroll
-      for (int c = 0; c < kCols; ++c) acc[rt][c] = zero;
-    f4 sc[kRT][2];
+    for (int c = 0; c < kCols; ++c) acc[c] = zero;
+    f4 sc[2];
     // (operands come from LDS kAhead reads ahead of the products that take them)
     constexpr int kAhead = kBf ? 2 : 4;
     const auto scores = [&](const uint16_t *kb) {
@@ -906,20 +896,17 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2)
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) A[i] = read(i);
       keep_order();
-#pragma unroll
-      for (int rt = 0; rt < kRT; ++rt) sc[rt][0] = sc[rt][1] = zero;
+      sc[0] = sc[1] = zero;
 #pragma unroll
       for (int i = 0; i < kReads; i += 2) {  // (both key tiles in turn: a sum waits for its last product)
 #pragma unroll
         for (int p = kP - 1; p >= 0; --p)
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int rt = 0; rt < kRT; ++rt) sc[rt][y] = half_mfma<kBf>(A[(i + y) % kAhead], qb[rt][i >> 1][p], sc[rt][y]);
+          for (int z = 0; z < 2; ++z) sc[z] = half_mfma<kBf>(A[(i + z) % kAhead], qb[i >> 1][p], sc[z]);
         keep_order();
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-          if (i + y + kAhead < kReads) A[(i + y) % kAhead] = read(i + y + kAhead);
+        for (int z = 0; z < 2; ++z)
+          if (i + z + kAhead < kReads) A[(i + z) % kAhead] = read(i + z + kAhead);
         keep_order();
       }
     };
@@ -934,24 +921,18 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2)
       fetch(a.k, b2, koff, lk[(at + 2) % 3]);
       fetch(a.v, b2, voff, lv[(at + 2) % 3]);
       scores(lk[at]);
-      float c[kRT][8];
+      float c[8];
 #pragma unroll
-      for (int rt = 0; rt < kRT; ++rt)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) c[rt][e] = sc[rt][e >> 2][e & 3];
+      for (int e = 0; e < 8; ++e) c[e] = sc[e >> 2][e & 3];
       const bool all = (b0.valid == kBlk) & full & all_seen(a, wp0, wp1, j0);
+      float alpha = 1.0f;
+      if (row.raise(c, back, all, [&] { return seen_of(a, pos, j0 + 8 * g, b0.valid - 8 * g); }, alpha))
 #pragma unroll
-      for (int rt = 0; rt < kRT; ++rt) {
-        float alpha = 1.0f;
-        if (row[rt].raise(c[rt], back[rt], all, [&] { return seen_of(a, pos[rt], j0 + 8 * g, b0.valid - 8 * g); }, alpha))
+        for (int cc = 0; cc < kCols; ++cc)
 #pragma unroll
-          for (int cc = 0; cc < kCols; ++cc)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[rt][cc][e] *= alpha;
-      }
-      u4 pb[kRT][kP];
-#pragma unroll
-      for (int rt = 0; rt < kRT; ++rt) row[rt].weights(c[rt], back[rt], pb[rt]);
+          for (int e = 0; e < 4; ++e) acc[cc][e] *= alpha;
+      u4 pb[kP];
+      row.weights(c, back, pb);
       // lane n of each 16: four values of row n / 4 of keys 8 g .. + 3, then of + 4 .. + 7
       const int vat = v_place();
       const auto read = [&](int cc) {
@@ -968,14 +949,11 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2)
 #pragma unroll
         for (int p = kP - 1; p >= 0; --p)
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-#pragma unroll
-            for (int rt = 0; rt < kRT; ++rt)
-              acc[rt][cc + y] = half_mfma<kBf>(A[(cc + y) % kAhead], pb[rt][p], acc[rt][cc + y]);
+          for (int z = 0; z < 2; ++z) acc[cc + z] = half_mfma<kBf>(A[(cc + z) % kAhead], pb[p], acc[cc + z]);
         keep_order();
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-          if (cc + y + kAhead < kCols) A[(cc + y) % kAhead] = read(cc + y + kAhead);
+        for (int z = 0; z < 2; ++z)
+          if (cc + z + kAhead < kCols) A[(cc + z) % kAhead] = read(cc + z + kAhead);
         keep_order();
       }
       fetched<2 * kMoves>();  // all but what this step sent for
@@ -989,35 +967,25 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 && !kBf ? 4 : 2)
       if (i + 2 < i1) step(i + 2, std::integral_constant<int, 2>{});
     }
     fetched<0>();  // (what was sent for behind the end lands before LDS is used again)
-    float l[kRT];
-    bool bad = false;
+    const float l = row.sum();
+    bool bad = !(l < INFINITY);
 #pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      l[rt] = row[rt].sum();
-      bad |= !(l[rt] < INFINITY);
+    for (int cc = 0; cc < kCols; ++cc)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[cc][e] *= 1.0f / Row<kBf>::kUp;
+        bad |= !(fabsf(acc[cc][e]) < INFINITY);
+      }
+    if (__any(bad)) {
+      for (int z = row0; z < w1; ++z) plain_store<kBf, kD / 64>(a, t, h, z, i0, i1, lane, to, kRows);
+    } else if (mine) {
+      const int64_t at = to.slot * kRows + y;
+      float *o = (to.whole ? row_out(a, t, h, y, kD) : a.part + at * kD) + 4 * g;
+      const float f = !to.whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
       for (int cc = 0; cc < kCols; ++cc)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          acc[rt][cc][e] *= 1.0f / Row<kBf>::kUp;
-          bad |= !(fabsf(acc[rt][cc][e]) < INFINITY);
-        }
-    }
-    if (__any(bad)) {
-      for (int y = row0; y < w1; ++y) plain_store<kBf, kD / 64>(a, t, h, y, i0, i1, lane, to, kRows);
-    } else {
-#pragma unroll
-      for (int rt = 0; rt < kRT; ++rt) {
-        const int y = row0 + 16 * rt + n;
-        if (y >= t.rows) continue;
-        const int64_t at = to.slot * kRows + y;
-        float *o = (to.whole ? row_out(a, t, h, y, kD) : a.part + at * kD) + 4 * g;
-        const float f = !to.whole ? 1.0f : l[rt] > 0.0f ? 1.0f / l[rt] : 0.0f;
-#pragma unroll
-        for (int cc = 0; cc < kCols; ++cc)
-          *reinterpret_cast<float4 *>(o + 16 * cc) = float4{acc[rt][cc][0] * f, acc[rt][cc][1] * f, acc[rt][cc][2] * f, acc[rt][cc][3] * f};
-        if (!to.whole && g == 0) a.ml[at] = float2{row[rt].m, l[rt]};
-      }
+        *reinterpret_cast<float4 *>(o + 16 * cc) = float4{acc[cc][0] * f, acc[cc][1] * f, acc[cc][2] * f, acc[cc][3] * f};
+      if (!to.whole && g == 0) a.ml[at] = float2{row.m, l};
     }
   }
 }
@@ -1144,15 +1112,21 @@ __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(
   }
 }
 
-// Rows a tile holds, the workgroups that share the blocks, and how many blocks a tile's start costs.
+// Rows a tile holds, the workgroups that share the blocks (as many as the chip runs at once), and how
+// many blocks a tile's start costs: 2 of a few rows, 6 of a prompt's (start, queries, first loads and
+// stores take 20000 cycles, a block 4300; 4 and 8 made 8001 tokens in a window 3% slower).
+// Tiles of few rows for requests of up to 48 rows on average: 80 drafted tokens of 40 rows each
+// take 48 us in tiles of 48 and 78 in LDS tiles of 64. Three waves a SIMD hold 16 rows of head_dim
+// 64 and 128 (24 requests of 64: 58 us by two, 44 by three), two anything else.
 struct Shape {
   int rows, shares, start;
+  bool prompts() const { return start == 6; }
 };
 Shape shape_of(int n, int64_t tokens, int group, int head_dim) {
   const int64_t rows = tokens * group;
   for (const int r : {16, 32, 48})
-    if (rows <= r * (int64_t)n) return Shape{r, 512 * 256 / head_dim, 2};
-  return Shape{128, head_dim > 128 ? 256 : 512, 6};
+    if (rows <= r * (int64_t)n) return Shape{r, (r == 16 && head_dim < 256 ? 768 : 512) * 256 / head_dim, 2};
+  return head_dim == 64 ? Shape{64, 1024, 6} : head_dim == 128 ? Shape{64, 768, 6} : Shape{128, 256, 6};
 }
 struct Layout {
   size_t tiles, before, firsts, count, ml, part, all;
@@ -1196,14 +1170,14 @@ template <bool kBf, int kD>
 int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
   // a head's units at most, as 32-bit sums of the workgroup's own plan
   const int64_t most = (int64_t)a.max_tiles * ((((int64_t)a.max_pages << a.page_lg) >> 5) + sh.start + 1);
-  if (sh.rows < 128 && a.n <= 64 && a.max_tiles <= kHereTiles && most < ((int64_t)1 << 31)) {
+  if (!sh.prompts() && a.n <= 64 && a.max_tiles <= kHereTiles && most < ((int64_t)1 << 31)) {
     few<kBf, kD, true>(a, sh, s);
   } else {
     hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, sh.rows);
-    if (sh.rows < 128) {
+    if (!sh.prompts()) {
       few<kBf, kD, false>(a, sh, s);
     } else {
-      hipLaunchKernelGGL((many_kernel<kBf, kD, (kD > 64 ? 8 : 4), (kD > 64 ? 1 : 2)>), dim3(sh.shares), dim3(kD > 64 ? 512 : 256), 0, s, a);
+      hipLaunchKernelGGL((many_kernel<kBf, kD, (kD > 128 ? 8 : 4)>), dim3(sh.shares), dim3(kD > 128 ? 512 : 256), 0, s, a);
       join<kD, false>(a, sh, s);
     }
   }

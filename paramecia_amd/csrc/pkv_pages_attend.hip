@@ -66,10 +66,10 @@ __device__ __forceinline__ void request_of(const AttendArgs &a, int b, int &q0, 
   len = len < 0 ? 0 : len > most ? (int)most : len;
 }
 
-__device__ __forceinline__ Tile tile_of(const AttendArgs &a, int b, int i, int rows_per_tile) {
+// Tile i of request b, whose queries begin at q0 of the step.
+__device__ __forceinline__ Tile tile_of(const AttendArgs &a, int b, int q0, int fresh, int len, int i, int rows_per_tile) {
   Tile t;
-  int fresh, len;
-  request_of(a, b, t.tok0, fresh, len);
+  t.tok0 = q0;
   const int all = fresh * a.group;
   t.b = b;
   t.row0 = i * rows_per_tile;
@@ -91,6 +91,12 @@ __device__ __forceinline__ Tile tile_of(const AttendArgs &a, int b, int i, int r
   return t;
 }
 
+__device__ __forceinline__ Tile tile_of(const AttendArgs &a, int b, int i, int rows_per_tile) {
+  int q0, fresh, len;
+  request_of(a, b, q0, fresh, len);
+  return tile_of(a, b, q0, fresh, len, i, rows_per_tile);
+}
+
 // Whether the query at position p sees key j.
 __device__ __forceinline__ bool sees(const AttendArgs &a, int p, int j) {
   return j <= p && (a.window <= 0 || j > p - a.window || j < a.sinks);
@@ -100,7 +106,19 @@ __device__ __forceinline__ bool sees(const AttendArgs &a, int p, int j) {
 struct Line {
   int tiles, shares;
   int64_t per_head, all;
-  __device__ __forceinline__ int64_t start(int w) const { return all * w / shares; }
+  int64_t each;  // units of a share; the first `more` have one more
+  int more;
+  __device__ __forceinline__ int64_t start(int w) const { return each * w + (w < more ? w : more); }
+  // The share that holds unit u.
+  __device__ __forceinline__ int share(int64_t u) const {
+    const int64_t longer = (each + 1) * more;
+    return (int)(u < longer ? quotient(u, each + 1) : more + quotient(u - longer, each));
+  }
+  __device__ __forceinline__ int head(int64_t u) const { return (int)quotient(u, per_head); }
+  // x / y of numbers of at least 0, in 32 bits where they fit (a 64-bit quotient takes 500 cycles)
+  static __device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+    return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+  }
 };
 __device__ __forceinline__ Line line_of(const AttendArgs &a, int tiles, int64_t per_head) {
   Line l;
@@ -108,6 +126,8 @@ __device__ __forceinline__ Line line_of(const AttendArgs &a, int tiles, int64_t 
   l.per_head = per_head;
   l.all = per_head * a.kv_heads;
   l.shares = l.all < a.shares ? (int)l.all : a.shares;
+  l.each = l.shares ? Line::quotient(l.all, l.shares) : 0;
+  l.more = (int)(l.all - l.each * l.shares);
   return l;
 }
 __device__ __forceinline__ Line line_of(const AttendArgs &a) {
@@ -199,7 +219,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int ro
   }
   __syncthreads();
   const Line line = line_of(a, count, blocks);
-  for (int w = tid; w < line.shares; w += kPlanThreads) a.firsts[w] = tile_at(a, count, line.start(w) % blocks);
+  for (int w = tid; w < line.shares; w += kPlanThreads) a.firsts[w] = tile_at(a, count, line.start(w) - line.head(line.start(w)) * blocks);
 }
 
 // What the plan says, from memory, or worked out by the workgroup itself: a launch less where the
@@ -215,6 +235,20 @@ __device__ __forceinline__ Tile uniform(const Tile &t) {
   return Tile{uniform(t.b), uniform(t.row0), uniform(t.rows), uniform(t.tok0), uniform(t.p0), uniform(t.p1),
               uniform(t.first), uniform(t.sink_blocks), uniform(t.lo), uniform(t.blocks)};
 }
+// Running sums of x over a wave's lanes.
+__device__ __forceinline__ int wave_running(int x) {
+  const auto add = [&](auto ctrl, auto rows) {
+    return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+  };
+  using std::integral_constant;
+  x += add(integral_constant<int, 0x111>{}, integral_constant<int, 0xF>{});  // row_shr 1, 2, 4, 8
+  x += add(integral_constant<int, 0x112>{}, integral_constant<int, 0xF>{});
+  x += add(integral_constant<int, 0x114>{}, integral_constant<int, 0xF>{});
+  x += add(integral_constant<int, 0x118>{}, integral_constant<int, 0xF>{});
+  x += add(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // row_bcast 15, 31
+  x += add(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});
+  return x;
+}
 template <bool kHere>
 struct Plan;
 template <>
@@ -225,61 +259,55 @@ struct Plan<false> {
   __device__ __forceinline__ int64_t before(const AttendArgs &a, int x) const { return a.before[x]; }
   __device__ __forceinline__ Tile tile(const AttendArgs &a, int x) const { return a.tiles[x]; }
   __device__ __forceinline__ int first(const AttendArgs &a, int share) const { return a.firsts[share]; }
-  __device__ __forceinline__ int at(const AttendArgs &a, int64_t u) const { return tile_at(a, line.tiles, u); }
 };
 template <>
 struct Plan<true> {
   Line line;
   using Lds = HerePlan;
   const HerePlan *lds;
-  // n at most 64, max_tiles at most kHereTiles, a head's units below 2^31
+  // n at most 64, max_tiles at most kHereTiles, a head's units below 2^31. The first workgroup leaves
+  // the plan in memory, for the join.
   __device__ __forceinline__ void make(const AttendArgs &a, Lds &p, int rows_per_tile, int threads) {
     const int tid = threadIdx.x;
     if (tid < 64) {
-      int q0, fresh = 0, len;
+      int q0 = 0, fresh = 0, len = 0;
       if (tid < a.n) request_of(a, tid, q0, fresh, len);
       const int mine = (fresh * a.group + rows_per_tile - 1) / rows_per_tile;
-      int y = mine;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int z = __shfl_up(y, o);
-        if (tid >= o) y += z;
+      if (!__any(mine > 1)) {  // a tile a request (of no rows, where it has none)
+        const Tile x = tile_of(a, tid, q0, fresh, len, 0, rows_per_tile);
+        if (tid < a.n) p.tiles[tid] = x;
+        const int y = wave_running((int)x.units(a.start));
+        p.before[tid + 1] = y;
+        if (tid == 0) p.before[0] = 0, p.count = a.n;
+      } else {
+        const int to = wave_running(mine);
+        const int count = uniform(__shfl(to, 63)) < a.max_tiles ? uniform(__shfl(to, 63)) : a.max_tiles;
+        for (int i = 0; i < mine && to - mine + i < count; ++i)
+          p.tiles[to - mine + i] = tile_of(a, tid, q0, fresh, len, i, rows_per_tile);
+        int sum = 0;
+        for (int t0 = 0; t0 < count; t0 += 64) {
+          const int t = t0 + tid;
+          const int y = sum + wave_running(t < count ? (int)p.tiles[t].units(a.start) : 0);
+          if (t < count) p.before[t + 1] = y;
+          sum = uniform(__shfl(y, 63));
+        }
+        if (tid == 0) p.before[0] = 0, p.count = count;
       }
-      for (int i = 0; i < mine && y - mine + i < a.max_tiles; ++i)
-        p.tiles[y - mine + i].b = tid, p.tiles[y - mine + i].row0 = i;
-      if (tid == 63) p.count = y < a.max_tiles ? y : a.max_tiles;
     }
     __syncthreads();
     const int count = uniform(p.count);
-    for (int t = tid; t < count; t += threads) {
-      const Tile x = tile_of(a, p.tiles[t].b, p.tiles[t].row0, rows_per_tile);
-      p.tiles[t] = x;
-      p.before[t + 1] = (int)x.units(a.start);
-    }
-    __syncthreads();
-    if (tid < 64) {
-      int sum = 0;
-      for (int t0 = 0; t0 < count; t0 += 64) {
-        const int t = t0 + tid;
-        int y = t < count ? p.before[t + 1] : 0;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const int z = __shfl_up(y, o);
-          if (tid >= o) y += z;
-        }
-        if (t < count) p.before[t + 1] = sum + y;
-        sum += __shfl(y, 63);
-      }
-      if (tid == 0) p.before[0] = 0;
-    }
-    __syncthreads();
     lds = &p;
     line = line_of(a, count, uniform(p.before[count]));
+    if (blockIdx.x == 0) {
+      for (int t = tid; t <= count; t += threads) a.before[t] = p.before[t];
+      for (int t = tid; t < count; t += threads) a.tiles[t] = p.tiles[t];
+      if (tid == 0) *a.count = count;
+    }
   }
   __device__ __forceinline__ int64_t before(const AttendArgs &, int x) const { return uniform(lds->before[x]); }
   __device__ __forceinline__ Tile tile(const AttendArgs &, int x) const { return uniform(lds->tiles[x]); }
-  __device__ __forceinline__ int first(const AttendArgs &a, int share) const { return at(a, line.start(share) % line.per_head); }
-  __device__ __forceinline__ int at(const AttendArgs &, int64_t u) const {
+  __device__ __forceinline__ int first(const AttendArgs &, int share) const {
+    const int64_t u = line.start(share) - line.head(line.start(share)) * line.per_head;
     int x = -1;  // tiles that begin at u or before it
     for (int t0 = 0; t0 < line.tiles; t0 += 64) {
       const int t = t0 + (int)(threadIdx.x & 63);
@@ -569,7 +597,7 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
   if (tid == 0) s_bad = 0u;
   int turn = 0;
   const uint32_t stride = (uint32_t)a.kv_heads * 2u * kD;
-  int x = plan.first(a, share), h = (int)(u / line.per_head);
+  int x = plan.first(a, share), h = line.head(u);
   for (; u < end; ++x) {
     if (x == line.tiles) x = 0, ++h;
     const Tile t = plan.tile(a, x);
@@ -823,7 +851,7 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
     const int ln = this_lane(), m = ln & 15, key = 8 * (ln >> 4) + (m >> 2);
     return key * kD + 8 * v_piece<kD>(key, (m & 3) >> 1) + 4 * (m & 1);
   };
-  int x = plan.first(a, share), h = (int)(u / line.per_head);
+  int x = plan.first(a, share), h = line.head(u);
   for (; u < end; ++x) {
     if (x == line.tiles) x = 0, ++h;
     const Tile t = plan.tile(a, x);
@@ -1044,38 +1072,32 @@ __device__ __forceinline__ void join_parts(const AttendArgs &a, Slot slot, int i
   }
 }
 
-template <int kD, int kAcross, bool kHere>
+template <int kD, int kAcross>
 __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(AttendArgs a, int rows_per_tile, int by_cut) {
   constexpr int kE = kD / 64;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  __shared__ typename Plan<kHere>::Lds s_plan;
-  Plan<kHere> plan;
-  plan.make(a, s_plan, rows_per_tile, (int)blockDim.x);
-  const Line line = plan.line;
+  const Line line = line_of(a);
   int h, x, w0;  // w0: the share that holds the tile's first block
   if (by_cut) {
     const int cut = blockIdx.x + 1;
     if (cut >= line.shares) return;
     const int64_t u = line.start(cut);
-    h = (int)(u / line.per_head);
-    x = plan.at(a, u - h * line.per_head);
-    const int64_t first = h * line.per_head + plan.before(a, x) + a.start;
+    h = line.head(u);
+    x = tile_at(a, line.tiles, u - h * line.per_head);
+    const int64_t first = h * line.per_head + a.before[x] + a.start;
     if (u <= first || (cut > 1 && line.start(cut - 1) > first)) return;
     w0 = cut - 1;
   } else {
     h = (int)blockIdx.x % a.kv_heads;
     x = (int)blockIdx.x / a.kv_heads;
-    if (x >= line.tiles || plan.before(a, x + 1) == plan.before(a, x)) return;
-    const int64_t first = h * line.per_head + plan.before(a, x) + a.start;
-    w0 = (int)(first * line.shares / line.all);  // (start(w0) <= first, maybe not the last such)
-    while (line.start(w0 + 1) <= first) ++w0;
+    if (x >= line.tiles || a.before[x + 1] == a.before[x]) return;
+    const int64_t first = h * line.per_head + a.before[x] + a.start;
+    w0 = line.share(first);
   }
-  const int64_t tile0 = h * line.per_head + plan.before(a, x), last = h * line.per_head + plan.before(a, x + 1);
+  const int64_t tile0 = h * line.per_head + a.before[x], last = h * line.per_head + a.before[x + 1];
   if (line.start(w0 + 1) >= last) return;  // not cut
-  int w1 = (int)((last - 1) * line.shares / line.all);
-  while (line.start(w1 + 1) < last) ++w1;
-  const int pieces = w1 - w0 + 1, odd = line.start(w0) < tile0 ? 1 : 0;
-  const Tile t = plan.tile(a, x);
+  const int pieces = line.share(last - 1) - w0 + 1, odd = line.start(w0) < tile0 ? 1 : 0;
+  const Tile t = a.tiles[x];
   const int row = kAcross > 1 ? (int)blockIdx.y : (int)blockIdx.y * 4 + wave;
   if (row >= t.rows) return;
   const auto slot = [&](int i) { return (2 * (int64_t)(w0 + i) + (i == 0 ? odd : 0)) * rows_per_tile + row; };
@@ -1146,17 +1168,17 @@ Layout layout_of(const Shape &sh, int n, int64_t tokens, int group, int head_dim
   return l;
 }
 
-template <int kD, bool kHere>
+template <int kD>
 void join(AttendArgs &a, const Shape &sh, hipStream_t s) {
   const int64_t tiles = (int64_t)a.max_tiles * a.kv_heads;
   const int by_cut = tiles > sh.shares;
   const unsigned x = by_cut ? (unsigned)sh.shares : (unsigned)tiles;
   if (tiles * 64 <= sh.shares)  // the parts a tile has on average
-    hipLaunchKernelGGL((join_kernel<kD, 16, kHere>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
+    hipLaunchKernelGGL((join_kernel<kD, 16>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
   else if (tiles * 4 <= sh.shares)
-    hipLaunchKernelGGL((join_kernel<kD, 4, kHere>), dim3(x, sh.rows), dim3(256), 0, s, a, sh.rows, by_cut);
+    hipLaunchKernelGGL((join_kernel<kD, 4>), dim3(x, sh.rows), dim3(256), 0, s, a, sh.rows, by_cut);
   else
-    hipLaunchKernelGGL((join_kernel<kD, 1, kHere>), dim3(x, sh.rows / 4), dim3(256), 0, s, a, sh.rows, by_cut);
+    hipLaunchKernelGGL((join_kernel<kD, 1>), dim3(x, sh.rows / 4), dim3(256), 0, s, a, sh.rows, by_cut);
 }
 template <bool kBf, int kD, bool kHere>
 void few(AttendArgs &a, const Shape &sh, hipStream_t s) {
@@ -1164,7 +1186,7 @@ void few(AttendArgs &a, const Shape &sh, hipStream_t s) {
   if (sh.rows == 16) hipLaunchKernelGGL((few_kernel<kBf, kD, 1, kHere>), grid, block, 0, s, a);
   else if (sh.rows == 32) hipLaunchKernelGGL((few_kernel<kBf, kD, 2, kHere>), grid, block, 0, s, a);
   else hipLaunchKernelGGL((few_kernel<kBf, kD, 3, kHere>), grid, block, 0, s, a);
-  join<kD, kHere>(a, sh, s);
+  join<kD>(a, sh, s);
 }
 template <bool kBf, int kD>
 int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
@@ -1178,7 +1200,7 @@ int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
       few<kBf, kD, false>(a, sh, s);
     } else {
       hipLaunchKernelGGL((many_kernel<kBf, kD, (kD > 128 ? 8 : 4)>), dim3(sh.shares), dim3(kD > 128 ? 512 : 256), 0, s, a);
-      join<kD, false>(a, sh, s);
+      join<kD>(a, sh, s);
     }
   }
   PKV_HIP(hipGetLastError());

@@ -758,8 +758,7 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
 }
 
 // ---- tiles of 16 kW rows, 16 a wave, for prompts. Blocks' rows of K and V go from memory
-// into LDS, three blocks of each, one in use and one or two on their way; every wave runs its rows
-// from there:
+// into LDS ahead of their use; every wave runs its rows from there:
 //   scores (transposed, A = K) with keys in the order of few_kernel; out (transposed, A = V): V's
 //   columns come by transposing reads; the result is columns 16 c + 4 g + i of row n.
 // Pieces of 16 bytes of a row are turned by the row, so that the 16 rows which a quarter of a wave
@@ -815,7 +814,12 @@ template <bool kBf, int kD, int kW>
 __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void many_kernel(AttendArgs a) {
   constexpr int kThreads = 64 * kW, kRows = 16 * kW, kSteps = kD / 32, kCols = kD / 16, kP = kParts<kBf>;
   constexpr int kMoves = 4 * kD / kThreads;  // 16-byte pieces of K, and of V, that a thread moves
-  __shared__ __attribute__((aligned(1024))) uint16_t lk[3][kBlk * kD], lv[3][kBlk * kD];
+  // Blocks of K and of V in LDS. Four: two between barriers, the two behind them on their way. Rows
+  // of 256 bytes take three, one and one or two, so that three workgroups fit a CU's LDS (8001 tokens in a
+  // window, 32 heads of 128: 360 us, with four 471; of 256, 16 heads: 304 by pairs, 317 one by one).
+  constexpr bool kPairs = kD != 128;
+  constexpr int kRing = kPairs ? 4 : 3;
+  __shared__ __attribute__((aligned(1024))) uint16_t lk[kRing][kBlk * kD], lv[kRing][kBlk * kD];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Plan<false> plan;
@@ -939,22 +943,18 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
       }
     };
 
-    fetched<2 * kMoves>();  // the first block
+    fetched<kPairs ? 0 : 2 * kMoves>();  // the first blocks, or the first
     lds_barrier();
-    // here: block i in LDS, the next one on its way
-    const auto step = [&](int i, auto third) {
-      constexpr int at = decltype(third)::value;  // (i - i0) % 3
+    const auto step = [&](int i, int valid, auto slot) {
+      constexpr int at = decltype(slot)::value;
       const int j0 = t.block(i) << 5;
-      const Block b2 = block(i + 2);
-      fetch(a.k, b2, koff, lk[(at + 2) % 3]);
-      fetch(a.v, b2, voff, lv[(at + 2) % 3]);
       scores(lk[at]);
       float c[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) c[e] = sc[e >> 2][e & 3];
-      const bool all = (b0.valid == kBlk) & full & all_seen(a, wp0, wp1, j0);
+      const bool all = (valid == kBlk) & full & all_seen(a, wp0, wp1, j0);
       float alpha = 1.0f;
-      if (row.raise(c, back, all, [&] { return seen_of(a, pos, j0 + 8 * g, b0.valid - 8 * g); }, alpha))
+      if (row.raise(c, back, all, [&] { return seen_of(a, pos, j0 + 8 * g, valid - 8 * g); }, alpha))
 #pragma unroll
         for (int cc = 0; cc < kCols; ++cc)
 #pragma unroll
@@ -984,15 +984,43 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
           if (cc + z + kAhead < kCols) A[(cc + z) % kAhead] = read(cc + z + kAhead);
         keep_order();
       }
-      fetched<2 * kMoves>();  // all but what this step sent for
-      lds_barrier();
-      b0 = b1;
-      b1 = b2;
     };
-    for (int i = i0; i < i1; i += 3) {
-      step(i, std::integral_constant<int, 0>{});
-      if (i + 1 < i1) step(i + 1, std::integral_constant<int, 1>{});
-      if (i + 2 < i1) step(i + 2, std::integral_constant<int, 2>{});
+    if constexpr (kPairs) {
+      const auto pair = [&](int i, auto which) {
+        constexpr int at = 2 * decltype(which)::value, other = 2 - at;
+        const Block b2 = block(i + 2), b3 = block(i + 3);
+        fetch(a.k, b2, koff, lk[other]);
+        fetch(a.v, b2, voff, lv[other]);
+        fetch(a.k, b3, koff, lk[other + 1]);
+        fetch(a.v, b3, voff, lv[other + 1]);
+        step(i, b0.valid, std::integral_constant<int, at>{});
+        if (i + 1 < i1) step(i + 1, b1.valid, std::integral_constant<int, at + 1>{});
+        fetched<0>();
+        lds_barrier();
+        b0 = b2;
+        b1 = b3;
+      };
+      for (int i = i0; i < i1; i += 4) {
+        pair(i, std::integral_constant<int, 0>{});
+        if (i + 2 < i1) pair(i + 2, std::integral_constant<int, 1>{});
+      }
+    } else {
+      const auto one = [&](int i, auto which) {
+        constexpr int at = decltype(which)::value, other = (at + 2) % 3;
+        const Block b2 = block(i + 2);
+        fetch(a.k, b2, koff, lk[other]);
+        fetch(a.v, b2, voff, lv[other]);
+        step(i, b0.valid, std::integral_constant<int, at>{});
+        fetched<2 * kMoves>();  // all but what was just sent for
+        lds_barrier();
+        b0 = b1;
+        b1 = b2;
+      };
+      for (int i = i0; i < i1; i += 3) {
+        one(i, std::integral_constant<int, 0>{});
+        if (i + 1 < i1) one(i + 1, std::integral_constant<int, 1>{});
+        if (i + 2 < i1) one(i + 2, std::integral_constant<int, 2>{});
+      }
     }
     fetched<0>();  // (what was sent for behind the end lands before LDS is used again)
     const float l = row.sum();

@@ -842,19 +842,29 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
     koff[j] = (uint32_t)key * stride + 16u * (uint32_t)k_piece<kD>(key, c);
     voff[j] = (uint32_t)key * stride + 16u * (uint32_t)v_piece<kD>(key, c);
   }
-  // Where the lane reads: K's piece g of key 8 (n / 4) + n % 4, V's row n / 4 of keys 8 g .. + 3 in the
-  // first 16 columns. Later steps and columns turn the place as they turn the piece, by an
-  // exclusive or; the next keys are four rows on. Worked out again in each block: held for all of
-  // them they take registers that the sums need, and what the compiler then puts into scratch
-  // memory comes back behind the loads of LDS.
-  const auto k_place = [] {
-    const int ln = this_lane(), m = ln & 15, key = 8 * (m >> 2) + (m & 3);
-    return key * kD + 8 * k_piece<kD>(key, ln >> 4);
+  // Where the lane reads: K's pieces 4 st + g of key 8 (n / 4) + n % 4 (the other keys are four rows on),
+  // V's row n / 4 of keys 8 g .. + 3 in tile cc of 16 columns (keys + 4 four rows on). Pieces are turned
+  // by an exclusive or of their low bits, so four steps and eight tiles on the place is 256 bytes on.
+  // BF16 rows of 512 bytes leave no registers for twelve places: they are worked out again in each
+  // block from the lane's two. (What the compiler puts into scratch memory instead comes back
+  // behind the loads of LDS: 8001 tokens 1020 us instead of 400.)
+  constexpr bool kAgain = kBf && kD == 256;
+  constexpr int kK = kAgain ? 1 : kSteps < 4 ? kSteps : 4, kV = kAgain ? 1 : kCols < 8 ? kCols : 8;
+  const auto k_place = [](int st) {
+    const int ln = kAgain ? this_lane() : (int)(threadIdx.x & 63), m = ln & 15, key = 8 * (m >> 2) + (m & 3);
+    return key * kD + 8 * k_piece<kD>(key, 4 * st + (ln >> 4));
   };
-  const auto v_place = [] {
-    const int ln = this_lane(), m = ln & 15, key = 8 * (ln >> 4) + (m >> 2);
-    return key * kD + 8 * v_piece<kD>(key, (m & 3) >> 1) + 4 * (m & 1);
+  const auto v_place = [](int cc) {
+    const int ln = kAgain ? this_lane() : (int)(threadIdx.x & 63), m = ln & 15, key = 8 * (ln >> 4) + (m >> 2);
+    return key * kD + 8 * v_piece<kD>(key, 2 * cc + ((m & 3) >> 1)) + 4 * (m & 1);
   };
+  int k_held[kK], v_held[kV];
+  if constexpr (!kAgain) {
+#pragma unroll
+    for (int st = 0; st < kK; ++st) k_held[st] = k_place(st);
+#pragma unroll
+    for (int cc = 0; cc < kV; ++cc) v_held[cc] = v_place(cc);
+  }
   int x = plan.first(a, share), h = line.head(u);
   for (; u < end; ++x) {
     if (x == line.tiles) x = 0, ++h;
@@ -920,9 +930,10 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
     constexpr int kAhead = kBf ? 2 : 4;
     const auto scores = [&](const uint16_t *kb) {
       constexpr int kReads = 2 * kSteps;
-      const int kat = k_place();
+      const int own = kAgain ? k_place(0) : 0;
       const auto read = [&](int i) {
-        return *reinterpret_cast<const u4 *>(kb + (kat ^ (32 * (i >> 1))) + (i & 1) * 4 * kD);
+        const int st = i >> 1, at = kAgain ? own ^ (32 * st) : k_held[st % kK] + st / kK * 128;
+        return *reinterpret_cast<const u4 *>(kb + at + (i & 1) * 4 * kD);
       };
       u4 A[kAhead];
 #pragma unroll
@@ -962,9 +973,9 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
       u4 pb[kP];
       row.weights(c, back, pb);
       // lane n of each 16: four values of row n / 4 of keys 8 g .. + 3, then of + 4 .. + 7
-      const int vat = v_place();
+      const int own = kAgain ? v_place(0) : 0;
       const auto read = [&](int cc) {
-        const uint16_t *vp = lv[at] + (vat ^ (16 * cc));
+        const uint16_t *vp = lv[at] + (kAgain ? own ^ (16 * cc) : v_held[cc % kV] + cc / kV * 128);
         const uint2 lo = load_columns(vp), hi = load_columns(vp + 4 * kD);
         return u4{lo.x, lo.y, hi.x, hi.y};
       };

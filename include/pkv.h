@@ -67,7 +67,8 @@ const char *pkv_last_error(void);
 const char *pkv_version(void);
 /* Waits for the current device, then reports and clears the errors its kernels flagged
  * instead of hanging: PKV_ERR_HIP if a fused decode step's bounded barrier gave up (the
- * step's appended row and output are then invalid), PKV_OK otherwise. No reference
+ * step's appended row and output are then invalid) or an adapter's id, a slot or a page of a
+ * table was out of range (what it named was left out), PKV_OK otherwise. No reference
  * counterpart (the reference's CPU path cannot hang a barrier). */
 int pkv_device_status(void);
 
@@ -438,7 +439,8 @@ int pkv_seq_get_kv(const pkv_seq *s, float *k_out, float *v_out);
  * other one of the call. */
 /* A pool's planes, and pages that the device may hand out: take moves n of the pool's free
  * pages (PKV_ERR_OVERFLOW, with none taken, when it lacks them) out of its sequences' reach,
- * give brings such pages back (PKV_ERR_ARG, with none given, for a page that is not taken). */
+ * give brings such pages back (PKV_ERR_ARG, with none given, for a page that is not taken). The
+ * caller orders work on such pages with the pool's stream, both ways. */
 int pkv_pool_storage(const pkv_pool *p, void **k_pages, void **v_pages, size_t *page_bytes,
                      int *page_tokens, int *n_pages);
 int pkv_pool_take_pages(pkv_pool *p, int n, int *pages_host);
@@ -471,7 +473,7 @@ int pkv_pages_map(const int *lens, const int *add, int n, int *tables, int max_p
  * to quant (PKV_QUANT_F16 or PKV_QUANT_BF16, else PKV_ERR_UNSUPPORTED) as the cache rounds
  * them. A negative slot: its token is left out; a slot of n_slots (n_pages * page_tokens) or
  * more too, and pkv_device_status reports it. Two tokens of one slot leave a row whose parts
- * may be either's. n * n_kv_heads * head_dim below 2^32 (else PKV_ERR_UNSUPPORTED). */
+ * may be either's. n * n_kv_heads * head_dim below 2^31 (else PKV_ERR_UNSUPPORTED). */
 int pkv_pages_append(int quant, const float *k, const float *v, int64_t k_stride, int64_t v_stride,
                      const int64_t *slots, int64_t n, void *k_pages, void *v_pages,
                      int64_t n_slots, int n_kv_heads, int head_dim, pkv_stream stream);

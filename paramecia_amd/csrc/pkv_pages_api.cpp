@@ -74,8 +74,8 @@ int pkv_pages_append(int quant, const float *k, const float *v, int64_t k_stride
   if (n == 0) return PKV_OK;
   if (!k || !v || !slots || !k_pages || !v_pages) return set_error(PKV_ERR_ARG, "null argument");
   const int64_t width = (int64_t)n_kv_heads * head_dim;
-  if (width >= kMost32 || n >= 2 * kMost32 || n * width >= 2 * kMost32)
-    return set_error(PKV_ERR_UNSUPPORTED, "n * n_kv_heads * head_dim must be below 2^32");
+  if (width >= kMost32 || n >= kMost32 || n * width >= kMost32)
+    return set_error(PKV_ERR_UNSUPPORTED, "n * n_kv_heads * head_dim must be below 2^31");
   if (n > 1 && (k_stride < width || v_stride < width))
     return set_error(PKV_ERR_ARG, "a token's row holds all its heads, and rows do not overlap");
   if (k_stride < 0 || v_stride < 0) return set_error(PKV_ERR_ARG, "strides must be >= 0");

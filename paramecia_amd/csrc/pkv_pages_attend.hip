@@ -9,11 +9,21 @@
 // gives zeros. Lengths, tables and row counts are read on the device: the launches of a step do
 // not depend on them, so a captured step serves every later one.
 //
-// Work: a tile is 16 kW rows of one request (row = token x query heads of a KV head); its keys
-// are blocks of 32 (one page each), the sinks' blocks first, then the window's. The blocks of all
-// tiles and KV heads lie in one line, which is cut into equal shares, one a workgroup, whatever
-// the lengths are. A share that holds a whole tile writes its rows of out; the parts of a tile
-// that is cut meet in the join, a launch of their own.
+// Mathematics: with x_j = clamp(scale q.k_j) log2(e), one pass over the keys holds per row the running
+// maximum m, l = sum 2^(x_j - m) and sum 2^(x_j - m) v_j in f32; a larger maximum rescales both. Two
+// parts of a row join as sums weighed with 2^(m_i - max m). The matrix cores take 16-bit operands, and
+// K and V are 16-bit rows already, so that only q and the weights are rounded: they go in as sums of
+// two fp16 parts (F16 pages) or three bf16 parts (BF16), 22 and 24 bits, which costs two or three
+// products for one and keeps a row within 2e-6 of 64-bit sums; one part alone is off by 2^-11 or 2^-8.
+//
+// Work: a tile is 16 to 128 rows of one request (row = token x query heads of a KV head, which share
+// their keys); its keys are blocks of 32 (one page each), the sinks' blocks first, then the window's. The
+// blocks of all tiles and KV heads lie in one line, which is cut into equal shares, one a workgroup,
+// whatever the lengths are: 24 requests of 100 to 17000 keys end together. A share that holds a whole
+// tile writes its rows of out; the parts of a tile that is cut meet in the join, a launch of their own.
+//
+// Bound: of few rows the bytes of the keys (2 rows of 16 bits a key and KV head), of prompts the matrix
+// cores: 4 head_dim flops a key and row, twice (F16) or three times (BF16).
 #include "pkv_half_common.hpp"
 #include "pkv_internal.hpp"
 
@@ -499,13 +509,13 @@ struct Queries {
 };
 
 // Of eight keys from j on, `valid` of them there, the i that the query at position p sees: i <= last,
-// and i > above or i < below.
+// and i > above or i < below. (No key is seen where p < j: the other limits must only not overflow.)
 struct Seen {
   int last, above, below;
 };
 __device__ __forceinline__ Seen seen_of(const AttendArgs &a, int p, int j, int valid) {
   const int x = p - j, y = valid - 1;
-  return Seen{x < y ? x : y, a.window > 0 ? x - a.window : -1, a.sinks - j};
+  return Seen{x < y ? x : y, a.window > 0 ? (x > 0 ? x : 0) - a.window : -1, a.sinks - j};
 }
 
 // A row's softmax, the lane's eight keys 8 g .. 8 g + 7 of a block of row n. Scores come in
@@ -565,10 +575,17 @@ struct Row {
 };
 // Every query of positions p0 .. p1 (p0 below 0: some see nothing) sees all keys j0 .. j0 + 31.
 __device__ __forceinline__ bool all_seen(const AttendArgs &a, int p0, int p1, int j0) {
-  return (j0 + 31 <= p0) & ((a.window <= 0) | (j0 > p1 - a.window) | (j0 + 31 < a.sinks));
+  return (j0 + 31 <= p0) & ((a.window <= 0) | ((int64_t)j0 + a.window > p1) | (j0 + 31 < a.sinks));
 }
 
-// ---- up to 16 kRT rows a tile, for one token and a few. A workgroup of kD / 64 waves: wave w takes
+// ---- up to 16 kRT rows a tile, for one token and a few.
+// Measured (MI355X; 16 query heads over 2 KV heads of 256): 24 tokens of 100 to 17000 BF16 keys each
+// 117 us, 5.0 to 5.4 TB/s of keys (a copy of 2 GiB: 4.8); one token of 131073 BF16 keys 47 us, 5.7 TB/s;
+// one of 1025 F16 keys 7.4 us, four dependent trips to memory (lengths, table, rows, sums of the
+// line); 16 x 5 drafted tokens, F16, a window of 4096: 35 us, 16 of it the keys' bytes, the rest each
+// workgroup's plan, its 40 rows of queries and its parts' rows. Straight into registers since a block's
+// rows serve one tile only: LDS as a stop on the way cost 221 against 166 us at 24 tokens.
+// A workgroup of kD / 64 waves: wave w takes
 // elements 64 w .. of all 32 keys of a block for the scores, and columns 64 w .. of V. Rows go from
 // memory straight into registers as MFMA operands, a block ahead; the waves' partial scores meet
 // in LDS, one barrier a block, and every wave runs the same softmax.
@@ -757,7 +774,17 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
   }
 }
 
-// ---- tiles of 16 kW rows, 16 a wave, for prompts. Blocks' rows of K and V go from memory
+// ---- tiles of 16 kW rows, 16 a wave, for prompts.
+// Measured (MI355X; 16 query heads over 2 KV heads of 256): 512 new tokens over 16896 BF16 keys 335 us,
+// 1.25 PFLOP/s of products in three parts (a library product of 8192^3 in BF16: 1.14); 8001 tokens of
+// F16 in a window of 4096 behind 4 first keys, 250 us, 0.54 PFLOP/s of the keys seen, in two parts. Bound:
+// instructions. Beside a block's 64 (F16) or 96 (BF16) products a wave runs some 290 vector
+// instructions (masks, maximum, exponents, parts), and a SIMD issues one or the other: products alone
+// run at 2.07 PFLOP/s with two waves a SIMD, at 1.35 beside four vector instructions each. Without the
+// softmax (a copy of this kernel) the chunk of 512 takes 258 us instead of 305 in F16, with
+// products and barriers alone 228. 16 rows a wave: 32 (half the reads of LDS) need more than 256
+// registers beside the sums of 256 columns, and one wave a SIMD took 970 us for the 8001 tokens.
+// Blocks' rows of K and V go from memory
 // into LDS ahead of their use; every wave runs its rows from there:
 //   scores (transposed, A = K) with keys in the order of few_kernel; out (transposed, A = V): V's
 //   columns come by transposing reads; the result is columns 16 c + 4 g + i of row n.
@@ -1057,7 +1084,8 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
   }
 }
 
-// ---- the parts of a tile that was cut, joined: a wave a row, or kAcross waves a row of a tile
+// ---- the parts of a tile that was cut, joined (5 us where one token's 1025 keys lie in 64 parts, 9 where
+// 131073 lie in 512, 27 behind 8001 prompt tokens: 256 parts of 128 rows twice over, 64 MB): a wave a row, or kAcross waves a row of a tile
 // of many parts. The parts' maxima and sums come side by side, a lane a part; then their rows, four
 // in flight. By tile where there are fewer tiles than cuts, else by cut: the first cut inside a
 // tile joins it.
@@ -1177,7 +1205,7 @@ __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(
 // many blocks a tile's start costs: 2 of a few rows, 6 of a prompt's (start, queries, first loads and
 // stores take 20000 cycles, a block 4300; 4 and 8 made 8001 tokens in a window 3% slower).
 // Tiles of few rows for requests of up to 48 rows on average: 80 drafted tokens of 40 rows each
-// take 48 us in tiles of 48 and 78 in LDS tiles of 64. Three waves a SIMD hold 16 rows of head_dim
+// take 48 us in tiles of 48 and 78 in the prompts' tiles. Three waves a SIMD hold 16 rows of head_dim
 // 64 and 128 (24 requests of 64: 58 us by two, 44 by three), two anything else.
 struct Shape {
   int rows, shares, start;

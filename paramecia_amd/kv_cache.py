@@ -342,7 +342,10 @@ class PagedKvPool:
         for p in (kp, vp):
             view = _DeviceBytes(p.value, self.n_pages * page_bytes.value)
             view.pool = self
-            planes.append(torch.as_tensor(view, device="cuda").view(dtype).view(shape))
+            plane = torch.as_tensor(view, device="cuda")
+            if plane.data_ptr() != p.value:  # (torch copies what lies on another device)
+                raise KvCacheError("storage: the pool is not on the current device")
+            planes.append(plane.view(dtype).view(shape))
         return tuple(planes)
 
     def take_pages(self, n: int) -> torch.Tensor:

@@ -247,6 +247,48 @@ def test_rows(pk, kind, heads, kv, dim, lens, new):
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,dim", [(64, 1, 64), (20, 1, 128), (96, 2, 256), (33, 11, 64)])
+def test_heads_of_a_kv_head(pk, kind, heads, kv, dim):
+    """More query heads than a row tile holds, and numbers that no tile divides by."""
+    say("heads", kind, heads, kv, dim)
+    Case(19, [70, 1, 0, 333], [1, 1, 1, 1], heads, kv, dim, kind).check(pk, 40, 2)
+    Case(20, [70, 500], [3, 41], heads, kv, dim, kind).check(pk)
+
+
+def test_largest_window_and_sinks(pk):
+    """A window and sinks as large as they can be see everything."""
+    c = Case(21, [300, 5, 0, 90], [20, 5, 3, 90], 16, 2, 256, "f16")
+    want = c.run(pk)
+    for window, sinks in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1), (7, 300)):
+        assert torch.equal(c.run(pk, window, sinks), want)
+    c = Case(22, [300, 5, 0, 90], [1] * 4, 16, 2, 256, "bf16")
+    want = c.run(pk)
+    for window, sinks in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1)):
+        assert torch.equal(c.run(pk, window, sinks), want)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 25])
+def test_queries_that_are_no_numbers(pk, kind, new):
+    """NaN makes its own row NaN, an infinite one scores that are clamped or NaN; zeros weigh all
+    keys alike. Other rows keep their bits where no piece is made again, their values where one is."""
+    c = Case(23, [200, 150], [new, new], 16, 2, 256, kind)
+    c.q = c.q.clone()
+    clean = c.run(pk)
+    c.q[0, 3, 7] = math.nan
+    c.q[new, 11] = 0
+    got = c.run(pk)
+    assert torch.isnan(got[0, 3]).all()
+    keep = torch.ones_like(got, dtype=torch.bool)
+    keep[0, 3], keep[new, 11] = False, False
+    assert torch.isfinite(got[keep]).all() and ((got - clean)[keep].abs() <= 1e-5).all()
+    p = 150 - new
+    rows = [int(c.tables[1, j // c.page]) * c.page + j % c.page for j in range(p + 1)]
+    mean = c.v.view(-1, 2, 256)[rows, 1].double().mean(0)
+    assert ((got[new, 11].double() - mean).abs() <= 1e-5).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("spread", [0.01, 4.0, 40.0])
 def test_scores_small_and_clamped(pk, kind, spread):
     """Scores near nothing, dominant keys, and many past the clamp at 100."""
@@ -495,6 +537,72 @@ def test_verify_at_the_ends(pk):
     tokens, accepted = pk.verify_drafts(target, drafts, u)
     want = verify64(target, drafts, u, None, None)
     assert torch.equal(accepted.cpu(), want[1]) and torch.equal(tokens.cpu(), want[0])
+
+
+def test_nothing_to_do(pk):
+    c = Case(24, [40], [0], 16, 2, 256, "f16")
+    assert c.run(pk).shape == (0, 16, 256)
+    pk.append_pages(c.q[:, :2], c.q[:, :2], torch.empty(0, dtype=torch.int64, device="cuda"), c.k, c.v)
+    tokens, accepted = pk.verify_drafts(torch.empty(0, 3, 9, device="cuda"), i32([]).view(0, 2), torch.empty(0, 3, device="cuda"))
+    assert tokens.shape == (0, 3) and accepted.shape == (0,)
+
+
+def test_verify_and_map_captured_on_another_stream(pk):
+    g = gen(9)
+    n, k, vocab = 3, 4, 5000
+    target, draft, u = probs(g, n, k + 1, vocab), probs(g, n, k, vocab), torch.rand(n, k + 1, device="cuda", generator=g)
+    drafts = draft.argmax(-1).to(torch.int32)
+    lens, add = i32([5, 70, 0]), i32([1, 1, 40])
+    t = Tables(random.Random(2), n, 8, 32, 12, [5, 70, 0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    start = [x.clone() for x in (t.t, t.h, t.free, t.count)]
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            m = pk.map_pages(lens, add, t.t, t.h, t.free, t.count, 32, 64)
+            tokens, accepted = pk.verify_drafts(target, drafts, u, draft_probs=draft)
+    for turn in range(4):
+        new = [[5 + turn, 70, 31 * turn], [1, turn, 40]]
+        with torch.cuda.stream(side):
+            for x, y in zip((t.t, t.h, t.free, t.count), start):
+                x.copy_(y)
+            lens.copy_(i32(new[0]))
+            add.copy_(i32(new[1]))
+            target.copy_(probs(g, n, k + 1, vocab))
+            u.uniform_(generator=g)
+            graph.replay()
+        side.synchronize()
+        want = map_pages64(*new, start[0].tolist(), start[1].tolist(), start[2].tolist()[:start[3].item()], 32, t.capacity, 64)
+        assert m.status.tolist() == [want[0]] == [0]
+        assert m.slots.tolist() == want[4] and m.starts.tolist() == want[6] and t.h.tolist() == want[2]
+        ok = verify64(target, drafts, u, draft, None)
+        assert torch.equal(tokens.cpu(), ok[0]) and torch.equal(accepted.cpu(), ok[1])
+
+
+def test_storage_outlives_the_pool_object(pk):
+    pool = pk.PagedKvPool(1, 64, 32, 4, pk.KvCacheQuantization.BF16)
+    k, v = pool.storage()
+    assert k.shape == (4, 32, 1, 64) and k.dtype is torch.bfloat16 and int((k != 0).sum()) == 0
+    ids = pool.take_pages(4)
+    assert sorted(ids.tolist()) == [0, 1, 2, 3] and pool.take_pages(0).numel() == 0
+    with pytest.raises(pk.KvCacheOverflow):
+        pool.take_pages(1)
+    with pytest.raises(pk.KvCacheOverflow):
+        pool.sequence().append_quantized(torch.zeros(1, 1, 1, 64, device="cuda"), torch.zeros(1, 1, 1, 64, device="cuda"))
+    for bad in ([0, 0], [1, 4], [-1]):
+        with pytest.raises(pk.KvCacheError, match="not taken"):
+            pool.give_pages(torch.tensor(bad, dtype=torch.int32))
+    pool.give_pages(ids[:2])
+    with pytest.raises(pk.KvCacheError, match="not taken"):
+        pool.give_pages(ids[1:3])
+    assert pool.free_pages == 2
+    del pool
+    k.fill_(1)
+    torch.cuda.synchronize()
+    assert float(k.float().sum()) == 4 * 32 * 64
+    with pytest.raises(pk.KvCacheError, match="F16 or BF16"):
+        pk.PagedKvPool(2, 256, 32, 2).storage()
 
 
 # ------------------------------------------------------------------ a step of all of them

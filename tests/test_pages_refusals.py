@@ -52,7 +52,7 @@ def append(**k):
     (dict(n=-1), ERR_ARG, "n must"), (dict(ns=0), ERR_ARG, "n_slots"), (dict(h=0), ERR_ARG, "n_kv_heads"), (dict(d=0), ERR_ARG, "head_dim"),
     (dict(quant=3), ERR_UNSUPPORTED, "F16 or BF16"), (dict(quant=4), ERR_UNSUPPORTED, "F16 or BF16"), (dict(quant=9), ERR_UNSUPPORTED, "F16"),
     (dict(ks=511), ERR_ARG, "overlap"), (dict(vs=256), ERR_ARG, "overlap"), (dict(n=1, ks=-1), ERR_ARG, "strides"),
-    (dict(n=1 << 23), ERR_UNSUPPORTED, "2^32"), (dict(h=1 << 20, d=1 << 20), ERR_UNSUPPORTED, "2^32"),
+    (dict(n=1 << 22), ERR_UNSUPPORTED, "2^31"), (dict(h=1 << 20, d=1 << 20), ERR_UNSUPPORTED, "2^31"),
     (dict(vp=D + 640 * 1024 - 2), ERR_ARG, "overlap"), (dict(kp=A + 20000), ERR_ARG, "overlap"), (dict(vp=C), ERR_ARG, "overlap"),
 ])
 def test_append(k, code, word):

@@ -775,9 +775,9 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
 }
 
 // ---- tiles of 16 kW rows, 16 a wave, for prompts.
-// Measured (MI355X; 16 query heads over 2 KV heads of 256): 512 new tokens over 16896 BF16 keys 335 us,
-// 1.25 PFLOP/s of products in three parts (a library product of 8192^3 in BF16: 1.14); 8001 tokens of
-// F16 in a window of 4096 behind 4 first keys, 250 us, 0.54 PFLOP/s of the keys seen, in two parts. Bound:
+// Measured (MI355X; 16 query heads over 2 KV heads of 256): 512 new tokens over 16896 BF16 keys 325 us,
+// 1.29 PFLOP/s of products in three parts (a library product of 8192^3 in BF16: 1.14); 8001 tokens of
+// F16 in a window of 4096 behind 4 first keys 265 us, 0.51 PFLOP/s of the keys seen, in two parts. Bound:
 // instructions. Beside a block's 64 (F16) or 96 (BF16) products a wave runs some 290 vector
 // instructions (masks, maximum, exponents, parts), and a SIMD issues one or the other: products alone
 // run at 2.07 PFLOP/s with two waves a SIMD, at 1.35 beside four vector instructions each. Without the
@@ -843,8 +843,10 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
   constexpr int kMoves = 4 * kD / kThreads;  // 16-byte pieces of K, and of V, that a thread moves
   // Blocks of K and of V in LDS. Four: two between barriers, the two behind them on their way. Rows
   // of 256 bytes take three, one and one or two, so that three workgroups fit a CU's LDS (8001 tokens in a
-  // window, 32 heads of 128: 360 us, with four 471; of 256, 16 heads: 304 by pairs, 317 one by one).
-  constexpr bool kPairs = kD != 128;
+  // window, 32 heads of 128: 360 us, with four 471; of 256, 16 heads: 304 by pairs, 317 one by one),
+  // and BF16 rows of 512 bytes, whose registers a pair's second block exceeds (512 tokens over 16896
+  // keys: 356 us, by pairs 361).
+  constexpr bool kPairs = kD == 64 || (kD == 256 && !kBf);
   constexpr int kRing = kPairs ? 4 : 3;
   __shared__ __attribute__((aligned(1024))) uint16_t lk[kRing][kBlk * kD], lv[kRing][kBlk * kD];
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
@@ -953,8 +955,9 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
 #pragma unroll
     for (int c = 0; c < kCols; ++c) acc[c] = zero;
     f4 sc[2];
-    // (operands come from LDS kAhead reads ahead of the products that take them)
-    constexpr int kAhead = kBf ? 2 : 4;
+    // operands come from LDS kAhead reads ahead of the products that take them (two: 512 tokens over
+    // 16896 BF16 keys 376 us instead of 356; six and eight: the same within 1%)
+    constexpr int kAhead = 4;
     const auto scores = [&](const uint16_t *kb) {
       constexpr int kReads = 2 * kSteps;
       const int own = kAgain ? k_place(0) : 0;

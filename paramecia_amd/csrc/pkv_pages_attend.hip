@@ -584,7 +584,7 @@ __device__ __forceinline__ bool all_seen(const AttendArgs &a, int p0, int p1, in
 // one of 1025 F16 keys 7.4 us, four dependent trips to memory (lengths, table, rows, sums of the
 // line); 16 x 5 drafted tokens, F16, a window of 4096: 35 us, 16 of it the keys' bytes, the rest each
 // workgroup's plan, its 40 rows of queries and its parts' rows. Straight into registers since a block's
-// rows serve one tile only: LDS as a stop on the way cost 221 against 166 us at 24 tokens.
+// rows serve one tile only (by way of LDS 24 tokens took 166 us, then 139).
 // A workgroup of kD / 64 waves: wave w takes
 // elements 64 w .. of all 32 keys of a block for the scores, and columns 64 w .. of V. Rows go from
 // memory straight into registers as MFMA operands, a block ahead; the waves' partial scores meet
@@ -778,8 +778,8 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
 // Measured (MI355X; 16 query heads over 2 KV heads of 256): 512 new tokens over 16896 BF16 keys 325 us,
 // 1.29 PFLOP/s of products in three parts (a library product of 8192^3 in BF16: 1.14); 8001 tokens of
 // F16 in a window of 4096 behind 4 first keys 265 us, 0.51 PFLOP/s of the keys seen, in two parts. Bound:
-// instructions. Beside a block's 64 (F16) or 96 (BF16) products a wave runs some 290 vector
-// instructions (masks, maximum, exponents, parts), and a SIMD issues one or the other: products alone
+// instructions. Beside a block's 64 (F16) or 96 (BF16) products a wave runs some 170 or 210 vector
+// instructions (maximum, exponents, parts, masks at the window's edges), and a SIMD issues one or the other: products alone
 // run at 2.07 PFLOP/s with two waves a SIMD, at 1.35 beside four vector instructions each. Without the
 // softmax (a copy of this kernel) the chunk of 512 takes 258 us instead of 305 in F16, with
 // products and barriers alone 228. 16 rows a wave: 32 (half the reads of LDS) need more than 256
@@ -1243,7 +1243,10 @@ void join(AttendArgs &a, const Shape &sh, hipStream_t s) {
   const int64_t tiles = (int64_t)a.max_tiles * a.kv_heads;
   const int by_cut = tiles > sh.shares;
   const unsigned x = by_cut ? (unsigned)sh.shares : (unsigned)tiles;
-  if (tiles * 64 <= sh.shares)  // the parts a tile has on average
+  // by the parts a tile has on average, waves a row: 131073 keys in 256 parts a tile 61 us with 16, 76
+  // with four, 140 with one; 8 requests of 3000 keys (32 parts) 20, 25 and 46; 80 drafted tokens (9) 52, 43 and
+  // 48; prompts of 8001 tokens (one or two) 574, 398 and 348
+  if (tiles * 16 <= sh.shares)
     hipLaunchKernelGGL((join_kernel<kD, 16>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
   else if (tiles * 4 <= sh.shares)
     hipLaunchKernelGGL((join_kernel<kD, 4>), dim3(x, sh.rows), dim3(256), 0, s, a, sh.rows, by_cut);

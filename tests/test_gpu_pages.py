@@ -298,6 +298,78 @@ def test_scores_small_and_clamped(pk, kind, spread):
     Case(7, [300, 90], [200, 30], 16, 2, 256, kind, spread=spread).check(pk)
 
 
+def parts(x, n, kind):
+    """x as the sum of n roundings to kind, in 64 bits."""
+    total = torch.zeros_like(x)
+    for _ in range(n):
+        total += (x - total).to(TYPES[kind]).double()
+    return total
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 3, 5, 60])
+@pytest.mark.parametrize("top", [0.5, 16.0])
+def test_precision_of_queries_and_weights(pk, kind, dim, new, top):
+    """Keys and values that are unit vectors: a score is one query element, an output one weight, so
+    that what is off is the roundings alone and a part of a query or a weight less would show.
+
+    In half steps of f32 (E), scores of at most `top` in log2 units: a query's element is off by 2
+    (its factor and the product) and 4 (its parts, F16's 22 bits), a score by 3 more (a part's product at a time) and
+    the exponent's difference by 2 more: 11 top E, times ln 2 below 8 top E of a weight, 2 of exp2, 4 of the
+    weight's parts, 3 of its sum over parts. The sum below it: 8 top + 2 each, a lane adds 8 weights a
+    block of 32 keys and four lanes meet: keys / 4 + 2. A larger maximum and a join: 4 a block and 8; the
+    quotient 4. F16's weights, of 2048 and more for the largest, end at 2^-25: 2^-36 of the sum."""
+    say("precision", kind, dim, new, top)
+    lens = [64, 60, 64]
+    c = Case(25, lens, [new] * 3, 8, 1, dim, kind)
+    c.k.zero_()
+    for b, length in enumerate(lens):
+        for j in range(length):
+            c.k[int(c.tables[b, j // 32]), j % 32, 0, j] = 1
+    c.v = c.k.clone()
+    unit = c.scale * math.log2(math.e)
+    c.q = (torch.rand(c.q.shape, device="cuda", generator=gen(3)) * 2 - 1).mul(top / unit)
+    want, _ = attend64(c.q, c.k, c.v, c.tables, lens, c.scale, c.starts, 0, 0, c.out)
+    bound = (16 * top + 45 + 64 / 4 + 4 * 3) * 2.0 ** -24 * want + 2.0 ** -36
+    got = c.run(pk)
+    off = (got.double() - want).abs()
+    say("   worst share of the bound", round(float((off / bound).max()), 3))
+    assert (off <= bound).all()
+    # the bound would see a part less of the weights (of few bits for small scores), or of the queries
+    few = 1 if kind == "f16" else 2
+    if top < 1:
+        total = parts(want / want.amax(-1, keepdim=True), few, kind) * want.amax(-1, keepdim=True)
+        assert ((total - want).abs() > bound).any()
+    else:
+        c.q = parts(c.q.double() * unit, few, kind) / unit
+        less, _ = attend64(c.q, c.k, c.v, c.tables, lens, c.scale, c.starts, 0, 0, c.out)
+        assert ((less - want).abs() > bound).any()
+
+
+def mix(seed):
+    """Requests, heads, pages and masks drawn together."""
+    r = random.Random(seed)
+    kv, group = r.choice([1, 1, 2, 2, 3, 8]), r.choice([1, 2, 3, 4, 7, 8, 8, 16, 20])
+    dim, kind, page = r.choice([64, 128, 256]), r.choice(["f16", "bf16"]), r.choice([32, 64, 128, 512])
+    most = r.choice([1, 6, 30, 300])
+    n = r.choice([1, 2, 3, 7, 24, 64, 65, 90]) if most < 10 else r.choice([1, 2, 5, 9])
+    longest = r.choice([3, 70, 700, 3000])
+    new = [1 if most == 1 else r.randrange(0, most + 1) for _ in range(n)]
+    lens = [(m if r.random() < 0.85 else 0) + r.randrange(0, longest) for m in new]
+    window = r.choice([0, 0, 1, 5, 31, 32, 33, 200, 1000])
+    return lens, new, group * kv, kv, dim, kind, page, window, r.choice([0, 1, 4, 40, 300])
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_mixes(pk, seed):
+    lens, new, heads, kv, dim, kind, page, window, sinks = mix(seed)
+    say("mix", seed, len(lens), sum(lens), sum(new), heads, kv, dim, kind, page, window, sinks)
+    c = Case(seed, lens, new, heads, kv, dim, kind, page=page, pad=seed % 3 + 1, spread=[0.2, 1, 6][seed % 3], gated=seed % 2 == 0)
+    got = c.check(pk, window, sinks)
+    assert torch.equal(c.run(pk, window, sinks), got)
+
+
 @pytest.mark.parametrize("kind,mag", [("f16", 6e4), ("f16", 1e-6), ("bf16", 1e30), ("bf16", 1e-30)])
 def test_values_near_the_ends_of_their_type(pk, kind, mag):
     c = Case(8, [500, 40], [1, 1], 16, 2, 256, kind)

@@ -31,6 +31,10 @@ namespace pkv {
 namespace {
 
 struct Tile;
+struct Count {
+  int64_t units;  // of a head
+  int tiles;
+};
 struct AttendArgs {
   const float *q;  // token t, head h at t * q_t + h * q_h
   int64_t q_t, q_h;
@@ -41,7 +45,7 @@ struct AttendArgs {
   Tile *tiles;      // [tile]
   int64_t *before;  // [tile + 1]: units of the tiles before it
   int *firsts;      // [share]: the tile that its first block is of
-  int *count;       // tiles
+  Count *count;
   float *part;      // [2 workgroup + (not its first piece)][row][head_dim]
   float2 *ml;       // [..][row]: running max (log2 units), sum
   unsigned *status;
@@ -141,8 +145,8 @@ __device__ __forceinline__ Line line_of(const AttendArgs &a, int tiles, int64_t 
   return l;
 }
 __device__ __forceinline__ Line line_of(const AttendArgs &a) {
-  const int tiles = *a.count;
-  return line_of(a, tiles, a.before[tiles]);
+  const Count c = *a.count;
+  return line_of(a, c.tiles, c.units);
 }
 // The tile that holds unit u of a head (u below the head's units).
 __device__ __forceinline__ int tile_at(const AttendArgs &a, int tiles, int64_t u) {
@@ -225,7 +229,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(AttendArgs a, int ro
   }
   if (tid == 0) {
     a.before[count] = blocks;
-    *a.count = count;
+    *a.count = Count{blocks, count};
   }
   __syncthreads();
   const Line line = line_of(a, count, blocks);
@@ -311,18 +315,19 @@ struct Plan<true> {
     if (blockIdx.x == 0) {
       for (int t = tid; t <= count; t += threads) a.before[t] = p.before[t];
       for (int t = tid; t < count; t += threads) a.tiles[t] = p.tiles[t];
-      if (tid == 0) *a.count = count;
+      if (tid == 0) *a.count = Count{line.per_head, count};
     }
   }
   __device__ __forceinline__ int64_t before(const AttendArgs &, int x) const { return uniform(lds->before[x]); }
   __device__ __forceinline__ Tile tile(const AttendArgs &, int x) const { return uniform(lds->tiles[x]); }
-  __device__ __forceinline__ int first(const AttendArgs &, int share) const {
+  __device__ __forceinline__ int first(const AttendArgs &a, int share) const {
     const int64_t u = line.start(share) - line.head(line.start(share)) * line.per_head;
     int x = -1;  // tiles that begin at u or before it
     for (int t0 = 0; t0 < line.tiles; t0 += 64) {
       const int t = t0 + (int)(threadIdx.x & 63);
       x += __builtin_popcountll(__ballot(t < line.tiles && lds->before[t < line.tiles ? t : 0] <= u));
     }
+    if (threadIdx.x == 0) a.firsts[share] = x;
     return x;
   }
 };
@@ -1115,6 +1120,13 @@ __device__ __forceinline__ void join_parts(const AttendArgs &a, Slot slot, int i
   for (int b = i0; b < i1; b += 64) {
     const int count = i1 - b < 64 ? i1 - b : 64;
     const float2 ml = lane < count ? a.ml[slot(b + lane)] : float2{-INFINITY, 0.0f};
+    float x[4][kE];
+    const auto load = [&](int i) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        load_elems<kE>(a.part + slot(b + (i + y < count ? i + y : count - 1)) * (64 * kE) + lane * kE, x[y]);
+    };
+    load(0);
     float top = xmax32(xmax16(ml.x));
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -1127,10 +1139,6 @@ __device__ __forceinline__ void join_parts(const AttendArgs &a, Slot slot, int i
     for (int e = 0; e < kE; ++e) acc[e] *= c;
     m = mn;
     for (int i = 0; i < count; i += 4) {
-      float x[4][kE];
-#pragma unroll
-      for (int y = 0; y < 4; ++y)
-        load_elems<kE>(a.part + slot(b + (i + y < count ? i + y : count - 1)) * (64 * kE) + lane * kE, x[y]);
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         if (i + y >= count) break;  // (the last part again, which may hold infinities)
@@ -1138,6 +1146,7 @@ __device__ __forceinline__ void join_parts(const AttendArgs &a, Slot slot, int i
 #pragma unroll
         for (int e = 0; e < kE; ++e) acc[e] += f * x[y][e];
       }
+      if (i + 4 < count) load(i + 4);
     }
   }
 }
@@ -1147,27 +1156,27 @@ __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(
   constexpr int kE = kD / 64;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Line line = line_of(a);
-  int h, x, w0;  // w0: the share that holds the tile's first block
+  // (what the plan says of the tile is asked for together, whether there is such a tile or not)
+  const int cut = (int)blockIdx.x + 1;
+  if (by_cut && cut >= line.shares) return;
+  const int x = by_cut ? a.firsts[cut] : (int)blockIdx.x / a.kv_heads;
+  const int64_t before = a.before[x], behind = a.before[x + 1];
+  const Tile t = a.tiles[x];
+  int h, w0;  // w0: the share that holds the tile's first block
   if (by_cut) {
-    const int cut = blockIdx.x + 1;
-    if (cut >= line.shares) return;
     const int64_t u = line.start(cut);
     h = line.head(u);
-    x = tile_at(a, line.tiles, u - h * line.per_head);
-    const int64_t first = h * line.per_head + a.before[x] + a.start;
+    const int64_t first = h * line.per_head + before + a.start;
     if (u <= first || (cut > 1 && line.start(cut - 1) > first)) return;
     w0 = cut - 1;
   } else {
     h = (int)blockIdx.x % a.kv_heads;
-    x = (int)blockIdx.x / a.kv_heads;
-    if (x >= line.tiles || a.before[x + 1] == a.before[x]) return;
-    const int64_t first = h * line.per_head + a.before[x] + a.start;
-    w0 = line.share(first);
+    if (x >= line.tiles || behind == before) return;
+    w0 = line.share(h * line.per_head + before + a.start);
   }
-  const int64_t tile0 = h * line.per_head + a.before[x], last = h * line.per_head + a.before[x + 1];
+  const int64_t tile0 = h * line.per_head + before, last = h * line.per_head + behind;
   if (line.start(w0 + 1) >= last) return;  // not cut
   const int pieces = line.share(last - 1) - w0 + 1, odd = line.start(w0) < tile0 ? 1 : 0;
-  const Tile t = a.tiles[x];
   const int row = kAcross > 1 ? (int)blockIdx.y : (int)blockIdx.y * 4 + wave;
   if (row >= t.rows) return;
   const auto slot = [&](int i) { return (2 * (int64_t)(w0 + i) + (i == 0 ? odd : 0)) * rows_per_tile + row; };
@@ -1306,7 +1315,7 @@ int launch_pages_attend(const PagesAttend &p, void *ws, hipStream_t s) {
   a.tiles = reinterpret_cast<Tile *>(w + l.tiles);
   a.before = reinterpret_cast<int64_t *>(w + l.before);
   a.firsts = reinterpret_cast<int *>(w + l.firsts);
-  a.count = reinterpret_cast<int *>(w + l.count);
+  a.count = reinterpret_cast<Count *>(w + l.count);
   a.ml = reinterpret_cast<float2 *>(w + l.ml);
   a.part = reinterpret_cast<float *>(w + l.part);
   a.n = p.n;

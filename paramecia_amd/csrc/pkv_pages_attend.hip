@@ -587,13 +587,15 @@ __device__ __forceinline__ bool all_seen(const AttendArgs &a, int p0, int p1, in
 // Measured (MI355X; 16 query heads over 2 KV heads of 256): 24 tokens of 100 to 17000 BF16 keys each
 // 117 us, 5.0 to 5.4 TB/s of keys (a copy of 2 GiB: 4.8); one token of 131073 BF16 keys 47 us, 5.7 TB/s;
 // one of 1025 F16 keys 7.4 us, four dependent trips to memory (lengths, table, rows, sums of the
-// line); 16 x 5 drafted tokens, F16, a window of 4096: 35 us, 16 of it the keys' bytes, the rest each
+// line); 16 x 5 drafted tokens, F16, a window of 4096: 30 us, 16 of it the keys' bytes, the rest each
 // workgroup's plan, its 40 rows of queries and its parts' rows. Straight into registers since a block's
 // rows serve one tile only (by way of LDS 24 tokens took 166 us, then 139).
 // A workgroup of kD / 64 waves: wave w takes
 // elements 64 w .. of all 32 keys of a block for the scores, and columns 64 w .. of V. Rows go from
 // memory straight into registers as MFMA operands, a block ahead; the waves' partial scores meet
-// in LDS, one barrier a block, and every wave runs the same softmax.
+// in LDS, one barrier a block, and of a single row tile every wave runs the softmax itself. Of two and
+// three each tile's softmax is one wave's, which hands the weights on behind a second barrier (80
+// drafted tokens: 30 us, 35 where every wave ran all three).
 //   scores (transposed, A = K): lane (r, g) holds 8 elements of key 8 (r / 4) + 4 t + r % 4 for
 //   tile t, so that the result (row n, keys 8 g + 4 t + i) is the weights' operand as it is;
 //   out (transposed, A = V): lane (m, g) holds columns 4 m + j (tile j) of keys 8 g .. + 7, pairs
@@ -603,7 +605,11 @@ constexpr int kScoreRow = 36;  // floats, 32 keys and a pad that spreads rows ov
 template <bool kBf, int kD, int kRT, bool kHere>
 __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
   constexpr int kW = kD / 64, kRows = 16 * kRT, kP = kParts<kBf>;
-  __shared__ __attribute__((aligned(16))) float sc[2][kW][kRows][kScoreRow];
+  // Of several row tiles each wave runs the softmax of its own and hands the weights on
+  constexpr bool kOwn = kRT > 1 && kW > 1;
+  __shared__ __attribute__((aligned(16))) float sc[kOwn ? 1 : 2][kW][kRows][kScoreRow];
+  __shared__ u4 s_weights[kOwn ? kRT : 1][kP][64];
+  __shared__ float s_alpha[kRT][16], s_l[kRT][16];
   __shared__ uint32_t s_bad;
   __shared__ typename Plan<kHere>::Lds s_plan;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
@@ -679,7 +685,7 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
     for (int i = i0; i < i1; ++i, turn ^= 1) {
       const int j0 = t.block(i) << 5;
       const bool more = i + 1 < i1;
-      float(*all_sc)[kRows][kScoreRow] = sc[turn];
+      float(*all_sc)[kRows][kScoreRow] = sc[kOwn ? 0 : turn];
 #pragma unroll
       for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
@@ -713,9 +719,7 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
       }
       lds_barrier();
       const bool all = (now_valid == kBlk) & (t.rows == kRows) & all_seen(a, t.p0, t.p1, j0);
-#pragma unroll
-      for (int rt = 0; rt < kRT; ++rt) {
-        float c[8];
+      const auto raise = [&](int rt, float (&c)[8], float &alpha) {
 #pragma unroll
         for (int w = 0; w < kW; ++w)
 #pragma unroll
@@ -726,18 +730,51 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
             c[4 * y + 2] = w ? c[4 * y + 2] + f.z : f.z;
             c[4 * y + 3] = w ? c[4 * y + 3] + f.w : f.w;
           }
-        float alpha = 1.0f;
-        if (row[rt].raise(c, 1.0f, all, [&] { return seen_of(a, pos[rt], j0 + 8 * g, now_valid - 8 * g); }, alpha))
+        return row[rt].raise(c, 1.0f, all, [&] { return seen_of(a, pos[rt], j0 + 8 * g, now_valid - 8 * g); }, alpha);
+      };
+      const auto rescale = [&](int rt, float alpha) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[rt][j][e] *= alpha;
-        u4 pb[kP];
-        row[rt].weights(c, 1.0f, pb);
+          for (int e = 0; e < 4; ++e) acc[rt][j][e] *= alpha;
+      };
+      const auto add = [&](int rt, const u4 (&pb)[kP]) {
 #pragma unroll
         for (int p = kP - 1; p >= 0; --p)
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[rt][j] = half_mfma<kBf>(A[j], pb[p], acc[rt][j]);
+      };
+      if constexpr (kOwn) {
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt) {
+          if (rt % kW != wave) continue;
+          u4 pb[kP];
+          float c[8], alpha = 1.0f;
+          raise(rt, c, alpha);
+          row[rt].weights(c, 1.0f, pb);
+#pragma unroll
+          for (int p = 0; p < kP; ++p) s_weights[rt][p][lane] = pb[p];
+          if (g == 0) s_alpha[rt][n] = alpha;
+        }
+        lds_barrier();  // (the next scores are written behind it, the next weights behind the barrier after)
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt) {
+          u4 pb[kP];
+#pragma unroll
+          for (int p = 0; p < kP; ++p) pb[p] = s_weights[rt][p][lane];
+          const float alpha = s_alpha[rt][n];
+          if (__any(alpha != 1.0f)) rescale(rt, alpha);
+          add(rt, pb);
+        }
+      } else {
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt) {
+          float c[8], alpha = 1.0f;
+          if (raise(rt, c, alpha)) rescale(rt, alpha);
+          u4 pb[kP];
+          row[rt].weights(c, 1.0f, pb);
+          add(rt, pb);
+        }
       }
     }
     // ---- the piece's rows
@@ -745,8 +782,11 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
     bool bad = false;
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt) {
-      l[rt] = row[rt].sum();
-      bad |= !(l[rt] < INFINITY);
+      if (!kOwn || rt % kW == wave) {
+        l[rt] = row[rt].sum();
+        bad |= !(l[rt] < INFINITY);
+        if (kOwn && g == 0) s_l[rt][n] = l[rt];
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -767,13 +807,14 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
       for (int rt = 0; rt < kRT; ++rt) {
         const int y = 16 * rt + n;
         if (y >= t.rows) continue;
+        if (kOwn) l[rt] = s_l[rt][n];
         const int64_t at = to.slot * kRows + y;
         float *o = (to.whole ? row_out(a, t, h, y, kD) : a.part + at * kD) + 64 * wave + 16 * g;
         const float f = !to.whole ? 1.0f : l[rt] > 0.0f ? 1.0f / l[rt] : 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           reinterpret_cast<float4 *>(o)[e] = float4{acc[rt][0][e] * f, acc[rt][1][e] * f, acc[rt][2][e] * f, acc[rt][3][e] * f};
-        if (!to.whole && wave == 0 && g == 0) a.ml[at] = float2{row[rt].m, l[rt]};
+        if (!to.whole && wave == (kOwn ? rt % kW : 0) && g == 0) a.ml[at] = float2{row[rt].m, l[rt]};
       }
     }
   }

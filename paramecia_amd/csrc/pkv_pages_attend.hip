@@ -19,7 +19,7 @@
 // Work: a tile is 16 to 128 rows of one request (row = token x query heads of a KV head, which share
 // their keys); its keys are blocks of 32 (one page each), the sinks' blocks first, then the window's. The
 // blocks of all tiles and KV heads lie in one line, which is cut into equal shares, one a workgroup,
-// whatever the lengths are: 24 requests of 100 to 17000 keys end together. A share that holds a whole
+// whatever the lengths are: 24 requests of 65 to 65536 keys end together. A share that holds a whole
 // tile writes its rows of out; the parts of a tile that is cut meet in the join, a launch of their own.
 //
 // Bound: of few rows the bytes of the keys (2 rows of 16 bits a key and KV head), of prompts the matrix
@@ -584,8 +584,8 @@ __device__ __forceinline__ bool all_seen(const AttendArgs &a, int p0, int p1, in
 }
 
 // ---- up to 16 kRT rows a tile, for one token and a few.
-// Measured (MI355X; 16 query heads over 2 KV heads of 256): 24 tokens of 100 to 17000 BF16 keys each
-// 117 us, 5.0 to 5.4 TB/s of keys (a copy of 2 GiB: 4.8); one token of 131073 BF16 keys 47 us, 5.7 TB/s;
+// Measured (MI355X; 16 query heads over 2 KV heads of 256): 24 tokens of 300000 BF16 keys in all
+// 117 us, 5.2 TB/s of keys (a copy of 2 GiB: 4.8); one token of 131073 BF16 keys 47 us, 5.7 TB/s;
 // one of 1025 F16 keys 7.4 us, four dependent trips to memory (lengths, table, rows, sums of the
 // line); 16 x 5 drafted tokens, F16, a window of 4096: 30 us, 16 of it the keys' bytes, the rest each
 // workgroup's plan, its 40 rows of queries and its parts' rows. Straight into registers since a block's
@@ -821,9 +821,9 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
 }
 
 // ---- tiles of 16 kW rows, 16 a wave, for prompts.
-// Measured (MI355X; 16 query heads over 2 KV heads of 256): 512 new tokens over 16896 BF16 keys 325 us,
-// 1.29 PFLOP/s of products in three parts (a library product of 8192^3 in BF16: 1.14); 8001 tokens of
-// F16 in a window of 4096 behind 4 first keys 265 us, 0.51 PFLOP/s of the keys seen, in two parts. Bound:
+// Measured (MI355X; 16 query heads over 2 KV heads of 256): 512 new tokens over 16896 BF16 keys 310 us,
+// 1.35 PFLOP/s of products in three parts (a library product of 8192^3 in BF16: 1.14); 8001 tokens of
+// F16 in a window of 1024 behind 4 first keys 265 us, 0.84 PFLOP/s of the keys seen in two parts. Bound:
 // instructions. Beside a block's 64 (F16) or 96 (BF16) products a wave runs some 170 or 210 vector
 // instructions (maximum, exponents, parts, masks at the window's edges), and a SIMD issues one or the other: products alone
 // run at 2.07 PFLOP/s with two waves a SIMD, at 1.35 beside four vector instructions each. Without the
@@ -1133,8 +1133,9 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
   }
 }
 
-// ---- the parts of a tile that was cut, joined (5 us where one token's 1025 keys lie in 64 parts, 9 where
-// 131073 lie in 512, 27 behind 8001 prompt tokens: 256 parts of 128 rows twice over, 64 MB): a wave a row, or kAcross waves a row of a tile
+// ---- the parts of a tile that was cut, joined (4.5 us where one token's 1025 keys lie in 64 parts, 7 for 24
+// requests and for 131073 keys in 512, 23 behind 8001 prompt tokens: 256 parts of 128 rows twice over, 64
+// MB). Bound: two trips to memory and a launch, or the parts' bytes. A wave a row, or kAcross waves a row of a tile
 // of many parts. The parts' maxima and sums come side by side, a lane a part; then their rows, four
 // in flight. By tile where there are fewer tiles than cuts, else by cut: the first cut inside a
 // tile joins it.

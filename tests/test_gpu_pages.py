@@ -611,6 +611,46 @@ def test_verify_at_the_ends(pk):
     assert torch.equal(accepted.cpu(), want[1]) and torch.equal(tokens.cpu(), want[0])
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_more_tiles_than_shares(pk, kind):
+    """Many KV heads of short requests: parts are joined by cut, from the workgroups' own plan and
+    from the plan's launch."""
+    r = random.Random(4)
+    for n, new in ((64, 16), (70, 16), (20, 40)):
+        lens = [r.choice([0, 16, 40, 300, 700]) for _ in range(n)]
+        say("more tiles", kind, n, new, sum(lens))
+        Case(26, lens, [min(new, x) if i % 9 else 0 for i, x in enumerate(lens)], 8, 8, 256, kind).check(pk, 200 if n == 70 else 0, 3)
+
+
+def test_two_calls_at_once(pk):
+    """Calls on two streams, eager and as two graphs that are replayed together, each with a workspace
+    of its own."""
+    cases = [(Case(27, [9000, 40, 700], [1, 1, 1], 16, 2, 256, "bf16"), 0), (Case(28, [900, 600], [700, 300], 16, 2, 256, "f16"), 256),
+             (Case(29, [3000] * 8, [5] * 8, 16, 2, 256, "bf16"), 1000), (Case(30, [2000] * 30, [1] * 30, 32, 8, 128, "f16"), 0)]
+    want = [c.run(pk, w, 2) for c, w in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    graphs = [torch.cuda.CUDAGraph() for _ in cases]
+    outs = [c.out.clone() for c, _ in cases]
+    lens = [i32(c.lens) for c, _ in cases]
+    call = lambda i: pk.attend_pages(cases[i][0].q, cases[i][0].k, cases[i][0].v, cases[i][0].tables, lens[i], cases[i][0].scale,  # noqa: E731
+                                     starts=cases[i][0].starts, window=cases[i][1], sinks=2, out=outs[i])
+    for i, stream in enumerate(streams):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream), torch.cuda.graph(graphs[i], stream=stream):
+            call(i)
+    for turn in range(6):
+        for x in outs:
+            x.fill_(turn)
+        torch.cuda.synchronize()
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                call(i) if turn % 2 else graphs[i].replay()
+        torch.cuda.synchronize()
+        for x, y in zip(outs, want):
+            assert torch.equal(x, y)
+
+
 def test_nothing_to_do(pk):
     c = Case(24, [40], [0], 16, 2, 256, "f16")
     assert c.run(pk).shape == (0, 16, 256)

@@ -81,6 +81,12 @@ class Tables:
     (1025, 300, 32, 3, 4097),            # more requests than threads
     (4500, 100, 64, 5, 4500 * 5),        # starts that do not fit LDS
     (3, 70000, 1024, 9000, 30000),       # one request takes many pages
+    (256, 2000, 64, 4, 1024),            # a thread a request, slots in the same launch
+    (257, 2000, 32, 4, 1024),
+    (256, 2000, 32, 5, 1025),            # and in one of their own
+    (1025, 100, 32, 1, 1000),
+    (4097, 70, 32, 1, 700),              # starts that do not fit LDS, few rows
+    (5000, 70, 32, 0, 0),
 ])
 def test_map_over_steps(pk, n, longest, page, most, max_tokens):
     say("map", n, longest, page, most)

@@ -824,13 +824,13 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
 // Measured (MI355X; 16 query heads over 2 KV heads of 256): 512 new tokens over 16896 BF16 keys 310 us,
 // 1.35 PFLOP/s of products in three parts (a library product of 8192^3 in BF16: 1.14); 8001 tokens of
 // F16 in a window of 1024 behind 4 first keys 265 us, 0.84 PFLOP/s of the keys seen in two parts. Bound:
-// products and, in F16, reads of LDS (32 KB a wave and block, so 2048 cycles a CU, as many as the products of
-// a SIMD's two waves), in turn with the softmax. Beside a block's 64 (F16) or 96 (BF16) products a wave runs some 170 or 210 vector
-// instructions (maximum, exponents, parts, masks at the window's edges), and a SIMD issues one or the other: products alone
-// run at 2.07 PFLOP/s with two waves a SIMD, at 1.35 beside four vector instructions each. Without the
-// softmax (a copy of this kernel) the chunk of 512 takes 258 us instead of 305 in F16, with
-// products and barriers alone 228. 16 rows a wave: 32 (half the reads of LDS) need more than 256
-// registers beside the sums of 256 columns, and one wave a SIMD took 970 us for the 8001 tokens.
+// instructions. Beside a block's 64 (F16) or 96 (BF16) products a wave runs some 170 or 210 vector
+// instructions (maximum, exponents, parts, masks at the window's edges), and a SIMD issues one or the
+// other: products alone run at 2.07 PFLOP/s with two waves a SIMD, at 1.35 beside four vector instructions
+// each. Without the softmax (a copy of this kernel) the chunk of 512 takes 258 us instead of 305 in F16,
+// with products and barriers alone 228. 16 rows a wave: 32, with half the reads of LDS, need more than 256
+// registers beside the sums of 256 columns (one wave a SIMD: 970 us for the 8001 tokens), and where they
+// fit (head_dim 128) gain 4% in F16 and nothing in BF16.
 // Blocks' rows of K and V go from memory
 // into LDS ahead of their use; every wave runs its rows from there:
 //   scores (transposed, A = K) with keys in the order of few_kernel; out (transposed, A = V): V's

@@ -10,8 +10,9 @@
 // not depend on them, so a captured step serves every later one.
 //
 // Mathematics: with x_j = clamp(scale q.k_j) log2(e), one pass over the keys holds per row the running
-// maximum m, l = sum 2^(x_j - m) and sum 2^(x_j - m) v_j in f32; a larger maximum rescales both. Two
-// parts of a row join as sums weighed with 2^(m_i - max m). The matrix cores take 16-bit operands, and
+// maximum m, l = sum 2^(x_j - m) and sum 2^(x_j - m) v_j in f32; a larger maximum rescales both. Parts
+// of a row are kept as means, and join as those weighed with their share 2^(m_i - max m) l_i of the
+// sum: BF16 values reach 3.4e38, whose mean f32 holds and whose sum it does not. The matrix cores take 16-bit operands, and
 // K and V are 16-bit rows already, so that only q and the weights are rounded: they go in as sums of
 // two fp16 parts (F16 pages) or three bf16 parts (BF16), 22 and 24 bits, which costs two or three
 // products for one and keeps a row within 2e-6 of 64-bit sums; one part alone is off by 2^-11 or 2^-8.
@@ -46,7 +47,7 @@ struct AttendArgs {
   int64_t *before;  // [tile + 1]: units of the tiles before it
   int *firsts;      // [share]: the tile that its first block is of
   Count *count;
-  float *part;      // [2 workgroup + (not its first piece)][row][head_dim]
+  float *part;      // [2 workgroup + (not its first piece)][row][head_dim]: means
   float2 *ml;       // [..][row]: running max (log2 units), sum
   unsigned *status;
   int n, tokens, heads, kv_heads, group, page_lg, n_pages, max_pages, window, sinks, max_tiles, shares, start;
@@ -370,7 +371,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const uint8_t *plane, 
 
 // Row `row` of a tile over its blocks [i0, i1) in plain f32 products of the keys that it sees
 // alone: for pieces that met infinities or NaN, where split operands and masked keys' zero
-// weights would make more NaN than the formula does. The lane owns kE elements; m in log2 units.
+// weights would make more NaN than the formula does, or whose sums passed f32: acc is the mean so far. The
+// lane owns kE elements; m in log2 units.
 template <bool kBf, int kE>
 __device__ __forceinline__ void plain_row(const AttendArgs &a, const Tile &t, int h, int row, int i0, int i1,
                                           int lane, float &m, float &l, float (&acc)[kE]) {
@@ -401,15 +403,17 @@ __device__ __forceinline__ void plain_row(const AttendArgs &a, const Tile &t, in
       s = s > kClampL2 ? kClampL2 : s < -kClampL2 ? -kClampL2 : s;  // (NaN stays)
       const float mn = fmaxf(m, s == s ? s : -kClampL2);             // (a key that was seen)
       const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(s - mn);
-      l = l * c + w;
+      const float before = l * c;
+      l = before + w;
+      const float by = 1.0f / l, kept = before * by, now = w * by;
 #pragma unroll
-      for (int e = 0; e < kE; ++e) acc[e] = acc[e] * c + w * half_value(v[j * stride + e], kBf);
+      for (int e = 0; e < kE; ++e) acc[e] = acc[e] * kept + now * half_value(v[j * stride + e], kBf);
       m = mn;
     }
   }
 }
 
-// Where a piece's rows go: out if it is the whole tile, else the share's slot.
+// Where a piece's rows go: out if it is the whole tile, else the share's slot, as means either way.
 struct Sink {
   bool whole;
   int64_t slot;
@@ -427,7 +431,7 @@ __device__ __forceinline__ void plain_store(const AttendArgs &a, const Tile &t, 
   const int64_t at = to.slot * rows_per_tile + row;
   float *o = to.whole ? row_out(a, t, h, row, kD) : a.part + at * kD;
 #pragma unroll
-  for (int e = 0; e < kE; ++e) o[lane * kE + e] = !to.whole ? acc[e] : m == -INFINITY ? 0.0f : acc[e] / l;
+  for (int e = 0; e < kE; ++e) o[lane * kE + e] = acc[e];
   if (!to.whole && lane == 0) a.ml[at] = float2{m, l};
 }
 
@@ -810,7 +814,7 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
         if (kOwn) l[rt] = s_l[rt][n];
         const int64_t at = to.slot * kRows + y;
         float *o = (to.whole ? row_out(a, t, h, y, kD) : a.part + at * kD) + 64 * wave + 16 * g;
-        const float f = !to.whole ? 1.0f : l[rt] > 0.0f ? 1.0f / l[rt] : 0.0f;
+        const float f = l[rt] > 0.0f ? 1.0f / l[rt] : 0.0f;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           reinterpret_cast<float4 *>(o)[e] = float4{acc[rt][0][e] * f, acc[rt][1][e] * f, acc[rt][2][e] * f, acc[rt][3][e] * f};
@@ -1125,7 +1129,7 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
     } else if (mine) {
       const int64_t at = to.slot * kRows + y;
       float *o = (to.whole ? row_out(a, t, h, y, kD) : a.part + at * kD) + 4 * g;
-      const float f = !to.whole ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+      const float f = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
       for (int cc = 0; cc < kCols; ++cc)
         *reinterpret_cast<float4 *>(o + 16 * cc) = float4{acc[cc][0] * f, acc[cc][1] * f, acc[cc][2] * f, acc[cc][3] * f};
@@ -1152,7 +1156,7 @@ __device__ __forceinline__ void load_elems(const float *p, float (&x)[kE]) {
     x[0] = *p;
   }
 }
-// Parts [i0, i1) of a row: slot(i) is where part i's row is.
+// Parts [i0, i1) of a row, their mean: slot(i) is where part i's row is.
 template <int kE, typename Slot>
 __device__ __forceinline__ void join_parts(const AttendArgs &a, Slot slot, int i0, int i1, int lane, float &m, float &l,
                                            float (&acc)[kE]) {
@@ -1175,11 +1179,12 @@ __device__ __forceinline__ void join_parts(const AttendArgs &a, Slot slot, int i
     for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
     if (top == -INFINITY) continue;
     const float mn = fmaxf(m, top), c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+    const float before = l * c, own = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn) * ml.y;
     // (a part that saw nothing wrote zeros: a weight of 0 takes it out)
-    l = l * c + wave_sum(w * ml.y);
+    l = before + wave_sum(own);
+    const float by = 1.0f / l, w = own * by;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) acc[e] *= c;
+    for (int e = 0; e < kE; ++e) acc[e] *= before * by;
     m = mn;
     for (int i = 0; i < count; i += 4) {
 #pragma unroll
@@ -1228,7 +1233,7 @@ __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(
     join_parts<kE>(a, slot, 0, pieces, lane, m, l, acc);
     float *o = row_out(a, t, h, row, kD) + lane * kE;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) o[e] = m == -INFINITY ? 0.0f : acc[e] / l;
+    for (int e = 0; e < kE; ++e) o[e] = acc[e];
   } else {
     __shared__ float part[kAcross][kD], s_m[kAcross], s_l[kAcross];
     const int per = (pieces + kAcross - 1) / kAcross;
@@ -1245,14 +1250,16 @@ __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < kAcross; ++i) top = fmaxf(top, s_m[i]);
-    float sum = 0.0f, all = 0.0f;
+    float w[kAcross], all = 0.0f, mean = 0.0f;
 #pragma unroll
     for (int i = 0; i < kAcross; ++i) {
-      const float w = s_m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[i] - top);
-      all += s_l[i] * w;
-      sum += part[i][threadIdx.x] * w;
+      w[i] = s_m[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[i] - top) * s_l[i];
+      all += w[i];
     }
-    row_out(a, t, h, row, kD)[threadIdx.x] = top == -INFINITY ? 0.0f : sum / all;
+    const float by = top == -INFINITY ? 0.0f : 1.0f / all;
+#pragma unroll
+    for (int i = 0; i < kAcross; ++i) mean += part[i][threadIdx.x] * (w[i] * by);
+    row_out(a, t, h, row, kD)[threadIdx.x] = mean;
   }
 }
 

@@ -64,6 +64,12 @@ def _call(rc: int) -> None:
         raise _ERRORS.get(rc, KvCacheError)(f"[pkv {rc}] {msg}")
 
 
+def _past_32_bits(names: str, *values) -> None:
+    """For numbers that C takes as int: ctypes would drop what is above 31 bits without a word, so
+    that a call asks `(a | b | ..) >> 31` of them first (0 for none below 0 or past 2^31 - 1)."""
+    raise KvCacheError(f"{names} must be in [0, 2^31), got {values}")
+
+
 # torch's own accessors of the current device and its current stream as plain integers:
 # torch.cuda.current_stream() builds a Stream object per call (2.8 us, of the 13 us a short
 # decode step took on the host; 0.3 us this way).
@@ -292,6 +298,8 @@ class PagedKvPool:
     def __init__(self, num_kv_heads: int, head_dim: int, page_tokens: int, n_pages: int,
                  quant: KvCacheQuantization = KvCacheQuantization.Q4K,
                  stream: Optional[int] = None):
+        if (num_kv_heads | head_dim | page_tokens | n_pages) >> 31:
+            _past_32_bits("num_kv_heads, head_dim, page_tokens and n_pages", num_kv_heads, head_dim, page_tokens, n_pages)
         h = ctypes.c_void_p()
         self._stream = stream if stream is not None else _stream()
         _call(lib().pkv_pool_create(int(quant), num_kv_heads, head_dim, page_tokens, n_pages,
@@ -351,7 +359,9 @@ class PagedKvPool:
     def take_pages(self, n: int) -> torch.Tensor:
         """n free pages out of the reach of the pool's sequences, for tables on the device
         (pkv_pool_take_pages): their ids, int32 on the host."""
-        ids = torch.empty(max(n, 0), dtype=torch.int32)
+        if n >> 31:
+            _past_32_bits("n", n)
+        ids = torch.empty(n, dtype=torch.int32)
         _call(lib().pkv_pool_take_pages(self._h, n, ctypes.cast(ids.data_ptr(), ctypes.POINTER(ctypes.c_int))))
         return ids
 
@@ -359,6 +369,8 @@ class PagedKvPool:
         """Pages of take_pages back to the pool's sequences; ids as take_pages gives them."""
         if ids.is_cuda or ids.dtype is not torch.int32 or ids.dim() != 1:
             raise KvCacheError("give_pages takes int32 ids on the host")
+        if ids.numel() >> 31:
+            _past_32_bits("their number", ids.numel())
         ids = ids.contiguous()
         _call(lib().pkv_pool_give_pages(self._h, ids.numel(), ctypes.cast(ids.data_ptr(), ctypes.POINTER(ctypes.c_int))))
 

@@ -15,7 +15,7 @@ import torch
 
 from . import _lib
 from ._lib import lib
-from .kv_cache import KvCacheError, _at, _call, _device, _stream, _take
+from .kv_cache import KvCacheError, _at, _call, _device, _past_32_bits, _stream, _take
 
 _PAGES = {torch.float16: _lib.QUANT_F16, torch.bfloat16: _lib.QUANT_BF16}
 
@@ -53,15 +53,16 @@ def map_pages(lens: torch.Tensor, add: torch.Tensor, tables: torch.Tensor, held:
     n = lens.shape[0] if lens.dim() == 1 else 0
     if n == 0 or tables.dim() != 2 or free_pages.dim() != 1:
         raise KvCacheError("map_pages expects lens [n], tables [n, max_pages] and free_pages [capacity]")
+    max_pages, capacity = tables.shape[1], free_pages.shape[0]
+    if (n | max_pages | capacity | page_tokens | max_tokens) >> 31:
+        _past_32_bits("n, max_pages, capacity, page_tokens and max_tokens", n, max_pages, capacity, page_tokens, max_tokens)
     i32 = torch.int32
     lens, add = _take(lens, "lens", (n,), dev, i32), _take(add, "add", (n,), dev, i32)
-    _take(tables, "tables", (n, tables.shape[1]), dev, i32, writes=True)
+    _take(tables, "tables", (n, max_pages), dev, i32, writes=True)
     _take(held, "held", (n,), dev, i32, writes=True)
-    _take(free_pages, "free_pages", free_pages.shape, dev, i32, writes=True)
+    _take(free_pages, "free_pages", (capacity,), dev, i32, writes=True)
     _take(free_count, "free_count", (1,), dev, i32, writes=True)
     if out is None:
-        if max_tokens < 0:
-            raise KvCacheError("map_pages: max_tokens must be >= 0")
         slots, positions, starts, totals, status = lens.new_empty(3 * max_tokens + 2 * n + 2).split_with_sizes(
             (2 * max_tokens, max_tokens, n + 1, n, 1))
         out = PageMap(slots.view(torch.int64), positions, starts, totals, status)
@@ -69,9 +70,9 @@ def map_pages(lens: torch.Tensor, add: torch.Tensor, tables: torch.Tensor, held:
         for t, name, size, dtype in zip(out, PageMap._fields, (max_tokens, max_tokens, n + 1, n, 1),
                                         (torch.int64, i32, i32, i32, i32)):
             _take(t, name, (size,), dev, dtype, writes=True)
-    _call(lib().pkv_pages_map(lens.data_ptr(), add.data_ptr(), n, tables.data_ptr(), tables.shape[1],
+    _call(lib().pkv_pages_map(lens.data_ptr(), add.data_ptr(), n, tables.data_ptr(), max_pages,
                               held.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
-                              free_pages.shape[0], page_tokens, out.slots.data_ptr(),
+                              capacity, page_tokens, out.slots.data_ptr(),
                               out.positions.data_ptr(), max_tokens, out.starts.data_ptr(),
                               out.totals.data_ptr(), out.status.data_ptr(), _stream()))
     return out
@@ -82,9 +83,12 @@ def _planes(k_pages: torch.Tensor, v_pages: torch.Tensor, dev: int):
     quant = _PAGES.get(k_pages.dtype)
     if quant is None or k_pages.dim() != 4:
         raise KvCacheError("pages are float16 or bfloat16 [n_pages, page_tokens, kv heads, head_dim]")
-    _take(k_pages, "k_pages", k_pages.shape, dev, k_pages.dtype, writes=True)
-    _take(v_pages, "v_pages", k_pages.shape, dev, k_pages.dtype, writes=True)
-    return quant, k_pages.shape
+    shape = k_pages.shape
+    if (shape[0] | shape[1] | shape[2] | shape[3]) >> 31:
+        _past_32_bits("the pages' sizes", *shape)
+    _take(k_pages, "k_pages", shape, dev, k_pages.dtype, writes=True)
+    _take(v_pages, "v_pages", shape, dev, k_pages.dtype, writes=True)
+    return quant, shape
 
 
 def append_pages(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor,
@@ -119,19 +123,22 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     all), sinks: the first keys that it sees all the same. Returns out [tokens, heads, head_dim];
     rows of no request are left as they were (zeros if out is not given)."""
     dev = _device()
+    expects = "attend_pages expects q [tokens, heads, head_dim], heads a multiple of the pages', and tables [n, max_pages]"
+    if q.dim() != 3 or tables.dim() != 2:
+        raise KvCacheError(expects)
+    (tokens, heads, width), (n, max_pages) = q.shape, tables.shape
+    if (window | sinks | n | max_pages | tokens | heads) >> 31:
+        _past_32_bits("window, sinks, n, max_pages, tokens and heads", window, sinks, n, max_pages, tokens, heads)
     quant, (n_pages, page, kv_heads, dim) = _planes(k_pages, v_pages, dev)
-    if q.dim() != 3 or q.shape[2] != dim or tables.dim() != 2 or q.shape[1] == 0 or q.shape[1] % kv_heads:
-        raise KvCacheError("attend_pages expects q [tokens, heads, head_dim], heads a multiple of the pages', "
-                           "and tables [n, max_pages]")
-    tokens, heads, _ = q.shape
-    n = tables.shape[0]
+    if width != dim or heads == 0 or heads % kv_heads:
+        raise KvCacheError(expects)
     st, sh, sd = q.stride()
     if (q.get_device() != dev or q.dtype is not torch.float32 or sd != 1 or sh < dim or sh % 4 or st % 4 or
             st < (heads - 1) * sh + dim or q.data_ptr() % 16):
         _take(q, "q", q.shape, dev)
         q = q.clone(memory_format=torch.contiguous_format)
         st, sh, sd = q.stride()
-    tables = _take(tables, "tables", tables.shape, dev, torch.int32)
+    tables = _take(tables, "tables", (n, max_pages), dev, torch.int32)
     lens = _take(lens, "lens", (n,), dev, torch.int32)
     starts = _take(starts, "starts", (n + 1,), dev, torch.int32)
     if out is None:
@@ -142,7 +149,7 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     # torch's allocator orders the workspace with the stream, and gives each graph its own
     ws = out.new_empty(need, dtype=torch.uint8) if need else None
     _call(lib().pkv_pages_attend(quant, q.data_ptr(), st, sh, k_pages.data_ptr(), v_pages.data_ptr(), n_pages,
-                                 page, tables.data_ptr(), tables.shape[1], lens.data_ptr(), _at(starts), n,
+                                 page, tables.data_ptr(), max_pages, lens.data_ptr(), _at(starts), n,
                                  tokens, heads, kv_heads, dim, scale, window, sinks, out.data_ptr(), _at(ws),
                                  need, _stream()))
     return out
@@ -160,6 +167,8 @@ def verify_drafts(target_probs: torch.Tensor, drafts: torch.Tensor, uniforms: to
         raise KvCacheError("verify_drafts expects target_probs [n, k + 1, vocab]")
     n, rows, vocab = target_probs.shape
     k = rows - 1
+    if (n | k | vocab) >> 31:
+        _past_32_bits("n, k and vocab", n, k, vocab)
     target_probs = _take(target_probs, "target_probs", (n, rows, vocab), dev)
     draft_probs = _take(draft_probs, "draft_probs", (n, k, vocab), dev)
     drafts = _take(drafts, "drafts", (n, k), dev, torch.int32)

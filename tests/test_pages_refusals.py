@@ -145,6 +145,44 @@ def test_python_refuses_host_tensors_and_shapes():
         pk.verify_drafts(t(1, 3, 9), i(1, 2), t(1, 3))
 
 
+@pytest.mark.parametrize("bad", [2 ** 31, 2 ** 32, 2 ** 32 + 64, 2 ** 64 + 64, -2 ** 32, -1])
+def test_python_refuses_numbers_past_32_bits(bad):
+    """ctypes drops the high bits of a number: what does not fit C's int is refused in front of it."""
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    h = lambda *s: torch.zeros(*s, dtype=torch.float16)  # noqa: E731
+    t = torch.zeros
+    words = r"must be in \[0, 2\^31\)"
+    for page, tokens in ((bad, 10), (64, bad)):
+        with pytest.raises(pk.KvCacheError, match=words):
+            pk.map_pages(i(2), i(2), i(2, 4), i(2), i(8), i(1), page, tokens)
+    for k in (dict(window=bad), dict(sinks=bad), dict(window=5, sinks=bad)):
+        with pytest.raises(pk.KvCacheError, match=words):
+            pk.attend_pages(t(1, 4, 64), h(4, 32, 2, 64), h(4, 32, 2, 64), i(1, 4), i(1), 0.1, **k)
+    pool = object.__new__(pk.PagedKvPool)
+    with pytest.raises(pk.KvCacheError, match=words):
+        pool.take_pages(bad)
+    for at in range(4):
+        with pytest.raises(pk.KvCacheError, match=words):
+            pk.PagedKvPool(*[bad if j == at else x for j, x in enumerate((2, 64, 32, 4))], pk.KvCacheQuantization.F16, stream=0)
+
+
+def test_python_refuses_shapes_past_32_bits():
+    i = lambda *s: torch.zeros(1, dtype=torch.int32).expand(*s)  # noqa: E731
+    h = lambda *s: torch.zeros(1, dtype=torch.float16).expand(*s)  # noqa: E731
+    f = lambda *s: torch.zeros(1).expand(*s)  # noqa: E731
+    big, words = 2 ** 32 + 2, r"must be in \[0, 2\^31\)"
+    with pytest.raises(pk.KvCacheError, match=words):
+        pk.map_pages(i(2), i(2), i(2, big), i(2), i(8), i(1), 64, 10)
+    with pytest.raises(pk.KvCacheError, match=words):
+        pk.map_pages(i(2), i(2), i(2, 4), i(2), i(big), i(1), 64, 10)
+    with pytest.raises(pk.KvCacheError, match=words):
+        pk.append_pages(f(1, 2, 64), f(1, 2, 64), torch.zeros(1, dtype=torch.int64), h(big, 32, 2, 64), h(big, 32, 2, 64))
+    with pytest.raises(pk.KvCacheError, match=words):
+        pk.attend_pages(f(1, 4, 64), h(4, 32, 2, 64), h(4, 32, 2, 64), i(1, big), i(1), 0.1)
+    with pytest.raises(pk.KvCacheError, match=words):
+        pk.verify_drafts(f(1, 3, big), i(1, 2), f(1, 3))
+
+
 # ------------------------------------------------------------------ the plain forms themselves
 def test_plain_map():
     # a request shrinks from three pages to one, one ends, one takes two pages: theirs, last given first

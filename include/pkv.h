@@ -489,7 +489,8 @@ int pkv_pages_append(int quant, const float *k, const float *v, int64_t k_stride
  * lens and starts are taken into what tables and tokens hold; pages that no key seen lies in are
  * not read; a key in a page outside [0, n_pages) is not seen, and pkv_device_status reports it.
  * workspace: at least pkv_pages_attend_workspace() bytes of device memory, 256-byte aligned,
- * which the call writes: calls that overlap in time, and graphs that do, need one each. */
+ * which the call writes: calls that overlap in time, and graphs that do, need one each. The size never
+ * falls as n or tokens grow: one for the most requests and tokens of any step serves all of them. */
 size_t pkv_pages_attend_workspace(int n, int64_t tokens, int num_heads, int num_kv_heads,
                                   int head_dim);
 int pkv_pages_attend(int quant, const float *q, int64_t q_stride_t, int64_t q_stride_h,

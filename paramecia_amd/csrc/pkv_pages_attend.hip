@@ -25,6 +25,8 @@
 //
 // Bound: of few rows the bytes of the keys (2 rows of 16 bits a key and KV head), of prompts the matrix
 // cores: 4 head_dim flops a key and row, twice (F16) or three times (BF16).
+#include <algorithm>
+
 #include "pkv_half_common.hpp"
 #include "pkv_internal.hpp"
 
@@ -1273,20 +1275,27 @@ struct Shape {
   int rows, shares, start;
   bool prompts() const { return start == 6; }
 };
-Shape shape_of(int n, int64_t tokens, int group, int head_dim) {
-  const int64_t rows = tokens * group;
-  for (const int r : {16, 32, 48})
-    if (rows <= r * (int64_t)n) return Shape{r, (r == 16 && head_dim < 256 ? 768 : 512) * 256 / head_dim, 2};
+constexpr int kFewRows[] = {16, 32, 48};
+Shape few_shape(int rows, int head_dim) {
+  return Shape{rows, (rows == 16 && head_dim < 256 ? 768 : 512) * 256 / head_dim, 2};
+}
+Shape prompt_shape(int head_dim) {
   return head_dim == 64 ? Shape{64, 1024, 6} : head_dim == 128 ? Shape{64, 768, 6} : Shape{128, 256, 6};
+}
+// rows: of the whole step, tokens x query heads of a KV head
+Shape shape_of(int n, int64_t rows, int head_dim) {
+  for (const int r : kFewRows)
+    if (rows <= r * (int64_t)n) return few_shape(r, head_dim);
+  return prompt_shape(head_dim);
 }
 struct Layout {
   size_t tiles, before, firsts, count, ml, part, all;
   int max_tiles;
 };
-Layout layout_of(const Shape &sh, int n, int64_t tokens, int group, int head_dim) {
+Layout layout_of(const Shape &sh, int n, int64_t rows, int head_dim) {
   Layout l;
   const auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  l.max_tiles = (int)(n + tokens * group / sh.rows);
+  l.max_tiles = (int)(n + rows / sh.rows);
   l.tiles = 0;
   l.before = up((size_t)l.max_tiles * sizeof(Tile));
   l.firsts = l.before + up(((size_t)l.max_tiles + 1) * sizeof(int64_t));
@@ -1341,15 +1350,25 @@ int go(AttendArgs &a, const Shape &sh, hipStream_t s) {
 
 }  // namespace
 
+// What any step of up to n requests and `tokens` tokens needs, so that a buffer for the largest step holds
+// the smaller ones: tiles of fewer rows have more shares and may need more (head_dim 64, 24 requests, 8
+// heads of a KV head: 52 MB for 144 tokens, 35 for 8192).
 size_t pages_attend_workspace(int n, int64_t tokens, int heads, int kv_heads, int head_dim) {
-  const int group = heads / kv_heads;
-  return layout_of(shape_of(n, tokens, group, head_dim), n, tokens, group, head_dim).all;
+  const int64_t rows = tokens * (heads / kv_heads);
+  size_t most = 0;
+  int64_t below = 0;  // one request of more rows takes the shape at hand, or a later one
+  for (const int r : kFewRows) {
+    const int64_t own = rows < r * (int64_t)n ? rows : r * (int64_t)n;  // as many as it is for
+    if (rows > below) most = std::max(most, layout_of(few_shape(r, head_dim), n, own, head_dim).all);
+    below = r;
+  }
+  return rows > below ? std::max(most, layout_of(prompt_shape(head_dim), n, rows, head_dim).all) : most;
 }
 
 int launch_pages_attend(const PagesAttend &p, void *ws, hipStream_t s) {
   const int group = p.heads / p.kv_heads;
-  const Shape sh = shape_of(p.n, p.tokens, group, p.head_dim);
-  const Layout l = layout_of(sh, p.n, p.tokens, group, p.head_dim);
+  const Shape sh = shape_of(p.n, p.tokens * group, p.head_dim);
+  const Layout l = layout_of(sh, p.n, p.tokens * group, p.head_dim);
   uint8_t *w = static_cast<uint8_t *>(ws);
   AttendArgs a;
   a.q = p.q;

@@ -94,6 +94,18 @@ def test_attend_workspace():
     assert 0 < f(1, 1, 16, 2, 256) <= 160 << 20 and 0 < f(8, 8001, 16, 2, 256) <= 160 << 20
 
 
+@pytest.mark.parametrize("heads,kv,dim", [(16, 2, 256), (8, 1, 64), (32, 8, 128), (28, 4, 128), (96, 2, 256), (6, 6, 128), (2, 2, 64)])
+def test_attend_workspace_for_the_largest_step_serves_all(heads, kv, dim):
+    counts = [1, 2, 3, 4, 6, 7, 9, 16, 24, 33, 64, 65, 100, 144, 300, 1025, 8192, 20000]
+    f = lambda n, t: lib().pkv_pages_attend_workspace(n, t, heads, kv, dim)  # noqa: E731
+    for n, more in zip(counts, counts[1:] + [100000]):
+        for t, longer in zip(counts, counts[1:] + [100000]):
+            assert 0 < f(n, t) <= f(n, longer) and f(n, t) <= f(more, t), (n, t)
+    # a buffer for 64 requests and 8192 tokens is taken by steps of fewer (that end at the next check)
+    for n, t in ((24, 144), (1, 1), (64, 64), (3, 8000)):
+        assert attend(n=n, t=t, h=heads, kv=kv, d=dim, qt=heads * dim, qh=dim, wb=f(64, 8192), ws=H) == ERR_ARG and "overlap" in err()
+
+
 def verify(**k):
     a = dict(p=A, ps=1000, q=B, qs=1000, x=C, c=D, u=F, n=3, k=4, v=1000, t=G, acc=H, ws=I, wb=None)
     a.update(k)

@@ -481,8 +481,8 @@ int pkv_pages_append(int quant, const float *k, const float *v, int64_t k_stride
 /* The attention of pkv_attend over pages: request b's queries are the rows [starts[b],
  * starts[b + 1]) of q (starts NULL: row b alone), the last tokens of its lens[b] keys (new ones
  * included), the pages of tables[b]. A query at position p sees key j iff j <= p and (window
- * == 0, j > p - window, or j < sinks); scores are scaled, clamped to [-100, 100] and
- * soft-maxed; a query that sees no key gives zeros. q: [tokens, num_heads, head_dim] f32, tokens
+ * == 0, j > p - window, or j < sinks); scores are scaled (scale times log2(e) must be finite in
+ * f32), clamped to [-100, 100] and soft-maxed; a query that sees no key gives zeros. q: [tokens, num_heads, head_dim] f32, tokens
  * q_stride_t and heads q_stride_h elements apart; out: [tokens, num_heads, head_dim] f32, whose
  * rows of no request are left as they were. quant PKV_QUANT_F16 or PKV_QUANT_BF16, head_dim 64,
  * 128 or 256 (else PKV_ERR_UNSUPPORTED); q and out 16-byte aligned, q's strides multiples of 4.

@@ -113,7 +113,8 @@ int pkv_pages_attend(int quant, const float *q, int64_t q_stride_t, int64_t q_st
   if ((int64_t)max_pages * page_tokens > kMost32 - 64)
     return set_error(PKV_ERR_ARG, "a table must name fewer than 2^31 - 64 tokens");
   if (window < 0 || sinks < 0) return set_error(PKV_ERR_ARG, "window and sinks must be >= 0");
-  if (!std::isfinite(scale)) return set_error(PKV_ERR_ARG, "scale must be finite");
+  // the kernels hold scores times log2(e)
+  if (!std::isfinite(scale * 1.4426950408889634f)) return set_error(PKV_ERR_ARG, "scale times log2(e) must be finite");
   if (!starts && tokens != n)
     return set_error(PKV_ERR_ARG, "without starts every request has one row: tokens must be n");
   if (quant == PKV_QUANT_NONE) quant = PKV_QUANT_F16;

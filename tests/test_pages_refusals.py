@@ -106,6 +106,17 @@ def test_attend_workspace_for_the_largest_step_serves_all(heads, kv, dim):
         assert attend(n=n, t=t, h=heads, kv=kv, d=dim, qt=heads * dim, qh=dim, wb=f(64, 8192), ws=H) == ERR_ARG and "overlap" in err()
 
 
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38, math.inf, -math.inf, math.nan, 1e39])
+def test_attend_refuses_scales_whose_product_passes_f32(scale):
+    """Scores are held times log2(e): 1.44 scale has to be a number too, or zeros would give NaN."""
+    assert attend(scale=scale) == ERR_ARG and "finite" in err()
+
+
+def test_attend_takes_the_largest_scale():
+    for scale in (2.3e38, -2.3e38, 0.0):  # (they end at the next check)
+        assert attend(scale=scale, starts=None) == ERR_ARG and "tokens must be n" in err()
+
+
 def verify(**k):
     a = dict(p=A, ps=1000, q=B, qs=1000, x=C, c=D, u=F, n=3, k=4, v=1000, t=G, acc=H, ws=I, wb=None)
     a.update(k)

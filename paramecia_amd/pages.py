@@ -98,7 +98,7 @@ def append_pages(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages:
     negative one: no row); k_pages, v_pages [n_pages, page_tokens, kv heads, head_dim]."""
     dev = _device()
     quant, (n_pages, page, heads, dim) = _planes(k_pages, v_pages, dev)
-    n = slots.shape[0]
+    n = slots.numel()
     rows, strides = [], []
     for t, name in ((k, "k"), (v, "v")):
         if (t.get_device() != dev or t.dtype is not torch.float32 or t.shape != (n, heads, dim) or
@@ -130,7 +130,7 @@ def attend_pages(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     if (window | sinks | n | max_pages | tokens | heads) >> 31:
         _past_32_bits("window, sinks, n, max_pages, tokens and heads", window, sinks, n, max_pages, tokens, heads)
     quant, (n_pages, page, kv_heads, dim) = _planes(k_pages, v_pages, dev)
-    if width != dim or heads == 0 or heads % kv_heads:
+    if width != dim or heads == 0 or kv_heads == 0 or heads % kv_heads:
         raise KvCacheError(expects)
     st, sh, sd = q.stride()
     if (q.get_device() != dev or q.dtype is not torch.float32 or sd != 1 or sh < dim or sh % 4 or st % 4 or

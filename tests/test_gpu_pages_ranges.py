@@ -5,7 +5,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from pages_checks import E, attend64  # noqa: E402
-from test_gpu_pages import Case, gen, pk, say  # noqa: E402, F401
+from test_gpu_pages import Case, gen, i32, pk, say  # noqa: E402, F401
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,18 @@ def test_means_of_the_largest_values(pk, dim, lens, new, mag, signed):
     weigh, _ = attend64(c.q, c.k, c.v.abs(), c.tables, c.lens, c.scale, c.starts, 100, 4, c.out)
     assert torch.isfinite(few).all()
     assert ((few.double() - want).abs() <= bound + 16 * 400 * E * weigh).all()
+
+
+def test_refusals_of_empty_shapes(pk):
+    """Slots that are no row of numbers, and pages without heads: the framework's error, and nothing moved."""
+    k, v = (torch.zeros(2, 32, 2, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    new = torch.ones(1, 2, 64, device="cuda")
+    for slots in (torch.tensor(3, device="cuda"), torch.zeros(1, 1, dtype=torch.int64, device="cuda")):
+        with pytest.raises(pk.KvCacheError, match="slots must have shape"):
+            pk.append_pages(new, new, slots, k, v)
+    none = k[:, :, :0].contiguous()
+    with pytest.raises(pk.KvCacheError, match="heads a multiple"):
+        pk.attend_pages(torch.zeros(1, 4, 64, device="cuda"), none, none, i32([[0]]), i32([1]), 0.1)
+    with pytest.raises(pk.KvCacheError, match="n_kv_heads"):
+        pk.append_pages(new[:, :0], new[:, :0], torch.zeros(1, dtype=torch.int64, device="cuda"), none, none)
+    assert int((k != 0).sum()) == 0

@@ -486,6 +486,9 @@ int pkv_pages_append(int quant, const float *k, const float *v, int64_t k_stride
  * q_stride_t and heads q_stride_h elements apart; out: [tokens, num_heads, head_dim] f32, whose
  * rows of no request are left as they were. quant PKV_QUANT_F16 or PKV_QUANT_BF16, head_dim 64,
  * 128 or 256 (else PKV_ERR_UNSUPPORTED); q and out 16-byte aligned, q's strides multiples of 4.
+ * The kernels' tiles are chosen by tokens * (num_heads / num_kv_heads) / n, rows of no request
+ * among them, as lengths are not known on the host: a step that is padded past some rows a request, or
+ * one prompt among single tokens, is right but slower than calls of their own.
  * lens and starts are taken into what tables and tokens hold; pages that no key seen lies in are
  * not read; a key in a page outside [0, n_pages) is not seen, and pkv_device_status reports it.
  * workspace: at least pkv_pages_attend_workspace() bytes of device memory, 256-byte aligned,

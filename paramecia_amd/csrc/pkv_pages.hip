@@ -12,8 +12,8 @@ namespace pkv {
 namespace {
 
 // Tokens up to which the mapping workgroup writes the slots itself; more are left to a launch
-// of their own (24 requests of 24 rows in all: 3.6 us, with the launch 4.8; of 1024 5.3 and 5.2; of
-// 4096 8.0 and 5.3).
+// of their own (24 requests of 24 rows in all: with the launch 1.2 us more; of 1024 as long; of 4096 2.7
+// less).
 constexpr int64_t kMapTokensInline = 1024;
 constexpr int kStartsInLds = 4096;
 
@@ -105,7 +105,7 @@ __device__ __forceinline__ void write_slot(const MapArgs &a, const Starts &start
 // moves the few pages of its request; those of a request that moves more its whole wave, a lane a
 // page. Bound: the chain of its loads and barriers (MI355X: 24 requests 4.0 us, 2.8 of it a launch;
 // 300 with 8001 rows 7.1, and 3.5 for their slots). All three sums take one scan: with one each the
-// kernel took 7.8 us for 24 requests.
+// kernel took 3.8 us more for 24 requests.
 constexpr int kLanePages = 4;
 template <int kThreads>
 __global__ __launch_bounds__(kThreads) void pages_map_kernel(MapArgs a) {
@@ -239,7 +239,7 @@ __device__ __forceinline__ uint32_t round2(float a, float b) {
 
 // Eight elements a thread (16-byte loads and stores), or one where a row's width, stride or
 // address allows no more. Bound: the bytes (MI355X: 8001 rows of 512 values of K and V in F16 9.1 us,
-// 5.4 TB/s, part of it in the last-level cache; 24 rows 2.7 us, a launch).
+// 5.4 TB/s, part of it in the last-level cache; 24 rows 2.6 us, a launch).
 template <bool kBf, int kPer>
 __global__ __launch_bounds__(256) void pages_append_kernel(RowsArgs a, int per_row) {
   const uint32_t i = blockIdx.x * 256 + threadIdx.x;  // (a launch holds fewer than 2^32)
@@ -288,7 +288,7 @@ int launch_pages_map(const int *lens, const int *add, int n, int *tables, int ma
   a.capacity = capacity;
   a.page_lg = __builtin_ctz((unsigned)page_tokens);
   a.fill = max_tokens <= kMapTokensInline;
-  // a thread a request: fewer waves have shorter barriers (24 requests: 3.6 us, with 1024 threads 5.7)
+  // a thread a request: fewer waves have shorter barriers (24 requests: with 1024 threads 2.1 us more)
   if (n <= 256)
     hipLaunchKernelGGL(pages_map_kernel<256>, dim3(1), dim3(256), 0, s, a);
   else

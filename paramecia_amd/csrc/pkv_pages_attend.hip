@@ -12,10 +12,11 @@
 // Mathematics: with x_j = clamp(scale q.k_j) log2(e), one pass over the keys holds per row the running
 // maximum m, l = sum 2^(x_j - m) and sum 2^(x_j - m) v_j in f32; a larger maximum rescales both. Parts
 // of a row are kept as means, and join as those weighed with their share 2^(m_i - max m) l_i of the
-// sum: BF16 values reach 3.4e38, whose mean f32 holds and whose sum it does not. The matrix cores take 16-bit operands, and
-// K and V are 16-bit rows already, so that only q and the weights are rounded: they go in as sums of
-// two fp16 parts (F16 pages) or three bf16 parts (BF16), 22 and 24 bits, which costs two or three
-// products for one and keeps a row within 2e-6 of 64-bit sums; one part alone is off by 2^-11 or 2^-8.
+// sum: BF16 values reach 3.4e38, whose mean f32 holds and whose sum it does not. The matrix cores
+// take 16-bit operands, and K and V are 16-bit rows already, so that only q and the weights are
+// rounded: they go in as sums of two fp16 parts (F16 pages) or three bf16 parts (BF16), 22 and 24
+// bits, which costs two or three products for one and keeps a row within 2e-6 of 64-bit sums; one
+// part alone is off by 2^-11 or 2^-8.
 //
 // Work: a tile is 16 to 128 rows of one request (row = token x query heads of a KV head, which share
 // their keys); its keys are blocks of 32 (one page each), the sinks' blocks first, then the window's. The
@@ -23,8 +24,8 @@
 // whatever the lengths are: 24 requests of 65 to 65536 keys end together. A share that holds a whole
 // tile writes its rows of out; the parts of a tile that is cut meet in the join, a launch of their own.
 //
-// Bound: of few rows the bytes of the keys (2 rows of 16 bits a key and KV head), of prompts the matrix
-// cores: 4 head_dim flops a key and row, twice (F16) or three times (BF16).
+// Bound: of few rows the bytes of the keys (2 rows of 16 bits a key and KV head); of prompts 4 head_dim
+// flops a key and row, twice (F16) or three times (BF16), and what brings them their operands.
 #include <algorithm>
 
 #include "pkv_half_common.hpp"
@@ -590,12 +591,12 @@ __device__ __forceinline__ bool all_seen(const AttendArgs &a, int p0, int p1, in
 }
 
 // ---- up to 16 kRT rows a tile, for one token and a few.
-// Measured (MI355X; 16 query heads over 2 KV heads of 256): 24 tokens of 300000 BF16 keys in all
-// 117 us, 5.2 TB/s of keys (a copy of 2 GiB: 4.8); one token of 131073 BF16 keys 47 us, 5.7 TB/s;
-// one of 1025 F16 keys 7.4 us, four dependent trips to memory (lengths, table, rows, sums of the
+// Measured (MI355X, the kernel alone; 16 query heads over 2 KV heads of 256): 24 tokens of 297000 BF16
+// keys in all 113 us, 5.4 TB/s of keys (a copy of 2 GiB: 4.8); one token of 131073 BF16 keys 46 us, 5.8
+// TB/s; one of 1025 F16 keys 7.2 us, four dependent trips to memory (lengths, table, rows, sums of the
 // line); 16 x 5 drafted tokens, F16, a window of 4096: 30 us, 16 of it the keys' bytes, the rest each
 // workgroup's plan, its 40 rows of queries and its parts' rows. Straight into registers since a block's
-// rows serve one tile only (by way of LDS 24 tokens took 166 us, then 139).
+// rows serve one tile only (by way of LDS 24 tokens took a fifth longer).
 // A workgroup of kD / 64 waves: wave w takes
 // elements 64 w .. of all 32 keys of a block for the scores, and columns 64 w .. of V. Rows go from
 // memory straight into registers as MFMA operands, a block ahead; the waves' partial scores meet
@@ -827,18 +828,18 @@ __global__ __launch_bounds__(kD, 2) void few_kernel(AttendArgs a) {
 }
 
 // ---- tiles of 16 kW rows, 16 a wave, for prompts.
-// Measured (MI355X; 16 query heads over 2 KV heads of 256): 512 new tokens over 16896 BF16 keys 310 us,
-// 1.35 PFLOP/s of products in three parts (a library product of 8192^3 in BF16: 1.14); 8001 tokens of
-// F16 in a window of 1024 behind 4 first keys 265 us, 0.84 PFLOP/s of the keys seen in two parts. Bound:
-// instructions. Beside a block's 64 (F16) or 96 (BF16) products a wave runs some 170 or 210 vector
-// instructions (maximum, exponents, parts, masks at the window's edges), and a SIMD issues one or the
-// other: products alone run at 2.07 PFLOP/s with two waves a SIMD, at 1.35 beside four vector instructions
-// each. Without the softmax (a copy of this kernel) the chunk of 512 takes 258 us instead of 305 in F16,
-// with products and barriers alone 228. 16 rows a wave: 32, with half the reads of LDS, need more than 256
-// registers beside the sums of 256 columns (one wave a SIMD: 970 us for the 8001 tokens), and where they
-// fit (head_dim 128) gain 4% in F16 and nothing in BF16.
-// Blocks' rows of K and V go from memory
-// into LDS ahead of their use; every wave runs its rows from there:
+// Measured (MI355X, a call less its plan and join; 16 query heads over 2 KV heads of 256): 512 new tokens
+// over 16896 BF16 keys 320 us, 1.31 PFLOP/s of products in three parts (a library product of 8192^3 in
+// BF16: 1.14); 8001 tokens of F16 in a window of 1024 behind 4 first keys 260 us, 0.84 PFLOP/s of the keys
+// seen in two parts. Bound, by copies of this kernel that leave a part out: no one part. Of the BF16
+// chunk's time the softmax is 10%, the reads of LDS 16, the loads into it 5, and products, barriers and
+// the tiles' starts what is left; a block takes 2.0 us in F16, 0.9 of them the products at the matrix
+// cores' full rate. A tile's start and end (queries, first blocks, rows of out) take 13 us with nothing
+// beside them, one workgroup a CU: a quarter of the 8001 tokens in a window, whose softmax is 5% and loads
+// 7. Of head_dim 128 and 64 the softmax is 18 and 28%. 16 rows a wave: 32, with half the reads of LDS, need
+// more than 256 registers beside the sums of 256 columns (one wave a SIMD: three times as long), and
+// where they fit (head_dim 128) gain 4% in F16 and nothing in BF16.
+// Blocks' rows of K and V go from memory into LDS ahead of their use; every wave runs its rows from there:
 //   scores (transposed, A = K) with keys in the order of few_kernel; out (transposed, A = V): V's
 //   columns come by transposing reads; the result is columns 16 c + 4 g + i of row n.
 // Pieces of 16 bytes of a row are turned by the row, so that the 16 rows which a quarter of a wave
@@ -896,9 +897,9 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
   constexpr int kMoves = 4 * kD / kThreads;  // 16-byte pieces of K, and of V, that a thread moves
   // Blocks of K and of V in LDS. Four: two between barriers, the two behind them on their way. Rows
   // of 256 bytes take three, one and one or two, so that three workgroups fit a CU's LDS (8001 tokens in a
-  // window, 32 heads of 128: 360 us, with four 471; of 256, 16 heads: 304 by pairs, 317 one by one),
+  // window, 32 heads of 128: with four 31% longer; of 256, 16 heads: one by one 4% longer than by pairs),
   // and BF16 rows of 512 bytes, whose registers a pair's second block exceeds (512 tokens over 16896
-  // keys: 356 us, by pairs 361).
+  // keys: by pairs 1% longer).
   constexpr bool kPairs = kD == 64 || (kD == 256 && !kBf);
   constexpr int kRing = kPairs ? 4 : 3;
   __shared__ __attribute__((aligned(1024))) uint16_t lk[kRing][kBlk * kD], lv[kRing][kBlk * kD];
@@ -929,7 +930,8 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
   // by an exclusive or of their low bits, so four steps and eight tiles on the place is 256 bytes on.
   // BF16 rows of 512 bytes leave no registers for twelve places: they are worked out again in each
   // block from the lane's two. (What the compiler puts into scratch memory instead comes back
-  // behind the loads of LDS: 8001 tokens 1020 us instead of 400.)
+  // behind the loads of LDS: 8001 tokens 2.5 times as long. Fifteen values still lie there, of which a
+  // block with masks reads two and one block in three another.)
   constexpr bool kAgain = kBf && kD == 256;
   constexpr int kK = kAgain ? 1 : kSteps < 4 ? kSteps : 4, kV = kAgain ? 1 : kCols < 8 ? kCols : 8;
   const auto k_place = [](int st) {
@@ -1009,7 +1011,7 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
     for (int c = 0; c < kCols; ++c) acc[c] = zero;
     f4 sc[2];
     // operands come from LDS kAhead reads ahead of the products that take them (two: 512 tokens over
-    // 16896 BF16 keys 376 us instead of 356; six and eight: the same within 1%)
+    // 16896 BF16 keys 6% longer; six and eight: the same within 1%)
     constexpr int kAhead = 4;
     const auto scores = [&](const uint16_t *kb) {
       constexpr int kReads = 2 * kSteps;
@@ -1140,9 +1142,9 @@ __global__ __launch_bounds__(64 * kW, kD == 256 ? 2 : kD == 128 ? 3 : 4) void ma
   }
 }
 
-// ---- the parts of a tile that was cut, joined (4.5 us where one token's 1025 keys lie in 64 parts, 7 for 24
-// requests and for 131073 keys in 512, 23 behind 8001 prompt tokens: 256 parts of 128 rows twice over, 64
-// MB). Bound: two trips to memory and a launch, or the parts' bytes. A wave a row, or kAcross waves a row of a tile
+// ---- the parts of a tile that was cut, joined (5 us where one token's 1025 keys lie in 64 parts, 7 for 24
+// requests, 8 for 131073 keys in 512 parts, 24 behind 8001 prompt tokens: 53 MB read, 26 written). Bound: two
+// trips to memory and a launch, or the parts' bytes. A wave a row, or kAcross waves a row of a tile
 // of many parts. The parts' maxima and sums come side by side, a lane a part; then their rows, four
 // in flight. By tile where there are fewer tiles than cuts, else by cut: the first cut inside a
 // tile joins it.
@@ -1267,10 +1269,13 @@ __global__ __launch_bounds__(kAcross > 1 ? 64 * kAcross : 256) void join_kernel(
 
 // Rows a tile holds, the workgroups that share the blocks (as many as the chip runs at once), and how
 // many blocks a tile's start costs: 2 of a few rows, 6 of a prompt's (start, queries, first loads and
-// stores take 20000 cycles, a block 4300; 4 and 8 made 8001 tokens in a window 3% slower).
+// stores take 13 us, a block 2; 4 and 8 made 8001 tokens in a window 3% slower).
 // Tiles of few rows for requests of up to 48 rows on average: 80 drafted tokens of 40 rows each
-// take 48 us in tiles of 48 and 78 in the prompts' tiles. Three waves a SIMD hold 16 rows of head_dim
-// 64 and 128 (24 requests of 64: 58 us by two, 44 by three), two anything else.
+// take 38 us in tiles of 48 and 53 in the prompts' tiles. The average is the step's, its rows of no request
+// among them, since lengths are not known here: one token of 65536 keys in a step of 9 rows or more takes
+// 67 us instead of 36, a chunk of 512 tokens over 4608 keys beside 23 tokens 184, in two calls 169.
+// Three waves a SIMD hold 16 rows of head_dim 64 and 128 (24 requests of 64: a quarter less than by two),
+// two anything else.
 struct Shape {
   int rows, shares, start;
   bool prompts() const { return start == 6; }
@@ -1311,9 +1316,10 @@ void join(AttendArgs &a, const Shape &sh, hipStream_t s) {
   const int64_t tiles = (int64_t)a.max_tiles * a.kv_heads;
   const int by_cut = tiles > sh.shares;
   const unsigned x = by_cut ? (unsigned)sh.shares : (unsigned)tiles;
-  // by the parts a tile has on average, waves a row: 131073 keys in 256 parts a tile 61 us with 16, 76
-  // with four, 140 with one; 8 requests of 3000 keys (32 parts) 20, 25 and 46; 80 drafted tokens (9) 52, 43 and
-  // 48; prompts of 8001 tokens (one or two) 574, 398 and 348
+  // by the parts a tile has on average, waves a row. What the others cost: 131073 keys in 256 parts a tile
+  // (16) 15 us more with four, 79 with one; 8 requests of 3000 keys (32 parts, 16) 5 and 26; 80 drafted
+  // tokens (9 parts, four) 9 us more with 16, 5 with one; 8001 prompt tokens (one or two parts, one) 226
+  // with 16, 50 with four
   if (tiles * 16 <= sh.shares)
     hipLaunchKernelGGL((join_kernel<kD, 16>), dim3(x, sh.rows), dim3(1024), 0, s, a, sh.rows, by_cut);
   else if (tiles * 4 <= sh.shares)

